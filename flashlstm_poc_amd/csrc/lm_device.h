@@ -1,0 +1,72 @@
+// Shared helpers of the language-model operators (lm_ops.h): element types, loads and stores of any alignment, reductions.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include "../../include/flashlstm/lm_ops.h"
+#include "../../include/flashlstm/lstm_core.h"
+#include "common.h"
+
+namespace flstm_hip {
+
+typedef __bf16 bfloat_t;
+typedef float float8 __attribute__((ext_vector_type(8)));
+
+template <class T> struct Vec8;
+template <> struct Vec8<half_t> { typedef half8 type; };
+template <> struct Vec8<bfloat_t> { typedef __bf16 type __attribute__((ext_vector_type(8))); };
+template <> struct Vec8<float> { typedef float8 type; };
+
+// Eight consecutive elements as floats.  The hardware loads 16 bytes from any address, so callers' tensors may begin anywhere;
+// only the element type's own alignment is assumed.
+template <class T> __device__ __forceinline__ float8 load8(const T* p) {
+    typename Vec8<T>::type v;
+    __builtin_memcpy(&v, __builtin_assume_aligned(p, sizeof(T)), sizeof(v));
+    return __builtin_convertvector(v, float8);
+}
+template <class T> __device__ __forceinline__ void store8(T* p, float8 v) {
+    const typename Vec8<T>::type r = __builtin_convertvector(v, typename Vec8<T>::type);
+    __builtin_memcpy(__builtin_assume_aligned(p, sizeof(T)), &r, sizeof(r));
+}
+// The same for a row's last vector, of which `n` elements exist (n <= 0: none; the others read as zero).
+template <class T> __device__ __forceinline__ float8 load8(const T* p, int n) {
+    if (n >= 8) return load8(p);
+    float8 v = 0.f;
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+        if (i < n) v[i] = float(p[i]);
+    return v;
+}
+template <class T> __device__ __forceinline__ void store8(T* p, float8 v, int n) {
+    if (n >= 8) return store8(p, v);
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+        if (i < n) p[i] = T(v[i]);
+}
+
+// Sum over groups of `N` neighbouring lanes (a power of two up to a wave), in every lane.
+template <int N> __device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+    for (int m = N / 2; m > 0; m /= 2) v += __shfl_xor(v, m, kWave);
+    return v;
+}
+template <int N> __device__ __forceinline__ float lanes_max(float v) {
+#pragma unroll
+    for (int m = N / 2; m > 0; m /= 2) v = fmaxf(v, __shfl_xor(v, m, kWave));
+    return v;
+}
+
+__host__ __device__ inline bool valid_dtype(int t) { return t == FLSTM_OP_F32 || t == FLSTM_OP_F16 || t == FLSTM_OP_BF16; }
+
+// Calls `f` with a value of the element type that `dtype` names.
+template <class F> inline int with_type(flstm_op_dtype dtype, F&& f) {
+    switch (dtype) {
+        case FLSTM_OP_F32: return f(float());
+        case FLSTM_OP_F16: return f(half_t());
+        case FLSTM_OP_BF16: return f(bfloat_t());
+    }
+    return FLSTM_E_INVALID;
+}
+
+inline int launched() { return int(hipGetLastError()); }
+
+}  // namespace flstm_hip
