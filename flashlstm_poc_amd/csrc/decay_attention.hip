@@ -1,0 +1,908 @@
+// Attention with a decaying state (lm_ops.h): prompts and training in chunks of tokens, single tokens by themselves.
+//
+// One sweep serves the forward pass and all three gradients.  For rows q, k (D wide) and v (E wide) it walks the tokens with a
+// D x E state X and a decay g:
+//     out_t = a g q_t X_{t-1} + b sum_{s in t's chunk, s <= t} g^(t-s) (q_t . k_s) v_s,   X_t = g X_{t-1} + c k_t v_t^T
+// Forward it is called with (q, k, v).  With A_s = scale q_s do_s^T + g A_{s+1} the gradients are
+//     dq_t = scale S_t do_t:  the sweep of (do, v, k) with the transposed state;
+//     dv_s = A_s^T k_s, dk_s = A_s v_s:  the sweeps of (k, q, do) and (v, do, q) from the last token to the first.
+//
+// A workgroup holds X of one head in its accumulators for a whole run of tokens, so that a token's rows are read once and its
+// output written once and nothing else leaves the chip: the sweep is bound by memory.  Each wave has 32 columns of X and forms
+// the scores of a chunk for itself: four times the products, which are a fraction of the time that the rows take to arrive, and
+// no exchange of them.  The layouts are chosen so that no accumulator passes through LDS: in every product below the operand
+// that was an accumulator before has its contraction index where the accumulator rows lie (see `perm`).
+#include "lm_device.h"
+
+namespace flstm_hip {
+namespace {
+
+constexpr int kMinHead = 8, kMaxHead = 256;     // dk, dv (8: a 16-byte slot of the narrower types)
+
+typedef unsigned uint4v __attribute__((ext_vector_type(4)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) short4v lds_short4;
+
+// Tokens a chunk: fp32 tiles are twice as large.
+template <class T> constexpr int kChunk = sizeof(T) == 4 ? 32 : 64;
+
+// Rows of one role: element (n, t, h, i) at data + n * sequence + t * token + (h / group) * head + i.
+struct Role {
+    void* data;
+    ptrdiff_t sequence, token, head;
+    int group;
+};
+
+struct Sweep {
+    Role q, k, v, out;
+    int d, e;              // widths of (q, k) and (v, out)
+    int out_f32;           // out holds floats whatever the type (shares of heads that are summed afterwards)
+    int reverse;           // from the last token to the first; x_in then belongs to the last token itself
+    const float* x_in;     // null: zeros
+    float* x_out;          // null: not written
+    int in_d, in_e, out_d, out_e;         // strides of a state's elements; states lie d * e apart
+    int in_slots, out_slots;              // states are counted by segment, not by sequence
+    float a, b, c;
+};
+
+struct Sweeps {
+    Sweep s[3];
+    int count;
+    size_t sequences, tokens, slots, segment;   // segment: tokens a workgroup walks at most, a multiple of every chunk
+    const int* cu_seqlens;
+    int heads, column_blocks;
+    const float* log_decay;
+};
+
+// The tokens of sequence n, whatever cu_seqlens holds; n == sequences: those behind the last.
+struct Span { long long first, length; };
+__device__ __forceinline__ Span span_of(const Sweeps& a, long long n) {
+    if (!a.cu_seqlens) return Span{0, (long long)a.tokens};
+    const long long all = (long long)a.tokens;
+    const auto bound = [&](long long i) {
+        if (i <= 0) return 0ll;
+        if (i > (long long)a.sequences) return all;
+        const long long v = a.cu_seqlens[i];
+        return v < 0 ? 0ll : v > all ? all : v;
+    };
+    const long long first = bound(n), end = bound(n + 1);
+    return Span{first, end > first ? end - first : 0};
+}
+// A sequence's segments have consecutive slots.  Packed: from first / segment + n on, which leaves each enough of them without
+// a sum over the sequences before.
+__device__ __forceinline__ long long first_slot(const Sweeps& a, long long n) {
+    if (!a.cu_seqlens) return n * (long long)(a.tokens ? (a.tokens + a.segment - 1) / a.segment : 1);
+    return span_of(a, n).first / (long long)a.segment + n;
+}
+__device__ __forceinline__ long long sequence_of(const Sweeps& a, long long slot) {
+    if (!a.cu_seqlens) return slot / (long long)(a.tokens ? (a.tokens + a.segment - 1) / a.segment : 1);
+    long long lo = 0, hi = (long long)a.sequences;   // the last n whose first slot is not behind this one
+    while (lo < hi) {
+        const long long mid = (lo + hi + 1) / 2;
+        if (first_slot(a, mid) <= slot) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+// exp2(n * l), 1 for n == 0 also where l is minus infinity.
+__device__ __forceinline__ float power(float l, float n) { return __builtin_amdgcn_exp2f(l * n); }
+__device__ __forceinline__ float log2_decay(const float* log_decay, int head) {
+    const float l = log_decay[head] * 1.4426950408889634f;
+    return l < -1e30f ? -1e30f : l;
+}
+
+__device__ __forceinline__ float uniform(float v) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v))); }
+
+// ---- matrix products.  An operand fragment is eight values a lane: lane l holds row (or column) l % 32 and, of a step of 16
+// along the contraction, the values 8 * (l / 32) .. + 7.
+
+template <class T> struct Frag { typedef typename Vec8<T>::type type; };
+
+__device__ __forceinline__ floatx16 mma(half8 a, half8 b, floatx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ floatx16 mma(Vec8<bfloat_t>::type a, Vec8<bfloat_t>::type b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ floatx16 mma(float8 a, float8 b, floatx16 c) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
+    return c;
+}
+
+// Accumulator row 8 * (r / 4) + 4 * (l / 32) + r % 4 sits in register r.  Where an operand's rows are handed over in the order
+// perm(0), perm(1), .. (the two inner blocks of four of every sixteen exchanged), register r of the result is row
+// 16 * (r / 8) + 8 * (l / 32) + r % 8: registers 0..7 and 8..15 are then each a fragment for a product along those rows.
+__device__ __forceinline__ int perm(int i) { return (i & ~12) | ((i & 4) << 1) | ((i & 8) >> 1); }
+
+// ---- tiles in LDS: blocks of 32 columns, in each of which the rows lie one behind the other, in 16-byte slots that a row's
+// number permutes.  Sixteen rows read at one column lie in different banks, and so do four neighbouring rows read over the
+// block's width (the transposing read); a lane's addresses differ between blocks, and every 16 rows, by constants alone.
+template <class T, int COLS> struct Tile {
+    static constexpr int kPer = 16 / int(sizeof(T)), kSlots = COLS / kPer;   // elements a slot, slots a row
+    static constexpr int kBlockSlots = 32 / kPer, kRow = kBlockSlots * 16;
+    static constexpr int kBlock = (kChunk<T> + 1) * kRow;   // (a row more: the blocks of one row lie in different banks too)
+    static constexpr int kBytes = COLS / 32 * kBlock;
+    static __device__ __forceinline__ int at(int row, int slot) {
+        const int swizzle = sizeof(T) == 2 ? (row >> 2) & 3 : (row >> 1) & 7;
+        return slot / kBlockSlots * kBlock + row * kRow + ((slot % kBlockSlots) ^ swizzle) * 16;
+    }
+    // row `row`, elements col + off .. + 7 (off: the lane's part, in the block of col; both multiples of 8)
+    static __device__ __forceinline__ typename Frag<T>::type row8(const char* tile, int row, int col) {
+        typename Frag<T>::type f;
+        if constexpr (sizeof(T) == 2) {
+            f = *reinterpret_cast<const typename Frag<T>::type*>(tile + at(row, col / 8));
+        } else {
+            const floatx4 lo = *reinterpret_cast<const floatx4*>(tile + at(row, col / 4));
+            const floatx4 hi = *reinterpret_cast<const floatx4*>(tile + at(row, col / 4 + 1));
+            f = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+        return f;
+    }
+    // column col + perm(l % 32), rows row + 8 * (l / 32) .. + 7 for lane l (col a multiple of 32, row of 16)
+    static __device__ __forceinline__ typename Frag<T>::type column8(const char* tile, int row, int col, int l) {
+        if constexpr (sizeof(T) == 2) {
+            // transposing read: of 16 lanes, lane j hands over four columns of row j / 4 and gets four rows of column j
+            const int r = 8 * (l / 32) + (l % 16) / 4;
+            const int b = l % 4, c = 16 * ((l / 16) % 2) + 4 * (((b & 1) << 1) | (b >> 1));
+            const char* p = tile + col / 32 * kBlock + row * kRow + (c % 8) * 2;
+            union { short4v s[2]; typename Frag<T>::type f; } u;
+            u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(p + at(r, c / 8)));
+            u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(p + at(r + 4, c / 8)));
+            return u.f;
+        } else {
+            const int c = perm(l % 32), r = 8 * (l / 32);
+            const char* p = tile + col / 32 * kBlock + row * kRow + (c % 4) * 4;
+            typename Frag<T>::type f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = *reinterpret_cast<const float*>(p + at(r + i, c / 4));
+            return f;
+        }
+    }
+};
+
+// A chunk's rows of one role on their way from memory to LDS, in registers: requested while the chunk before is worked on.
+// `column0`: the first of the tile's columns; the row has `width` (at least eight).  Rows from `valid` on, and columns from
+// `width` on, become zeros.  A row's last slot is read where it ends, and shifted down, so that nothing behind a row is touched.
+template <class T, int COLS, int THREADS> struct Staged {
+    typedef Tile<T, COLS> tile;
+    static constexpr int kCount = kChunk<T> * tile::kSlots / THREADS, kStep = THREADS / tile::kSlots;
+    static_assert(kCount * THREADS == kChunk<T> * tile::kSlots && kStep * tile::kSlots == THREADS, "whole rows a turn");
+    uint4v r[kCount];
+
+    static __device__ __forceinline__ int slot(int tid) { return tid % tile::kSlots; }
+    static __device__ __forceinline__ int row(int tid, int i) { return tid / tile::kSlots + i * kStep; }
+
+    // row i of the walk at first + i * step bytes; |step| * rows < 2^31
+    __device__ __forceinline__ void load(int tid, const char* first, long long step, int valid, int column0, int width) {
+        const bool down = step < 0;
+        const char* low = down ? first + (valid - 1) * step : first;
+        const unsigned distance = unsigned(down ? -step : step);
+        const int wanted = column0 + slot(tid) * tile::kPer, last = width - tile::kPer;
+        const unsigned at = unsigned(wanted < last ? wanted : last) * unsigned(sizeof(T));
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) {
+            int n = row(tid, i);
+            if (valid < kChunk<T>) n = n < valid ? n : valid - 1;
+            const unsigned offset = unsigned(down ? valid - 1 - n : n) * distance + at;
+            __builtin_memcpy(&r[i], __builtin_assume_aligned(low + offset, sizeof(T)), 16);
+        }
+    }
+    // in place: zeros behind the row, and what the last slot read too much of in front of its elements shifted out
+    __device__ __forceinline__ void trim(int tid, int valid, int column0, int width) {
+        if (valid < kChunk<T>) {
+#pragma unroll
+            for (int i = 0; i < kCount; ++i) {
+                const uint4v zero = 0u;
+                r[i] = row(tid, i) < valid ? r[i] : zero;
+            }
+        }
+        if (width - column0 >= COLS) return;
+        const int more = column0 + (slot(tid) + 1) * tile::kPer - width;   // elements of the slot that do not exist
+        constexpr int kPerWord = 4 / int(sizeof(T));
+        const int words = more <= 0 ? 0 : more / kPerWord, part = more <= 0 ? 0 : more % kPerWord;
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) {
+            uint4v v;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const auto word = [&](int from) {   // word `from` + words, zero behind the last
+                    unsigned u = 0;
+#pragma unroll
+                    for (int j = from; j < 4; ++j) u = words == j - from ? r[i][j] : u;
+                    return u;
+                };
+                v[w] = part ? word(w) >> 16 | word(w + 1) << 16 : word(w);
+            }
+            r[i] = v;
+        }
+    }
+    __device__ __forceinline__ void store(int tid, char* lds) const {
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) *reinterpret_cast<uint4v*>(lds + tile::at(row(tid, i), slot(tid))) = r[i];
+    }
+    // whether an element is an infinity or a NaN: an exponent of ones, found by the carry out of it
+    __device__ __forceinline__ bool not_finite() const {
+        constexpr unsigned ones = std::is_same<T, half_t>::value ? 0x7c007c00u : std::is_same<T, bfloat_t>::value ? 0x7f807f80u : 0x7f800000u;
+        constexpr unsigned low = std::is_same<T, half_t>::value ? 0x04000400u : std::is_same<T, bfloat_t>::value ? 0x00800080u : 0x00800000u;
+        constexpr unsigned top = sizeof(T) == 2 ? 0x80008000u : 0x80000000u;
+        unsigned found = 0;
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) {
+            const uint4v c = (r[i] & ones) + low;
+            found |= c[0] | c[1] | c[2] | c[3];
+        }
+        return (found & top) != 0;
+    }
+};
+
+template <class T> __device__ __forceinline__ typename Frag<T>::type to_frag(float8 v) { return __builtin_convertvector(v, typename Frag<T>::type); }
+
+// The range of fp16: what becomes an operand is multiplied with a power of two where its largest magnitude in the wave lies
+// outside [low, 2^15], to some 2^13; returns that power, or 1.  (bf16 and fp32 have a float's range.)
+template <class T> __device__ __forceinline__ float range_scale(float most_of_lane, float low) {
+    if constexpr (!std::is_same<T, half_t>::value) return 1.f;
+    if (!__any(most_of_lane > 32768.f) && __any(most_of_lane >= low)) return 1.f;
+    const float most = lanes_max<kWave>(most_of_lane);
+    if (!(most > 0.f)) return 1.f;
+    const int e = 14 - __builtin_amdgcn_frexp_expf(most);
+    return uniform(ldexpf(1.f, e < -100 ? -100 : e > 100 ? 100 : e));
+}
+template <int N> __device__ __forceinline__ float most8(const float8 (&v)[N]) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[i][j]));
+    return m;
+}
+__device__ __forceinline__ float8 half_of(const floatx16& v, int u) {
+    return u == 0 ? __builtin_shufflevector(v, v, 0, 1, 2, 3, 4, 5, 6, 7) : __builtin_shufflevector(v, v, 8, 9, 10, 11, 12, 13, 14, 15);
+}
+
+template <class T, int D, int WAVES, bool kOut>
+__global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2 : 1) void sweep_kernel(Sweeps a) {
+    constexpr int kThreads = WAVES * 64, kTokens = kChunk<T>, kTiles = D / 32, kBlocks = kTokens / 32;
+    typedef Tile<T, D> tile_d;
+    typedef Tile<T, WAVES * 32> tile_e;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    char* const lds_k = lds;
+    char* const lds_v = lds_k + tile_d::kBytes;
+    char* const lds_q = lds_v + tile_e::kBytes;      // (these two where there is output)
+    char* const lds_near = lds_q + tile_d::kBytes;
+
+    const int lane = threadIdx.x % kWave, half = lane / 32, wave = threadIdx.x / kWave;
+    long long id = blockIdx.x;
+    const int which = int(id % a.count);
+    id /= a.count;
+    const Sweep& s = a.s[which];
+    const int column0 = int(id % a.column_blocks) * (WAVES * 32);
+    id /= a.column_blocks;
+    const int head = int(id % a.heads);
+    const long long slot = id / a.heads;
+    if (column0 >= s.e) return;
+    const long long n = sequence_of(a, slot), segment = slot - first_slot(a, n);
+    const Span span = span_of(a, n);
+    const bool behind = n >= (long long)a.sequences;   // tokens of no sequence: their outputs are zeros
+    const long long begin = segment * (long long)a.segment;
+    const long long end = begin + (long long)a.segment < span.length ? begin + (long long)a.segment : span.length;
+    if (begin >= end && !(span.length == 0 && segment == 0 && !behind)) return;
+
+    // the rows in the order of the walk: row p of the walk at first_of + p * step_of
+    const auto first_of = [&](const Role& r, int size) {
+        const long long first = span.first + (s.reverse ? span.length - 1 : 0);
+        return static_cast<char*>(r.data) + ((a.cu_seqlens ? 0 : n * r.sequence) + first * r.token + (head / r.group) * r.head) * size;
+    };
+    const auto step_of = [&](const Role& r, int size) { return (s.reverse ? -r.token : r.token) * size; };
+    const int e0 = wave * 32;                                            // this wave's columns of the workgroup's
+    const int out_size = s.out_f32 ? 4 : int(sizeof(T));
+
+    if (behind) {
+        if constexpr (kOut) {
+            char* out = first_of(s.out, out_size);
+            const int columns = s.e - column0 < WAVES * 32 ? s.e - column0 : WAVES * 32;
+            for (long long p = begin + threadIdx.x / 32; p < end; p += kThreads / 32)
+                for (int c = threadIdx.x % 32; c < columns; c += 32) {
+                    char* at = out + p * step_of(s.out, out_size) + (column0 + c) * out_size;
+                    if (s.out_f32) *reinterpret_cast<float*>(at) = 0.f;
+                    else *reinterpret_cast<T*>(at) = T(0.f);
+                }
+        }
+        return;
+    }
+
+    const float l2 = log2_decay(a.log_decay, head);
+    floatx16 x[kTiles];
+    // register r of tile i is X[32 i + 16 (r / 8) + 8 half + r % 8][column]
+    const int column = column0 + e0 + perm(lane % 32);
+    const auto x_row = [&](int i, int r) { return 32 * i + 16 * (r / 8) + 8 * half + r % 8; };
+    const int state_size = s.d * s.e;
+    {
+        const float* in = s.x_in ? s.x_in + ((s.in_slots ? slot : n) * a.heads + head) * (long long)state_size : nullptr;
+        const int near_column = column < s.e ? column : 0;
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+            x[i] = 0.f;
+            if (in) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int d = x_row(i, r);
+                    const float v = in[unsigned((d < s.d ? d : 0) * s.in_d + near_column * s.in_e)];
+                    x[i][r] = d < s.d && column < s.e ? v : 0.f;
+                }
+            }
+        }
+    }
+
+    // Decays.  The same in every lane, g^0 .. g^7, of which with a factor a lane the others are made (both at most 1, so that none
+    // overflows); and in LDS, b among them, those from row to column of the scores' tiles on the diagonal, where no such factor is.
+    float few[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) few[j] = uniform(power(l2, float(j)));
+    const auto diagonal = [&](int u, int j4, int lane) { return lds_near + ((u * 2 + j4) * kWave + lane) * 16; };
+    if constexpr (kOut) {
+        if (wave == 0) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int j4 = 0; j4 < 2; ++j4) {
+                    floatx4 v;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int apart = lane % 32 - (16 * u + 8 * half + 4 * j4 + j);
+                        v[j] = s.b * power(l2, float(apart < 0 ? 0 : apart));
+                    }
+                    *reinterpret_cast<floatx4*>(diagonal(u, j4, lane)) = v;
+                }
+        }
+    }
+    float x_scale = 1.f;   // x holds X times this power of two (fp16 alone)
+
+    Staged<T, D, kThreads> next_q, next_k;
+    Staged<T, WAVES * 32, kThreads> next_v;
+    const long long step_q = step_of(s.q, sizeof(T)), step_k = step_of(s.k, sizeof(T)), step_v = step_of(s.v, sizeof(T));
+    const char* at_q = kOut ? first_of(s.q, sizeof(T)) + begin * step_q : nullptr;   // the first row of the chunk that is requested next
+    const char* at_k = first_of(s.k, sizeof(T)) + begin * step_k;
+    const char* at_v = first_of(s.v, sizeof(T)) + begin * step_v;
+    const auto request = [&](int tid, int valid) {
+        if constexpr (kOut) next_q.load(tid, at_q, step_q, valid, 0, s.d);
+        next_k.load(tid, at_k, step_k, valid, 0, s.d);
+        next_v.load(tid, at_v, step_v, valid, column0, s.e);
+    };
+    const long long step_out = kOut ? step_of(s.out, out_size) : 0;
+    char* at_out = kOut ? first_of(s.out, out_size) + begin * step_out + (column0 + e0) * out_size : nullptr;
+    const auto chunk_at = [&](long long p) { return int(end - p < kTokens ? end - p : kTokens); };
+
+    // Rows of a chunk that hold an infinity or a NaN in v would spread it to the tokens before (0 * inf in a product over the
+    // chunk): such a chunk is walked a token at a time.
+    const bool ragged = s.d < D || s.e - column0 < WAVES * 32;
+    long long careful_until = begin;
+    int valid = begin < end ? chunk_at(begin) : 0;
+    if (valid > 0) request(threadIdx.x, valid);
+    for (long long p = begin; p < end;) {
+        // (What depends on the lane alone, addresses and powers, is formed anew for every chunk: kept over the loop it would take
+        // registers that the products need.)
+        int tid = threadIdx.x;
+        float l = l2;
+        asm volatile("" : "+v"(tid), "+v"(l));
+        const int lane = tid % kWave, half = lane / 32;
+        __syncthreads();   // the chunk before has been read
+        if (valid < kTokens || ragged) {
+            next_k.trim(tid, valid, 0, s.d);
+            next_v.trim(tid, valid, column0, s.e);
+            if constexpr (kOut) next_q.trim(tid, valid, 0, s.d);
+        }
+        next_k.store(tid, lds_k);
+        next_v.store(tid, lds_v);
+        if constexpr (kOut) next_q.store(tid, lds_q);
+        if (__syncthreads_or(valid > 1 && next_v.not_finite())) {
+            careful_until = p + valid;
+            valid = 1;
+            request(tid, 1);
+            continue;
+        }
+        const long long after = p + valid;
+        const int next_valid = after >= end ? 0 : after < careful_until ? 1 : chunk_at(after);
+        at_k += valid * step_k;
+        at_v += valid * step_v;
+        at_q += valid * step_q;
+        if (next_valid > 0) request(tid, next_valid);
+
+        // x_in of a walk from the back is the state behind the last token, and has met that token's decay already
+        const float lead = s.reverse && p == 0 ? 0.f : 1.f;
+
+        if constexpr (kOut) {
+            if constexpr (std::is_same<T, half_t>::value) {
+                float most = 0.f;
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i) most = fmaxf(most, most8({half_of(x[i], 0), half_of(x[i], 1)}));
+                const float r = range_scale<T>(most, 0x1p-8f);
+                if (r != 1.f) {
+                    x_scale *= r;
+#pragma unroll
+                    for (int i = 0; i < kTiles; ++i) x[i] *= r;
+                }
+            }
+            // along the width: the rows against the state and against the chunk's other rows
+            floatx16 o[kBlocks], scores[kBlocks][kBlocks];
+#pragma unroll
+            for (int tb = 0; tb < kBlocks; ++tb) {
+                o[tb] = 0.f;
+#pragma unroll
+                for (int sb = 0; sb <= tb; ++sb) scores[tb][sb] = 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) {
+                __builtin_amdgcn_sched_barrier(0);   // (left to itself the compiler requests all operands first and runs out of registers)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    typename Frag<T>::type kf[kBlocks];
+                    const typename Frag<T>::type xf = to_frag<T>(half_of(x[i], u));
+#pragma unroll
+                    for (int sb = 0; sb < kBlocks; ++sb) kf[sb] = tile_d::row8(lds_k, sb * 32 + perm(lane % 32), 32 * i + 16 * u + 8 * half);
+#pragma unroll
+                    for (int tb = 0; tb < kBlocks; ++tb) {
+                        const typename Frag<T>::type qf = tile_d::row8(lds_q, tb * 32 + lane % 32, 32 * i + 16 * u + 8 * half);
+                        o[tb] = mma(xf, qf, o[tb]);
+#pragma unroll
+                        for (int sb = 0; sb <= tb; ++sb) scores[tb][sb] = mma(kf[sb], qf, scores[tb][sb]);
+                    }
+                }
+            }
+            const int columns = s.e - column0 - e0;
+#pragma unroll
+            for (int tb = 0; tb < kBlocks; ++tb) {
+                if (tb * 32 >= valid) break;
+                float8 w[2 * kBlocks];
+#pragma unroll
+                for (int sb = 0; sb <= tb; ++sb)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        float8& to = w[2 * sb + u];
+                        to = half_of(scores[tb][sb], u);
+                        if (sb == tb) {
+                            const floatx4 n0 = *reinterpret_cast<const floatx4*>(diagonal(u, 0, lane)), n1 = *reinterpret_cast<const floatx4*>(diagonal(u, 1, lane));
+                            const float8 near = __builtin_shufflevector(n0, n1, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {   // (behind the token: not a product with zero, the score may be anything)
+                                const float v = to[j] * near[j];
+                                to[j] = 16 * u + 8 * half + j > lane % 32 ? 0.f : v;
+                            }
+                        } else {   // g^(32 + t - s) = g^(25 + t - 16 u - 8 half) g^(7 - j)
+                            to *= s.b * power(l, float(lane % 32 + 25 - 16 * u - 8 * half));
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) to[j] *= few[7 - j];
+                        }
+                    }
+                float w_scale = 1.f;
+                if constexpr (std::is_same<T, half_t>::value) {
+                    float most = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 2 * (tb + 1); ++j) most = fmaxf(most, most8({w[j]}));
+                    w_scale = range_scale<T>(most, 0x1p-8f);
+                    if (w_scale != 1.f)
+#pragma unroll
+                        for (int j = 0; j < 2 * (tb + 1); ++j) w[j] *= w_scale;
+                }
+                o[tb] *= s.a * power(l, float(tb * 32 + lane % 32) + lead) * (w_scale / x_scale);
+#pragma unroll
+                for (int j = 0; j < 2 * (tb + 1); ++j) o[tb] = mma(tile_e::column8(lds_v, 16 * j, e0, lane), to_frag<T>(w[j]), o[tb]);
+                if (w_scale != 1.f) o[tb] *= 1.f / w_scale;
+                const int t = tb * 32 + lane % 32;
+                if (t < valid) {
+                    char* const row = at_out + t * step_out;
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const int c = 16 * u + 8 * half;
+                        if (s.out_f32) store8(reinterpret_cast<float*>(row) + c, half_of(o[tb], u), columns - c);
+                        else store8(reinterpret_cast<T*>(row) + c, half_of(o[tb], u), columns - c);
+                    }
+                }
+            }
+        }
+
+        const float keep = power(l, float(valid - 1) + lead);
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) x[i] *= keep;
+#pragma unroll
+        for (int kk = 0; kk < kTokens / 16; ++kk) {
+            if (kk * 16 >= valid) break;
+            float8 w = __builtin_convertvector(tile_e::column8(lds_v, kk * 16, e0, lane), float8);
+            const float c = s.c * x_scale;
+            if (valid == kTokens) {
+                w *= c * power(l, float(kTokens - 16 * kk - 8 - 8 * half));
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[j] *= few[7 - j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int left = valid - 1 - (kk * 16 + 8 * half + j);
+                    w[j] *= c * power(l, float(left < 0 ? 0 : left));
+                }
+            }
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i) x[i] = mma(tile_d::column8(lds_k, kk * 16, i * 32, lane), w, x[i]);
+            } else {
+                // The state is a sum over the whole sequence: the weighted values go into it in parts that hold 22 (fp16) and
+                // 24 (bf16) bits, not in one rounding to 11 or 8.
+                float r = 1.f;
+                if constexpr (std::is_same<T, half_t>::value) {
+                    r = range_scale<T>(most8({w}), 0x1p-3f);
+                    if (r != 1.f) {
+                        w *= r;
+#pragma unroll
+                        for (int i = 0; i < kTiles; ++i) x[i] *= r;
+                    }
+                }
+                const typename Frag<T>::type hi = to_frag<T>(w);
+                w -= __builtin_convertvector(hi, float8);
+                const typename Frag<T>::type mid = to_frag<T>(w);
+                w -= __builtin_convertvector(mid, float8);
+                const typename Frag<T>::type lo = to_frag<T>(w);
+                typename Frag<T>::type kf[kTiles];
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i) kf[i] = tile_d::column8(lds_k, kk * 16, i * 32, lane);
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i) x[i] = mma(kf[i], hi, x[i]);
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i) x[i] = mma(kf[i], mid, x[i]);
+                if constexpr (std::is_same<T, bfloat_t>::value)
+#pragma unroll
+                    for (int i = 0; i < kTiles; ++i) x[i] = mma(kf[i], lo, x[i]);
+                if (r != 1.f) {
+#pragma unroll
+                    for (int i = 0; i < kTiles; ++i) x[i] *= 1.f / r;
+                }
+            }
+        }
+        at_out += valid * step_out;
+        p = after;
+        valid = next_valid;
+    }
+
+    if (s.x_out && (s.out_slots || end == span.length)) {
+        float* out = s.x_out + ((s.out_slots ? slot : n) * a.heads + head) * (long long)state_size;
+        // (a walk from the back ends with the gradient of the state behind the first token; the initial one is a decay away)
+        const float last = (s.reverse && !s.out_slots && span.length > 0 ? power(l2, 1.f) : 1.f) / x_scale;
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int d = x_row(i, r);
+                if (d < s.d && column < s.e) out[unsigned(d * s.out_d + column * s.out_e)] = x[i][r] * last;
+            }
+    }
+}
+
+// From the states that each segment adds (in place, one behind the other) to the states that it starts with.
+struct Scan {
+    Sweeps a;
+    float* states;          // [slot][head][d * e]
+    const float* x_in;      // [sequence][head][d * e] or null
+    float* x_out;           // [sequence][head][d * e] or null
+    int size, reverse;
+};
+
+__global__ __launch_bounds__(256) void scan_kernel(Scan c) {
+    const long long pair = blockIdx.y;
+    const int head = int(pair % c.a.heads);
+    const long long n = pair / c.a.heads;
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= c.size) return;
+    const Span span = span_of(c.a, n);
+    const long long slot0 = first_slot(c.a, n), segments = (span.length + c.a.segment - 1) / c.a.segment;
+    const float l2 = log2_decay(c.a.log_decay, head);
+    float run = c.x_in ? c.x_in[(n * c.a.heads + head) * c.size + i] : 0.f;
+    for (long long j = 0; j < segments && slot0 + j < (long long)c.a.slots; ++j) {
+        float* at = c.states + ((slot0 + j) * c.a.heads + head) * c.size + i;
+        const long long left = span.length - j * (long long)c.a.segment;
+        const float length = float(left < (long long)c.a.segment ? left : (long long)c.a.segment);
+        const float added = *at;
+        *at = run;
+        run = power(l2, c.reverse && j == 0 ? length - 1.f : length) * run + added;
+    }
+    if (c.x_out) c.x_out[(n * c.a.heads + head) * c.size + i] = c.reverse && segments > 0 ? run * power(l2, 1.f) : run;
+}
+
+// Sums the shares of the heads that have one key and value head: in [row][heads][width] floats, out one row per group.
+struct Fold {
+    const float* in;
+    Role out;
+    size_t sequences, tokens;   // rows of `in`: sequence * tokens + token
+    int heads, group, width;
+};
+
+template <class T> __global__ __launch_bounds__(256) void fold_kernel(Fold f) {
+    const int kv = f.heads / f.group;
+    const size_t row = blockIdx.x, n = row / f.tokens, t = row % f.tokens;
+    for (int i = threadIdx.x; i < kv * f.width; i += 256) {
+        const int h = i / f.width, c = i % f.width;
+        const float* in = f.in + (row * f.heads + size_t(h) * f.group) * f.width + c;
+        float v = 0.f;
+        for (int g = 0; g < f.group; ++g) v += in[size_t(g) * f.width];
+        static_cast<T*>(f.out.data)[ptrdiff_t(n) * f.out.sequence + ptrdiff_t(t) * f.out.token + h * f.out.head + c] = T(v);
+    }
+}
+
+// ---- single tokens: bound by reading and writing the state once.  A workgroup has 64 columns of one state (a thread four of them, of every 16th row).
+struct Step {
+    Role q, k, v, out;
+    int heads, d, e;
+    float scale;
+    const float* log_decay;
+    float* state;
+};
+
+template <class T> __global__ __launch_bounds__(256) void step_kernel(Step s) {
+    __shared__ float qs[kMaxHead], ks[kMaxHead];
+    __shared__ float sums[16][64];
+    const long long n = blockIdx.x / s.heads;
+    const int head = blockIdx.x % s.heads, column0 = blockIdx.y * 64;
+    const auto row_of = [&](const Role& r) { return static_cast<T*>(r.data) + n * r.sequence + (head / r.group) * r.head; };
+    for (int i = threadIdx.x; i < s.d; i += 256) {
+        qs[i] = float(row_of(s.q)[i]) * s.scale;
+        ks[i] = float(row_of(s.k)[i]);
+    }
+    const int x = threadIdx.x % 16, y = threadIdx.x / 16, c = column0 + 4 * x, count = s.e - c;
+    const float g = power(log2_decay(s.log_decay, head), 1.f);
+    float v[4], o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = j < count ? float(row_of(s.v)[c + j]) : 0.f;
+    __syncthreads();
+    float* state = s.state + (n * s.heads + head) * s.d * (long long)s.e + c;
+    if (count >= 4) {
+#pragma unroll 4
+        for (int d = y; d < s.d; d += 16) {
+            floatx4 r;
+            __builtin_memcpy(&r, __builtin_assume_aligned(state + (long long)d * s.e, 4), 16);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                r[j] = g * r[j] + ks[d] * v[j];
+                o[j] += qs[d] * r[j];
+            }
+            __builtin_memcpy(__builtin_assume_aligned(state + (long long)d * s.e, 4), &r, 16);
+        }
+    } else if (count > 0) {
+        for (int d = y; d < s.d; d += 16) {
+#pragma unroll
+            for (int j = 0; j < 3; ++j)
+                if (j < count) {
+                    const float r = g * state[(long long)d * s.e + j] + ks[d] * v[j];
+                    o[j] += qs[d] * r;
+                    state[(long long)d * s.e + j] = r;
+                }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sums[y][4 * x + j] = o[j];
+    __syncthreads();
+    if (threadIdx.x < 64 && column0 + int(threadIdx.x) < s.e) {
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) t += sums[i][threadIdx.x];
+        row_of(s.out)[column0 + threadIdx.x] = T(t);
+    }
+}
+
+// ---- host side
+
+int padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+
+bool valid_shape(const flstm_decay_attention* p) {
+    return p && valid_dtype(p->dtype) && p->heads > 0 && p->kv_heads > 0 && p->heads % p->kv_heads == 0 && p->heads <= 65535 && p->dk >= kMinHead &&
+           p->dv >= kMinHead && p->dk <= kMaxHead && p->dv <= kMaxHead && p->scale == p->scale && p->log_decay &&
+           p->sequences < (size_t(1) << 31) && p->tokens < (size_t(1) << 40) && (!p->cu_seqlens || p->tokens < (size_t(1) << 31));
+}
+
+// Tokens a workgroup walks.
+size_t segment_of(const flstm_decay_attention* p) {
+    const size_t blocks = size_t(p->heads) * ceil_div(size_t(p->dv), 128), whole = p->sequences * blocks;
+    if (whole >= 512) return size_t(1) << 41;
+    const size_t rows = p->cu_seqlens ? p->tokens : p->sequences * p->tokens;
+    const size_t segment = round_up(ceil_div(rows * blocks, 1024), 64);
+    return segment < 512 ? 512 : segment;
+}
+size_t slots_of(const flstm_decay_attention* p) {
+    const size_t segment = segment_of(p);
+    if (p->cu_seqlens) return p->tokens / segment + p->sequences + 1;
+    return p->sequences * (p->tokens ? ceil_div(p->tokens, segment) : 1);
+}
+size_t states_bytes(const flstm_decay_attention* p) {
+    const size_t slots = slots_of(p);
+    const bool split = p->tokens > segment_of(p);
+    return split ? round_up(slots * p->heads * size_t(p->dk) * p->dv * sizeof(float), 256) : 0;
+}
+// Whether a chunk's rows lie within 32-bit offsets.
+bool reachable(const flstm_rows& r) { return r.token < (ptrdiff_t(1) << 23) && r.token > -(ptrdiff_t(1) << 23); }
+
+size_t rows_of(const flstm_decay_attention* p) { return p->cu_seqlens ? p->tokens : p->sequences * p->tokens; }
+size_t shares_bytes(const flstm_decay_attention* p, int width) {
+    return p->heads == p->kv_heads ? 0 : round_up(rows_of(p) * p->heads * size_t(width) * sizeof(float), 256);
+}
+
+Role role(flstm_rows r, int group) { return Role{r.data, r.sequence, r.token, r.head, group}; }
+
+Sweeps sweeps_of(const flstm_decay_attention* p) {
+    Sweeps a{};
+    a.sequences = p->sequences; a.tokens = p->tokens; a.slots = slots_of(p); a.segment = segment_of(p);
+    a.cu_seqlens = p->cu_seqlens; a.heads = p->heads; a.log_decay = p->log_decay;
+    return a;
+}
+
+template <class T, int D, int WAVES, bool kOut> int launch_sweeps(Sweeps a, hipStream_t stream) {
+    int widest = 0;
+    for (int i = 0; i < a.count; ++i) widest = a.s[i].e > widest ? a.s[i].e : widest;
+    a.column_blocks = int(ceil_div(size_t(widest), WAVES * 32));
+    const size_t grid = a.slots * size_t(a.heads) * a.column_blocks * a.count;
+    if (grid == 0) return 0;
+    if (grid >= (size_t(1) << 31)) return FLSTM_E_TOO_LARGE;
+    constexpr int lds = Tile<T, D>::kBytes * (kOut ? 2 : 1) + Tile<T, WAVES * 32>::kBytes + (kOut ? 4 * kWave * 16 : 0);
+    const auto kernel = sweep_kernel<T, D, WAVES, kOut>;
+    if (lds > 65536) {
+        const hipError_t rc = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (rc != hipSuccess) return int(rc);
+    }
+    kernel<<<unsigned(grid), WAVES * 64, lds, stream>>>(a);
+    return launched();
+}
+
+// Waves a workgroup, of 32 columns each.  (Two of 256 rows would have to hold more than their registers.)
+int waves_of(int d, int e) { return e <= 64 && d <= 128 ? 2 : 4; }
+
+// Runs the sweeps of `a`, those of one padded width in one launch.
+int run_sweeps(const Sweeps& all, flstm_op_dtype dtype, bool out, hipStream_t stream) {
+    for (const int d : {64, 128, 256})
+        for (const int waves : {2, 4}) {
+            Sweeps a = all;
+            a.count = 0;
+            for (int i = 0; i < all.count; ++i)
+                if (padded(all.s[i].d) == d && waves_of(d, all.s[i].e) == waves) a.s[a.count++] = all.s[i];
+            if (a.count == 0) continue;
+            const int rc = with_type(dtype, [&](auto zero) {
+                typedef decltype(zero) T;
+                const auto go = [&](auto width) {
+                    constexpr int D = decltype(width)::value;
+                    if (out) return waves == 2 ? launch_sweeps<T, D, 2, true>(a, stream) : launch_sweeps<T, D, 4, true>(a, stream);
+                    return waves == 2 ? launch_sweeps<T, D, 2, false>(a, stream) : launch_sweeps<T, D, 4, false>(a, stream);
+                };
+                if (d == 256) {
+                    if (out) return launch_sweeps<T, 256, 4, true>(a, stream);
+                    return launch_sweeps<T, 256, 4, false>(a, stream);
+                }
+                if (d == 64) return go(std::integral_constant<int, 64>());
+                return go(std::integral_constant<int, 128>());
+            });
+            if (rc != 0) return rc;
+        }
+    return 0;
+}
+
+int run_scan(const Sweeps& a, float* states, const float* x_in, float* x_out, int size, int reverse, hipStream_t stream) {
+    if (a.sequences * a.heads > 65535) return FLSTM_E_TOO_LARGE;
+    if (a.sequences == 0) return 0;
+    const Scan c{a, states, x_in, x_out, size, reverse};
+    scan_kernel<<<dim3(unsigned(ceil_div(size_t(size), 256)), unsigned(a.sequences * a.heads)), 256, 0, stream>>>(c);
+    return launched();
+}
+
+}  // namespace
+}  // namespace flstm_hip
+
+using namespace flstm_hip;
+
+extern "C" size_t flstm_decay_attention_workspace_bytes(const flstm_decay_attention* p, int backward) {
+    if (!valid_shape(p)) return 0;
+    return backward ? 2 * states_bytes(p) + shares_bytes(p, p->dk) + shares_bytes(p, p->dv) : states_bytes(p);
+}
+
+extern "C" int flstm_decay_attention_forward(const flstm_decay_attention* p, flstm_rows q, flstm_rows k, flstm_rows v,
+                                             const float* state_in, flstm_rows o, float* state_out, void* workspace, void* stream) {
+    if (!valid_shape(p)) return FLSTM_E_INVALID;
+    if (rows_of(p) > 0 && (!q.data || !k.data || !v.data)) return FLSTM_E_INVALID;
+    if (states_bytes(p) > 0 && !workspace) return FLSTM_E_INVALID;
+    if (!reachable(q) || !reachable(k) || !reachable(v)) return FLSTM_E_TOO_LARGE;
+    if (p->sequences == 0 && !p->cu_seqlens) return 0;
+    hipStream_t stream_ = static_cast<hipStream_t>(stream);
+    const int group = p->heads / p->kv_heads;
+    Sweeps a = sweeps_of(p);
+    Sweep& s = a.s[0];
+    a.count = 1;
+    s = Sweep{role(q, 1), role(k, group), role(v, group), role(o, 1), p->dk, p->dv, 0, 0, state_in, state_out, p->dv, 1, p->dv, 1, 0, 0,
+              p->scale, p->scale, 1.f};
+    if (states_bytes(p) > 0) {
+        float* states = static_cast<float*>(workspace);
+        s.x_in = nullptr; s.x_out = states; s.out_slots = 1;
+        int rc = run_sweeps(a, p->dtype, false, stream_);
+        if (rc == 0) rc = run_scan(a, states, state_in, state_out, p->dk * p->dv, 0, stream_);
+        if (rc != 0) return rc;
+        s.x_in = states; s.in_slots = 1; s.x_out = nullptr; s.out_slots = 0;
+    }
+    if (!o.data) return !s.x_out ? 0 : run_sweeps(a, p->dtype, false, stream_);
+    return run_sweeps(a, p->dtype, true, stream_);
+}
+
+extern "C" int flstm_decay_attention_backward(const flstm_decay_attention* p, flstm_rows d_o, flstm_rows q, flstm_rows k, flstm_rows v,
+                                              const float* state_in, const float* d_state_out, flstm_rows dq, flstm_rows dk,
+                                              flstm_rows dv, float* d_state_in, void* workspace, void* stream) {
+    if (!valid_shape(p)) return FLSTM_E_INVALID;
+    if (rows_of(p) > 0 && (!d_o.data || !q.data || !k.data || !v.data)) return FLSTM_E_INVALID;
+    if (flstm_decay_attention_workspace_bytes(p, 1) > 0 && !workspace) return FLSTM_E_INVALID;
+    if (!reachable(d_o) || !reachable(q) || !reachable(k) || !reachable(v)) return FLSTM_E_TOO_LARGE;
+    if (p->sequences == 0 && !p->cu_seqlens) return 0;
+    hipStream_t stream_ = static_cast<hipStream_t>(stream);
+    const int group = p->heads / p->kv_heads;
+    char* room = static_cast<char*>(workspace);
+    const bool split = states_bytes(p) > 0;
+    float* const states = reinterpret_cast<float*>(room);                      // S at the segments' starts
+    float* const adjoints = reinterpret_cast<float*>(room + states_bytes(p));  // A behind the segments' ends
+    char* const shares_k = room + 2 * states_bytes(p);
+    char* const shares_v = shares_k + shares_bytes(p, p->dk);
+    const Role rq = role(q, 1), rk = role(k, group), rv = role(v, group), rdo = role(d_o, 1);
+    const auto shared = [&](flstm_rows r, char* room, int width) {   // where a sweep leaves a head's share
+        if (group == 1 || !r.data) return role(r, 1);
+        return Role{room, ptrdiff_t(p->tokens) * p->heads * width, ptrdiff_t(p->heads) * width, width, 1};
+    };
+    const int f32 = group > 1;
+    const Sweep to_q{rdo, rv, rk, role(dq, 1), p->dv, p->dk, 0, 0, state_in, nullptr, 1, p->dv, 1, p->dv, 0, 0, p->scale, p->scale, 1.f};
+    const Sweep to_v{rk, rq, rdo, shared(dv, shares_v, p->dv), p->dk, p->dv, f32, 1, d_state_out, d_state_in, p->dv, 1, p->dv, 1, 0, 0,
+                     1.f, p->scale, p->scale};
+    const Sweep to_k{rv, rdo, rq, shared(dk, shares_k, p->dk), p->dv, p->dk, f32, 1, d_state_out, nullptr, 1, p->dv, 1, p->dv, 0, 0,
+                     1.f, p->scale, p->scale};
+    Sweeps a = sweeps_of(p);
+    a.count = 0;
+    if (split) {
+        // what each segment adds to S and to A, then what each starts with
+        Sweep s = to_v;   // (k, q, do) from the back: A
+        s.x_in = nullptr; s.x_out = adjoints; s.out_slots = 1;
+        a.s[a.count++] = s;
+        if (dq.data) {
+            s = Sweep{rq, rk, rv, Role{}, p->dk, p->dv, 0, 0, nullptr, states, p->dv, 1, p->dv, 1, 0, 1, 1.f, 1.f, 1.f};
+            a.s[a.count++] = s;
+        }
+        int rc = run_sweeps(a, p->dtype, false, stream_);
+        if (rc == 0) rc = run_scan(a, adjoints, d_state_out, d_state_in, p->dk * p->dv, 1, stream_);
+        if (rc == 0 && dq.data) rc = run_scan(a, states, state_in, nullptr, p->dk * p->dv, 0, stream_);
+        if (rc != 0) return rc;
+    }
+    a.count = 0;
+    const auto add = [&](Sweep s, const float* at) {
+        if (split) { s.x_in = at; s.in_slots = 1; s.x_out = nullptr; }
+        a.s[a.count++] = s;
+    };
+    if (dq.data) add(to_q, states);
+    if (dv.data) add(to_v, adjoints);
+    if (dk.data) add(to_k, adjoints);
+    int rc = run_sweeps(a, p->dtype, true, stream_);
+    if (rc == 0 && !dv.data && d_state_in && !split) {   // nothing but the state is asked of this walk
+        a.count = 1;
+        a.s[0] = to_v;
+        rc = run_sweeps(a, p->dtype, false, stream_);
+    }
+    if (rc != 0 || group == 1 || rows_of(p) == 0) return rc;
+    if (rows_of(p) >= (size_t(1) << 31)) return FLSTM_E_TOO_LARGE;
+    const auto fold = [&](flstm_rows r, char* shares, int width) {
+        if (!r.data) return 0;
+        const size_t rows = rows_of(p), tokens = p->cu_seqlens ? rows : p->tokens;
+        const Fold f{reinterpret_cast<const float*>(shares), role(r, 1), rows / tokens, tokens, p->heads, group, width};
+        return with_type(p->dtype, [&](auto zero) {
+            fold_kernel<decltype(zero)><<<unsigned(rows), 256, 0, stream_>>>(f);
+            return launched();
+        });
+    };
+    rc = fold(dk, shares_k, p->dk);
+    return rc != 0 ? rc : fold(dv, shares_v, p->dv);
+}
+
+extern "C" int flstm_decay_attention_step(const flstm_decay_attention* p, flstm_rows q, flstm_rows k, flstm_rows v, flstm_rows o,
+                                          float* state, void* stream) {
+    if (!valid_shape(p)) return FLSTM_E_INVALID;
+    if (p->sequences == 0) return 0;
+    if (!q.data || !k.data || !v.data || !o.data || !state) return FLSTM_E_INVALID;
+    const size_t grid = p->sequences * size_t(p->heads);
+    if (grid >= (size_t(1) << 31)) return FLSTM_E_TOO_LARGE;
+    const int group = p->heads / p->kv_heads;
+    const Step s{role(q, 1), role(k, group), role(v, group), role(o, 1), p->heads, p->dk, p->dv, p->scale, p->log_decay, state};
+    return with_type(p->dtype, [&](auto zero) {
+        step_kernel<decltype(zero)><<<dim3(unsigned(grid), unsigned(ceil_div(size_t(p->dv), 64))), 256, 0, static_cast<hipStream_t>(stream)>>>(s);
+        return launched();
+    });
+}

@@ -126,7 +126,7 @@ __global__ __launch_bounds__(L > kNormThreads ? L : kNormThreads) void norm_back
     __shared__ float8 share[kParameters && kRows > 1 ? kThreads : 1];
     const int lane = threadIdx.x % L;
     const float inverse = 1.f / float(a.width);
-    // (a workgroup of 1024 has 128 registers a lane: it reads the weight again for every row, from the caches)
+    // (512 lanes with four vectors would need more than their 256 registers: they read the weight for every row, from the caches)
     constexpr bool kKeepWeight = L <= kNormThreads;
     const auto weight = [&](int c) { return a.weight ? load8(a.weight + c, a.width - c) : ones8(); };
     float8 w[V], dw[V], db[V];
@@ -227,7 +227,7 @@ template <class F> int with_hold(size_t width, F&& f) {
     if (width <= 2048) return f(Hold<64, 4>());
     if (width <= 4096) return f(Hold<256, 2>());
     if (width <= 8192) return f(Hold<256, 4>());
-    return f(Hold<1024, 2>());
+    return f(Hold<512, 4>());
 }
 
 int rows_per_workgroup(size_t width) {

@@ -27,20 +27,44 @@ template <class T> __device__ __forceinline__ void store8(T* p, float8 v) {
     const typename Vec8<T>::type r = __builtin_convertvector(v, typename Vec8<T>::type);
     __builtin_memcpy(__builtin_assume_aligned(p, sizeof(T)), &r, sizeof(r));
 }
-// The same for a row's last vector, of which `n` elements exist (n <= 0: none; the others read as zero).
+// N consecutive elements, N a power of two up to 4, at places `at` .. of a vector of eight
+template <class T, int N> __device__ __forceinline__ void load_part(float8& v, int at, const T* p) {
+    T e[N];
+    __builtin_memcpy(e, __builtin_assume_aligned(p, sizeof(T)), sizeof(e));
+#pragma unroll
+    for (int i = 0; i < 8; i += N)
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[i + j] = at == i ? float(e[j]) : v[i + j];
+}
+template <class T, int N> __device__ __forceinline__ void store_part(float8 v, int at, T* p) {
+    T e[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        float x = v[j];
+#pragma unroll
+        for (int i = N; i < 8; i += N) x = at == i ? v[i + j] : x;
+        e[j] = T(x);
+    }
+    __builtin_memcpy(__builtin_assume_aligned(p, sizeof(T)), e, sizeof(e));
+}
+// The same for a row's last vector, of which `n` elements exist (n <= 0: none; the others read as zero): in parts of 4, 2 and 1.
 template <class T> __device__ __forceinline__ float8 load8(const T* p, int n) {
     if (n >= 8) return load8(p);
     float8 v = 0.f;
-#pragma unroll
-    for (int i = 0; i < 7; ++i)
-        if (i < n) v[i] = float(p[i]);
+    if (n > 0) {
+        if (n & 4) load_part<T, 4>(v, 0, p);
+        if (n & 2) load_part<T, 2>(v, n & 4, p + (n & 4));
+        if (n & 1) load_part<T, 1>(v, n & 6, p + (n & 6));
+    }
     return v;
 }
 template <class T> __device__ __forceinline__ void store8(T* p, float8 v, int n) {
     if (n >= 8) return store8(p, v);
-#pragma unroll
-    for (int i = 0; i < 7; ++i)
-        if (i < n) p[i] = T(v[i]);
+    if (n > 0) {
+        if (n & 4) store_part<T, 4>(v, 0, p);
+        if (n & 2) store_part<T, 2>(v, n & 4, p + (n & 4));
+        if (n & 1) store_part<T, 1>(v, n & 6, p + (n & 6));
+    }
 }
 
 // Sum over groups of `N` neighbouring lanes (a power of two up to a wave), in every lane.

@@ -28,6 +28,12 @@ def _bind() -> ctypes.CDLL:
         lib.flstm_layer_norm_workspace_bytes.argtypes = [sz, sz]
         lib.flstm_layer_norm_workspace_bytes.restype = sz
         lib.flstm_layer_norm_backward.argtypes = [sz, sz, vp, sz, vp, sz, vp, sz, i32] + [vp] * 8
+        shape = ctypes.POINTER(_DecayShape)
+        lib.flstm_decay_attention_forward.argtypes = [shape, _Rows, _Rows, _Rows, vp, _Rows, vp, vp, vp]
+        lib.flstm_decay_attention_backward.argtypes = [shape, _Rows, _Rows, _Rows, _Rows, vp, vp, _Rows, _Rows, _Rows, vp, vp, vp]
+        lib.flstm_decay_attention_workspace_bytes.argtypes = [shape, i32]
+        lib.flstm_decay_attention_workspace_bytes.restype = sz
+        lib.flstm_decay_attention_step.argtypes = [shape, _Rows, _Rows, _Rows, _Rows, vp, vp]
         _BOUND = lib
     return _BOUND
 
@@ -189,3 +195,176 @@ class LayerNorm(torch.nn.Module):
 
     def forward(self, x, residual=None):
         return layer_norm(x, self.weight, self.bias, eps=self.eps, residual=residual)
+
+
+# ---- attention with a decaying state
+
+class _Rows(ctypes.Structure):
+    """flstm_rows: where element (sequence, token, head, i) of a tensor lies."""
+    _fields_ = [("data", ctypes.c_void_p), ("sequence", ctypes.c_ssize_t), ("token", ctypes.c_ssize_t), ("head", ctypes.c_ssize_t)]
+
+
+class _DecayShape(ctypes.Structure):
+    """flstm_decay_attention."""
+    _fields_ = [("sequences", ctypes.c_size_t), ("tokens", ctypes.c_size_t), ("cu_seqlens", ctypes.c_void_p), ("heads", ctypes.c_int),
+                ("kv_heads", ctypes.c_int), ("dk", ctypes.c_int), ("dv", ctypes.c_int), ("dtype", ctypes.c_int),
+                ("scale", ctypes.c_float), ("log_decay", ctypes.c_void_p)]
+
+
+def _rows_of(t) -> _Rows:
+    """Strides of (sequences, tokens, heads, D) or, packed, (tokens, heads, D); for a single token (sequences, heads, D) too, where
+    the token's stride is not read."""
+    if t is None:
+        return _Rows()
+    s = t.stride()
+    return _Rows(t.data_ptr(), s[0], s[-3], s[-2])
+
+
+def _last_axis_contiguous(t):
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _decay_shape(q, k, v, log_decay, scale, state, cu_seqlens, axes: int):
+    """Checks q (.., heads, dk), k (.., kv_heads, dk) and v (.., kv_heads, dv) of `axes` axes, and what goes with them."""
+    code = _device_tensor("q", q)
+    if q.dim() != axes:
+        raise ValueError(f"q must have {axes} axes, not {q.dim()}")
+    for name, t in (("k", k), ("v", v)):
+        _device_tensor(name, t, q.dtype)
+        if t.dim() != axes or t.shape[:-2] != q.shape[:-2]:
+            raise ValueError(f"{name} must have q's leading axes {tuple(q.shape[:-2])}: got {tuple(t.shape)}")
+    heads, dk = q.shape[-2:]
+    kv_heads, dv = v.shape[-2:]
+    if tuple(k.shape[-2:]) != (kv_heads, dk):
+        raise ValueError(f"k must have v's heads and q's width ({kv_heads}, {dk}): got {tuple(k.shape[-2:])}")
+    if kv_heads < 1 or heads < 1 or heads % kv_heads != 0:
+        raise ValueError(f"the number of query heads ({heads}) must be a multiple of that of key and value heads ({kv_heads})")
+    if not (8 <= dk <= 256 and 8 <= dv <= 256):
+        raise ValueError(f"head widths must lie in 8 .. 256: got {dk} and {dv}")
+    _device_tensor("log_decay", log_decay, torch.float32)
+    if tuple(log_decay.shape) != (heads,) or not log_decay.is_contiguous():
+        raise ValueError(f"log_decay must be a contiguous tensor of shape ({heads},)")
+    if log_decay.requires_grad:
+        raise ValueError("log_decay is a constant of the model: it has no gradient")
+    scale = dk ** -0.5 if scale is None else float(scale)
+    if scale != scale:
+        raise ValueError("scale must be a number")
+    if cu_seqlens is not None:
+        _device_tensor_int("cu_seqlens", cu_seqlens)
+        if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1 or not cu_seqlens.is_contiguous():
+            raise ValueError("cu_seqlens must be a contiguous tensor of one more entry than there are sequences")
+        sequences, tokens = cu_seqlens.shape[0] - 1, q.shape[0]
+    else:
+        sequences, tokens = q.shape[0], q.shape[1] if axes == 4 else 1
+    shape = _DecayShape(sequences, tokens, _ptr(cu_seqlens), heads, kv_heads, dk, dv, code, scale, log_decay.data_ptr())
+    _check_state("state", state, (sequences, heads, dk, dv))
+    return shape, (sequences, heads, dk, dv)
+
+
+def _device_tensor_int(name: str, t) -> None:
+    if not torch.is_tensor(t) or not t.is_cuda or t.get_device() != torch.cuda.current_device():
+        raise ValueError(f"{name} must be a CUDA tensor on the current device")
+    if t.dtype != torch.int32:
+        raise ValueError(f"{name} must be of type {torch.int32}, not {t.dtype}")
+
+
+def _check_state(name: str, t, shape) -> None:
+    if t is not None:
+        _device_tensor(name, t, torch.float32)
+        if tuple(t.shape) != shape or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous tensor of shape {shape}")
+
+
+def _like_rows(q, heads: int, width: int):
+    """An output in the memory order of q's rows: (T, B, ..) below a transposed (B, T, ..) stays that."""
+    if q.dim() == 4 and q.stride(0) < q.stride(1) and q.shape[0] > 1:
+        return torch.empty((q.shape[1], q.shape[0], heads, width), device=q.device, dtype=q.dtype).transpose(0, 1)
+    return torch.empty((*q.shape[:-2], heads, width), device=q.device, dtype=q.dtype)
+
+
+def _workspace(shape: _DecayShape, backward: int, device):
+    size = _bind().flstm_decay_attention_workspace_bytes(ctypes.byref(shape), backward)
+    return torch.empty(size, device=device, dtype=torch.uint8) if size else None
+
+
+def decay_attention_forward(q, k, v, log_decay, *, scale: Optional[float] = None, state=None, cu_seqlens=None,
+                            want_state: bool = True) -> Tuple:
+    """S_t = exp(log_decay) S_{t-1} + k_t v_t^T, o_t = scale * S_t^T q_t, for every sequence and head.
+
+    q (sequences, tokens, heads, dk), k (.., kv_heads, dk), v (.., kv_heads, dv), float32 / float16 / bfloat16, of any strides
+    (a transposed (tokens, sequences, ..) among them); head h reads key and value head h // (heads // kv_heads).  Or packed,
+    (tokens, heads, dk) and so on, with cu_seqlens (sequences + 1,) int32, from 0 on.  log_decay (heads,) float32, <= 0, a constant.
+    scale: dk ** -0.5 where None.  state (sequences, heads, dk, dv) float32: the state in front of the first tokens (None: zeros).
+    Returns (o, state behind the last tokens or, without want_state, None)."""
+    axes = 4 if cu_seqlens is None else 3
+    shape, states = _decay_shape(q, k, v, log_decay, scale, state, cu_seqlens, axes)
+    q, k, v = (_last_axis_contiguous(t) for t in (q, k, v))
+    o = _like_rows(q, shape.heads, shape.dv)
+    final = torch.empty(states, device=q.device, dtype=torch.float32) if want_state else None
+    workspace = _workspace(shape, 0, q.device)
+    _check(_bind().flstm_decay_attention_forward(ctypes.byref(shape), _rows_of(q), _rows_of(k), _rows_of(v), _ptr(state), _rows_of(o),
+                                                 _ptr(final), _ptr(workspace), _stream()), "flstm_decay_attention_forward")
+    return o, final
+
+
+def decay_attention_backward(do, q, k, v, log_decay, *, scale: Optional[float] = None, state=None, cu_seqlens=None, d_state=None,
+                             want=(True, True, True, True)) -> Tuple:
+    """Gradients (dq, dk, dv, d_initial_state) of decay_attention_forward from those of o and of the final state (None: zeros);
+    `want` tells which (None for the others)."""
+    axes = 4 if cu_seqlens is None else 3
+    shape, states = _decay_shape(q, k, v, log_decay, scale, state, cu_seqlens, axes)
+    _device_tensor("do", do, q.dtype)
+    if tuple(do.shape) != (*q.shape[:-1], shape.dv):
+        raise ValueError(f"do must have shape {(*q.shape[:-1], shape.dv)}: got {tuple(do.shape)}")
+    _check_state("d_state", d_state, states)
+    do, q, k, v = (_last_axis_contiguous(t) for t in (do, q, k, v))
+    dq = _like_rows(q, shape.heads, shape.dk) if want[0] else None
+    dk = _like_rows(k, shape.kv_heads, shape.dk) if want[1] else None
+    dv = _like_rows(v, shape.kv_heads, shape.dv) if want[2] else None
+    d_initial = torch.empty(states, device=q.device, dtype=torch.float32) if want[3] else None
+    workspace = _workspace(shape, 1, q.device)
+    _check(_bind().flstm_decay_attention_backward(
+        ctypes.byref(shape), _rows_of(do), _rows_of(q), _rows_of(k), _rows_of(v), _ptr(state), _ptr(d_state), _rows_of(dq), _rows_of(dk),
+        _rows_of(dv), _ptr(d_initial), _ptr(workspace), _stream()), "flstm_decay_attention_backward")
+    return dq, dk, dv, d_initial
+
+
+def decay_attention_step(q, k, v, log_decay, state, *, scale: Optional[float] = None):
+    """One token of every sequence: q (sequences, heads, dk), k (sequences, kv_heads, dk), v (sequences, kv_heads, dv); `state`
+    (sequences, heads, dk, dv) float32 is updated in place.  Returns o (sequences, heads, dv).  No autograd."""
+    if state is None:
+        raise ValueError("state must be a tensor: it is updated in place")
+    shape, _ = _decay_shape(q, k, v, log_decay, scale, state, None, 3)
+    q, k, v = (_last_axis_contiguous(t) for t in (q, k, v))
+    o = torch.empty((shape.sequences, shape.heads, shape.dv), device=q.device, dtype=q.dtype)
+    _check(_bind().flstm_decay_attention_step(ctypes.byref(shape), _rows_of(q), _rows_of(k), _rows_of(v), _rows_of(o), state.data_ptr(),
+                                              _stream()), "flstm_decay_attention_step")
+    return o
+
+
+class _DecayAttentionFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, state, log_decay, scale, cu_seqlens):
+        o, final = decay_attention_forward(q, k, v, log_decay, scale=scale, state=state, cu_seqlens=cu_seqlens)
+        ctx.save_for_backward(q, k, v, state, log_decay, cu_seqlens)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        return o, final
+
+    @staticmethod
+    def backward(ctx, do, d_final):
+        q, k, v, state, log_decay, cu_seqlens = ctx.saved_tensors
+        if do is None:
+            do = torch.zeros((*q.shape[:-1], v.shape[-1]), device=q.device, dtype=q.dtype)
+        if d_final is not None:
+            d_final = d_final.contiguous()
+        grads = decay_attention_backward(do, q, k, v, log_decay, scale=ctx.scale, state=state, cu_seqlens=cu_seqlens, d_state=d_final,
+                                         want=ctx.needs_input_grad[:4])
+        return (*grads, None, None, None)
+
+
+def decay_attention(q, k, v, log_decay, *, scale: Optional[float] = None, state=None, cu_seqlens=None) -> Tuple:
+    """decay_attention_forward with autograd in q, k, v and state: (o, final state)."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, state)):
+        return _DecayAttentionFunction.apply(q, k, v, state, log_decay, scale, cu_seqlens)
+    return decay_attention_forward(q, k, v, log_decay, scale=scale, state=state, cu_seqlens=cu_seqlens)

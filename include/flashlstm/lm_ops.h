@@ -1,4 +1,5 @@
-/* Operators around the recurrent layers of a language model, for MI355X (gfx950): layer norm on a residual stream.
+/* Operators around the recurrent layers of a language model, for MI355X (gfx950): layer norm on a residual stream, and
+ * attention whose memory is a decaying state of fixed size.
  * They have no counterpart in the reference, which is an LSTM layer alone.
  *
  * All pointers are device pointers.  Every function only enqueues work on `stream`: it allocates nothing, waits for nothing and
@@ -41,6 +42,49 @@ size_t flstm_layer_norm_workspace_bytes(size_t rows, size_t width);
 int flstm_layer_norm_backward(size_t rows, size_t width, const void* dy, size_t lddy, const void* total, size_t ldt,
                               const void* d_total, size_t lddt, flstm_op_dtype dtype, const float* weight, const float* mean,
                               const float* rstd, void* dx, float* dweight, float* dbias, void* workspace, void* stream);
+
+/* ---- attention with a decaying state
+ *
+ * For every sequence and head, with a decay g = exp(log_decay[head]) of the head's own (log_decay <= 0; minus infinity: no
+ * memory), over the sequence's tokens t:
+ *   S_t = g S_{t-1} + k_t v_t^T   (dk x dv, S before the first token = state_in or zeros)
+ *   o_t = scale * S_t^T q_t
+ * heads must be a multiple of kv_heads; query head h reads key and value head h / (heads / kv_heads).
+ * 8 <= dk, dv <= 256.  States are contiguous fp32 (sequences, heads, dk, dv).
+ *
+ * A tensor's element (sequence, token, head, i) lies at data + sequence * .sequence + token * .token + head * .head + i elements.
+ * With cu_seqlens (sequences + 1 int32 on the device) sequences are packed along the token axis: sequence n is tokens
+ * [cu_seqlens[n], cu_seqlens[n + 1]) of `tokens` in all, and .sequence is not used.  A tensor's tokens may be any distance apart up to 2^23 elements
+ * (FLSTM_E_TOO_LARGE beyond).  Bounds are clamped to 0 .. tokens and to
+ * ascending order; tokens in no sequence get zeros.  An empty sequence's final state is its initial one. */
+typedef struct {
+    void* data;
+    ptrdiff_t sequence, token, head;
+} flstm_rows;
+
+typedef struct {
+    size_t sequences, tokens;
+    const int* cu_seqlens;
+    int heads, kv_heads, dk, dv;
+    flstm_op_dtype dtype;
+    float scale;
+    const float* log_decay;
+} flstm_decay_attention;
+
+/* o, state_out: either may be null, o.data too.  state_out may be state_in.
+ * `workspace` has flstm_decay_attention_workspace_bytes(shape, 0) bytes (16-byte aligned; null where that is 0). */
+int flstm_decay_attention_forward(const flstm_decay_attention* shape, flstm_rows q, flstm_rows k, flstm_rows v,
+                                  const float* state_in, flstm_rows o, float* state_out, void* workspace, void* stream);
+/* Gradients, of d_o and d_state_out (null: zeros): dq, dk and dv (type and head counts of q, k and v; .data may be null) and
+ * d_state_in (may be null).  None of them may lie in an input.  `workspace`: flstm_decay_attention_workspace_bytes(shape, 1).
+ * log_decay is a constant of the model and has no gradient. */
+int flstm_decay_attention_backward(const flstm_decay_attention* shape, flstm_rows d_o, flstm_rows q, flstm_rows k, flstm_rows v,
+                                   const float* state_in, const float* d_state_out, flstm_rows dq, flstm_rows dk, flstm_rows dv,
+                                   float* d_state_in, void* workspace, void* stream);
+size_t flstm_decay_attention_workspace_bytes(const flstm_decay_attention* shape, int backward);
+/* One token of every sequence (shape->tokens and cu_seqlens are not read), the state updated in place. */
+int flstm_decay_attention_step(const flstm_decay_attention* shape, flstm_rows q, flstm_rows k, flstm_rows v, flstm_rows o,
+                               float* state, void* stream);
 
 #ifdef __cplusplus
 }

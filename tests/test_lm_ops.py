@@ -17,7 +17,8 @@ def test_header_functions_are_exported():
     text = open(os.path.join(ROOT, "include/flashlstm/lm_ops.h")).read()
     text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
     names = set(re.findall(r"\b(flstm_\w+)\s*\(", text))
-    assert {"flstm_layer_norm_forward", "flstm_layer_norm_backward", "flstm_layer_norm_workspace_bytes"} <= names
+    assert {"flstm_layer_norm_forward", "flstm_layer_norm_backward", "flstm_layer_norm_workspace_bytes",
+            "flstm_decay_attention_forward", "flstm_decay_attention_backward", "flstm_decay_attention_step"} <= names
     for name in sorted(names):
         assert hasattr(fl.load_library(), name), f"{name} declared but not exported"
 
@@ -42,3 +43,33 @@ def test_layer_norm_refuses_host_tensors():
         fl.layer_norm_forward(torch.zeros(2, 8))
     with pytest.raises(ValueError, match="CUDA"):
         fl.layer_norm(torch.zeros(2, 8, requires_grad=True))
+
+
+def test_decay_attention_refuses_before_device_work():
+    from flashlstm_poc_amd import lm_ops
+    lib = lm_ops._bind()
+    rows = lambda data=SOME, token=64: lm_ops._Rows(data.value if data else None, 64 * 5, token, 32)
+
+    def shape(**change):
+        s = lm_ops._DecayShape(2, 5, None, 2, 1, 32, 32, 1, 0.5, SOME.value)
+        for name, value in change.items():
+            setattr(s, name, value)
+        return ctypes.byref(s)
+
+    forward = lambda s=shape(), q=rows(), o=rows(): lib.flstm_decay_attention_forward(s, q, rows(), rows(), None, o, None, None, None)
+    for change in (dict(dtype=3), dict(heads=0), dict(kv_heads=0), dict(heads=3, kv_heads=2), dict(dk=7), dict(dk=257), dict(dv=0), dict(dv=300),
+                   dict(scale=float("nan")), dict(log_decay=None)):
+        assert forward(shape(**change)) == 1, change
+    assert forward(q=rows(None)) == 1 and forward(q=rows(token=1 << 23)) == 2004
+    assert lib.flstm_decay_attention_forward(None, rows(), rows(), rows(), None, rows(), None, None, None) == 1
+    assert lib.flstm_decay_attention_forward(shape(tokens=1 << 20, heads=1), rows(), rows(), rows(), None, rows(), None, None, None) == 1   # no workspace
+    assert lib.flstm_decay_attention_step(shape(), rows(), rows(), rows(), rows(), None, None) == 1
+    assert lib.flstm_decay_attention_step(shape(sequences=0), rows(None), rows(None), rows(None), rows(None), None, None) == 0
+    assert lib.flstm_decay_attention_workspace_bytes(shape(dk=1), 0) == 0
+    assert lib.flstm_decay_attention_workspace_bytes(shape(heads=1), 1) == 0
+
+
+def test_decay_attention_refuses_host_tensors():
+    q = torch.zeros(1, 4, 2, 32)
+    with pytest.raises(ValueError, match="CUDA"):
+        fl.decay_attention_forward(q, q, q, torch.zeros(2))
