@@ -5,9 +5,11 @@ the drop-in `flashlstm` Python package of the streaming surface lives in `flashl
 """
 from .core import LstmCore, load_library, library_path, LibraryMissing, add_flashlstm_to_path
 from .stack import LstmStack, StackedLSTM
-from .lm_ops import (LayerNorm, decay_attention, decay_attention_backward, decay_attention_forward, decay_attention_step, layer_norm,
-                     layer_norm_backward, layer_norm_forward)
+from .lm_ops import (LayerNorm, decay_attention, decay_attention_backward, decay_attention_forward, decay_attention_step,
+                     distillation_backward, distillation_forward, distillation_loss, distillation_train, layer_norm, layer_norm_backward,
+                     layer_norm_forward)
 
 __all__ = ["LstmCore", "LstmStack", "StackedLSTM", "load_library", "library_path", "LibraryMissing", "add_flashlstm_to_path",
-           "LayerNorm", "decay_attention", "decay_attention_backward", "decay_attention_forward", "decay_attention_step", "layer_norm",
-           "layer_norm_backward", "layer_norm_forward"]
+           "LayerNorm", "decay_attention", "decay_attention_backward", "decay_attention_forward", "decay_attention_step",
+           "distillation_backward", "distillation_forward", "distillation_loss", "distillation_train", "layer_norm", "layer_norm_backward",
+           "layer_norm_forward"]

@@ -129,7 +129,7 @@ __global__ __launch_bounds__(L > kNormThreads ? L : kNormThreads) void norm_back
     // (512 lanes with four vectors would need more than their 256 registers: they read the weight for every row, from the caches)
     constexpr bool kKeepWeight = L <= kNormThreads;
     const auto weight = [&](int c) { return a.weight ? load8(a.weight + c, a.width - c) : ones8(); };
-    float8 w[V], dw[V], db[V];
+    float8 w[kKeepWeight ? V : 1], dw[V], db[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         if constexpr (kKeepWeight) w[j] = weight((j * L + lane) * 8);
@@ -137,25 +137,27 @@ __global__ __launch_bounds__(L > kNormThreads ? L : kNormThreads) void norm_back
     }
     for (size_t row = size_t(blockIdx.x) * kRows + threadIdx.x / L; row < a.rows; row += size_t(gridDim.x) * kRows) {
         const T *dy = static_cast<const T*>(a.dy) + row * a.lddy, *total = static_cast<const T*>(a.total) + row * a.ldt;
+        int at = threadIdx.x % L;
+        asm volatile("" : "+v"(at));   // (columns and addresses are formed for every row: kept, they take registers)
         const T* dt = a.d_total ? static_cast<const T*>(a.d_total) + row * a.lddt : nullptr;
         const float mean = a.mean[row], rstd = a.rstd[row];
         float8 h[V], n[V];
         float sh = 0.f, shn = 0.f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const int c = (j * L + lane) * 8;
+            const int c = (j * L + at) * 8;
             h[j] = load8(dy + c, a.width - c);
             n[j] = load8(total + c, a.width - c);
         }
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            n[j] = keep8((n[j] - mean) * rstd, a.width - (j * L + lane) * 8);
+            n[j] = keep8((n[j] - mean) * rstd, a.width - (j * L + at) * 8);
             if constexpr (kParameters) {
                 dw[j] += h[j] * n[j];
                 db[j] += h[j];
             }
-            if constexpr (kKeepWeight) h[j] *= w[j];
-            else h[j] *= weight((j * L + lane) * 8);
+            if constexpr (!kKeepWeight) w[0] = weight((j * L + at) * 8);
+            h[j] *= w[kKeepWeight ? j : 0];
             sh += sum8(h[j]);
             shn += sum8(h[j] * n[j]);
         }
@@ -163,7 +165,7 @@ __global__ __launch_bounds__(L > kNormThreads ? L : kNormThreads) void norm_back
         T* dx = static_cast<T*>(a.dx) + row * a.width;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const int c = (j * L + lane) * 8;
+            const int c = (j * L + at) * 8;
             float8 o = rstd * (h[j] - mh - n[j] * mhn);
             if (dt) o += load8(dt + c, a.width - c);
             store8(dx + c, o, a.width - c);

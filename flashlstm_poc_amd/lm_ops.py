@@ -34,6 +34,12 @@ def _bind() -> ctypes.CDLL:
         lib.flstm_decay_attention_workspace_bytes.argtypes = [shape, i32]
         lib.flstm_decay_attention_workspace_bytes.restype = sz
         lib.flstm_decay_attention_step.argtypes = [shape, _Rows, _Rows, _Rows, _Rows, vp, vp]
+        problem = ctypes.POINTER(_Distillation)
+        lib.flstm_distillation_forward.argtypes = [problem, vp, vp, vp]
+        lib.flstm_distillation_backward.argtypes = [problem, vp, vp, sz, vp, sz, vp]
+        lib.flstm_distillation_workspace_bytes.argtypes = [problem]
+        lib.flstm_distillation_workspace_bytes.restype = sz
+        lib.flstm_distillation_train.argtypes = [problem, vp, sz, vp, vp, sz, vp, vp]
         _BOUND = lib
     return _BOUND
 
@@ -368,3 +374,119 @@ def decay_attention(q, k, v, log_decay, *, scale: Optional[float] = None, state=
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, state)):
         return _DecayAttentionFunction.apply(q, k, v, state, log_decay, scale, cu_seqlens)
     return decay_attention_forward(q, k, v, log_decay, scale=scale, state=state, cu_seqlens=cu_seqlens)
+
+
+# ---- distillation from a teacher's top logits
+
+class _Distillation(ctypes.Structure):
+    """flstm_distillation."""
+    _fields_ = [("rows", ctypes.c_size_t), ("vocabulary", ctypes.c_size_t), ("logits", ctypes.c_void_p), ("ld", ctypes.c_size_t),
+                ("dtype", ctypes.c_int), ("top", ctypes.c_int), ("teacher_logits", ctypes.c_void_p), ("teacher_dtype", ctypes.c_int),
+                ("teacher_index", ctypes.c_void_p), ("index_64", ctypes.c_int), ("temperature", ctypes.c_float)]
+
+
+def _distillation(logits, teacher_logits, teacher_index, temperature: float):
+    """The checked problem and the tensors that it points into, which the caller keeps until its call is enqueued."""
+    code = _device_tensor("logits", logits)
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError("logits must have a last axis of at least one entry")
+    teacher_code = _device_tensor("teacher_logits", teacher_logits)
+    if not torch.is_tensor(teacher_index) or not teacher_index.is_cuda or teacher_index.get_device() != logits.get_device():
+        raise ValueError("teacher_index must be a CUDA tensor on the device of logits")
+    if teacher_index.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"teacher_index must be of type int32 or int64, not {teacher_index.dtype}")
+    if teacher_logits.shape != teacher_index.shape or teacher_logits.shape[:-1] != logits.shape[:-1] or teacher_logits.dim() != logits.dim():
+        raise ValueError(f"teacher_logits and teacher_index must have shape {(*logits.shape[:-1], 'top')}: got {tuple(teacher_logits.shape)} "
+                         f"and {tuple(teacher_index.shape)}")
+    top = teacher_logits.shape[-1]
+    if not 1 <= top <= 1024:
+        raise ValueError(f"between 1 and 1024 teacher entries a row: got {top}")
+    temperature = float(temperature)
+    if not 0 < temperature < float("inf"):
+        raise ValueError("temperature must be a positive number")
+    rows, vocabulary = logits.shape[:-1].numel(), logits.shape[-1]
+    kept = (_rows(logits) if rows else logits, teacher_logits.contiguous(), teacher_index.contiguous())
+    # (rows that share memory, an expanded tensor, are told apart by nothing but their number)
+    ld = kept[0].stride(0) if rows > 1 else vocabulary
+    if ld < vocabulary:
+        kept = (kept[0].contiguous(), *kept[1:])
+        ld = vocabulary
+    return _Distillation(rows, vocabulary, kept[0].data_ptr(), ld, code, top, kept[1].data_ptr(), teacher_code, kept[2].data_ptr(),
+                         int(teacher_index.dtype == torch.int64), temperature), kept
+
+
+def _per_row(name: str, t, problem: _Distillation):
+    """`t` as (rows,) float32 with any stride (0: one value for all rows)."""
+    _device_tensor(name, t, torch.float32)
+    if t.numel() == 1 and problem.rows != 1:
+        return t.reshape(1).expand(problem.rows)
+    if t.numel() != problem.rows:
+        raise ValueError(f"{name} must hold one value a row ({problem.rows}) or one for all: got {t.numel()}")
+    return t.reshape(-1)
+
+
+def distillation_forward(logits, teacher_logits, teacher_index, *, temperature: float = 1.0) -> Tuple:
+    """temperature^2 KL(p || q) for every row, p = softmax(teacher_logits / temperature) over the row's entries and
+    q = softmax(logits / temperature) over the vocabulary.
+
+    logits (.., vocabulary), teacher_logits (.., top) float32 / float16 / bfloat16, teacher_index (.., top) int32 / int64.  Entries
+    with an index outside the vocabulary (-1, say) or a logit of minus infinity do not count; a row without others has loss 0.
+    Returns (loss, stats), float32: loss of logits' leading shape, stats (rows, 2), which distillation_backward takes (a row's
+    largest logit, and log2 of the sum of exp((logit - largest) / temperature))."""
+    problem, kept = _distillation(logits, teacher_logits, teacher_index, temperature)
+    loss = torch.empty(logits.shape[:-1], device=logits.device, dtype=torch.float32)
+    stats = torch.empty((problem.rows, 2), device=logits.device, dtype=torch.float32)
+    _check(_bind().flstm_distillation_forward(ctypes.byref(problem), loss.data_ptr(), stats.data_ptr(), _stream()), "flstm_distillation_forward")
+    return loss, stats
+
+
+def distillation_backward(d_loss, logits, teacher_logits, teacher_index, stats, *, temperature: float = 1.0):
+    """The gradient of logits (in their type) from that of every row's loss (one value a row, or one for all)."""
+    problem, kept = _distillation(logits, teacher_logits, teacher_index, temperature)
+    d_loss = _per_row("d_loss", d_loss, problem)
+    _device_tensor("stats", stats, torch.float32)
+    if tuple(stats.shape) != (problem.rows, 2) or not stats.is_contiguous():
+        raise ValueError(f"stats must be a contiguous tensor of shape ({problem.rows}, 2)")
+    dlogits = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+    _check(_bind().flstm_distillation_backward(ctypes.byref(problem), stats.data_ptr(), d_loss.data_ptr(), d_loss.stride(0) if problem.rows else 0,
+                                               dlogits.data_ptr(), problem.vocabulary, _stream()), "flstm_distillation_backward")
+    return dlogits
+
+
+def distillation_train(logits, teacher_logits, teacher_index, d_loss, *, temperature: float = 1.0, in_place: bool = False) -> Tuple:
+    """(loss, dlogits) in one call, for a d_loss that is known beforehand (1 / rows for a mean): the logits are read once.
+    in_place: the gradient takes the place of the logits, which must then have contiguous rows."""
+    problem, kept = _distillation(logits, teacher_logits, teacher_index, temperature)
+    d_loss = _per_row("d_loss", d_loss, problem)
+    if in_place and problem.rows and problem.logits != logits.data_ptr():
+        raise ValueError("in place, logits must have contiguous rows of their own")
+    loss = torch.empty(logits.shape[:-1], device=logits.device, dtype=torch.float32)
+    dlogits = logits if in_place else torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+    lib = _bind()
+    size = lib.flstm_distillation_workspace_bytes(ctypes.byref(problem))
+    workspace = torch.empty(size, device=logits.device, dtype=torch.uint8) if size else None
+    _check(lib.flstm_distillation_train(ctypes.byref(problem), d_loss.data_ptr(), d_loss.stride(0) if problem.rows else 0, loss.data_ptr(),
+                                        dlogits.data_ptr(), problem.ld if in_place else problem.vocabulary, _ptr(workspace), _stream()),
+           "flstm_distillation_train")
+    return loss, dlogits
+
+
+class _DistillationFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, teacher_logits, teacher_index, temperature):
+        loss, stats = distillation_forward(logits, teacher_logits, teacher_index, temperature=temperature)
+        ctx.save_for_backward(logits, teacher_logits, teacher_index, stats)
+        ctx.temperature = temperature
+        return loss
+
+    @staticmethod
+    def backward(ctx, d_loss):
+        logits, teacher_logits, teacher_index, stats = ctx.saved_tensors
+        return distillation_backward(d_loss, logits, teacher_logits, teacher_index, stats, temperature=ctx.temperature), None, None, None
+
+
+def distillation_loss(logits, teacher_logits, teacher_index, *, temperature: float = 1.0):
+    """distillation_forward's loss of every row, with autograd in logits (the teacher gets no gradient)."""
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _DistillationFunction.apply(logits, teacher_logits, teacher_index, temperature)
+    return distillation_forward(logits, teacher_logits, teacher_index, temperature=temperature)[0]

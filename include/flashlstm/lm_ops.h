@@ -1,5 +1,5 @@
-/* Operators around the recurrent layers of a language model, for MI355X (gfx950): layer norm on a residual stream, and
- * attention whose memory is a decaying state of fixed size.
+/* Operators around the recurrent layers of a language model, for MI355X (gfx950): layer norm on a residual stream, attention
+ * whose memory is a decaying state of fixed size, and the distillation loss against a teacher's top logits.
  * They have no counterpart in the reference, which is an LSTM layer alone.
  *
  * All pointers are device pointers.  Every function only enqueues work on `stream`: it allocates nothing, waits for nothing and
@@ -85,6 +85,43 @@ size_t flstm_decay_attention_workspace_bytes(const flstm_decay_attention* shape,
 /* One token of every sequence (shape->tokens and cu_seqlens are not read), the state updated in place. */
 int flstm_decay_attention_step(const flstm_decay_attention* shape, flstm_rows q, flstm_rows k, flstm_rows v, flstm_rows o,
                                float* state, void* stream);
+
+/* ---- distillation from a teacher's top logits
+ *
+ * Row r of the student's logits z (rows x vocabulary, ld elements apart) is held against `top` entries (teacher_logits,
+ * teacher_index) of the teacher's, at temperature t > 0:
+ *   p = softmax(teacher_logits / t) over the row's entries;  q = softmax(z / t) over the vocabulary
+ *   loss = t^2 * sum over entries of p * (log p - log q[index])
+ *   dlogits[j] = d_loss * t * (q[j] - sum of p over the entries whose index is j)
+ * Entries whose index lies outside 0 .. vocabulary - 1 and entries of minus infinity do not count.  A row without any other
+ * entry has loss 0 and a gradient of zeros, whatever its logits hold.  1 <= top <= 1024, vocabulary below 2^31 - 65536.
+ * teacher_logits: teacher_dtype; teacher_index: int32, or int64 where index_64 is not 0; both contiguous.
+ * d_loss's elements are d_stride apart (0: one for all rows).  dlogits may be logits (same place and ld).
+ */
+typedef struct {
+    size_t rows, vocabulary;
+    const void* logits;
+    size_t ld;
+    flstm_op_dtype dtype;
+    int top;
+    const void* teacher_logits;
+    flstm_op_dtype teacher_dtype;
+    const void* teacher_index;
+    int index_64;
+    float temperature;
+} flstm_distillation;
+
+/* stats (rows x 2, 8-byte aligned, may be null): a row's largest logit m, and log2 of the sum of exp((z - m) / t).  The backward
+ * pass takes them apart because their sum would lose the second in a row whose logits all lie at the lowest value of their type. */
+int flstm_distillation_forward(const flstm_distillation* problem, float* loss, float* stats, void* stream);
+int flstm_distillation_backward(const flstm_distillation* problem, const float* stats, const float* d_loss, size_t d_stride,
+                                void* dlogits, size_t ldd, void* stream);
+/* Both in one call, for a d_loss known beforehand (a mean over rows, say): a row's logits are read from memory once, as
+ * long as they fit a workgroup's registers (131072 of 16 bits, 65536 of fp32).  `workspace`:
+ * flstm_distillation_workspace_bytes() bytes, 16-byte aligned (null where that is 0). */
+size_t flstm_distillation_workspace_bytes(const flstm_distillation* problem);
+int flstm_distillation_train(const flstm_distillation* problem, const float* d_loss, size_t d_stride, float* loss,
+                             void* dlogits, size_t ldd, void* workspace, void* stream);
 
 #ifdef __cplusplus
 }

@@ -18,7 +18,8 @@ def test_header_functions_are_exported():
     text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
     names = set(re.findall(r"\b(flstm_\w+)\s*\(", text))
     assert {"flstm_layer_norm_forward", "flstm_layer_norm_backward", "flstm_layer_norm_workspace_bytes",
-            "flstm_decay_attention_forward", "flstm_decay_attention_backward", "flstm_decay_attention_step"} <= names
+            "flstm_decay_attention_forward", "flstm_decay_attention_backward", "flstm_decay_attention_step",
+            "flstm_distillation_forward", "flstm_distillation_backward", "flstm_distillation_train"} <= names
     for name in sorted(names):
         assert hasattr(fl.load_library(), name), f"{name} declared but not exported"
 
@@ -73,3 +74,32 @@ def test_decay_attention_refuses_host_tensors():
     q = torch.zeros(1, 4, 2, 32)
     with pytest.raises(ValueError, match="CUDA"):
         fl.decay_attention_forward(q, q, q, torch.zeros(2))
+
+
+def test_distillation_refuses_before_device_work():
+    from flashlstm_poc_amd import lm_ops
+    lib = lm_ops._bind()
+
+    def problem(**change):
+        p = lm_ops._Distillation(4, 100, SOME.value, 100, 1, 5, SOME.value, 0, SOME.value, 0, 1.0)
+        for name, value in change.items():
+            setattr(p, name, value)
+        return ctypes.byref(p)
+
+    for change in (dict(dtype=3), dict(teacher_dtype=-1), dict(top=0), dict(top=1025), dict(temperature=0.0), dict(temperature=float("nan")),
+                   dict(temperature=float("inf")), dict(temperature=1e-40), dict(vocabulary=0), dict(vocabulary=1 << 31), dict(ld=99),
+                   dict(logits=None), dict(teacher_logits=None), dict(teacher_index=None)):
+        assert lib.flstm_distillation_forward(problem(**change), SOME, None, None) == 1, change
+    assert lib.flstm_distillation_forward(None, SOME, None, None) == 1 and lib.flstm_distillation_forward(problem(), None, None, None) == 1
+    assert lib.flstm_distillation_backward(problem(), None, SOME, 1, SOME, 100, None) == 1
+    assert lib.flstm_distillation_backward(problem(), SOME, SOME, 1, SOME, 99, None) == 1
+    assert lib.flstm_distillation_train(problem(), SOME, 1, SOME, None, 100, None, None) == 1
+    assert lib.flstm_distillation_train(problem(vocabulary=200000, ld=200000), SOME, 1, SOME, SOME, 200000, None, None) == 1   # no workspace
+    assert lib.flstm_distillation_forward(problem(rows=0, logits=None), None, None, None) == 0
+    assert lib.flstm_distillation_workspace_bytes(problem()) == 0
+    assert lib.flstm_distillation_workspace_bytes(problem(vocabulary=200000, ld=200000)) == 32
+
+
+def test_distillation_refuses_host_tensors():
+    with pytest.raises(ValueError, match="CUDA"):
+        fl.distillation_forward(torch.zeros(2, 8), torch.zeros(2, 1), torch.zeros(2, 1, dtype=torch.int32))
