@@ -111,7 +111,7 @@ __device__ __forceinline__ floatx16 mma(float8 a, float8 b, floatx16 c) {
 // Accumulator row 8 * (r / 4) + 4 * (l / 32) + r % 4 sits in register r.  Where an operand's rows are handed over in the order
 // perm(0), perm(1), .. (the two inner blocks of four of every sixteen exchanged), register r of the result is row
 // 16 * (r / 8) + 8 * (l / 32) + r % 8: registers 0..7 and 8..15 are then each a fragment for a product along those rows.
-__device__ __forceinline__ int perm(int i) { return (i & ~12) | ((i & 4) << 1) | ((i & 8) >> 1); }
+__device__ __forceinline__ unsigned perm(unsigned i) { return (i & ~12u) | ((i & 4) << 1) | ((i & 8) >> 1); }
 
 // ---- tiles in LDS: blocks of 32 columns, in each of which the rows lie one behind the other, in 16-byte slots that a row's
 // number permutes.  Sixteen rows read at one column lie in different banks, and so do four neighbouring rows read over the
@@ -121,58 +121,59 @@ template <class T, int COLS> struct Tile {
     static constexpr int kBlockSlots = 32 / kPer, kRow = kBlockSlots * 16;
     static constexpr int kBlock = (kChunk<T> + 1) * kRow;   // (a row more: the blocks of one row lie in different banks too)
     static constexpr int kBytes = COLS / 32 * kBlock;
-    static __device__ __forceinline__ int at(int row, int slot) {
-        const int swizzle = sizeof(T) == 2 ? (row >> 2) & 3 : (row >> 1) & 7;
-        return slot / kBlockSlots * kBlock + row * kRow + ((slot % kBlockSlots) ^ swizzle) * 16;
+    static __device__ __forceinline__ unsigned swizzled(unsigned row, unsigned slot) {   // of one block
+        return row * kRow + (slot ^ (sizeof(T) == 2 ? (row >> 2) & 3 : (row >> 1) & 7)) * 16;
     }
-    // row `row`, elements col + off .. + 7 (off: the lane's part, in the block of col; both multiples of 8)
-    static __device__ __forceinline__ typename Frag<T>::type row8(const char* tile, int row, int col) {
-        typename Frag<T>::type f;
+    static __device__ __forceinline__ unsigned at(unsigned row, unsigned slot) { return slot / kBlockSlots * kBlock + swizzled(row, slot % kBlockSlots); }
+
+    // Eight values of row rows + r from column 32 * block + 16 * step + 8 * half on (rows, block and step: the same in every lane;
+    // rows a multiple of 32, r below 32).
+    static __device__ __forceinline__ typename Frag<T>::type row8(const char* tile, int block, int step, int rows, unsigned r, unsigned half) {
+        const char* p = tile + block * kBlock + rows * kRow;
         if constexpr (sizeof(T) == 2) {
-            f = *reinterpret_cast<const typename Frag<T>::type*>(tile + at(row, col / 8));
+            return *reinterpret_cast<const typename Frag<T>::type*>(p + swizzled(r, 2 * step + half));
         } else {
-            const floatx4 lo = *reinterpret_cast<const floatx4*>(tile + at(row, col / 4));
-            const floatx4 hi = *reinterpret_cast<const floatx4*>(tile + at(row, col / 4 + 1));
-            f = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            const floatx4 lo = *reinterpret_cast<const floatx4*>(p + swizzled(r, 4 * step + 2 * half));
+            const floatx4 hi = *reinterpret_cast<const floatx4*>(p + swizzled(r, 4 * step + 2 * half + 1));
+            return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         }
-        return f;
     }
-    // column col + perm(l % 32), rows row + 8 * (l / 32) .. + 7 for lane l (col a multiple of 32, row of 16)
-    static __device__ __forceinline__ typename Frag<T>::type column8(const char* tile, int row, int col, int l) {
+    // Column 32 * block + perm(l % 32), rows rows + 8 * (l / 32) .. + 7, for lane l (rows a multiple of 16).
+    static __device__ __forceinline__ typename Frag<T>::type column8(const char* tile, int block, int rows, unsigned l) {
+        const char* p = tile + block * kBlock + rows * kRow;
         if constexpr (sizeof(T) == 2) {
             // transposing read: of 16 lanes, lane j hands over four columns of row j / 4 and gets four rows of column j
-            const int r = 8 * (l / 32) + (l % 16) / 4;
-            const int b = l % 4, c = 16 * ((l / 16) % 2) + 4 * (((b & 1) << 1) | (b >> 1));
-            const char* p = tile + col / 32 * kBlock + row * kRow + (c % 8) * 2;
+            const unsigned r = 8 * (l / 32) + (l % 16) / 4;
+            const unsigned b = l % 4, c = 16 * ((l / 16) % 2) + 4 * (((b & 1) << 1) | (b >> 1));
             union { short4v s[2]; typename Frag<T>::type f; } u;
-            u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(p + at(r, c / 8)));
-            u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(p + at(r + 4, c / 8)));
+            u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(p + swizzled(r, c / 8) + (c % 8) * 2));
+            u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(p + swizzled(r + 4, c / 8) + (c % 8) * 2));
             return u.f;
         } else {
-            const int c = perm(l % 32), r = 8 * (l / 32);
-            const char* p = tile + col / 32 * kBlock + row * kRow + (c % 4) * 4;
+            const unsigned c = perm(l % 32), r = 8 * (l / 32);
             typename Frag<T>::type f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = *reinterpret_cast<const float*>(p + at(r + i, c / 4));
+            for (int i = 0; i < 8; ++i) f[i] = *reinterpret_cast<const float*>(p + swizzled(r + i, c / 4) + (c % 4) * 4);
             return f;
         }
     }
 };
 
 // A chunk's rows of one role on their way from memory to LDS, in registers: requested while the chunk before is worked on.
-// `column0`: the first of the tile's columns; the row has `width` (at least eight).  Rows from `valid` on, and columns from
-// `width` on, become zeros.  A row's last slot is read where it ends, and shifted down, so that nothing behind a row is touched.
+// A chunk of fewer tokens lies at the tile's end: what depends on the distance to the chunk's end is then the same for all chunks.
+// `column0`: the first of the tile's columns; the row has `width` (at least eight).  Rows in front of the last `valid`, and columns
+// from `width` on, become zeros.  A row's last slot is read where it ends, and shifted down, so that nothing behind a row is touched.
 template <class T, int COLS, int THREADS> struct Staged {
     typedef Tile<T, COLS> tile;
     static constexpr int kCount = kChunk<T> * tile::kSlots / THREADS, kStep = THREADS / tile::kSlots;
     static_assert(kCount * THREADS == kChunk<T> * tile::kSlots && kStep * tile::kSlots == THREADS, "whole rows a turn");
     uint4v r[kCount];
 
-    static __device__ __forceinline__ int slot(int tid) { return tid % tile::kSlots; }
-    static __device__ __forceinline__ int row(int tid, int i) { return tid / tile::kSlots + i * kStep; }
+    static __device__ __forceinline__ int slot(unsigned tid) { return tid % tile::kSlots; }
+    static __device__ __forceinline__ int row(unsigned tid, int i) { return tid / tile::kSlots + i * kStep; }
 
-    // row i of the walk at first + i * step bytes; |step| * rows < 2^31
-    __device__ __forceinline__ void load(int tid, const char* first, long long step, int valid, int column0, int width) {
+    // the chunk's row i at first + i * step bytes; |step| * rows < 2^31
+    __device__ __forceinline__ void load(unsigned tid, const char* first, long long step, int valid, int column0, int width) {
         const bool down = step < 0;
         const char* low = down ? first + (valid - 1) * step : first;
         const unsigned distance = unsigned(down ? -step : step);
@@ -181,18 +182,18 @@ template <class T, int COLS, int THREADS> struct Staged {
 #pragma unroll
         for (int i = 0; i < kCount; ++i) {
             int n = row(tid, i);
-            if (valid < kChunk<T>) n = n < valid ? n : valid - 1;
+            if (valid < kChunk<T>) n = n + valid > kChunk<T> ? n + valid - kChunk<T> : 0;
             const unsigned offset = unsigned(down ? valid - 1 - n : n) * distance + at;
             __builtin_memcpy(&r[i], __builtin_assume_aligned(low + offset, sizeof(T)), 16);
         }
     }
     // in place: zeros behind the row, and what the last slot read too much of in front of its elements shifted out
-    __device__ __forceinline__ void trim(int tid, int valid, int column0, int width) {
+    __device__ __forceinline__ void trim(unsigned tid, int valid, int column0, int width) {
         if (valid < kChunk<T>) {
 #pragma unroll
             for (int i = 0; i < kCount; ++i) {
                 const uint4v zero = 0u;
-                r[i] = row(tid, i) < valid ? r[i] : zero;
+                r[i] = row(tid, i) + valid >= kChunk<T> ? r[i] : zero;
             }
         }
         if (width - column0 >= COLS) return;
@@ -215,7 +216,7 @@ template <class T, int COLS, int THREADS> struct Staged {
             r[i] = v;
         }
     }
-    __device__ __forceinline__ void store(int tid, char* lds) const {
+    __device__ __forceinline__ void store(unsigned tid, char* lds) const {
 #pragma unroll
         for (int i = 0; i < kCount; ++i) *reinterpret_cast<uint4v*>(lds + tile::at(row(tid, i), slot(tid))) = r[i];
     }
@@ -236,15 +237,35 @@ template <class T, int COLS, int THREADS> struct Staged {
 
 template <class T> __device__ __forceinline__ typename Frag<T>::type to_frag(float8 v) { return __builtin_convertvector(v, typename Frag<T>::type); }
 
-// The range of fp16: what becomes an operand is multiplied with a power of two where its largest magnitude in the wave lies
-// outside [low, 2^15], to some 2^13; returns that power, or 1.  (bf16 and fp32 have a float's range.)
-template <class T> __device__ __forceinline__ float range_scale(float most_of_lane, float low) {
-    if constexpr (!std::is_same<T, half_t>::value) return 1.f;
-    if (!__any(most_of_lane > 32768.f) && __any(most_of_lane >= low)) return 1.f;
-    const float most = lanes_max<kWave>(most_of_lane);
-    if (!(most > 0.f)) return 1.f;
+// w - part, eight times
+template <class T> __device__ __forceinline__ float8 less(float8 w, typename Frag<T>::type part) {
+    if constexpr (std::is_same<T, bfloat_t>::value) {   // (a bf16 is the upper half of a float: taken from the packed pairs as they are)
+        const uint4v p = __builtin_bit_cast(uint4v, part);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            w[2 * j] -= __builtin_bit_cast(float, p[j] << 16);
+            w[2 * j + 1] -= __builtin_bit_cast(float, p[j] & 0xffff0000u);
+        }
+        return w;
+    } else {
+        return w - __builtin_convertvector(part, float8);
+    }
+}
+
+// The range of fp16: what becomes an operand is multiplied with a power of two that brings its largest magnitude in the wave to some
+// 2^13, where that lies outside [low, 2^15].  (bf16 and fp32 have a float's range.)
+__device__ __forceinline__ float to_range(float most) {
     const int e = 14 - __builtin_amdgcn_frexp_expf(most);
-    return uniform(ldexpf(1.f, e < -100 ? -100 : e > 100 ? 100 : e));
+    return most > 0.f ? uniform(ldexpf(1.f, e < -100 ? -100 : e > 100 ? 100 : e)) : 1.f;
+}
+__device__ __forceinline__ float range_scale(float most_of_lane, float low) {
+    if (!__any(most_of_lane > 32768.f) && __any(most_of_lane >= low)) return 1.f;
+    return to_range(lanes_max<kWave>(most_of_lane));
+}
+__device__ __forceinline__ float most_of(half8 v) {
+    half8 m = __builtin_elementwise_abs(v);
+    const half4 n = __builtin_elementwise_max(__builtin_shufflevector(m, m, 0, 1, 2, 3), __builtin_shufflevector(m, m, 4, 5, 6, 7));
+    return fmaxf(fmaxf(float(n[0]), float(n[1])), fmaxf(float(n[2]), float(n[3])));
 }
 template <int N> __device__ __forceinline__ float most8(const float8 (&v)[N]) {
     float m = 0.f;
@@ -269,7 +290,7 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
     char* const lds_q = lds_v + tile_e::kBytes;      // (these two where there is output)
     char* const lds_near = lds_q + tile_d::kBytes;
 
-    const int lane = threadIdx.x % kWave, half = lane / 32, wave = threadIdx.x / kWave;
+    const int lane = threadIdx.x % kWave, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     long long id = blockIdx.x;
     const int which = int(id % a.count);
     id /= a.count;
@@ -285,6 +306,7 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
     const long long begin = segment * (long long)a.segment;
     const long long end = begin + (long long)a.segment < span.length ? begin + (long long)a.segment : span.length;
     if (begin >= end && !(span.length == 0 && segment == 0 && !behind)) return;
+    if (s.out_slots && end == span.length) return;   // (nothing starts with what the last segment adds)
 
     // the rows in the order of the walk: row p of the walk at first_of + p * step_of
     const auto first_of = [&](const Role& r, int size) {
@@ -333,10 +355,14 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
     }
 
     // Decays.  The same in every lane, g^0 .. g^7, of which with a factor a lane the others are made (both at most 1, so that none
-    // overflows); and in LDS, b among them, those from row to column of the scores' tiles on the diagonal, where no such factor is.
+    // overflows); and in LDS, b among them, those from row to column of the scores' tiles on the diagonal, where
+    // no such factor is, and which of these tiles' places count.
     float few[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) few[j] = uniform(power(l2, float(j)));
+    typedef typename Frag<T>::type frag;
+    typedef unsigned mask __attribute__((ext_vector_type(sizeof(frag) / 4)));
+    const auto causal = [&](int u, int lane) { return lds_near + 4 * kWave * 16 + (u * kWave + lane) * int(sizeof(frag)); };
     const auto diagonal = [&](int u, int j4, int lane) { return lds_near + ((u * 2 + j4) * kWave + lane) * 16; };
     if constexpr (kOut) {
         if (wave == 0) {
@@ -348,10 +374,21 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const int apart = lane % 32 - (16 * u + 8 * half + 4 * j4 + j);
-                        v[j] = s.b * power(l2, float(apart < 0 ? 0 : apart));
+                        v[j] = apart < 0 ? 0.f : s.b * power(l2, float(apart));
                     }
                     *reinterpret_cast<floatx4*>(diagonal(u, j4, lane)) = v;
                 }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                mask m;
+#pragma unroll
+                for (int j = 0; j < int(sizeof(frag) / 4); ++j) {
+                    const int row = 16 * u + 8 * half + j * 4 / int(sizeof(T));   // (the first of the word's)
+                    const unsigned second = sizeof(T) == 2 && row + 1 <= lane % 32 ? 0xffff0000u : 0u;
+                    m[j] = row > lane % 32 ? 0u : sizeof(T) == 2 ? 0x0000ffffu | second : 0xffffffffu;
+                }
+                *reinterpret_cast<mask*>(causal(u, lane)) = m;
+            }
         }
     }
     float x_scale = 1.f;   // x holds X times this power of two (fp16 alone)
@@ -362,7 +399,7 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
     const char* at_q = kOut ? first_of(s.q, sizeof(T)) + begin * step_q : nullptr;   // the first row of the chunk that is requested next
     const char* at_k = first_of(s.k, sizeof(T)) + begin * step_k;
     const char* at_v = first_of(s.v, sizeof(T)) + begin * step_v;
-    const auto request = [&](int tid, int valid) {
+    const auto request = [&](unsigned tid, int valid) {
         if constexpr (kOut) next_q.load(tid, at_q, step_q, valid, 0, s.d);
         next_k.load(tid, at_k, step_k, valid, 0, s.d);
         next_v.load(tid, at_v, step_v, valid, column0, s.e);
@@ -374,16 +411,20 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
     // Rows of a chunk that hold an infinity or a NaN in v would spread it to the tokens before (0 * inf in a product over the
     // chunk): such a chunk is walked a token at a time.
     const bool ragged = s.d < D || s.e - column0 < WAVES * 32;
+    __shared__ int bad[2];
+    if (threadIdx.x == 0) bad[0] = 0;   // (the first turn's; a barrier comes before its use)
+    int turn = 0;
     long long careful_until = begin;
     int valid = begin < end ? chunk_at(begin) : 0;
     if (valid > 0) request(threadIdx.x, valid);
     for (long long p = begin; p < end;) {
         // (What depends on the lane alone, addresses and powers, is formed anew for every chunk: kept over the loop it would take
         // registers that the products need.)
-        int tid = threadIdx.x;
+        unsigned tid = threadIdx.x;
         float l = l2;
         asm volatile("" : "+v"(tid), "+v"(l));
-        const int lane = tid % kWave, half = lane / 32;
+        const unsigned ulane = tid % kWave, uhalf = ulane / 32;
+        const int lane = ulane, half = uhalf;
         __syncthreads();   // the chunk before has been read
         if (valid < kTokens || ragged) {
             next_k.trim(tid, valid, 0, s.d);
@@ -393,10 +434,14 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
         next_k.store(tid, lds_k);
         next_v.store(tid, lds_v);
         if constexpr (kOut) next_q.store(tid, lds_q);
-        if (__syncthreads_or(valid > 1 && next_v.not_finite())) {
+        if (valid > 1 && __any(next_v.not_finite()) && lane == 0) bad[turn & 1] = 1;
+        if (threadIdx.x == 0) bad[~turn & 1] = 0;   // (read in the turn before, used in the next)
+        __syncthreads();
+        if (__builtin_amdgcn_readfirstlane(bad[turn++ & 1])) {
             careful_until = p + valid;
             valid = 1;
             request(tid, 1);
+            __builtin_amdgcn_s_waitcnt(0);   // (rare: no load of this branch is left to be waited for elsewhere)
             continue;
         }
         const long long after = p + valid;
@@ -404,8 +449,13 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
         at_k += valid * step_k;
         at_v += valid * step_v;
         at_q += valid * step_q;
-        if (next_valid > 0) request(tid, next_valid);
-
+        const int shift = kTokens - valid;   // rows of the tiles in front of the chunk's first
+        frag values[kTokens / 16];   // of this wave's columns: operands of the product with the scores and of the state's update
+        const auto read_values = [&] {
+#pragma unroll
+            for (int kk = 0; kk < kTokens / 16; ++kk) values[kk] = tile_e::column8(lds_v, wave, 16 * kk, ulane);
+        };
+        if constexpr (!kOut) read_values();
         // x_in of a walk from the back is the state behind the last token, and has met that token's decay already
         const float lead = s.reverse && p == 0 ? 0.f : 1.f;
 
@@ -414,7 +464,7 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
                 float most = 0.f;
 #pragma unroll
                 for (int i = 0; i < kTiles; ++i) most = fmaxf(most, most8({half_of(x[i], 0), half_of(x[i], 1)}));
-                const float r = range_scale<T>(most, 0x1p-8f);
+                const float r = range_scale(most, 0x1p-8f);
                 if (r != 1.f) {
                     x_scale *= r;
 #pragma unroll
@@ -437,20 +487,23 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
                     typename Frag<T>::type kf[kBlocks];
                     const typename Frag<T>::type xf = to_frag<T>(half_of(x[i], u));
 #pragma unroll
-                    for (int sb = 0; sb < kBlocks; ++sb) kf[sb] = tile_d::row8(lds_k, sb * 32 + perm(lane % 32), 32 * i + 16 * u + 8 * half);
+                    for (int sb = 0; sb < kBlocks; ++sb) kf[sb] = tile_d::row8(lds_k, i, u, sb * 32, perm(ulane % 32), uhalf);
 #pragma unroll
                     for (int tb = 0; tb < kBlocks; ++tb) {
-                        const typename Frag<T>::type qf = tile_d::row8(lds_q, tb * 32 + lane % 32, 32 * i + 16 * u + 8 * half);
+                        const typename Frag<T>::type qf = tile_d::row8(lds_q, i, u, tb * 32, ulane % 32, uhalf);
                         o[tb] = mma(xf, qf, o[tb]);
 #pragma unroll
                         for (int sb = 0; sb <= tb; ++sb) scores[tb][sb] = mma(kf[sb], qf, scores[tb][sb]);
                     }
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
+            read_values();
             const int columns = s.e - column0 - e0;
 #pragma unroll
             for (int tb = 0; tb < kBlocks; ++tb) {
-                if (tb * 32 >= valid) break;
+                __builtin_amdgcn_sched_barrier(0);
+                const int t = tb * 32 + lane % 32 - shift;   // (below zero: a row of zeros)
                 float8 w[2 * kBlocks];
 #pragma unroll
                 for (int sb = 0; sb <= tb; ++sb)
@@ -462,10 +515,7 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
                             const floatx4 n0 = *reinterpret_cast<const floatx4*>(diagonal(u, 0, lane)), n1 = *reinterpret_cast<const floatx4*>(diagonal(u, 1, lane));
                             const float8 near = __builtin_shufflevector(n0, n1, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) {   // (behind the token: not a product with zero, the score may be anything)
-                                const float v = to[j] * near[j];
-                                to[j] = 16 * u + 8 * half + j > lane % 32 ? 0.f : v;
-                            }
+                            for (int j = 0; j < 8; ++j) to[j] *= near[j];
                         } else {   // g^(32 + t - s) = g^(25 + t - 16 u - 8 half) g^(7 - j)
                             to *= s.b * power(l, float(lane % 32 + 25 - 16 * u - 8 * half));
 #pragma unroll
@@ -477,17 +527,21 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
                     float most = 0.f;
 #pragma unroll
                     for (int j = 0; j < 2 * (tb + 1); ++j) most = fmaxf(most, most8({w[j]}));
-                    w_scale = range_scale<T>(most, 0x1p-8f);
+                    w_scale = range_scale(most, 0x1p-8f);
                     if (w_scale != 1.f)
 #pragma unroll
                         for (int j = 0; j < 2 * (tb + 1); ++j) w[j] *= w_scale;
                 }
-                o[tb] *= s.a * power(l, float(tb * 32 + lane % 32) + lead) * (w_scale / x_scale);
+                o[tb] *= s.a * power(l, float(t < 0 ? 0 : t) + lead) * (w_scale / x_scale);
 #pragma unroll
-                for (int j = 0; j < 2 * (tb + 1); ++j) o[tb] = mma(tile_e::column8(lds_v, 16 * j, e0, lane), to_frag<T>(w[j]), o[tb]);
+                for (int j = 0; j < 2 * (tb + 1); ++j) {
+                    frag weights = to_frag<T>(w[j]);
+                    // tokens behind the row's own: by bits, not a product with zero, for the score there may be anything
+                    if (j / 2 == tb) weights = __builtin_bit_cast(frag, __builtin_bit_cast(mask, weights) & *reinterpret_cast<const mask*>(causal(j % 2, lane)));
+                    o[tb] = mma(values[j], weights, o[tb]);
+                }
                 if (w_scale != 1.f) o[tb] *= 1.f / w_scale;
-                const int t = tb * 32 + lane % 32;
-                if (t < valid) {
+                if (t >= 0) {
                     char* const row = at_out + t * step_out;
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
@@ -499,59 +553,52 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
             }
         }
 
-        const float keep = power(l, float(valid - 1) + lead);
+        // (the next chunk's rows: earlier, the scores leave no registers for them)
+        if (next_valid > 0) request(tid, next_valid);
+        float keep = power(l, float(valid - 1) + lead);
+        if constexpr (std::is_same<T, half_t>::value) {
+            // What the chunk adds becomes operands in two parts, the smaller of which has to keep bits that count in the state.
+            float most = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < kTokens / 16; ++kk) most = fmaxf(most, most_of(values[kk]) * power(l, float(kTokens - 16 - 16 * kk)));
+            most *= fabsf(s.c) * x_scale;
+            if (__any(most > 32768.f) || !__any(most >= 0x1p-3f)) {
+                float held = 0.f;
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i) held = fmaxf(held, most8({half_of(x[i], 0), half_of(x[i], 1)}));
+                most = lanes_max<kWave>(most);
+                const float larger = fmaxf(most, lanes_max<kWave>(held) * keep);
+                if (most > 32768.f || larger < 0x1p-3f) {
+                    const float r = to_range(larger);
+                    x_scale *= r;
+                    keep *= r;
+                }
+            }
+        }
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) x[i] *= keep;
 #pragma unroll
         for (int kk = 0; kk < kTokens / 16; ++kk) {
-            if (kk * 16 >= valid) break;
-            float8 w = __builtin_convertvector(tile_e::column8(lds_v, kk * 16, e0, lane), float8);
-            const float c = s.c * x_scale;
-            if (valid == kTokens) {
-                w *= c * power(l, float(kTokens - 16 * kk - 8 - 8 * half));
+            if constexpr (kOut && D >= 128) __builtin_amdgcn_sched_barrier(0);
+            float8 w = __builtin_convertvector(values[kk], float8);
+            const float to_end = s.c * x_scale * power(l, float(kTokens - 16 * kk - 8 - 8 * half));
 #pragma unroll
-                for (int j = 0; j < 8; ++j) w[j] *= few[7 - j];
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int left = valid - 1 - (kk * 16 + 8 * half + j);
-                    w[j] *= c * power(l, float(left < 0 ? 0 : left));
-                }
-            }
+            for (int j = 0; j < 8; ++j) w[j] *= to_end * few[7 - j];
             if constexpr (sizeof(T) == 4) {
 #pragma unroll
-                for (int i = 0; i < kTiles; ++i) x[i] = mma(tile_d::column8(lds_k, kk * 16, i * 32, lane), w, x[i]);
+                for (int i = 0; i < kTiles; ++i) x[i] = mma(tile_d::column8(lds_k, i, kk * 16, ulane), w, x[i]);
             } else {
-                // The state is a sum over the whole sequence: the weighted values go into it in parts that hold 22 (fp16) and
-                // 24 (bf16) bits, not in one rounding to 11 or 8.
-                float r = 1.f;
-                if constexpr (std::is_same<T, half_t>::value) {
-                    r = range_scale<T>(most8({w}), 0x1p-3f);
-                    if (r != 1.f) {
-                        w *= r;
-#pragma unroll
-                        for (int i = 0; i < kTiles; ++i) x[i] *= r;
-                    }
-                }
-                const typename Frag<T>::type hi = to_frag<T>(w);
-                w -= __builtin_convertvector(hi, float8);
-                const typename Frag<T>::type mid = to_frag<T>(w);
-                w -= __builtin_convertvector(mid, float8);
-                const typename Frag<T>::type lo = to_frag<T>(w);
+                // The state is a sum over the whole sequence, in 32 bits: the weighted values go into it in two parts, which hold 22
+                // (fp16) and 17 (bf16) bits, not in one rounding to 11 or 8.  (A third part of bf16 took 4 % more time; with two the
+                // states are 7e-7 off, relative to their norm, where sums in 32 bits alone are 2e-7 to 1e-6 off.)
+                const frag hi = to_frag<T>(w), lo = to_frag<T>(less<T>(w, hi));
                 typename Frag<T>::type kf[kTiles];
 #pragma unroll
-                for (int i = 0; i < kTiles; ++i) kf[i] = tile_d::column8(lds_k, kk * 16, i * 32, lane);
+                for (int i = 0; i < kTiles; ++i) kf[i] = tile_d::column8(lds_k, i, kk * 16, ulane);
 #pragma unroll
                 for (int i = 0; i < kTiles; ++i) x[i] = mma(kf[i], hi, x[i]);
 #pragma unroll
-                for (int i = 0; i < kTiles; ++i) x[i] = mma(kf[i], mid, x[i]);
-                if constexpr (std::is_same<T, bfloat_t>::value)
-#pragma unroll
-                    for (int i = 0; i < kTiles; ++i) x[i] = mma(kf[i], lo, x[i]);
-                if (r != 1.f) {
-#pragma unroll
-                    for (int i = 0; i < kTiles; ++i) x[i] *= 1.f / r;
-                }
+                for (int i = 0; i < kTiles; ++i) x[i] = mma(kf[i], lo, x[i]);
             }
         }
         at_out += valid * step_out;
@@ -573,12 +620,12 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
     }
 }
 
-// From the states that each segment adds (in place, one behind the other) to the states that it starts with.
+// From the states that each segment adds (in place, one behind the other) to the states that it starts with.  The last one's is
+// not read, and not there.
 struct Scan {
     Sweeps a;
     float* states;          // [slot][head][d * e]
     const float* x_in;      // [sequence][head][d * e] or null
-    float* x_out;           // [sequence][head][d * e] or null
     int size, reverse;
 };
 
@@ -592,15 +639,22 @@ __global__ __launch_bounds__(256) void scan_kernel(Scan c) {
     const long long slot0 = first_slot(c.a, n), segments = (span.length + c.a.segment - 1) / c.a.segment;
     const float l2 = log2_decay(c.a.log_decay, head);
     float run = c.x_in ? c.x_in[(n * c.a.heads + head) * c.size + i] : 0.f;
-    for (long long j = 0; j < segments && slot0 + j < (long long)c.a.slots; ++j) {
-        float* at = c.states + ((slot0 + j) * c.a.heads + head) * c.size + i;
-        const long long left = span.length - j * (long long)c.a.segment;
-        const float length = float(left < (long long)c.a.segment ? left : (long long)c.a.segment);
-        const float added = *at;
-        *at = run;
-        run = power(l2, c.reverse && j == 0 ? length - 1.f : length) * run + added;
+    const long long room = (long long)c.a.slots - slot0, some = segments > 0 ? segments : 1;   // (an empty sequence has a state too)
+    const long long count = some < room ? some : room;                                           // (what cu_seqlens holds is not trusted)
+    const ptrdiff_t step = ptrdiff_t(c.a.heads) * c.size;
+    float* at = c.states + (slot0 * c.a.heads + head) * c.size + i;
+    constexpr int kAhead = 16;   // segments whose sums are requested together
+    for (long long j = 0; j < count; j += kAhead, at += kAhead * step) {
+        float added[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) added[u] = j + u + 1 < count ? at[u * step] : 0.f;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            if (j + u >= count) break;
+            at[u * step] = run;
+            run = power(l2, float(c.a.segment) - (c.reverse && j + u == 0 ? 1.f : 0.f)) * run + added[u];
+        }
     }
-    if (c.x_out) c.x_out[(n * c.a.heads + head) * c.size + i] = c.reverse && segments > 0 ? run * power(l2, 1.f) : run;
 }
 
 // Sums the shares of the heads that have one key and value head: in [row][heads][width] floats, out one row per group.
@@ -695,6 +749,7 @@ bool valid_shape(const flstm_decay_attention* p) {
 
 // Tokens a workgroup walks.
 size_t segment_of(const flstm_decay_attention* p) {
+    if (const char* e = getenv("FL_SEG")) { const size_t v = atoll(e); return v ? v : size_t(1) << 41; }   // TEMP
     const size_t blocks = size_t(p->heads) * ceil_div(size_t(p->dv), 128), whole = p->sequences * blocks;
     if (whole >= 512) return size_t(1) << 41;
     const size_t rows = p->cu_seqlens ? p->tokens : p->sequences * p->tokens;
@@ -735,7 +790,7 @@ template <class T, int D, int WAVES, bool kOut> int launch_sweeps(Sweeps a, hipS
     const size_t grid = a.slots * size_t(a.heads) * a.column_blocks * a.count;
     if (grid == 0) return 0;
     if (grid >= (size_t(1) << 31)) return FLSTM_E_TOO_LARGE;
-    constexpr int lds = Tile<T, D>::kBytes * (kOut ? 2 : 1) + Tile<T, WAVES * 32>::kBytes + (kOut ? 4 * kWave * 16 : 0);
+    constexpr int lds = Tile<T, D>::kBytes * (kOut ? 2 : 1) + Tile<T, WAVES * 32>::kBytes + (kOut ? kWave * (4 * 16 + 2 * 8 * int(sizeof(T))) : 0);
     const auto kernel = sweep_kernel<T, D, WAVES, kOut>;
     if (lds > 65536) {
         const hipError_t rc = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
@@ -776,10 +831,10 @@ int run_sweeps(const Sweeps& all, flstm_op_dtype dtype, bool out, hipStream_t st
     return 0;
 }
 
-int run_scan(const Sweeps& a, float* states, const float* x_in, float* x_out, int size, int reverse, hipStream_t stream) {
+int run_scan(const Sweeps& a, float* states, const float* x_in, int size, int reverse, hipStream_t stream) {
     if (a.sequences * a.heads > 65535) return FLSTM_E_TOO_LARGE;
     if (a.sequences == 0) return 0;
-    const Scan c{a, states, x_in, x_out, size, reverse};
+    const Scan c{a, states, x_in, size, reverse};
     scan_kernel<<<dim3(unsigned(ceil_div(size_t(size), 256)), unsigned(a.sequences * a.heads)), 256, 0, stream>>>(c);
     return launched();
 }
@@ -797,7 +852,7 @@ extern "C" size_t flstm_decay_attention_workspace_bytes(const flstm_decay_attent
 extern "C" int flstm_decay_attention_forward(const flstm_decay_attention* p, flstm_rows q, flstm_rows k, flstm_rows v,
                                              const float* state_in, flstm_rows o, float* state_out, void* workspace, void* stream) {
     if (!valid_shape(p)) return FLSTM_E_INVALID;
-    if (rows_of(p) > 0 && (!q.data || !k.data || !v.data)) return FLSTM_E_INVALID;
+    if (rows_of(p) > 0 && (!q.data || !k.data || !v.data || !o.data)) return FLSTM_E_INVALID;
     if (states_bytes(p) > 0 && !workspace) return FLSTM_E_INVALID;
     if (!reachable(q) || !reachable(k) || !reachable(v)) return FLSTM_E_TOO_LARGE;
     if (p->sequences == 0 && !p->cu_seqlens) return 0;
@@ -812,11 +867,10 @@ extern "C" int flstm_decay_attention_forward(const flstm_decay_attention* p, fls
         float* states = static_cast<float*>(workspace);
         s.x_in = nullptr; s.x_out = states; s.out_slots = 1;
         int rc = run_sweeps(a, p->dtype, false, stream_);
-        if (rc == 0) rc = run_scan(a, states, state_in, state_out, p->dk * p->dv, 0, stream_);
+        if (rc == 0) rc = run_scan(a, states, state_in, p->dk * p->dv, 0, stream_);
         if (rc != 0) return rc;
-        s.x_in = states; s.in_slots = 1; s.x_out = nullptr; s.out_slots = 0;
+        s.x_in = states; s.in_slots = 1; s.x_out = state_out; s.out_slots = 0;
     }
-    if (!o.data) return !s.x_out ? 0 : run_sweeps(a, p->dtype, false, stream_);
     return run_sweeps(a, p->dtype, true, stream_);
 }
 
@@ -859,22 +913,22 @@ extern "C" int flstm_decay_attention_backward(const flstm_decay_attention* p, fl
             a.s[a.count++] = s;
         }
         int rc = run_sweeps(a, p->dtype, false, stream_);
-        if (rc == 0) rc = run_scan(a, adjoints, d_state_out, d_state_in, p->dk * p->dv, 1, stream_);
-        if (rc == 0 && dq.data) rc = run_scan(a, states, state_in, nullptr, p->dk * p->dv, 0, stream_);
+        if (rc == 0) rc = run_scan(a, adjoints, d_state_out, p->dk * p->dv, 1, stream_);
+        if (rc == 0 && dq.data) rc = run_scan(a, states, state_in, p->dk * p->dv, 0, stream_);
         if (rc != 0) return rc;
     }
-    a.count = 0;
     const auto add = [&](Sweep s, const float* at) {
-        if (split) { s.x_in = at; s.in_slots = 1; s.x_out = nullptr; }
+        if (split) { s.x_in = at; s.in_slots = 1; }
         a.s[a.count++] = s;
     };
+    a.count = 0;
     if (dq.data) add(to_q, states);
     if (dv.data) add(to_v, adjoints);
     if (dk.data) add(to_k, adjoints);
     int rc = run_sweeps(a, p->dtype, true, stream_);
-    if (rc == 0 && !dv.data && d_state_in && !split) {   // nothing but the state is asked of this walk
-        a.count = 1;
-        a.s[0] = to_v;
+    if (rc == 0 && !dv.data && d_state_in) {   // nothing but the state is asked of this walk
+        a.count = 0;
+        add(to_v, adjoints);
         rc = run_sweeps(a, p->dtype, false, stream_);
     }
     if (rc != 0 || group == 1 || rows_of(p) == 0) return rc;

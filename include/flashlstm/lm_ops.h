@@ -71,7 +71,7 @@ typedef struct {
     const float* log_decay;
 } flstm_decay_attention;
 
-/* o, state_out: either may be null, o.data too.  state_out may be state_in.
+/* state_in (null: zeros) and state_out may be null; they must not be one buffer.
  * `workspace` has flstm_decay_attention_workspace_bytes(shape, 0) bytes (16-byte aligned; null where that is 0). */
 int flstm_decay_attention_forward(const flstm_decay_attention* shape, flstm_rows q, flstm_rows k, flstm_rows v,
                                   const float* state_in, flstm_rows o, float* state_out, void* workspace, void* stream);
