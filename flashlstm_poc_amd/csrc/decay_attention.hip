@@ -295,11 +295,15 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
     const int which = int(id % a.count);
     id /= a.count;
     const Sweep& s = a.s[which];
+    // (What the loop needs of it is read once: the compiler would otherwise load it again in every chunk, and wait.)
+    const int width_d = __builtin_amdgcn_readfirstlane(s.d), width_e = __builtin_amdgcn_readfirstlane(s.e);
+    const bool reverse = __builtin_amdgcn_readfirstlane(s.reverse) != 0, out_f32 = __builtin_amdgcn_readfirstlane(s.out_f32) != 0;
+    const float factor_a = uniform(s.a), factor_b = uniform(s.b), factor_c = uniform(s.c);
     const int column0 = int(id % a.column_blocks) * (WAVES * 32);
     id /= a.column_blocks;
     const int head = int(id % a.heads);
     const long long slot = id / a.heads;
-    if (column0 >= s.e) return;
+    if (column0 >= width_e) return;
     const long long n = sequence_of(a, slot), segment = slot - first_slot(a, n);
     const Span span = span_of(a, n);
     const bool behind = n >= (long long)a.sequences;   // tokens of no sequence: their outputs are zeros
@@ -310,21 +314,22 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
 
     // the rows in the order of the walk: row p of the walk at first_of + p * step_of
     const auto first_of = [&](const Role& r, int size) {
-        const long long first = span.first + (s.reverse ? span.length - 1 : 0);
+        const long long first = span.first + (reverse ? span.length - 1 : 0);
         return static_cast<char*>(r.data) + ((a.cu_seqlens ? 0 : n * r.sequence) + first * r.token + (head / r.group) * r.head) * size;
     };
-    const auto step_of = [&](const Role& r, int size) { return (s.reverse ? -r.token : r.token) * size; };
+    const auto step_of = [&](const Role& r, int size) { return (reverse ? -r.token : r.token) * size; };
     const int e0 = wave * 32;                                            // this wave's columns of the workgroup's
-    const int out_size = s.out_f32 ? 4 : int(sizeof(T));
+    const int out_size = out_f32 ? 4 : int(sizeof(T));
+    const bool whole = !out_f32 && width_e - column0 - e0 >= 32;   // 32 columns of the tensors' type to write
 
     if (behind) {
         if constexpr (kOut) {
             char* out = first_of(s.out, out_size);
-            const int columns = s.e - column0 < WAVES * 32 ? s.e - column0 : WAVES * 32;
+            const int columns = width_e - column0 < WAVES * 32 ? width_e - column0 : WAVES * 32;
             for (long long p = begin + threadIdx.x / 32; p < end; p += kThreads / 32)
                 for (int c = threadIdx.x % 32; c < columns; c += 32) {
                     char* at = out + p * step_of(s.out, out_size) + (column0 + c) * out_size;
-                    if (s.out_f32) *reinterpret_cast<float*>(at) = 0.f;
+                    if (out_f32) *reinterpret_cast<float*>(at) = 0.f;
                     else *reinterpret_cast<T*>(at) = T(0.f);
                 }
         }
@@ -336,10 +341,10 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
     // register r of tile i is X[32 i + 16 (r / 8) + 8 half + r % 8][column]
     const int column = column0 + e0 + perm(lane % 32);
     const auto x_row = [&](int i, int r) { return 32 * i + 16 * (r / 8) + 8 * half + r % 8; };
-    const int state_size = s.d * s.e;
+    const int state_size = width_d * width_e;
     {
         const float* in = s.x_in ? s.x_in + ((s.in_slots ? slot : n) * a.heads + head) * (long long)state_size : nullptr;
-        const int near_column = column < s.e ? column : 0;
+        const int near_column = column < width_e ? column : 0;
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) {
             x[i] = 0.f;
@@ -347,8 +352,8 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const int d = x_row(i, r);
-                    const float v = in[unsigned((d < s.d ? d : 0) * s.in_d + near_column * s.in_e)];
-                    x[i][r] = d < s.d && column < s.e ? v : 0.f;
+                    const float v = in[unsigned((d < width_d ? d : 0) * s.in_d + near_column * s.in_e)];
+                    x[i][r] = d < width_d && column < width_e ? v : 0.f;
                 }
             }
         }
@@ -374,7 +379,7 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const int apart = lane % 32 - (16 * u + 8 * half + 4 * j4 + j);
-                        v[j] = apart < 0 ? 0.f : s.b * power(l2, float(apart));
+                        v[j] = apart < 0 ? 0.f : factor_b * power(l2, float(apart));
                     }
                     *reinterpret_cast<floatx4*>(diagonal(u, j4, lane)) = v;
                 }
@@ -399,10 +404,13 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
     const char* at_q = kOut ? first_of(s.q, sizeof(T)) + begin * step_q : nullptr;   // the first row of the chunk that is requested next
     const char* at_k = first_of(s.k, sizeof(T)) + begin * step_k;
     const char* at_v = first_of(s.v, sizeof(T)) + begin * step_v;
+    const auto request_q = [&](unsigned tid, int valid) { next_q.load(tid, at_q, step_q, valid, 0, width_d); };
+    const auto request_k = [&](unsigned tid, int valid) { next_k.load(tid, at_k, step_k, valid, 0, width_d); };
+    const auto request_v = [&](unsigned tid, int valid) { next_v.load(tid, at_v, step_v, valid, column0, width_e); };
     const auto request = [&](unsigned tid, int valid) {
-        if constexpr (kOut) next_q.load(tid, at_q, step_q, valid, 0, s.d);
-        next_k.load(tid, at_k, step_k, valid, 0, s.d);
-        next_v.load(tid, at_v, step_v, valid, column0, s.e);
+        request_k(tid, valid);
+        request_v(tid, valid);
+        if constexpr (kOut) request_q(tid, valid);
     };
     const long long step_out = kOut ? step_of(s.out, out_size) : 0;
     char* at_out = kOut ? first_of(s.out, out_size) + begin * step_out + (column0 + e0) * out_size : nullptr;
@@ -410,7 +418,7 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
 
     // Rows of a chunk that hold an infinity or a NaN in v would spread it to the tokens before (0 * inf in a product over the
     // chunk): such a chunk is walked a token at a time.
-    const bool ragged = s.d < D || s.e - column0 < WAVES * 32;
+    const bool ragged = width_d < D || width_e - column0 < WAVES * 32;
     __shared__ int bad[2];
     if (threadIdx.x == 0) bad[0] = 0;   // (the first turn's; a barrier comes before its use)
     int turn = 0;
@@ -427,9 +435,9 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
         const int lane = ulane, half = uhalf;
         __syncthreads();   // the chunk before has been read
         if (valid < kTokens || ragged) {
-            next_k.trim(tid, valid, 0, s.d);
-            next_v.trim(tid, valid, column0, s.e);
-            if constexpr (kOut) next_q.trim(tid, valid, 0, s.d);
+            next_k.trim(tid, valid, 0, width_d);
+            next_v.trim(tid, valid, column0, width_e);
+            if constexpr (kOut) next_q.trim(tid, valid, 0, width_d);
         }
         next_k.store(tid, lds_k);
         next_v.store(tid, lds_v);
@@ -457,7 +465,7 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
         };
         if constexpr (!kOut) read_values();
         // x_in of a walk from the back is the state behind the last token, and has met that token's decay already
-        const float lead = s.reverse && p == 0 ? 0.f : 1.f;
+        const float lead = reverse && p == 0 ? 0.f : 1.f;
 
         if constexpr (kOut) {
             if constexpr (std::is_same<T, half_t>::value) {
@@ -479,27 +487,40 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
 #pragma unroll
                 for (int sb = 0; sb <= tb; ++sb) scores[tb][sb] = 0.f;
             }
+            // A step's operands are requested during the step before, and no earlier: left to itself the compiler requests them all
+            // first and runs out of registers.
+            struct Operands {
+                frag k[kBlocks], q[kBlocks];
+            };
+            const auto operands = [&](int step) {
+                Operands f;
 #pragma unroll
-            for (int i = 0; i < kTiles; ++i) {
-                __builtin_amdgcn_sched_barrier(0);   // (left to itself the compiler requests all operands first and runs out of registers)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    typename Frag<T>::type kf[kBlocks];
-                    const typename Frag<T>::type xf = to_frag<T>(half_of(x[i], u));
-#pragma unroll
-                    for (int sb = 0; sb < kBlocks; ++sb) kf[sb] = tile_d::row8(lds_k, i, u, sb * 32, perm(ulane % 32), uhalf);
-#pragma unroll
-                    for (int tb = 0; tb < kBlocks; ++tb) {
-                        const typename Frag<T>::type qf = tile_d::row8(lds_q, i, u, tb * 32, ulane % 32, uhalf);
-                        o[tb] = mma(xf, qf, o[tb]);
-#pragma unroll
-                        for (int sb = 0; sb <= tb; ++sb) scores[tb][sb] = mma(kf[sb], qf, scores[tb][sb]);
-                    }
+                for (int b = 0; b < kBlocks; ++b) {
+                    f.k[b] = tile_d::row8(lds_k, step / 2, step % 2, b * 32, perm(ulane % 32), uhalf);
+                    f.q[b] = tile_d::row8(lds_q, step / 2, step % 2, b * 32, ulane % 32, uhalf);
                 }
+                return f;
+            };
+            Operands now = operands(0);
+#pragma unroll
+            for (int step = 0; step < 2 * kTiles; ++step) {
+                __builtin_amdgcn_sched_barrier(0);
+                Operands then = now;
+                if (step + 1 < 2 * kTiles) then = operands(step + 1);
+                const frag xf = to_frag<T>(half_of(x[step / 2], step % 2));
+#pragma unroll
+                for (int tb = 0; tb < kBlocks; ++tb) {
+                    o[tb] = mma(xf, now.q[tb], o[tb]);
+#pragma unroll
+                    for (int sb = 0; sb <= tb; ++sb) scores[tb][sb] = mma(now.k[sb], now.q[tb], scores[tb][sb]);
+                }
+                now = then;
             }
             __builtin_amdgcn_sched_barrier(0);
+            // (The next chunk's rows, a role at a time: all at once the requests would queue up, and the wave with them.)
+            if (next_valid > 0) request_k(tid, next_valid);
             read_values();
-            const int columns = s.e - column0 - e0;
+            const int columns = width_e - column0 - e0;
 #pragma unroll
             for (int tb = 0; tb < kBlocks; ++tb) {
                 __builtin_amdgcn_sched_barrier(0);
@@ -517,7 +538,7 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
 #pragma unroll
                             for (int j = 0; j < 8; ++j) to[j] *= near[j];
                         } else {   // g^(32 + t - s) = g^(25 + t - 16 u - 8 half) g^(7 - j)
-                            to *= s.b * power(l, float(lane % 32 + 25 - 16 * u - 8 * half));
+                            to *= factor_b * power(l, float(lane % 32 + 25 - 16 * u - 8 * half));
 #pragma unroll
                             for (int j = 0; j < 8; ++j) to[j] *= few[7 - j];
                         }
@@ -532,7 +553,7 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
 #pragma unroll
                         for (int j = 0; j < 2 * (tb + 1); ++j) w[j] *= w_scale;
                 }
-                o[tb] *= s.a * power(l, float(t < 0 ? 0 : t) + lead) * (w_scale / x_scale);
+                o[tb] *= factor_a * power(l, float(t < 0 ? 0 : t) + lead) * (w_scale / x_scale);
 #pragma unroll
                 for (int j = 0; j < 2 * (tb + 1); ++j) {
                     frag weights = to_frag<T>(w[j]);
@@ -541,27 +562,34 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
                     o[tb] = mma(values[j], weights, o[tb]);
                 }
                 if (w_scale != 1.f) o[tb] *= 1.f / w_scale;
-                if (t >= 0) {
-                    char* const row = at_out + t * step_out;
+                if (tb == 0 && next_valid > 0) request_v(tid, next_valid);
+                char* const row = at_out + t * step_out;
+                if (t < 0) {
+                } else if (whole) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) store8(reinterpret_cast<T*>(row) + 16 * u + 8 * half, half_of(o[tb], u));
+                } else {
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         const int c = 16 * u + 8 * half;
-                        if (s.out_f32) store8(reinterpret_cast<float*>(row) + c, half_of(o[tb], u), columns - c);
+                        if (out_f32) store8(reinterpret_cast<float*>(row) + c, half_of(o[tb], u), columns - c);
                         else store8(reinterpret_cast<T*>(row) + c, half_of(o[tb], u), columns - c);
                     }
                 }
             }
         }
 
-        // (the next chunk's rows: earlier, the scores leave no registers for them)
-        if (next_valid > 0) request(tid, next_valid);
+        if (next_valid > 0) {
+            if constexpr (kOut) request_q(tid, next_valid);
+            else request(tid, next_valid);
+        }
         float keep = power(l, float(valid - 1) + lead);
         if constexpr (std::is_same<T, half_t>::value) {
             // What the chunk adds becomes operands in two parts, the smaller of which has to keep bits that count in the state.
             float most = 0.f;
 #pragma unroll
             for (int kk = 0; kk < kTokens / 16; ++kk) most = fmaxf(most, most_of(values[kk]) * power(l, float(kTokens - 16 - 16 * kk)));
-            most *= fabsf(s.c) * x_scale;
+            most *= fabsf(factor_c) * x_scale;
             if (__any(most > 32768.f) || !__any(most >= 0x1p-3f)) {
                 float held = 0.f;
 #pragma unroll
@@ -577,29 +605,39 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
         }
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) x[i] *= keep;
+        // The state is a sum over the whole sequence, in 32 bits: of the narrower types the weighted values go into it in parts that
+        // hold 22 (two of fp16) and 24 (three of bf16) bits, not in one rounding to 11 or 8.  (Two of bf16 leave the states 3e-6
+        // off, relative to their norm, where sums in 32 bits alone are 2e-7 to 1e-6 off.)
+        constexpr int kParts = sizeof(T) == 4 ? 1 : std::is_same<T, half_t>::value ? 2 : 3;
+        struct Update {
+            frag k[kTiles], v[kParts];
+        };
+        const auto update = [&](int kk) {
+            Update f;
 #pragma unroll
-        for (int kk = 0; kk < kTokens / 16; ++kk) {
-            if constexpr (kOut && D >= 128) __builtin_amdgcn_sched_barrier(0);
+            for (int i = 0; i < kTiles; ++i) f.k[i] = tile_d::column8(lds_k, i, kk * 16, ulane);
             float8 w = __builtin_convertvector(values[kk], float8);
-            const float to_end = s.c * x_scale * power(l, float(kTokens - 16 * kk - 8 - 8 * half));
+            const float to_end = factor_c * x_scale * power(l, float(kTokens - 16 * kk - 8 - 8 * half));
 #pragma unroll
             for (int j = 0; j < 8; ++j) w[j] *= to_end * few[7 - j];
-            if constexpr (sizeof(T) == 4) {
 #pragma unroll
-                for (int i = 0; i < kTiles; ++i) x[i] = mma(tile_d::column8(lds_k, i, kk * 16, ulane), w, x[i]);
-            } else {
-                // The state is a sum over the whole sequence, in 32 bits: the weighted values go into it in two parts, which hold 22
-                // (fp16) and 17 (bf16) bits, not in one rounding to 11 or 8.  (A third part of bf16 took 4 % more time; with two the
-                // states are 7e-7 off, relative to their norm, where sums in 32 bits alone are 2e-7 to 1e-6 off.)
-                const frag hi = to_frag<T>(w), lo = to_frag<T>(less<T>(w, hi));
-                typename Frag<T>::type kf[kTiles];
-#pragma unroll
-                for (int i = 0; i < kTiles; ++i) kf[i] = tile_d::column8(lds_k, i, kk * 16, ulane);
-#pragma unroll
-                for (int i = 0; i < kTiles; ++i) x[i] = mma(kf[i], hi, x[i]);
-#pragma unroll
-                for (int i = 0; i < kTiles; ++i) x[i] = mma(kf[i], lo, x[i]);
+            for (int part = 0; part < kParts; ++part) {
+                f.v[part] = to_frag<T>(w);
+                if (part + 1 < kParts) w = less<T>(w, f.v[part]);
             }
+            return f;
+        };
+        Update now = update(0);
+#pragma unroll
+        for (int kk = 0; kk < kTokens / 16; ++kk) {
+            __builtin_amdgcn_sched_barrier(0);
+            Update then = now;
+            if (kk + 1 < kTokens / 16) then = update(kk + 1);
+#pragma unroll
+            for (int part = 0; part < kParts; ++part)
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i) x[i] = mma(now.k[i], now.v[part], x[i]);
+            now = then;
         }
         at_out += valid * step_out;
         p = after;
@@ -609,13 +647,13 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
     if (s.x_out && (s.out_slots || end == span.length)) {
         float* out = s.x_out + ((s.out_slots ? slot : n) * a.heads + head) * (long long)state_size;
         // (a walk from the back ends with the gradient of the state behind the first token; the initial one is a decay away)
-        const float last = (s.reverse && !s.out_slots && span.length > 0 ? power(l2, 1.f) : 1.f) / x_scale;
+        const float last = (reverse && !s.out_slots && span.length > 0 ? power(l2, 1.f) : 1.f) / x_scale;
 #pragma unroll
         for (int i = 0; i < kTiles; ++i)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int d = x_row(i, r);
-                if (d < s.d && column < s.e) out[unsigned(d * s.out_d + column * s.out_e)] = x[i][r] * last;
+                if (d < width_d && column < width_e) out[unsigned(d * s.out_d + column * s.out_e)] = x[i][r] * last;
             }
     }
 }
@@ -739,6 +777,8 @@ template <class T> __global__ __launch_bounds__(256) void step_kernel(Step s) {
 
 // ---- host side
 
+constexpr size_t kWhole = size_t(1) << 41;   // a segment that holds any sequence
+
 int padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
 bool valid_shape(const flstm_decay_attention* p) {
@@ -747,23 +787,30 @@ bool valid_shape(const flstm_decay_attention* p) {
            p->sequences < (size_t(1) << 31) && p->tokens < (size_t(1) << 40) && (!p->cu_seqlens || p->tokens < (size_t(1) << 31));
 }
 
-// Tokens a workgroup walks.
-size_t segment_of(const flstm_decay_attention* p) {
-    if (const char* e = getenv("FL_SEG")) { const size_t v = atoll(e); return v ? v : size_t(1) << 41; }   // TEMP
-    const size_t blocks = size_t(p->heads) * ceil_div(size_t(p->dv), 128), whole = p->sequences * blocks;
-    if (whole >= 512) return size_t(1) << 41;
+// Tokens a workgroup walks.  A walk over a whole sequence reads everything once, but few heads leave most of the chip idle; cut
+// into segments it reads keys and values twice, for what each segment adds to the state comes first.  Measured with heads of 128
+// x 128 (us, whole walks / segments): forward, 192 workgroups of 2048 tokens 162 / 200, 128 of them 156 / 135, 32 of 2100 packed tokens
+// on average (8192 the longest) 450 / 81, four of 4096 238 / 59; packed, 192 with up to 4096 tokens 240 / 207, since the longest
+// decides; both directions (three walks backward), 128 workgroups 365 / 448, 32 packed ones 905 / 254.
+// Segments are as long as leaves 512 workgroups, two a CU: 131072 tokens of 8 heads take 425 us in segments of 2048, 496 of 1024,
+// 740 of 4096.  256 where a workgroup's registers fill a CU, and for packed sequences, which have a segment more each that is not
+// full: 12 of them with 16 heads take 183 us in segments of 1024, 215 of 576.
+size_t segment_of(const flstm_decay_attention* p, bool backward) {
+    const size_t blocks = size_t(p->heads) * ceil_div(size_t(p->dv), 128), walks = p->sequences * blocks;
+    if (walks >= (backward ? 128 : p->cu_seqlens ? 256 : 129)) return kWhole;
     const size_t rows = p->cu_seqlens ? p->tokens : p->sequences * p->tokens;
-    const size_t segment = round_up(ceil_div(rows * blocks, 1024), 64);
-    return segment < 512 ? 512 : segment;
+    const size_t wanted = p->cu_seqlens || p->dk > 128 || p->dv > 128 ? 256 : 512;
+    const size_t segment = round_up(ceil_div(rows * blocks, wanted), 64);
+    return segment < 256 ? 256 : segment;
 }
-size_t slots_of(const flstm_decay_attention* p) {
-    const size_t segment = segment_of(p);
+size_t slots_of(const flstm_decay_attention* p, bool backward) {
+    const size_t segment = segment_of(p, backward);
     if (p->cu_seqlens) return p->tokens / segment + p->sequences + 1;
     return p->sequences * (p->tokens ? ceil_div(p->tokens, segment) : 1);
 }
-size_t states_bytes(const flstm_decay_attention* p) {
-    const size_t slots = slots_of(p);
-    const bool split = p->tokens > segment_of(p);
+size_t states_bytes(const flstm_decay_attention* p, bool backward) {
+    const size_t slots = slots_of(p, backward);
+    const bool split = p->tokens > segment_of(p, backward);
     return split ? round_up(slots * p->heads * size_t(p->dk) * p->dv * sizeof(float), 256) : 0;
 }
 // Whether a chunk's rows lie within 32-bit offsets.
@@ -776,9 +823,9 @@ size_t shares_bytes(const flstm_decay_attention* p, int width) {
 
 Role role(flstm_rows r, int group) { return Role{r.data, r.sequence, r.token, r.head, group}; }
 
-Sweeps sweeps_of(const flstm_decay_attention* p) {
+Sweeps sweeps_of(const flstm_decay_attention* p, bool backward) {
     Sweeps a{};
-    a.sequences = p->sequences; a.tokens = p->tokens; a.slots = slots_of(p); a.segment = segment_of(p);
+    a.sequences = p->sequences; a.tokens = p->tokens; a.slots = slots_of(p, backward); a.segment = segment_of(p, backward);
     a.cu_seqlens = p->cu_seqlens; a.heads = p->heads; a.log_decay = p->log_decay;
     return a;
 }
@@ -846,24 +893,24 @@ using namespace flstm_hip;
 
 extern "C" size_t flstm_decay_attention_workspace_bytes(const flstm_decay_attention* p, int backward) {
     if (!valid_shape(p)) return 0;
-    return backward ? 2 * states_bytes(p) + shares_bytes(p, p->dk) + shares_bytes(p, p->dv) : states_bytes(p);
+    return backward ? 2 * states_bytes(p, true) + shares_bytes(p, p->dk) + shares_bytes(p, p->dv) : states_bytes(p, false);
 }
 
 extern "C" int flstm_decay_attention_forward(const flstm_decay_attention* p, flstm_rows q, flstm_rows k, flstm_rows v,
                                              const float* state_in, flstm_rows o, float* state_out, void* workspace, void* stream) {
     if (!valid_shape(p)) return FLSTM_E_INVALID;
     if (rows_of(p) > 0 && (!q.data || !k.data || !v.data || !o.data)) return FLSTM_E_INVALID;
-    if (states_bytes(p) > 0 && !workspace) return FLSTM_E_INVALID;
+    if (states_bytes(p, false) > 0 && !workspace) return FLSTM_E_INVALID;
     if (!reachable(q) || !reachable(k) || !reachable(v)) return FLSTM_E_TOO_LARGE;
     if (p->sequences == 0 && !p->cu_seqlens) return 0;
     hipStream_t stream_ = static_cast<hipStream_t>(stream);
     const int group = p->heads / p->kv_heads;
-    Sweeps a = sweeps_of(p);
+    Sweeps a = sweeps_of(p, false);
     Sweep& s = a.s[0];
     a.count = 1;
     s = Sweep{role(q, 1), role(k, group), role(v, group), role(o, 1), p->dk, p->dv, 0, 0, state_in, state_out, p->dv, 1, p->dv, 1, 0, 0,
               p->scale, p->scale, 1.f};
-    if (states_bytes(p) > 0) {
+    if (states_bytes(p, false) > 0) {
         float* states = static_cast<float*>(workspace);
         s.x_in = nullptr; s.x_out = states; s.out_slots = 1;
         int rc = run_sweeps(a, p->dtype, false, stream_);
@@ -885,10 +932,10 @@ extern "C" int flstm_decay_attention_backward(const flstm_decay_attention* p, fl
     hipStream_t stream_ = static_cast<hipStream_t>(stream);
     const int group = p->heads / p->kv_heads;
     char* room = static_cast<char*>(workspace);
-    const bool split = states_bytes(p) > 0;
+    const bool split = states_bytes(p, true) > 0;
     float* const states = reinterpret_cast<float*>(room);                      // S at the segments' starts
-    float* const adjoints = reinterpret_cast<float*>(room + states_bytes(p));  // A behind the segments' ends
-    char* const shares_k = room + 2 * states_bytes(p);
+    float* const adjoints = reinterpret_cast<float*>(room + states_bytes(p, true));  // A behind the segments' ends
+    char* const shares_k = room + 2 * states_bytes(p, true);
     char* const shares_v = shares_k + shares_bytes(p, p->dk);
     const Role rq = role(q, 1), rk = role(k, group), rv = role(v, group), rdo = role(d_o, 1);
     const auto shared = [&](flstm_rows r, char* room, int width) {   // where a sweep leaves a head's share
@@ -901,7 +948,7 @@ extern "C" int flstm_decay_attention_backward(const flstm_decay_attention* p, fl
                      1.f, p->scale, p->scale};
     const Sweep to_k{rv, rdo, rq, shared(dk, shares_k, p->dk), p->dv, p->dk, f32, 1, d_state_out, nullptr, 1, p->dv, 1, p->dv, 0, 0,
                      1.f, p->scale, p->scale};
-    Sweeps a = sweeps_of(p);
+    Sweeps a = sweeps_of(p, true);
     a.count = 0;
     if (split) {
         // what each segment adds to S and to A, then what each starts with
