@@ -792,16 +792,22 @@ bool valid_shape(const flstm_decay_attention* p) {
 // x 128 (us, whole walks / segments): forward, 192 workgroups of 2048 tokens 162 / 200, 128 of them 156 / 135, 32 of 2100 packed tokens
 // on average (8192 the longest) 450 / 81, four of 4096 238 / 59; packed, 192 with up to 4096 tokens 240 / 207, since the longest
 // decides; both directions (three walks backward), 128 workgroups 365 / 448, 32 packed ones 905 / 254.
-// Segments are as long as leaves 512 workgroups, two a CU: 131072 tokens of 8 heads take 425 us in segments of 2048, 496 of 1024,
-// 740 of 4096.  256 where a workgroup's registers fill a CU, and for packed sequences, which have a segment more each that is not
-// full: 12 of them with 16 heads take 183 us in segments of 1024, 215 of 576.
+// Segments are as long as leaves 512 workgroups, which is two a CU and one round (256 where a workgroup's registers fill a CU):
+// 131072 tokens of 8 heads take 425 us in segments of 2048, 496 of 1024, 740 of 4096.  Of packed sequences, whose last segments are
+// not full, three quarters of one more each are reckoned with: 12 of them with 16 heads take 200 us so, 251 in
+// segments of 1408.
 size_t segment_of(const flstm_decay_attention* p, bool backward) {
     const size_t blocks = size_t(p->heads) * ceil_div(size_t(p->dv), 128), walks = p->sequences * blocks;
-    if (walks >= (backward ? 128 : p->cu_seqlens ? 256 : 129)) return kWhole;
-    const size_t rows = p->cu_seqlens ? p->tokens : p->sequences * p->tokens;
-    const size_t wanted = p->cu_seqlens || p->dk > 128 || p->dv > 128 ? 256 : 512;
-    const size_t segment = round_up(ceil_div(rows * blocks, wanted), 64);
-    return segment < 256 ? 256 : segment;
+    if (walks == 0 || walks >= (backward ? 128 : p->cu_seqlens ? 256 : 129)) return kWhole;
+    const size_t room = p->dk > 128 || p->dv > 128 ? 256 : 512;
+    size_t segment;
+    if (p->cu_seqlens) {
+        const size_t partial = walks * 3 / 4;
+        segment = ceil_div(p->tokens * blocks, partial * 2 < room ? room - partial : room / 2);
+    } else {
+        segment = ceil_div(p->tokens, walks < room ? room / walks : 1);
+    }
+    return segment < 256 ? 256 : round_up(segment, 64);
 }
 size_t slots_of(const flstm_decay_attention* p, bool backward) {
     const size_t segment = segment_of(p, backward);
@@ -821,7 +827,8 @@ size_t shares_bytes(const flstm_decay_attention* p, int width) {
     return p->heads == p->kv_heads ? 0 : round_up(rows_of(p) * p->heads * size_t(width) * sizeof(float), 256);
 }
 
-Role role(flstm_rows r, int group) { return Role{r.data, r.sequence, r.token, r.head, group}; }
+flstm_rows or_none(const flstm_rows* r) { return r ? *r : flstm_rows{}; }
+Role role(const flstm_rows& r, int group) { return Role{r.data, r.sequence, r.token, r.head, group}; }
 
 Sweeps sweeps_of(const flstm_decay_attention* p, bool backward) {
     Sweeps a{};
@@ -896,9 +903,10 @@ extern "C" size_t flstm_decay_attention_workspace_bytes(const flstm_decay_attent
     return backward ? 2 * states_bytes(p, true) + shares_bytes(p, p->dk) + shares_bytes(p, p->dv) : states_bytes(p, false);
 }
 
-extern "C" int flstm_decay_attention_forward(const flstm_decay_attention* p, flstm_rows q, flstm_rows k, flstm_rows v,
-                                             const float* state_in, flstm_rows o, float* state_out, void* workspace, void* stream) {
+extern "C" int flstm_decay_attention_forward(const flstm_decay_attention* p, const flstm_rows* q_, const flstm_rows* k_, const flstm_rows* v_,
+                                             const float* state_in, const flstm_rows* o_, float* state_out, void* workspace, void* stream) {
     if (!valid_shape(p)) return FLSTM_E_INVALID;
+    const flstm_rows q = or_none(q_), k = or_none(k_), v = or_none(v_), o = or_none(o_);
     if (rows_of(p) > 0 && (!q.data || !k.data || !v.data || !o.data)) return FLSTM_E_INVALID;
     if (states_bytes(p, false) > 0 && !workspace) return FLSTM_E_INVALID;
     if (!reachable(q) || !reachable(k) || !reachable(v)) return FLSTM_E_TOO_LARGE;
@@ -921,10 +929,11 @@ extern "C" int flstm_decay_attention_forward(const flstm_decay_attention* p, fls
     return run_sweeps(a, p->dtype, true, stream_);
 }
 
-extern "C" int flstm_decay_attention_backward(const flstm_decay_attention* p, flstm_rows d_o, flstm_rows q, flstm_rows k, flstm_rows v,
-                                              const float* state_in, const float* d_state_out, flstm_rows dq, flstm_rows dk,
-                                              flstm_rows dv, float* d_state_in, void* workspace, void* stream) {
+extern "C" int flstm_decay_attention_backward(const flstm_decay_attention* p, const flstm_rows* d_o_, const flstm_rows* q_, const flstm_rows* k_, const flstm_rows* v_,
+                                              const float* state_in, const float* d_state_out, const flstm_rows* dq_, const flstm_rows* dk_,
+                                              const flstm_rows* dv_, float* d_state_in, void* workspace, void* stream) {
     if (!valid_shape(p)) return FLSTM_E_INVALID;
+    const flstm_rows d_o = or_none(d_o_), q = or_none(q_), k = or_none(k_), v = or_none(v_), dq = or_none(dq_), dk = or_none(dk_), dv = or_none(dv_);
     if (rows_of(p) > 0 && (!d_o.data || !q.data || !k.data || !v.data)) return FLSTM_E_INVALID;
     if (flstm_decay_attention_workspace_bytes(p, 1) > 0 && !workspace) return FLSTM_E_INVALID;
     if (!reachable(d_o) || !reachable(q) || !reachable(k) || !reachable(v)) return FLSTM_E_TOO_LARGE;
@@ -938,7 +947,7 @@ extern "C" int flstm_decay_attention_backward(const flstm_decay_attention* p, fl
     char* const shares_k = room + 2 * states_bytes(p, true);
     char* const shares_v = shares_k + shares_bytes(p, p->dk);
     const Role rq = role(q, 1), rk = role(k, group), rv = role(v, group), rdo = role(d_o, 1);
-    const auto shared = [&](flstm_rows r, char* room, int width) {   // where a sweep leaves a head's share
+    const auto shared = [&](const flstm_rows& r, char* room, int width) {   // where a sweep leaves a head's share
         if (group == 1 || !r.data) return role(r, 1);
         return Role{room, ptrdiff_t(p->tokens) * p->heads * width, ptrdiff_t(p->heads) * width, width, 1};
     };
@@ -980,7 +989,7 @@ extern "C" int flstm_decay_attention_backward(const flstm_decay_attention* p, fl
     }
     if (rc != 0 || group == 1 || rows_of(p) == 0) return rc;
     if (rows_of(p) >= (size_t(1) << 31)) return FLSTM_E_TOO_LARGE;
-    const auto fold = [&](flstm_rows r, char* shares, int width) {
+    const auto fold = [&](const flstm_rows& r, char* shares, int width) {
         if (!r.data) return 0;
         const size_t rows = rows_of(p), tokens = p->cu_seqlens ? rows : p->tokens;
         const Fold f{reinterpret_cast<const float*>(shares), role(r, 1), rows / tokens, tokens, p->heads, group, width};
@@ -993,10 +1002,11 @@ extern "C" int flstm_decay_attention_backward(const flstm_decay_attention* p, fl
     return rc != 0 ? rc : fold(dv, shares_v, p->dv);
 }
 
-extern "C" int flstm_decay_attention_step(const flstm_decay_attention* p, flstm_rows q, flstm_rows k, flstm_rows v, flstm_rows o,
+extern "C" int flstm_decay_attention_step(const flstm_decay_attention* p, const flstm_rows* q_, const flstm_rows* k_, const flstm_rows* v_, const flstm_rows* o_,
                                           float* state, void* stream) {
     if (!valid_shape(p)) return FLSTM_E_INVALID;
     if (p->sequences == 0) return 0;
+    const flstm_rows q = or_none(q_), k = or_none(k_), v = or_none(v_), o = or_none(o_);
     if (!q.data || !k.data || !v.data || !o.data || !state) return FLSTM_E_INVALID;
     const size_t grid = p->sequences * size_t(p->heads);
     if (grid >= (size_t(1) << 31)) return FLSTM_E_TOO_LARGE;

@@ -43,6 +43,32 @@ __device__ __forceinline__ float8 share8(float8 z, float most, float log_sum, fl
     return e;
 }
 
+// A row as its workgroup takes it: whole vectors of eight from a 16-byte boundary of `at` on, what is left in front of them with the
+// first thread and what is left behind with the last.  (Rows of a vocabulary that is a multiple of nothing begin anywhere; read and
+// written as they lie, 8192 of 50001 bf16 logits take 424 us instead of 376.)
+struct Cut {
+    int whole;        // vectors
+    int head;         // elements in front of them
+    int first, left;  // this thread's elements beside its vectors
+};
+template <class T, int THREADS> __device__ __forceinline__ Cut cut_row(const T* at, int vocabulary) {
+    const int ahead = int((16 - reinterpret_cast<uintptr_t>(at) % 16) % 16 / sizeof(T));
+    Cut c;
+    c.head = ahead < vocabulary ? ahead : vocabulary;
+    c.whole = (vocabulary - c.head) / 8;
+    const int behind = c.head + c.whole * 8;
+    c.first = threadIdx.x == 0 ? 0 : behind;
+    c.left = threadIdx.x == 0 ? c.head : threadIdx.x == THREADS - 1 ? vocabulary - behind : 0;
+    return c;
+}
+// This thread's elements beside its vectors, minus infinity behind them, which adds nothing to a sum.
+template <class T> __device__ __forceinline__ float8 beside(const T* z, const Cut& c) {
+    float8 v = load8(z + c.first, c.left);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < c.left ? v[i] : -__builtin_inff();
+    return v;
+}
+
 // A pair of values over the workgroup, in all threads.
 template <int THREADS, class Op> __device__ __forceinline__ float2 all_threads(float2 v, float2* scratch, Op op) {
 #pragma unroll
@@ -136,33 +162,25 @@ template <class T, int THREADS> __global__ __launch_bounds__(THREADS) void loss_
     __shared__ float2 scratch[THREADS / kWave];
     const size_t row = blockIdx.x;
     const T* z = static_cast<const T*>(a.logits) + row * a.ld;
-    // running maximum and sum
-    float most = kLowest, sum = 0.f;
+    // running maximum and sum, several vectors at a time
+    const Cut cut = cut_row<T, THREADS>(z, a.vocabulary);
+    const float8 rest = beside(z, cut);
+    float most = fmaxf(kLowest, max8(rest)), sum = sum8(share8(rest, most, 0.f, a.to_log2));
     constexpr int kAhead = 4;
-    int c = int(threadIdx.x) * 8;
-    for (; c + (kAhead - 1) * THREADS * 8 + 8 <= a.vocabulary; c += kAhead * THREADS * 8) {
-        float8 v[kAhead];
+    for (int base = threadIdx.x; base < cut.whole; base += kAhead * THREADS) {
+        typename Vec8<T>::type v[kAhead];
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) v[j] = load8(z + c + j * THREADS * 8);
-        float m = max8(v[0]);
-#pragma unroll
-        for (int j = 1; j < kAhead; ++j) m = fmaxf(m, max8(v[j]));
-        m = fmaxf(most, m);
-        sum *= __builtin_amdgcn_exp2f((most - m) * a.to_log2);
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j) sum += sum8(share8(v[j], m, 0.f, a.to_log2));
-        most = m;
-    }
-    for (; c < a.vocabulary; c += THREADS * 8) {
-        const int n = a.vocabulary - c;
-        const float8 v = load8(z + c, n);
+        for (int j = 0; j < kAhead; ++j) {
+            const int i = base + j * THREADS;
+            if (i < cut.whole) __builtin_memcpy(&v[j], __builtin_assume_aligned(z + cut.head + size_t(i) * 8, sizeof(T)), sizeof(v[j]));
+            else v[j] = T(-__builtin_inff());
+        }
         float m = most;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = i < n ? fmaxf(m, v[i]) : m;
+        for (int j = 0; j < kAhead; ++j) m = fmaxf(m, max8(__builtin_convertvector(v[j], float8)));
         sum *= __builtin_amdgcn_exp2f((most - m) * a.to_log2);
-        const float8 e = share8(v, m, 0.f, a.to_log2);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum += i < n ? e[i] : 0.f;
+        for (int j = 0; j < kAhead; ++j) sum += sum8(share8(__builtin_convertvector(v[j], float8), m, 0.f, a.to_log2));
         most = m;
     }
     bool any;
@@ -206,8 +224,14 @@ template <class T> __global__ __launch_bounds__(kGradientThreads) void gradient_
     to_weights<THREADS>(a, teacher, Norm{m, __builtin_amdgcn_logf(mass)});
     const Norm norm{a.stats[row].x, a.stats[row].y};
     const float factor = a.d_loss[row * a.d_stride] * a.temperature;
-    for (int c = begin + int(threadIdx.x) * 8; c < end; c += THREADS * 8)
-        store8(out + c, factor * share8(load8(z + c, end - c), norm.most, norm.log_sum, a.to_log2), end - c);
+    const Cut cut = cut_row<T, THREADS>(out + begin, end - begin);
+    z += begin;
+    out += begin;
+    for (int i = threadIdx.x; i < cut.whole; i += THREADS) {
+        const size_t c = cut.head + size_t(i) * 8;
+        store8(out + c, factor * share8(load8(z + c), norm.most, norm.log_sum, a.to_log2));
+    }
+    store8(out + cut.first, factor * share8(beside(z, cut), norm.most, norm.log_sum, a.to_log2), cut.left);
     __syncthreads();
     write_entries<T, THREADS>(a, row, teacher, factor, norm, begin, end);
 }
@@ -222,21 +246,16 @@ template <class T, int THREADS, int R> __global__ __launch_bounds__(THREADS) voi
     const T* z = static_cast<const T*>(a.logits) + row * a.ld;
     T* out = static_cast<T*>(a.dlogits) + row * a.ldd;
     typedef typename Vec8<T>::type vec;
-    // whole vectors of the row, and what is left behind them with the last thread; behind the row minus infinity, which adds nothing
-    const int tid = threadIdx.x, whole = a.vocabulary / 8, left = tid == THREADS - 1 ? a.vocabulary % 8 : 0;
+    const int tid = threadIdx.x;
+    const Cut cut = cut_row<T, THREADS>(out, a.vocabulary);
     vec v[R + 1];
 #pragma unroll
     for (int j = 0; j < R; ++j) {
         const int i = j * THREADS + tid;
-        if (i < whole) __builtin_memcpy(&v[j], __builtin_assume_aligned(z + size_t(i) * 8, sizeof(T)), sizeof(vec));
+        if (i < cut.whole) __builtin_memcpy(&v[j], __builtin_assume_aligned(z + cut.head + size_t(i) * 8, sizeof(T)), sizeof(vec));
         else v[j] = T(-__builtin_inff());
     }
-    {
-        float8 tail = load8(z + size_t(whole) * 8, left);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) tail[i] = i < left ? tail[i] : -__builtin_inff();
-        v[R] = __builtin_convertvector(tail, vec);
-    }
+    v[R] = __builtin_convertvector(beside(z, cut), vec);
     // (Between the three readings the row is hidden from the compiler, which would otherwise keep it converted, in twice the registers.)
     const auto hide = [&] {
 #pragma unroll
@@ -265,8 +284,8 @@ template <class T, int THREADS, int R> __global__ __launch_bounds__(THREADS) voi
         const int i = j * THREADS + tid;
         float8 g = 0.f;
         if (counts) g = factor * share8(__builtin_convertvector(v[j], float8), q_norm.most, q_norm.log_sum, a.to_log2);
-        if (j == R) store8(out + size_t(whole) * 8, g, left);
-        else if (i < whole) store8(out + size_t(i) * 8, g);
+        if (j == R) store8(out + cut.first, g, cut.left);
+        else if (i < cut.whole) store8(out + cut.head + size_t(i) * 8, g);
     }
     if (!counts) return;
     to_weights<THREADS>(a, teacher, p_norm);
@@ -290,8 +309,11 @@ Distill distill_of(const flstm_distillation* p) {
     return a;
 }
 
-// The most that a row in registers may have: 16 vectors of eight 16-bit values a thread, or eight of fp32.
-size_t held_vocabulary(flstm_op_dtype dtype) { return dtype == FLSTM_OP_F32 ? 65536 : 131072; }
+// The most that a row in registers may have: 16 vectors of eight 16-bit values a thread of 512, or eight of fp32 a thread of 1024.
+// Two workgroups of 512 threads fit a CU, so that one's row arrives while the other's gradient leaves: 8192 rows of 50048 bf16
+// logits take 366 us (4.5 TB/s), where one of 1024 threads took 472.  (100000 of them with 16 vectors a thread of 1024, alone on
+// its CU, took 457 us for 4096 rows: no less than the two passes that read the logits twice.)
+constexpr size_t kHeld = 65536;
 
 }  // namespace
 }  // namespace flstm_hip
@@ -305,7 +327,9 @@ extern "C" int flstm_distillation_forward(const flstm_distillation* p, float* lo
     a.loss = loss; a.stats = reinterpret_cast<float2*>(stats);
     return with_type(p->dtype, [&](auto zero) {
         typedef decltype(zero) T;
-        if (p->vocabulary <= 8192) loss_kernel<T, 256><<<unsigned(p->rows), 256, 0, static_cast<hipStream_t>(stream)>>>(a);
+        // (256 threads a row where the rows fill the chip, so that eight of them are under way in a CU: 1024 rows of 32000 bf16 16 us
+        // instead of 20, 2048 of fp16 26 instead of 35; 1024 threads where they do not.)
+        if (p->vocabulary <= 8192 || p->rows >= 256) loss_kernel<T, 256><<<unsigned(p->rows), 256, 0, static_cast<hipStream_t>(stream)>>>(a);
         else loss_kernel<T, 1024><<<unsigned(p->rows), 1024, 0, static_cast<hipStream_t>(stream)>>>(a);
         return launched();
     });
@@ -326,14 +350,14 @@ extern "C" int flstm_distillation_backward(const flstm_distillation* p, const fl
 }
 
 extern "C" size_t flstm_distillation_workspace_bytes(const flstm_distillation* p) {
-    return valid_problem(p) && p->vocabulary > held_vocabulary(p->dtype) ? round_up(p->rows * 2 * sizeof(float), 16) : 0;
+    return valid_problem(p) && p->vocabulary > kHeld ? round_up(p->rows * 2 * sizeof(float), 16) : 0;
 }
 
 extern "C" int flstm_distillation_train(const flstm_distillation* p, const float* d_loss, size_t d_stride, float* loss, void* dlogits,
                                         size_t ldd, void* workspace, void* stream) {
     if (!valid_problem(p) || (p->rows > 0 && (!loss || !d_loss || !dlogits)) || ldd < p->vocabulary) return FLSTM_E_INVALID;
     if (p->rows == 0) return 0;
-    if (p->vocabulary > held_vocabulary(p->dtype)) {   // one pass behind the other, the rows' statistics in the workspace
+    if (p->vocabulary > kHeld) {   // one pass behind the other, the rows' statistics in the workspace
         if (!workspace) return FLSTM_E_INVALID;
         const int rc = flstm_distillation_forward(p, loss, static_cast<float*>(workspace), stream);
         return rc != 0 ? rc : flstm_distillation_backward(p, static_cast<const float*>(workspace), d_loss, d_stride, dlogits, ldd, stream);
@@ -348,14 +372,13 @@ extern "C" int flstm_distillation_train(const flstm_distillation* p, const float
             return launched();
         };
         const std::integral_constant<int, 256> few;
+        const std::integral_constant<int, 512> some;
         const std::integral_constant<int, 1024> many;
         if (p->vocabulary <= 2048) return go(few, std::integral_constant<int, 1>());
         if (p->vocabulary <= 8192) return go(few, std::integral_constant<int, 4>());
         if (p->vocabulary <= 16384) return go(many, std::integral_constant<int, 2>());
-        if (p->vocabulary <= 32768) return go(many, std::integral_constant<int, 4>());
-        if constexpr (sizeof(T) == 2) {
-            if (p->vocabulary > 65536) return go(many, std::integral_constant<int, 16>());
-        }
-        return go(many, std::integral_constant<int, 8>());
+        if (p->vocabulary <= 32768) return go(some, std::integral_constant<int, 8>());
+        if constexpr (sizeof(T) == 2) return go(some, std::integral_constant<int, 16>());
+        else return go(many, std::integral_constant<int, 8>());
     });
 }

@@ -8,6 +8,7 @@ current stream of the tensors' device, which has to be the current device, and n
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -28,13 +29,13 @@ def _bind() -> ctypes.CDLL:
         lib.flstm_layer_norm_workspace_bytes.argtypes = [sz, sz]
         lib.flstm_layer_norm_workspace_bytes.restype = sz
         lib.flstm_layer_norm_backward.argtypes = [sz, sz, vp, sz, vp, sz, vp, sz, i32] + [vp] * 8
-        shape = ctypes.POINTER(_DecayShape)
-        lib.flstm_decay_attention_forward.argtypes = [shape, _Rows, _Rows, _Rows, vp, _Rows, vp, vp, vp]
-        lib.flstm_decay_attention_backward.argtypes = [shape, _Rows, _Rows, _Rows, _Rows, vp, vp, _Rows, _Rows, _Rows, vp, vp, vp]
+        rows = shape = ctypes.c_char_p   # (packed structures)
+        lib.flstm_decay_attention_forward.argtypes = [shape, rows, rows, rows, vp, rows, vp, vp, vp]
+        lib.flstm_decay_attention_backward.argtypes = [shape, rows, rows, rows, rows, vp, vp, rows, rows, rows, vp, vp, vp]
         lib.flstm_decay_attention_workspace_bytes.argtypes = [shape, i32]
         lib.flstm_decay_attention_workspace_bytes.restype = sz
-        lib.flstm_decay_attention_step.argtypes = [shape, _Rows, _Rows, _Rows, _Rows, vp, vp]
-        problem = ctypes.POINTER(_Distillation)
+        lib.flstm_decay_attention_step.argtypes = [shape, rows, rows, rows, rows, vp, vp]
+        problem = ctypes.c_char_p
         lib.flstm_distillation_forward.argtypes = [problem, vp, vp, vp]
         lib.flstm_distillation_backward.argtypes = [problem, vp, vp, sz, vp, sz, vp]
         lib.flstm_distillation_workspace_bytes.argtypes = [problem]
@@ -51,20 +52,22 @@ def _check(rc: int, name: str) -> None:
 
 def _device_tensor(name: str, t, dtype=None) -> int:
     """Refuses what is no tensor on the current device or of a type that the operators do not have; returns the type's code."""
-    if not torch.is_tensor(t) or not t.is_cuda:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
-    if t.get_device() != torch.cuda.current_device():
+    if t.get_device() != torch._C._cuda_getDevice():
         raise ValueError(f"{name} is on {t.device}, which is not the current device")
-    if dtype is not None and t.dtype != dtype:
-        raise ValueError(f"{name} must be of type {dtype}, not {t.dtype}")
-    code = _DTYPES.get(t.dtype)
+    kind = t.dtype
+    if dtype is not None and kind != dtype:
+        raise ValueError(f"{name} must be of type {dtype}, not {kind}")
+    code = _DTYPES.get(kind)
     if code is None:
-        raise ValueError(f"unsupported dtype {t.dtype} of {name}: tensors must be float32, float16 or bfloat16")
+        raise ValueError(f"unsupported dtype {kind} of {name}: tensors must be float32, float16 or bfloat16")
     return code
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """The current stream of the current device (torch.cuda.current_stream().cuda_stream without the object around it: 2 us less)."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _ptr(t) -> Optional[int]:
@@ -75,7 +78,8 @@ def _ptr(t) -> Optional[int]:
 
 def _rows(t):
     """`t` as (rows, width) with contiguous rows; a copy only where its layout has no such view."""
-    t = t.reshape(-1, t.shape[-1])
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
@@ -112,8 +116,7 @@ def layer_norm_forward(x, weight=None, bias=None, *, eps: float = 1e-5, residual
     rows = rows_x.shape[0]
     y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     total = x if residual is None else torch.empty_like(y)
-    stats = torch.empty((2, rows), device=x.device, dtype=torch.float32)
-    mean, rstd = stats[0], stats[1]
+    mean, rstd = torch.empty((2, rows), device=x.device, dtype=torch.float32).unbind(0)
     _check(_bind().flstm_layer_norm_forward(rows, width, rows_x.data_ptr(), rows_x.stride(0), _ptr(rows_r),
                                             0 if rows_r is None else rows_r.stride(0), code, _ptr(weight), _ptr(bias), eps,
                                             None if residual is None else total.data_ptr(), y.data_ptr(), mean.data_ptr(),
@@ -205,25 +208,18 @@ class LayerNorm(torch.nn.Module):
 
 # ---- attention with a decaying state
 
-class _Rows(ctypes.Structure):
-    """flstm_rows: where element (sequence, token, head, i) of a tensor lies."""
-    _fields_ = [("data", ctypes.c_void_p), ("sequence", ctypes.c_ssize_t), ("token", ctypes.c_ssize_t), ("head", ctypes.c_ssize_t)]
+# flstm_rows and flstm_decay_attention, packed: a call of a few microseconds has no time for ctypes structures
+_ROWS = struct.Struct("@Pnnn")
+_SHAPE = struct.Struct("@NNPiiiiifP")
 
 
-class _DecayShape(ctypes.Structure):
-    """flstm_decay_attention."""
-    _fields_ = [("sequences", ctypes.c_size_t), ("tokens", ctypes.c_size_t), ("cu_seqlens", ctypes.c_void_p), ("heads", ctypes.c_int),
-                ("kv_heads", ctypes.c_int), ("dk", ctypes.c_int), ("dv", ctypes.c_int), ("dtype", ctypes.c_int),
-                ("scale", ctypes.c_float), ("log_decay", ctypes.c_void_p)]
-
-
-def _rows_of(t) -> _Rows:
-    """Strides of (sequences, tokens, heads, D) or, packed, (tokens, heads, D); for a single token (sequences, heads, D) too, where
-    the token's stride is not read."""
+def _rows_of(t):
+    """Where (sequences, tokens, heads, D) or, packed, (tokens, heads, D) lies; for a single token (sequences, heads, D) too, where the
+    token's stride is not read."""
     if t is None:
-        return _Rows()
+        return None
     s = t.stride()
-    return _Rows(t.data_ptr(), s[0], s[-3], s[-2])
+    return _ROWS.pack(t.data_ptr(), s[0], s[-3], s[-2])
 
 
 def _last_axis_contiguous(t):
@@ -262,7 +258,7 @@ def _decay_shape(q, k, v, log_decay, scale, state, cu_seqlens, axes: int):
         sequences, tokens = cu_seqlens.shape[0] - 1, q.shape[0]
     else:
         sequences, tokens = q.shape[0], q.shape[1] if axes == 4 else 1
-    shape = _DecayShape(sequences, tokens, _ptr(cu_seqlens), heads, kv_heads, dk, dv, code, scale, log_decay.data_ptr())
+    shape = _SHAPE.pack(sequences, tokens, _ptr(cu_seqlens) or 0, heads, kv_heads, dk, dv, code, scale, log_decay.data_ptr())
     _check_state("state", state, (sequences, heads, dk, dv))
     return shape, (sequences, heads, dk, dv)
 
@@ -288,8 +284,8 @@ def _like_rows(q, heads: int, width: int):
     return torch.empty((*q.shape[:-2], heads, width), device=q.device, dtype=q.dtype)
 
 
-def _workspace(shape: _DecayShape, backward: int, device):
-    size = _bind().flstm_decay_attention_workspace_bytes(ctypes.byref(shape), backward)
+def _workspace(shape: bytes, backward: int, device):
+    size = _bind().flstm_decay_attention_workspace_bytes(shape, backward)
     return torch.empty(size, device=device, dtype=torch.uint8) if size else None
 
 
@@ -305,10 +301,10 @@ def decay_attention_forward(q, k, v, log_decay, *, scale: Optional[float] = None
     axes = 4 if cu_seqlens is None else 3
     shape, states = _decay_shape(q, k, v, log_decay, scale, state, cu_seqlens, axes)
     q, k, v = (_last_axis_contiguous(t) for t in (q, k, v))
-    o = _like_rows(q, shape.heads, shape.dv)
+    o = _like_rows(q, states[1], states[3])
     final = torch.empty(states, device=q.device, dtype=torch.float32) if want_state else None
     workspace = _workspace(shape, 0, q.device)
-    _check(_bind().flstm_decay_attention_forward(ctypes.byref(shape), _rows_of(q), _rows_of(k), _rows_of(v), _ptr(state), _rows_of(o),
+    _check(_bind().flstm_decay_attention_forward(shape, _rows_of(q), _rows_of(k), _rows_of(v), _ptr(state), _rows_of(o),
                                                  _ptr(final), _ptr(workspace), _stream()), "flstm_decay_attention_forward")
     return o, final
 
@@ -320,17 +316,17 @@ def decay_attention_backward(do, q, k, v, log_decay, *, scale: Optional[float] =
     axes = 4 if cu_seqlens is None else 3
     shape, states = _decay_shape(q, k, v, log_decay, scale, state, cu_seqlens, axes)
     _device_tensor("do", do, q.dtype)
-    if tuple(do.shape) != (*q.shape[:-1], shape.dv):
-        raise ValueError(f"do must have shape {(*q.shape[:-1], shape.dv)}: got {tuple(do.shape)}")
+    if tuple(do.shape) != (*q.shape[:-1], states[3]):
+        raise ValueError(f"do must have shape {(*q.shape[:-1], states[3])}: got {tuple(do.shape)}")
     _check_state("d_state", d_state, states)
     do, q, k, v = (_last_axis_contiguous(t) for t in (do, q, k, v))
-    dq = _like_rows(q, shape.heads, shape.dk) if want[0] else None
-    dk = _like_rows(k, shape.kv_heads, shape.dk) if want[1] else None
-    dv = _like_rows(v, shape.kv_heads, shape.dv) if want[2] else None
+    dq = _like_rows(q, *q.shape[-2:]) if want[0] else None
+    dk = _like_rows(k, *k.shape[-2:]) if want[1] else None
+    dv = _like_rows(v, *v.shape[-2:]) if want[2] else None
     d_initial = torch.empty(states, device=q.device, dtype=torch.float32) if want[3] else None
     workspace = _workspace(shape, 1, q.device)
     _check(_bind().flstm_decay_attention_backward(
-        ctypes.byref(shape), _rows_of(do), _rows_of(q), _rows_of(k), _rows_of(v), _ptr(state), _ptr(d_state), _rows_of(dq), _rows_of(dk),
+        shape, _rows_of(do), _rows_of(q), _rows_of(k), _rows_of(v), _ptr(state), _ptr(d_state), _rows_of(dq), _rows_of(dk),
         _rows_of(dv), _ptr(d_initial), _ptr(workspace), _stream()), "flstm_decay_attention_backward")
     return dq, dk, dv, d_initial
 
@@ -340,10 +336,10 @@ def decay_attention_step(q, k, v, log_decay, state, *, scale: Optional[float] = 
     (sequences, heads, dk, dv) float32 is updated in place.  Returns o (sequences, heads, dv).  No autograd."""
     if state is None:
         raise ValueError("state must be a tensor: it is updated in place")
-    shape, _ = _decay_shape(q, k, v, log_decay, scale, state, None, 3)
+    shape, states = _decay_shape(q, k, v, log_decay, scale, state, None, 3)
     q, k, v = (_last_axis_contiguous(t) for t in (q, k, v))
-    o = torch.empty((shape.sequences, shape.heads, shape.dv), device=q.device, dtype=q.dtype)
-    _check(_bind().flstm_decay_attention_step(ctypes.byref(shape), _rows_of(q), _rows_of(k), _rows_of(v), _rows_of(o), state.data_ptr(),
+    o = torch.empty((states[0], states[1], states[3]), device=q.device, dtype=q.dtype)
+    _check(_bind().flstm_decay_attention_step(shape, _rows_of(q), _rows_of(k), _rows_of(v), _rows_of(o), state.data_ptr(),
                                               _stream()), "flstm_decay_attention_step")
     return o
 
@@ -378,11 +374,7 @@ def decay_attention(q, k, v, log_decay, *, scale: Optional[float] = None, state=
 
 # ---- distillation from a teacher's top logits
 
-class _Distillation(ctypes.Structure):
-    """flstm_distillation."""
-    _fields_ = [("rows", ctypes.c_size_t), ("vocabulary", ctypes.c_size_t), ("logits", ctypes.c_void_p), ("ld", ctypes.c_size_t),
-                ("dtype", ctypes.c_int), ("top", ctypes.c_int), ("teacher_logits", ctypes.c_void_p), ("teacher_dtype", ctypes.c_int),
-                ("teacher_index", ctypes.c_void_p), ("index_64", ctypes.c_int), ("temperature", ctypes.c_float)]
+_PROBLEM = struct.Struct("@NNPNiiPiPif")   # flstm_distillation
 
 
 def _distillation(logits, teacher_logits, teacher_index, temperature: float):
@@ -411,18 +403,19 @@ def _distillation(logits, teacher_logits, teacher_index, temperature: float):
     if ld < vocabulary:
         kept = (kept[0].contiguous(), *kept[1:])
         ld = vocabulary
-    return _Distillation(rows, vocabulary, kept[0].data_ptr(), ld, code, top, kept[1].data_ptr(), teacher_code, kept[2].data_ptr(),
-                         int(teacher_index.dtype == torch.int64), temperature), kept
+    problem = _PROBLEM.pack(rows, vocabulary, kept[0].data_ptr(), ld, code, top, kept[1].data_ptr(), teacher_code, kept[2].data_ptr(),
+                            teacher_index.dtype == torch.int64, temperature)
+    return problem, rows, vocabulary, ld, kept
 
 
-def _per_row(name: str, t, problem: _Distillation):
+def _per_row(name: str, t, rows: int):
     """`t` as (rows,) float32 with any stride (0: one value for all rows)."""
     _device_tensor(name, t, torch.float32)
-    if t.numel() == 1 and problem.rows != 1:
-        return t.reshape(1).expand(problem.rows)
-    if t.numel() != problem.rows:
-        raise ValueError(f"{name} must hold one value a row ({problem.rows}) or one for all: got {t.numel()}")
-    return t.reshape(-1)
+    if t.numel() == 1 and rows != 1:
+        return t.reshape(1).expand(rows)
+    if t.numel() != rows:
+        raise ValueError(f"{name} must hold one value a row ({rows}) or one for all: got {t.numel()}")
+    return t if t.dim() == 1 else t.reshape(-1)
 
 
 def distillation_forward(logits, teacher_logits, teacher_index, *, temperature: float = 1.0) -> Tuple:
@@ -433,40 +426,40 @@ def distillation_forward(logits, teacher_logits, teacher_index, *, temperature: 
     with an index outside the vocabulary (-1, say) or a logit of minus infinity do not count; a row without others has loss 0.
     Returns (loss, stats), float32: loss of logits' leading shape, stats (rows, 2), which distillation_backward takes (a row's
     largest logit, and log2 of the sum of exp((logit - largest) / temperature))."""
-    problem, kept = _distillation(logits, teacher_logits, teacher_index, temperature)
+    problem, rows, vocabulary, ld, kept = _distillation(logits, teacher_logits, teacher_index, temperature)
     loss = torch.empty(logits.shape[:-1], device=logits.device, dtype=torch.float32)
-    stats = torch.empty((problem.rows, 2), device=logits.device, dtype=torch.float32)
-    _check(_bind().flstm_distillation_forward(ctypes.byref(problem), loss.data_ptr(), stats.data_ptr(), _stream()), "flstm_distillation_forward")
+    stats = torch.empty((rows, 2), device=logits.device, dtype=torch.float32)
+    _check(_bind().flstm_distillation_forward(problem, loss.data_ptr(), stats.data_ptr(), _stream()), "flstm_distillation_forward")
     return loss, stats
 
 
 def distillation_backward(d_loss, logits, teacher_logits, teacher_index, stats, *, temperature: float = 1.0):
     """The gradient of logits (in their type) from that of every row's loss (one value a row, or one for all)."""
-    problem, kept = _distillation(logits, teacher_logits, teacher_index, temperature)
-    d_loss = _per_row("d_loss", d_loss, problem)
+    problem, rows, vocabulary, ld, kept = _distillation(logits, teacher_logits, teacher_index, temperature)
+    d_loss = _per_row("d_loss", d_loss, rows)
     _device_tensor("stats", stats, torch.float32)
-    if tuple(stats.shape) != (problem.rows, 2) or not stats.is_contiguous():
-        raise ValueError(f"stats must be a contiguous tensor of shape ({problem.rows}, 2)")
+    if tuple(stats.shape) != (rows, 2) or not stats.is_contiguous():
+        raise ValueError(f"stats must be a contiguous tensor of shape ({rows}, 2)")
     dlogits = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
-    _check(_bind().flstm_distillation_backward(ctypes.byref(problem), stats.data_ptr(), d_loss.data_ptr(), d_loss.stride(0) if problem.rows else 0,
-                                               dlogits.data_ptr(), problem.vocabulary, _stream()), "flstm_distillation_backward")
+    _check(_bind().flstm_distillation_backward(problem, stats.data_ptr(), d_loss.data_ptr(), d_loss.stride(0) if rows else 0,
+                                               dlogits.data_ptr(), vocabulary, _stream()), "flstm_distillation_backward")
     return dlogits
 
 
 def distillation_train(logits, teacher_logits, teacher_index, d_loss, *, temperature: float = 1.0, in_place: bool = False) -> Tuple:
     """(loss, dlogits) in one call, for a d_loss that is known beforehand (1 / rows for a mean): the logits are read once.
     in_place: the gradient takes the place of the logits, which must then have contiguous rows."""
-    problem, kept = _distillation(logits, teacher_logits, teacher_index, temperature)
-    d_loss = _per_row("d_loss", d_loss, problem)
-    if in_place and problem.rows and problem.logits != logits.data_ptr():
+    problem, rows, vocabulary, ld, kept = _distillation(logits, teacher_logits, teacher_index, temperature)
+    d_loss = _per_row("d_loss", d_loss, rows)
+    if in_place and rows and kept[0].data_ptr() != logits.data_ptr():
         raise ValueError("in place, logits must have contiguous rows of their own")
     loss = torch.empty(logits.shape[:-1], device=logits.device, dtype=torch.float32)
     dlogits = logits if in_place else torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
     lib = _bind()
-    size = lib.flstm_distillation_workspace_bytes(ctypes.byref(problem))
+    size = lib.flstm_distillation_workspace_bytes(problem)
     workspace = torch.empty(size, device=logits.device, dtype=torch.uint8) if size else None
-    _check(lib.flstm_distillation_train(ctypes.byref(problem), d_loss.data_ptr(), d_loss.stride(0) if problem.rows else 0, loss.data_ptr(),
-                                        dlogits.data_ptr(), problem.ld if in_place else problem.vocabulary, _ptr(workspace), _stream()),
+    _check(lib.flstm_distillation_train(problem, d_loss.data_ptr(), d_loss.stride(0) if rows else 0, loss.data_ptr(),
+                                        dlogits.data_ptr(), ld if in_place else vocabulary, _ptr(workspace), _stream()),
            "flstm_distillation_train")
     return loss, dlogits
 

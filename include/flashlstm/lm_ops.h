@@ -73,18 +73,18 @@ typedef struct {
 
 /* state_in (null: zeros) and state_out may be null; they must not be one buffer.
  * `workspace` has flstm_decay_attention_workspace_bytes(shape, 0) bytes (16-byte aligned; null where that is 0). */
-int flstm_decay_attention_forward(const flstm_decay_attention* shape, flstm_rows q, flstm_rows k, flstm_rows v,
-                                  const float* state_in, flstm_rows o, float* state_out, void* workspace, void* stream);
-/* Gradients, of d_o and d_state_out (null: zeros): dq, dk and dv (type and head counts of q, k and v; .data may be null) and
+int flstm_decay_attention_forward(const flstm_decay_attention* shape, const flstm_rows* q, const flstm_rows* k, const flstm_rows* v,
+                                  const float* state_in, const flstm_rows* o, float* state_out, void* workspace, void* stream);
+/* Gradients, of d_o and d_state_out (null: zeros): dq, dk and dv (type and head counts of q, k and v; each may be null) and
  * d_state_in (may be null).  None of them may lie in an input.  `workspace`: flstm_decay_attention_workspace_bytes(shape, 1).
  * log_decay is a constant of the model and has no gradient. */
-int flstm_decay_attention_backward(const flstm_decay_attention* shape, flstm_rows d_o, flstm_rows q, flstm_rows k, flstm_rows v,
-                                   const float* state_in, const float* d_state_out, flstm_rows dq, flstm_rows dk, flstm_rows dv,
-                                   float* d_state_in, void* workspace, void* stream);
+int flstm_decay_attention_backward(const flstm_decay_attention* shape, const flstm_rows* d_o, const flstm_rows* q, const flstm_rows* k,
+                                   const flstm_rows* v, const float* state_in, const float* d_state_out, const flstm_rows* dq,
+                                   const flstm_rows* dk, const flstm_rows* dv, float* d_state_in, void* workspace, void* stream);
 size_t flstm_decay_attention_workspace_bytes(const flstm_decay_attention* shape, int backward);
 /* One token of every sequence (shape->tokens and cu_seqlens are not read), the state updated in place. */
-int flstm_decay_attention_step(const flstm_decay_attention* shape, flstm_rows q, flstm_rows k, flstm_rows v, flstm_rows o,
-                               float* state, void* stream);
+int flstm_decay_attention_step(const flstm_decay_attention* shape, const flstm_rows* q, const flstm_rows* k, const flstm_rows* v,
+                               const flstm_rows* o, float* state, void* stream);
 
 /* ---- distillation from a teacher's top logits
  *
@@ -117,7 +117,7 @@ int flstm_distillation_forward(const flstm_distillation* problem, float* loss, f
 int flstm_distillation_backward(const flstm_distillation* problem, const float* stats, const float* d_loss, size_t d_stride,
                                 void* dlogits, size_t ldd, void* stream);
 /* Both in one call, for a d_loss known beforehand (a mean over rows, say): a row's logits are read from memory once, as
- * long as they fit a workgroup's registers (131072 of 16 bits, 65536 of fp32).  `workspace`:
+ * long as they fit a workgroup's registers (65536).  `workspace`:
  * flstm_distillation_workspace_bytes() bytes, 16-byte aligned (null where that is 0). */
 size_t flstm_distillation_workspace_bytes(const flstm_distillation* problem);
 int flstm_distillation_train(const flstm_distillation* problem, const float* d_loss, size_t d_stride, float* loss,

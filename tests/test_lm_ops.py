@@ -49,19 +49,17 @@ def test_layer_norm_refuses_host_tensors():
 def test_decay_attention_refuses_before_device_work():
     from flashlstm_poc_amd import lm_ops
     lib = lm_ops._bind()
-    rows = lambda data=SOME, token=64: lm_ops._Rows(data.value if data else None, 64 * 5, token, 32)
+    rows = lambda data=SOME, token=64: lm_ops._ROWS.pack(data.value if data else 0, 64 * 5, token, 32)
 
     def shape(**change):
-        s = lm_ops._DecayShape(2, 5, None, 2, 1, 32, 32, 1, 0.5, SOME.value)
-        for name, value in change.items():
-            setattr(s, name, value)
-        return ctypes.byref(s)
+        values = dict(sequences=2, tokens=5, cu_seqlens=0, heads=2, kv_heads=1, dk=32, dv=32, dtype=1, scale=0.5, log_decay=SOME.value)
+        return lm_ops._SHAPE.pack(*{**values, **change}.values())
 
     forward = lambda s=shape(), q=rows(), o=rows(): lib.flstm_decay_attention_forward(s, q, rows(), rows(), None, o, None, None, None)
     for change in (dict(dtype=3), dict(heads=0), dict(kv_heads=0), dict(heads=3, kv_heads=2), dict(dk=7), dict(dk=257), dict(dv=0), dict(dv=300),
-                   dict(scale=float("nan")), dict(log_decay=None)):
+                   dict(scale=float("nan")), dict(log_decay=0)):
         assert forward(shape(**change)) == 1, change
-    assert forward(q=rows(None)) == 1 and forward(q=rows(token=1 << 23)) == 2004
+    assert forward(q=rows(None)) == 1 and forward(q=None) == 1 and forward(o=rows(None)) == 1 and forward(q=rows(token=1 << 23)) == 2004
     assert lib.flstm_decay_attention_forward(None, rows(), rows(), rows(), None, rows(), None, None, None) == 1
     assert lib.flstm_decay_attention_forward(shape(tokens=1 << 20, heads=1), rows(), rows(), rows(), None, rows(), None, None, None) == 1   # no workspace
     assert lib.flstm_decay_attention_step(shape(), rows(), rows(), rows(), rows(), None, None) == 1
@@ -81,21 +79,20 @@ def test_distillation_refuses_before_device_work():
     lib = lm_ops._bind()
 
     def problem(**change):
-        p = lm_ops._Distillation(4, 100, SOME.value, 100, 1, 5, SOME.value, 0, SOME.value, 0, 1.0)
-        for name, value in change.items():
-            setattr(p, name, value)
-        return ctypes.byref(p)
+        values = dict(rows=4, vocabulary=100, logits=SOME.value, ld=100, dtype=1, top=5, teacher_logits=SOME.value, teacher_dtype=0,
+                      teacher_index=SOME.value, index_64=0, temperature=1.0)
+        return lm_ops._PROBLEM.pack(*{**values, **change}.values())
 
     for change in (dict(dtype=3), dict(teacher_dtype=-1), dict(top=0), dict(top=1025), dict(temperature=0.0), dict(temperature=float("nan")),
                    dict(temperature=float("inf")), dict(temperature=1e-40), dict(vocabulary=0), dict(vocabulary=1 << 31), dict(ld=99),
-                   dict(logits=None), dict(teacher_logits=None), dict(teacher_index=None)):
+                   dict(logits=0), dict(teacher_logits=0), dict(teacher_index=0)):
         assert lib.flstm_distillation_forward(problem(**change), SOME, None, None) == 1, change
     assert lib.flstm_distillation_forward(None, SOME, None, None) == 1 and lib.flstm_distillation_forward(problem(), None, None, None) == 1
     assert lib.flstm_distillation_backward(problem(), None, SOME, 1, SOME, 100, None) == 1
     assert lib.flstm_distillation_backward(problem(), SOME, SOME, 1, SOME, 99, None) == 1
     assert lib.flstm_distillation_train(problem(), SOME, 1, SOME, None, 100, None, None) == 1
     assert lib.flstm_distillation_train(problem(vocabulary=200000, ld=200000), SOME, 1, SOME, SOME, 200000, None, None) == 1   # no workspace
-    assert lib.flstm_distillation_forward(problem(rows=0, logits=None), None, None, None) == 0
+    assert lib.flstm_distillation_forward(problem(rows=0, logits=0), None, None, None) == 0
     assert lib.flstm_distillation_workspace_bytes(problem()) == 0
     assert lib.flstm_distillation_workspace_bytes(problem(vocabulary=200000, ld=200000)) == 32
 
