@@ -71,11 +71,8 @@ template <class T> __device__ __forceinline__ float8 beside(const T* z, const Cu
 
 // A pair of values over the workgroup, in all threads.
 template <int THREADS, class Op> __device__ __forceinline__ float2 all_threads(float2 v, float2* scratch, Op op) {
-#pragma unroll
-    for (int m = kWave / 2; m > 0; m /= 2) {
-        v.x = op(v.x, __shfl_xor(v.x, m, kWave));
-        v.y = op(v.y, __shfl_xor(v.y, m, kWave));
-    }
+    v.x = lanes_fold<kWave>(v.x, op);
+    v.y = lanes_fold<kWave>(v.y, op);
     __syncthreads();   // (the last one's readers are done)
     if (threadIdx.x % kWave == 0) scratch[threadIdx.x / kWave] = v;
     __syncthreads();

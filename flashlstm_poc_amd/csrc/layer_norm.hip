@@ -142,12 +142,15 @@ __global__ __launch_bounds__(L > kNormThreads ? L : kNormThreads) void norm_back
         const T* dt = a.d_total ? static_cast<const T*>(a.d_total) + row * a.lddt : nullptr;
         const float mean = a.mean[row], rstd = a.rstd[row];
         float8 h[V], n[V];
+        typename Vec8<T>::type more[V];   // of d_total, as it came: requested with the others, used at the end
         float sh = 0.f, shn = 0.f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const int c = (j * L + at) * 8;
             h[j] = load8(dy + c, a.width - c);
             n[j] = load8(total + c, a.width - c);
+            more[j] = T(0.f);
+            if (dt) more[j] = __builtin_convertvector(load8(dt + c, a.width - c), typename Vec8<T>::type);
         }
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -166,9 +169,7 @@ __global__ __launch_bounds__(L > kNormThreads ? L : kNormThreads) void norm_back
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const int c = (j * L + at) * 8;
-            float8 o = rstd * (h[j] - mh - n[j] * mhn);
-            if (dt) o += load8(dt + c, a.width - c);
-            store8(dx + c, o, a.width - c);
+            store8(dx + c, rstd * (h[j] - mh - n[j] * mhn) + __builtin_convertvector(more[j], float8), a.width - c);
         }
     }
     if constexpr (kParameters) {

@@ -67,16 +67,35 @@ template <class T> __device__ __forceinline__ void store8(T* p, float8 v, int n)
     }
 }
 
-// Sum over groups of `N` neighbouring lanes (a power of two up to a wave), in every lane.
-template <int N> __device__ __forceinline__ float lanes_sum(float v) {
-#pragma unroll
-    for (int m = N / 2; m > 0; m /= 2) v += __shfl_xor(v, m, kWave);
+// A value folded over groups of `N` neighbouring lanes (a power of two up to a wave), in every lane: lanes 1 and 2 apart, mirrored
+// halves of eight and of sixteen (each half holds one value by then), then rows of sixteen and of thirty-two exchanged.  Moves
+// inside the vector unit, a few clocks each, where a shuffle goes through LDS.
+template <int CTRL> __device__ __forceinline__ float lane_moved(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+template <int N, class Op> __device__ __forceinline__ float lanes_fold(float v, Op op) {
+    static_assert(N == 8 || N == 16 || N == 32 || N == 64, "whole groups of eight");
+    v = op(v, lane_moved<0xb1>(v));            // quad_perm 1, 0, 3, 2
+    v = op(v, lane_moved<0x4e>(v));            // quad_perm 2, 3, 0, 1
+    v = op(v, lane_moved<0x141>(v));           // row_half_mirror
+    if constexpr (N >= 16) v = op(v, lane_moved<0x140>(v));   // row_mirror
+    if constexpr (N >= 32) {
+        const unsigned u = __builtin_bit_cast(unsigned, v);
+        const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        v = op(__builtin_bit_cast(float, unsigned(r[0])), __builtin_bit_cast(float, unsigned(r[1])));
+    }
+    if constexpr (N >= 64) {
+        const unsigned u = __builtin_bit_cast(unsigned, v);
+        const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        v = op(__builtin_bit_cast(float, unsigned(r[0])), __builtin_bit_cast(float, unsigned(r[1])));
+    }
     return v;
 }
+template <int N> __device__ __forceinline__ float lanes_sum(float v) {
+    return lanes_fold<N>(v, [](float a, float b) { return a + b; });
+}
 template <int N> __device__ __forceinline__ float lanes_max(float v) {
-#pragma unroll
-    for (int m = N / 2; m > 0; m /= 2) v = fmaxf(v, __shfl_xor(v, m, kWave));
-    return v;
+    return lanes_fold<N>(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
 __host__ __device__ inline bool valid_dtype(int t) { return t == FLSTM_OP_F32 || t == FLSTM_OP_F16 || t == FLSTM_OP_BF16; }

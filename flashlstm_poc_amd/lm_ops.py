@@ -114,7 +114,7 @@ def layer_norm_forward(x, weight=None, bias=None, *, eps: float = 1e-5, residual
     rows_x = _rows(x)
     rows_r = None if residual is None else _rows(residual)
     rows = rows_x.shape[0]
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    y = torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, device=x.device, dtype=x.dtype)
     total = x if residual is None else torch.empty_like(y)
     mean, rstd = torch.empty((2, rows), device=x.device, dtype=torch.float32).unbind(0)
     _check(_bind().flstm_layer_norm_forward(rows, width, rows_x.data_ptr(), rows_x.stride(0), _ptr(rows_r),
@@ -338,7 +338,7 @@ def decay_attention_step(q, k, v, log_decay, state, *, scale: Optional[float] = 
         raise ValueError("state must be a tensor: it is updated in place")
     shape, states = _decay_shape(q, k, v, log_decay, scale, state, None, 3)
     q, k, v = (_last_axis_contiguous(t) for t in (q, k, v))
-    o = torch.empty((states[0], states[1], states[3]), device=q.device, dtype=q.dtype)
+    o = torch.empty_like(q) if states[2] == states[3] and q.is_contiguous() else torch.empty((states[0], states[1], states[3]), device=q.device, dtype=q.dtype)
     _check(_bind().flstm_decay_attention_step(shape, _rows_of(q), _rows_of(k), _rows_of(v), _rows_of(o), state.data_ptr(),
                                               _stream()), "flstm_decay_attention_step")
     return o
