@@ -252,15 +252,23 @@ template <class T> __device__ __forceinline__ float8 less(float8 w, typename Fra
     }
 }
 
-// The range of fp16: what becomes an operand is multiplied with a power of two that brings its largest magnitude in the wave to some
-// 2^13, where that lies outside [low, 2^15].  (bf16 and fp32 have a float's range.)
+// The range of fp16: what becomes an operand is multiplied with a power of two that brings its largest magnitude to some 2^13, where
+// that lies outside [low, 2^15].  (bf16 and fp32 have a float's range.)  Infinities and NaN do not count: they stay what they are,
+// and beside them the others have to keep their range.
+__device__ __forceinline__ bool in_range(float most, float low) { return most >= low && most <= 32768.f; }
 __device__ __forceinline__ float to_range(float most) {
     const int e = 14 - __builtin_amdgcn_frexp_expf(most);
     return most > 0.f ? uniform(ldexpf(1.f, e < -100 ? -100 : e > 100 ? 100 : e)) : 1.f;
 }
-__device__ __forceinline__ float range_scale(float most_of_lane, float low) {
-    if (!__any(most_of_lane > 32768.f) && __any(most_of_lane >= low)) return 1.f;
-    return to_range(lanes_max<kWave>(most_of_lane));
+__device__ __forceinline__ float finite_magnitude(float v) { return fabsf(v) < __builtin_inff() ? fabsf(v) : 0.f; }
+// The largest finite magnitude in the wave's state.
+template <int TILES> __device__ __forceinline__ float most_finite(const floatx16 (&x)[TILES]) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < TILES; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) m = fmaxf(m, finite_magnitude(x[i][r]));
+    return lanes_max<kWave>(m);
 }
 __device__ __forceinline__ float most_of(half8 v) {
     half8 m = __builtin_elementwise_abs(v);
@@ -472,8 +480,9 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
                 float most = 0.f;
 #pragma unroll
                 for (int i = 0; i < kTiles; ++i) most = fmaxf(most, most8({half_of(x[i], 0), half_of(x[i], 1)}));
-                const float r = range_scale(most, 0x1p-8f);
-                if (r != 1.f) {
+                if (__any(most > 32768.f) || !__any(most >= 0x1p-8f)) {
+                    most = most_finite(x);
+                    const float r = in_range(most, 0x1p-8f) ? 1.f : to_range(most);
                     x_scale *= r;
 #pragma unroll
                     for (int i = 0; i < kTiles; ++i) x[i] *= r;
@@ -548,10 +557,17 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
                     float most = 0.f;
 #pragma unroll
                     for (int j = 0; j < 2 * (tb + 1); ++j) most = fmaxf(most, most8({w[j]}));
-                    w_scale = range_scale(most, 0x1p-8f);
-                    if (w_scale != 1.f)
+                    if (__any(most > 32768.f) || !__any(most >= 0x1p-8f)) {
+                        most = 0.f;   // (behind the diagonal there are zeros, or where a score was infinite NaN, which do not count)
+#pragma unroll
+                        for (int j = 0; j < 2 * (tb + 1); ++j)
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) most = fmaxf(most, finite_magnitude(w[j][i]));
+                        most = lanes_max<kWave>(most);
+                        w_scale = in_range(most, 0x1p-8f) ? 1.f : to_range(most);
 #pragma unroll
                         for (int j = 0; j < 2 * (tb + 1); ++j) w[j] *= w_scale;
+                    }
                 }
                 o[tb] *= factor_a * power(l, float(t < 0 ? 0 : t) + lead) * (w_scale / x_scale);
 #pragma unroll
@@ -591,11 +607,14 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
             for (int kk = 0; kk < kTokens / 16; ++kk) most = fmaxf(most, most_of(values[kk]) * power(l, float(kTokens - 16 - 16 * kk)));
             most *= fabsf(factor_c) * x_scale;
             if (__any(most > 32768.f) || !__any(most >= 0x1p-3f)) {
-                float held = 0.f;
+                most = 0.f;
 #pragma unroll
-                for (int i = 0; i < kTiles; ++i) held = fmaxf(held, most8({half_of(x[i], 0), half_of(x[i], 1)}));
-                most = lanes_max<kWave>(most);
-                const float larger = fmaxf(most, lanes_max<kWave>(held) * keep);
+                for (int kk = 0; kk < kTokens / 16; ++kk)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        most = fmaxf(most, finite_magnitude(float(values[kk][j])) * power(l, float(kTokens - 16 - 16 * kk)));
+                most = lanes_max<kWave>(most) * fabsf(factor_c) * x_scale;
+                const float larger = fmaxf(most, most_finite(x) * keep);
                 if (most > 32768.f || larger < 0x1p-3f) {
                     const float r = to_range(larger);
                     x_scale *= r;

@@ -212,6 +212,24 @@ def test_nan_and_infinity_reach_later_tokens_alone(dtype):
     assert bool(torch.isfinite(o[clean]).all()) and not bool(torch.isfinite(o[0, 10, 0]).any())
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_an_infinite_value_leaves_the_others_their_range(dtype):
+    p = _problem(1, 150, dtype=dtype, dk=32, dv=48, train=False)
+    p["q"][0, 20, 1] *= 1000                                    # (a row whose scores fp16 holds scaled alone)
+    want, most = _definition(p), _definition(p, magnitudes=True)
+    bad = dict(p, q=p["q"].clone())
+    bad["q"][0, 10, 0, 2], bad["q"][0, 70, 1, 3] = float("inf"), float("-inf")
+    o = _own(bad)["o"]
+    clean = torch.ones(want["o"].shape, dtype=torch.bool, device="cuda")
+    clean[0, 10, 0] = clean[0, 70, 1] = False
+    unit = UNIT[dtype] if dtype != torch.float32 else 0.0
+    # (fp16: the scores of a chunk share a power of two; the smallest that it leaves, 2^-25 of a largest of 2^13, is far below the
+    # rounding of the row that decides it)
+    slack = (1.05 * unit + 64 * U32) * most["o"] + (2.0 ** -38 * most["o"].amax() if dtype == torch.float16 else 0.0)
+    assert_within(torch.where(clean, o, torch.zeros_like(o)), torch.where(clean, want["o"], 0.0), slack, "o")
+    assert not bool(torch.isfinite(o[0, 10, 0]).any()) and not bool(torch.isfinite(o[0, 70, 1]).any())
+
+
 def test_strides_and_alignment():
     for dtype in DTYPES:
         p = _problem(3, 70, heads=4, kv_heads=2, dk=40, dv=24, dtype=dtype)
