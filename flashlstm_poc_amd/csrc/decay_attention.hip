@@ -7,11 +7,18 @@
 //     dq_t = scale S_t do_t:  the sweep of (do, v, k) with the transposed state;
 //     dv_s = A_s^T k_s, dk_s = A_s v_s:  the sweeps of (k, q, do) and (v, do, q) from the last token to the first.
 //
-// A workgroup holds X of one head in its accumulators for a whole run of tokens, so that a token's rows are read once and its
-// output written once and nothing else leaves the chip: the sweep is bound by memory.  Each wave has 32 columns of X and forms
-// the scores of a chunk for itself: four times the products, which are a fraction of the time that the rows take to arrive, and
-// no exchange of them.  The layouts are chosen so that no accumulator passes through LDS: in every product below the operand
-// that was an accumulator before has its contraction index where the accumulator rows lie (see `perm`).
+// A workgroup holds X of one head (128 columns of it at most) in its accumulators for a whole run of tokens, so that a token's rows
+// are read once, its output written once, and nothing else leaves the chip.  Each wave has 32 columns of X and forms the scores of
+// a chunk for itself: four times these products, and no exchange.  (Shared out through LDS, in tiles of 16 x 16 and with a third
+// barrier a chunk, they took the same time for heads of 128, 13 to 17 % more for heads of 64 and 6 % less for fp32.)  The layouts
+// are chosen so that no accumulator passes through LDS: in every product below the operand that was an accumulator before has its
+// contraction index where the accumulator rows lie (see `perm`).
+//
+// What bounds it is the chain of a chunk, not one unit: the next rows are requested under the products, written to LDS between two
+// barriers, multiplied, weighted, multiplied again.  A workgroup alone on its CU takes 8700 clocks for a chunk of 64 tokens of a
+// head of 128 x 128 (staging 1500, products with rows and state 2100, weights and outputs 1800, requests 1100, the state 1750; 2500
+// to 3000 of them MFMA), each of two 11900.  Measured, bf16 but for the second: 16 x 2048 tokens of 16 heads of 128 forward 175 us
+// (3.1 TB/s of rows), their gradients 400; 131072 tokens of 8 heads, fp16, 425; a copy reaches 5.1 TB/s.
 #include "lm_device.h"
 
 namespace flstm_hip {
@@ -734,7 +741,8 @@ template <class T> __global__ __launch_bounds__(256) void fold_kernel(Fold f) {
     }
 }
 
-// ---- single tokens: bound by reading and writing the state once.  A workgroup has 64 columns of one state (a thread four of them, of every 16th row).
+// ---- single tokens: bound by reading and writing the state once (256 sequences of 16 heads of 128 x 128: 105 us, 5.1 TB/s, the rate
+// of a copy).  A workgroup has 64 columns of one state, a thread four of them of every 16th row.
 struct Step {
     Role q, k, v, out;
     int heads, d, e;
@@ -839,7 +847,9 @@ size_t states_bytes(const flstm_decay_attention* p, bool backward) {
     return split ? round_up(slots * p->heads * size_t(p->dk) * p->dv * sizeof(float), 256) : 0;
 }
 // Whether a chunk's rows lie within 32-bit offsets.
-bool reachable(const flstm_rows& r) { return r.token < (ptrdiff_t(1) << 23) && r.token > -(ptrdiff_t(1) << 23); }
+bool reachable(const flstm_decay_attention* p, const flstm_rows& r) {
+    return p->tokens <= 1 || (r.token < (ptrdiff_t(1) << 23) && r.token > -(ptrdiff_t(1) << 23));
+}
 
 size_t rows_of(const flstm_decay_attention* p) { return p->cu_seqlens ? p->tokens : p->sequences * p->tokens; }
 size_t shares_bytes(const flstm_decay_attention* p, int width) {
@@ -928,7 +938,7 @@ extern "C" int flstm_decay_attention_forward(const flstm_decay_attention* p, con
     const flstm_rows q = or_none(q_), k = or_none(k_), v = or_none(v_), o = or_none(o_);
     if (rows_of(p) > 0 && (!q.data || !k.data || !v.data || !o.data)) return FLSTM_E_INVALID;
     if (states_bytes(p, false) > 0 && !workspace) return FLSTM_E_INVALID;
-    if (!reachable(q) || !reachable(k) || !reachable(v)) return FLSTM_E_TOO_LARGE;
+    if (!reachable(p, q) || !reachable(p, k) || !reachable(p, v)) return FLSTM_E_TOO_LARGE;
     if (p->sequences == 0 && !p->cu_seqlens) return 0;
     hipStream_t stream_ = static_cast<hipStream_t>(stream);
     const int group = p->heads / p->kv_heads;
@@ -955,7 +965,7 @@ extern "C" int flstm_decay_attention_backward(const flstm_decay_attention* p, co
     const flstm_rows d_o = or_none(d_o_), q = or_none(q_), k = or_none(k_), v = or_none(v_), dq = or_none(dq_), dk = or_none(dk_), dv = or_none(dv_);
     if (rows_of(p) > 0 && (!d_o.data || !q.data || !k.data || !v.data)) return FLSTM_E_INVALID;
     if (flstm_decay_attention_workspace_bytes(p, 1) > 0 && !workspace) return FLSTM_E_INVALID;
-    if (!reachable(d_o) || !reachable(q) || !reachable(k) || !reachable(v)) return FLSTM_E_TOO_LARGE;
+    if (!reachable(p, d_o) || !reachable(p, q) || !reachable(p, k) || !reachable(p, v)) return FLSTM_E_TOO_LARGE;
     if (p->sequences == 0 && !p->cu_seqlens) return 0;
     hipStream_t stream_ = static_cast<hipStream_t>(stream);
     const int group = p->heads / p->kv_heads;

@@ -12,6 +12,7 @@ import struct
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .core import load_library
 
@@ -170,6 +171,7 @@ class _LayerNormFunction(torch.autograd.Function):
         return (y, total) if residual is not None else (y, None)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, d_total):
         total, weight, mean, rstd = ctx.saved_tensors
         if dy is None:
@@ -354,6 +356,7 @@ class _DecayAttentionFunction(torch.autograd.Function):
         return o, final
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, do, d_final):
         q, k, v, state, log_decay, cu_seqlens = ctx.saved_tensors
         if do is None:
@@ -473,6 +476,7 @@ class _DistillationFunction(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_loss):
         logits, teacher_logits, teacher_index, stats = ctx.saved_tensors
         return distillation_backward(d_loss, logits, teacher_logits, teacher_index, stats, temperature=ctx.temperature), None, None, None

@@ -268,6 +268,12 @@ def test_offsets_beyond_32_bits():
             assert torch.equal(want[key], got[key]), (name, key)
 
 
+def test_a_single_token_of_any_stride():
+    p = _problem(3, 1, heads=2, kv_heads=1, dk=32, dv=32, train=False)
+    wide = {name: p[name].as_strided(p[name].shape, (p[name].stride(0), 1 << 24, *p[name].stride()[2:])) for name in ("q", "k", "v")}
+    assert torch.equal(_own(dict(p, **wide))["o"], _own(p)["o"])
+
+
 def test_a_sequence_in_pieces_and_token_by_token():
     for dtype in DTYPES:
         p = _problem(3, 150, heads=4, kv_heads=2, dk=72, dv=100, dtype=dtype, train=False)
