@@ -47,7 +47,7 @@ __device__ __forceinline__ float8 share8(float8 z, float most, float log_sum, fl
 
 // A row as its workgroup takes it: whole vectors of eight from a 16-byte boundary of `at` on, what is left in front of them with the
 // first thread and what is left behind with the last.  (Rows of a vocabulary that is a multiple of nothing begin anywhere; read and
-// written as they lie, 8192 of 50001 bf16 logits take 424 us instead of 376.)
+// written as they lie, 8192 of 50001 bf16 logits take 424 us instead of 388.)
 struct Cut {
     int whole;        // vectors
     int head;         // elements in front of them

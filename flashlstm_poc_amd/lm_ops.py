@@ -66,6 +66,18 @@ def _device_tensor(name: str, t, dtype=None) -> int:
     return code
 
 
+def _all_here(dtype, *tensors) -> bool:
+    """Whether all are tensors of `dtype` on the current device: the common case, asked at once."""
+    try:
+        index = tensors[0].get_device()   # -1 of a host tensor
+        for t in tensors:
+            if t.get_device() != index or t.dtype is not dtype:
+                return False
+    except AttributeError:   # no tensor
+        return False
+    return index >= 0 and index == torch._C._cuda_getDevice()
+
+
 def _stream() -> int:
     """The current stream of the current device (torch.cuda.current_stream().cuda_stream without the object around it: 2 us less)."""
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
@@ -86,8 +98,9 @@ def _rows(t):
 
 def _check_parameter(name: str, t, width: int) -> None:
     if t is not None:
-        _device_tensor(name, t, torch.float32)
-        if tuple(t.shape) != (width,) or not t.is_contiguous():
+        if not _all_here(torch.float32, t):
+            _device_tensor(name, t, torch.float32)
+        if t.shape != (width,) or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous tensor of shape ({width},)")
 
 
@@ -98,12 +111,13 @@ def layer_norm_forward(x, weight=None, bias=None, *, eps: float = 1e-5, residual
     Returns (y, total, mean, rstd): y and total of x's shape and type, mean and rstd (rows,) float32, which
     layer_norm_backward takes."""
     code = _device_tensor("x", x)
-    if x.dim() < 1:
+    shape = x.shape
+    if not shape:
         raise ValueError("x must have a last axis to normalise over")
-    width = x.shape[-1]
+    width = shape[-1]
     if residual is not None:
         _device_tensor("residual", residual, x.dtype)
-        if residual.shape != x.shape:
+        if residual.shape != shape:
             raise ValueError(f"residual must have x's shape {tuple(x.shape)}, not {tuple(residual.shape)}")
     _check_parameter("weight", weight, width)
     _check_parameter("bias", bias, width)
@@ -230,23 +244,26 @@ def _last_axis_contiguous(t):
 
 def _decay_shape(q, k, v, log_decay, scale, state, cu_seqlens, axes: int):
     """Checks q (.., heads, dk), k (.., kv_heads, dk) and v (.., kv_heads, dv) of `axes` axes, and what goes with them."""
-    code = _device_tensor("q", q)
-    if q.dim() != axes:
-        raise ValueError(f"q must have {axes} axes, not {q.dim()}")
-    for name, t in (("k", k), ("v", v)):
-        _device_tensor(name, t, q.dtype)
-        if t.dim() != axes or t.shape[:-2] != q.shape[:-2]:
-            raise ValueError(f"{name} must have q's leading axes {tuple(q.shape[:-2])}: got {tuple(t.shape)}")
-    heads, dk = q.shape[-2:]
-    kv_heads, dv = v.shape[-2:]
-    if tuple(k.shape[-2:]) != (kv_heads, dk):
-        raise ValueError(f"k must have v's heads and q's width ({kv_heads}, {dk}): got {tuple(k.shape[-2:])}")
+    if not (_all_here(torch.float32, log_decay) and isinstance(q, torch.Tensor) and q.dtype in _DTYPES and _all_here(q.dtype, q, k, v)):
+        _device_tensor("q", q)
+        for name, t in (("k", k), ("v", v)):
+            _device_tensor(name, t, q.dtype)
+        _device_tensor("log_decay", log_decay, torch.float32)
+    code, of_q, of_k, of_v = _DTYPES[q.dtype], q.shape, k.shape, v.shape
+    if len(of_q) != axes:
+        raise ValueError(f"q must have {axes} axes, not {len(of_q)}")
+    heads, dk = of_q[-2:]
+    for name, shape in (("k", of_k), ("v", of_v)):
+        if len(shape) != axes or shape[:-2] != of_q[:-2]:
+            raise ValueError(f"{name} must have q's leading axes {tuple(of_q[:-2])}: got {tuple(shape)}")
+    kv_heads, dv = of_v[-2:]
+    if of_k[-2:] != (kv_heads, dk):
+        raise ValueError(f"k must have v's heads and q's width ({kv_heads}, {dk}): got {tuple(of_k[-2:])}")
     if kv_heads < 1 or heads < 1 or heads % kv_heads != 0:
         raise ValueError(f"the number of query heads ({heads}) must be a multiple of that of key and value heads ({kv_heads})")
     if not (8 <= dk <= 256 and 8 <= dv <= 256):
         raise ValueError(f"head widths must lie in 8 .. 256: got {dk} and {dv}")
-    _device_tensor("log_decay", log_decay, torch.float32)
-    if tuple(log_decay.shape) != (heads,) or not log_decay.is_contiguous():
+    if log_decay.shape != (heads,) or not log_decay.is_contiguous():
         raise ValueError(f"log_decay must be a contiguous tensor of shape ({heads},)")
     if log_decay.requires_grad:
         raise ValueError("log_decay is a constant of the model: it has no gradient")
@@ -257,9 +274,9 @@ def _decay_shape(q, k, v, log_decay, scale, state, cu_seqlens, axes: int):
         _device_tensor_int("cu_seqlens", cu_seqlens)
         if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1 or not cu_seqlens.is_contiguous():
             raise ValueError("cu_seqlens must be a contiguous tensor of one more entry than there are sequences")
-        sequences, tokens = cu_seqlens.shape[0] - 1, q.shape[0]
+        sequences, tokens = cu_seqlens.shape[0] - 1, of_q[0]
     else:
-        sequences, tokens = q.shape[0], q.shape[1] if axes == 4 else 1
+        sequences, tokens = of_q[0], of_q[1] if axes == 4 else 1
     shape = _SHAPE.pack(sequences, tokens, _ptr(cu_seqlens) or 0, heads, kv_heads, dk, dv, code, scale, log_decay.data_ptr())
     _check_state("state", state, (sequences, heads, dk, dv))
     return shape, (sequences, heads, dk, dv)
@@ -274,8 +291,9 @@ def _device_tensor_int(name: str, t) -> None:
 
 def _check_state(name: str, t, shape) -> None:
     if t is not None:
-        _device_tensor(name, t, torch.float32)
-        if tuple(t.shape) != shape or not t.is_contiguous():
+        if not _all_here(torch.float32, t):
+            _device_tensor(name, t, torch.float32)
+        if t.shape != shape or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous tensor of shape {shape}")
 
 
