@@ -731,13 +731,15 @@ struct Fold {
 
 template <class T> __global__ __launch_bounds__(256) void fold_kernel(Fold f) {
     const int kv = f.heads / f.group;
-    const size_t row = blockIdx.x, n = row / f.tokens, t = row % f.tokens;
-    for (int i = threadIdx.x; i < kv * f.width; i += 256) {
-        const int h = i / f.width, c = i % f.width;
-        const float* in = f.in + (row * f.heads + size_t(h) * f.group) * f.width + c;
-        float v = 0.f;
-        for (int g = 0; g < f.group; ++g) v += in[size_t(g) * f.width];
-        static_cast<T*>(f.out.data)[ptrdiff_t(n) * f.out.sequence + ptrdiff_t(t) * f.out.token + h * f.out.head + c] = T(v);
+    for (size_t row = blockIdx.x; row < f.sequences * f.tokens; row += gridDim.x) {
+        const size_t n = row / f.tokens, t = row % f.tokens;
+        for (int i = threadIdx.x; i < kv * f.width; i += 256) {
+            const int h = i / f.width, c = i % f.width;
+            const float* in = f.in + (row * f.heads + size_t(h) * f.group) * f.width + c;
+            float v = 0.f;
+            for (int g = 0; g < f.group; ++g) v += in[size_t(g) * f.width];
+            static_cast<T*>(f.out.data)[ptrdiff_t(n) * f.out.sequence + ptrdiff_t(t) * f.out.token + h * f.out.head + c] = T(v);
+        }
     }
 }
 
@@ -804,6 +806,7 @@ template <class T> __global__ __launch_bounds__(256) void step_kernel(Step s) {
 
 // ---- host side
 
+constexpr size_t kMaxThreads = 0xffffffffu;   // along one axis of a launch
 constexpr size_t kWhole = size_t(1) << 41;   // a segment that holds any sequence
 
 int padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
@@ -872,7 +875,7 @@ template <class T, int D, int WAVES, bool kOut> int launch_sweeps(Sweeps a, hipS
     a.column_blocks = int(ceil_div(size_t(widest), WAVES * 32));
     const size_t grid = a.slots * size_t(a.heads) * a.column_blocks * a.count;
     if (grid == 0) return 0;
-    if (grid >= (size_t(1) << 31)) return FLSTM_E_TOO_LARGE;
+    if (grid > kMaxThreads / (WAVES * 64)) return FLSTM_E_TOO_LARGE;
     constexpr int lds = Tile<T, D>::kBytes * (kOut ? 2 : 1) + Tile<T, WAVES * 32>::kBytes + (kOut ? kWave * (4 * 16 + 2 * 8 * int(sizeof(T))) : 0);
     const auto kernel = sweep_kernel<T, D, WAVES, kOut>;
     if (lds > 65536) {
@@ -1017,13 +1020,12 @@ extern "C" int flstm_decay_attention_backward(const flstm_decay_attention* p, co
         rc = run_sweeps(a, p->dtype, false, stream_);
     }
     if (rc != 0 || group == 1 || rows_of(p) == 0) return rc;
-    if (rows_of(p) >= (size_t(1) << 31)) return FLSTM_E_TOO_LARGE;
     const auto fold = [&](const flstm_rows& r, char* shares, int width) {
         if (!r.data) return 0;
         const size_t rows = rows_of(p), tokens = p->cu_seqlens ? rows : p->tokens;
         const Fold f{reinterpret_cast<const float*>(shares), role(r, 1), rows / tokens, tokens, p->heads, group, width};
         return with_type(p->dtype, [&](auto zero) {
-            fold_kernel<decltype(zero)><<<unsigned(rows), 256, 0, stream_>>>(f);
+            fold_kernel<decltype(zero)><<<unsigned(rows < (1u << 20) ? rows : (1u << 20)), 256, 0, stream_>>>(f);
             return launched();
         });
     };
@@ -1038,7 +1040,7 @@ extern "C" int flstm_decay_attention_step(const flstm_decay_attention* p, const 
     const flstm_rows q = or_none(q_), k = or_none(k_), v = or_none(v_), o = or_none(o_);
     if (!q.data || !k.data || !v.data || !o.data || !state) return FLSTM_E_INVALID;
     const size_t grid = p->sequences * size_t(p->heads);
-    if (grid >= (size_t(1) << 31)) return FLSTM_E_TOO_LARGE;
+    if (grid > kMaxThreads / 256) return FLSTM_E_TOO_LARGE;
     const int group = p->heads / p->kv_heads;
     const Step s{role(q, 1), role(k, group), role(v, group), role(o, 1), p->heads, p->dk, p->dv, p->scale, p->log_decay, state};
     return with_type(p->dtype, [&](auto zero) {

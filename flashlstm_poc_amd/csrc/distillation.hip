@@ -20,7 +20,7 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -3.4028234663852886e38f;   // starts a maximum: finite, so that differences to it are numbers
 
 struct Distill {
-    size_t rows, ld, ldd, d_stride;
+    size_t first, ld, ldd, d_stride;   // first: the launch's first row
     const void *logits, *teacher_logits, *teacher_index;
     void* dlogits;
     const float* d_loss;
@@ -159,7 +159,7 @@ __device__ __forceinline__ void write_entries(const Distill& a, size_t row, cons
 template <class T, int THREADS> __global__ __launch_bounds__(THREADS) void loss_kernel(Distill a) {
     __shared__ Teacher teacher;
     __shared__ float2 scratch[THREADS / kWave];
-    const size_t row = blockIdx.x;
+    const size_t row = a.first + blockIdx.x;
     const T* z = static_cast<const T*>(a.logits) + row * a.ld;
     // running maximum and sum, several vectors at a time
     const Cut cut = cut_row<T, THREADS>(z, a.vocabulary);
@@ -204,7 +204,7 @@ template <class T> __global__ __launch_bounds__(kGradientThreads) void gradient_
     __shared__ Teacher teacher;
     __shared__ float2 scratch[THREADS / kWave];
     const unsigned blocks = unsigned((a.vocabulary + kGradientColumns - 1) / kGradientColumns);
-    const size_t row = blockIdx.x / blocks;
+    const size_t row = a.first + blockIdx.x / blocks;
     const int begin = int(blockIdx.x % blocks) * kGradientColumns;
     const int end = a.vocabulary - begin < kGradientColumns ? a.vocabulary : begin + kGradientColumns;
     const T* z = static_cast<const T*>(a.logits) + row * a.ld;
@@ -241,7 +241,7 @@ template <class T> __global__ __launch_bounds__(kGradientThreads) void gradient_
 template <class T, int THREADS, int R> __global__ __launch_bounds__(THREADS) void train_kernel(Distill a) {
     __shared__ Teacher teacher;
     __shared__ float2 scratch[THREADS / kWave];
-    const size_t row = blockIdx.x;
+    const size_t row = a.first + blockIdx.x;
     const T* z = static_cast<const T*>(a.logits) + row * a.ld;
     T* out = static_cast<T*>(a.dlogits) + row * a.ldd;
     typedef typename Vec8<T>::type vec;
@@ -302,7 +302,7 @@ bool valid_problem(const flstm_distillation* p) {
 
 Distill distill_of(const flstm_distillation* p) {
     Distill a{};
-    a.rows = p->rows; a.ld = p->ld; a.logits = p->logits; a.teacher_logits = p->teacher_logits; a.teacher_index = p->teacher_index;
+    a.ld = p->ld; a.logits = p->logits; a.teacher_logits = p->teacher_logits; a.teacher_index = p->teacher_index;
     a.vocabulary = int(p->vocabulary); a.top = p->top; a.teacher_dtype = p->teacher_dtype; a.index_64 = p->index_64;
     a.temperature = p->temperature; a.to_log2 = kLog2e / p->temperature;
     return a;
@@ -313,6 +313,15 @@ Distill distill_of(const flstm_distillation* p) {
 // logits take 366 us (4.5 TB/s), where one of 1024 threads took 472.  (100000 of them with 16 vectors a thread of 1024, alone on
 // its CU, took 457 us for 4096 rows: no less than the two passes that read the logits twice.)
 constexpr size_t kHeld = 65536;
+
+// Launches `go(problem, rows)` for so many rows at a time that a launch stays below its limit of 2^32 threads: of at most 1024 for
+// each of `workgroups` a row.
+template <class F> int in_launches(Distill a, size_t rows, size_t workgroups, F&& go) {
+    const size_t most = (size_t(1) << 21) / workgroups;
+    for (a.first = 0; a.first < rows; a.first += most)
+        if (const int rc = go(a, unsigned(rows - a.first < most ? rows - a.first : most))) return rc;
+    return 0;
+}
 
 }  // namespace
 }  // namespace flstm_hip
@@ -328,9 +337,11 @@ extern "C" int flstm_distillation_forward(const flstm_distillation* p, float* lo
         typedef decltype(zero) T;
         // (256 threads a row where the rows fill the chip, so that eight of them are under way in a CU: 1024 rows of 32000 bf16 16 us
         // instead of 20, 2048 of fp16 26 instead of 35; 1024 threads where they do not.)
-        if (p->vocabulary <= 8192 || p->rows >= 256) loss_kernel<T, 256><<<unsigned(p->rows), 256, 0, static_cast<hipStream_t>(stream)>>>(a);
-        else loss_kernel<T, 1024><<<unsigned(p->rows), 1024, 0, static_cast<hipStream_t>(stream)>>>(a);
-        return launched();
+        return in_launches(a, p->rows, 1, [&](const Distill& part, unsigned rows) {
+            if (p->vocabulary <= 8192 || p->rows >= 256) loss_kernel<T, 256><<<rows, 256, 0, static_cast<hipStream_t>(stream)>>>(part);
+            else loss_kernel<T, 1024><<<rows, 1024, 0, static_cast<hipStream_t>(stream)>>>(part);
+            return launched();
+        });
     });
 }
 
@@ -340,11 +351,12 @@ extern "C" int flstm_distillation_backward(const flstm_distillation* p, const fl
     if (p->rows == 0) return 0;
     Distill a = distill_of(p);
     a.stats = reinterpret_cast<float2*>(const_cast<float*>(stats)); a.d_loss = d_loss; a.d_stride = d_stride; a.dlogits = dlogits; a.ldd = ldd;
-    const size_t grid = p->rows * ceil_div(p->vocabulary, size_t(kGradientColumns));
-    if (grid >= (size_t(1) << 31)) return FLSTM_E_TOO_LARGE;
+    const unsigned blocks = unsigned(ceil_div(p->vocabulary, size_t(kGradientColumns)));
     return with_type(p->dtype, [&](auto zero) {
-        gradient_kernel<decltype(zero)><<<unsigned(grid), kGradientThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
-        return launched();
+        return in_launches(a, p->rows, blocks, [&](const Distill& part, unsigned rows) {
+            gradient_kernel<decltype(zero)><<<rows * blocks, kGradientThreads, 0, static_cast<hipStream_t>(stream)>>>(part);
+            return launched();
+        });
     });
 }
 
@@ -366,9 +378,10 @@ extern "C" int flstm_distillation_train(const flstm_distillation* p, const float
     return with_type(p->dtype, [&](auto zero) {
         typedef decltype(zero) T;
         const auto go = [&](auto threads, auto vectors) {
-            train_kernel<T, decltype(threads)::value, decltype(vectors)::value>
-                <<<unsigned(p->rows), threads.value, 0, static_cast<hipStream_t>(stream)>>>(a);
-            return launched();
+            return in_launches(a, p->rows, 1, [&](const Distill& part, unsigned rows) {
+                train_kernel<T, decltype(threads)::value, decltype(vectors)::value><<<rows, threads.value, 0, static_cast<hipStream_t>(stream)>>>(part);
+                return launched();
+            });
         };
         const std::integral_constant<int, 256> few;
         const std::integral_constant<int, 512> some;

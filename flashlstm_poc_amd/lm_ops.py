@@ -83,6 +83,12 @@ def _stream() -> int:
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
+def _written(t) -> None:
+    """Tells autograd that `t` was changed in place, so that a backward pass which needs its old values refuses."""
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+
+
 def _ptr(t) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
@@ -361,6 +367,7 @@ def decay_attention_step(q, k, v, log_decay, state, *, scale: Optional[float] = 
     o = torch.empty_like(q) if states[2] == states[3] and q.is_contiguous() else torch.empty((states[0], states[1], states[3]), device=q.device, dtype=q.dtype)
     _check(_bind().flstm_decay_attention_step(shape, _rows_of(q), _rows_of(k), _rows_of(v), _rows_of(o), state.data_ptr(),
                                               _stream()), "flstm_decay_attention_step")
+    _written(state)
     return o
 
 
@@ -482,6 +489,8 @@ def distillation_train(logits, teacher_logits, teacher_index, d_loss, *, tempera
     _check(lib.flstm_distillation_train(problem, d_loss.data_ptr(), d_loss.stride(0) if rows else 0, loss.data_ptr(),
                                         dlogits.data_ptr(), ld if in_place else vocabulary, _ptr(workspace), _stream()),
            "flstm_distillation_train")
+    if in_place:
+        _written(logits)
     return loss, dlogits
 
 

@@ -55,8 +55,10 @@ int flstm_layer_norm_backward(size_t rows, size_t width, const void* dy, size_t 
  * A tensor's element (sequence, token, head, i) lies at data + sequence * .sequence + token * .token + head * .head + i elements.
  * With cu_seqlens (sequences + 1 int32 on the device) sequences are packed along the token axis: sequence n is tokens
  * [cu_seqlens[n], cu_seqlens[n + 1]) of `tokens` in all, and .sequence is not used.  A tensor's tokens may be any distance apart up to 2^23 elements
- * (FLSTM_E_TOO_LARGE beyond).  Bounds are clamped to 0 .. tokens and to
- * ascending order; tokens in no sequence get zeros.  An empty sequence's final state is its initial one. */
+ * (FLSTM_E_TOO_LARGE beyond; from 2^21 pairs of a sequence and a head on it may also be the answer, where their workgroups are
+ * more than a launch can have).  cu_seqlens must ascend from 0.  Bounds are clamped to 0 .. tokens, so that nothing
+ * outside the tensors is touched whatever they are, but where they do not ascend outputs are not specified.  Tokens behind the last
+ * bound get zeros.  An empty sequence's final state is its initial one. */
 typedef struct {
     void* data;
     ptrdiff_t sequence, token, head;

@@ -405,6 +405,36 @@ def test_other_streams_and_graphs():
         assert torch.equal(step, fl.decay_attention_step(p["q"][:, 0], p["k"][:, 0], p["v"][:, 0], p["log_decay"], again)) and torch.equal(state, again)
 
 
+def test_more_tokens_than_a_launch_has_rows():
+    """The shares of heads are summed for 2^20 tokens at a time.  (Sequences of one token each: their recurrence is a product.)"""
+    sequences, heads, width, scale = 2 ** 20 + 5, 2, 8, 0.5
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v, do = (torch.randn(sequences, 1, n, width, device="cuda", generator=g).to(torch.bfloat16) for n in (heads, 1, 1, heads))
+    decay = torch.tensor([-0.5, -0.25], device="cuda")
+    dq, dk, dv, _ = fl.decay_attention_backward(do, q, k, v, decay, scale=scale, want=(True, True, True, False))
+    q64, k64, v64, do64 = (t.double() for t in (q, k, v, do))
+    slack = lambda most: (1.05 * UNIT[torch.bfloat16] + 64 * U32) * most
+    dot = lambda a, b: (a * b).sum(-1, keepdim=True)
+    for got, want, most, name in (
+            (dq, scale * dot(do64, v64) * k64, scale * dot(do64.abs(), v64.abs()) * k64.abs(), "dq"),
+            (dk, (scale * dot(do64, v64) * q64).sum(2, True), (scale * dot(do64.abs(), v64.abs()) * q64.abs()).sum(2, True), "dk"),
+            (dv, (scale * dot(q64, k64) * do64).sum(2, True), (scale * dot(q64.abs(), k64.abs()) * do64.abs()).sum(2, True), "dv")):
+        assert_within(got, want, slack(most), name)
+
+
+def test_a_step_is_known_to_autograd():
+    p = _problem(2, 1, train=False, dtype=torch.float32)
+    state = (p["state"].requires_grad_() * 1.0)
+    square = state * state
+    fl.decay_attention_step(p["q"][:, 0], p["k"][:, 0], p["v"][:, 0], p["log_decay"], state.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        square.sum().backward()
+    with torch.inference_mode():
+        held = torch.zeros_like(p["state"])
+    fl.decay_attention_step(p["q"][:, 0], p["k"][:, 0], p["v"][:, 0], p["log_decay"], held)   # (such a tensor has no version)
+    assert bool(held.any())
+
+
 def test_refusals():
     p = _problem(2, 10, heads=4, kv_heads=2, dk=32, dv=32)
     q, k, v, g, s = p["q"], p["k"], p["v"], p["log_decay"], p["state"]

@@ -267,3 +267,19 @@ def test_refusals():
         fl.distillation_train(z, t, i, d.half())
     with pytest.raises(ValueError, match="stats"):
         fl.distillation_backward(d, z, t, i, stats[:2])
+
+
+def test_more_rows_than_a_launch_has():
+    """Rows are launched at most 2^21 at a time."""
+    p = _problem(2 ** 21 + 3, 5, 3, torch.bfloat16, distinct=False)
+    _check(p, _own(p))
+
+
+def test_in_place_is_known_to_autograd():
+    p = _problem(4, 100, 8, torch.float32)
+    logits = p["logits"].requires_grad_()
+    kept = logits * 1.0
+    square = kept * kept
+    fl.distillation_train(kept.detach(), p["teacher_logits"], p["teacher_index"], p["d_loss"], in_place=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        square.sum().backward()

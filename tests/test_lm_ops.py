@@ -100,3 +100,13 @@ def test_distillation_refuses_before_device_work():
 def test_distillation_refuses_host_tensors():
     with pytest.raises(ValueError, match="CUDA"):
         fl.distillation_forward(torch.zeros(2, 8), torch.zeros(2, 1), torch.zeros(2, 1, dtype=torch.int32))
+
+
+def test_decay_attention_refuses_more_workgroups_than_a_launch_has():
+    from flashlstm_poc_amd import lm_ops
+    lib = lm_ops._bind()
+    rows = lm_ops._ROWS.pack(SOME.value, 64, 64, 32)
+    shape = lambda heads: lm_ops._SHAPE.pack(2 ** 24, 1, 0, heads, 1, 32, 32, 1, 0.5, SOME.value)
+    assert lib.flstm_decay_attention_step(shape(1), rows, rows, rows, rows, SOME, None) == 2004
+    assert lib.flstm_decay_attention_forward(shape(2), rows, rows, rows, None, rows, None, None, None) == 2004
+    assert lib.flstm_decay_attention_backward(shape(2), rows, rows, rows, rows, None, None, rows, rows, rows, None, SOME, None) == 2004
