@@ -826,9 +826,13 @@ bool valid_shape(const flstm_decay_attention* p) {
 // 131072 tokens of 8 heads take 425 us in segments of 2048, 496 of 1024, 740 of 4096.  Of packed sequences, whose last segments are
 // not full, three quarters of one more each are reckoned with: 12 of them with 16 heads take 200 us so, 251 in
 // segments of 1408.
+// Segments shorter than 256 tokens come with fewer workgroups than that: more of them are states to be written, scanned and read for few
+// tokens, and backward there are three walks.  Up to 256 tokens a sequence is walked as a whole.  Segments of 64 tokens / of 256, both
+// directions: fp32, seven packed sequences of up to 200 tokens, 6 heads of 40 x 65, 118 / 195; one of 512, 16 heads of 128 x 128, 143 /
+// 251; bf16 100 / 119 for the latter.  (Four of 512 with 16 heads, bf16, gradients: 145 / 91; there segments stay at 256.)
 size_t segment_of(const flstm_decay_attention* p, bool backward) {
     const size_t blocks = size_t(p->heads) * ceil_div(size_t(p->dv), 128), walks = p->sequences * blocks;
-    if (walks == 0 || walks >= (backward ? 128 : p->cu_seqlens ? 256 : 129)) return kWhole;
+    if (walks == 0 || p->tokens <= 256 || walks >= (backward ? 128 : p->cu_seqlens ? 256 : 129)) return kWhole;
     const size_t room = p->dk > 128 || p->dv > 128 ? 256 : 512;
     size_t segment;
     if (p->cu_seqlens) {
@@ -837,7 +841,11 @@ size_t segment_of(const flstm_decay_attention* p, bool backward) {
     } else {
         segment = ceil_div(p->tokens, walks < room ? room / walks : 1);
     }
-    return segment < 256 ? 256 : round_up(segment, 64);
+    if (segment < 256) {
+        const size_t least = ceil_div(p->cu_seqlens ? p->tokens * blocks : p->tokens * walks, room / (backward ? 3 : 2));
+        segment = segment > least ? segment : least < 256 ? least : 256;
+    }
+    return round_up(segment, 64);
 }
 size_t slots_of(const flstm_decay_attention* p, bool backward) {
     const size_t segment = segment_of(p, backward);

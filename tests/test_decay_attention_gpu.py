@@ -133,6 +133,14 @@ def test_split_along_the_sequence(sequences, length, lengths, kv_heads):
     _check(p, _own(p))
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("sequences,length,lengths,dk,dv", [(1, 257, None, 64, 64), (2, 300, None, 40, 65), (1, 256, None, 64, 64), (5, None, [64, 128, 0, 63, 65], 65, 40),
+                                                            (1, 330, None, 200, 136), (3, None, [257, 1, 190], 16, 256)])
+def test_short_segments(sequences, length, lengths, dk, dv, dtype):
+    p = _problem(sequences, length, kv_heads=1, dk=dk, dv=dv, dtype=dtype, lengths=lengths, seed=4)
+    _check(p, _own(p))
+
+
 def test_tokens_of_no_sequence():
     p = _problem(2, None, lengths=[40, 70], heads=2, kv_heads=1, dk=32, dv=32)
     want = _own(p)
