@@ -263,9 +263,21 @@ template <class T> __device__ __forceinline__ float8 less(float8 w, typename Fra
 // that lies outside [low, 2^15].  (bf16 and fp32 have a float's range.)  Infinities and NaN do not count: they stay what they are,
 // and beside them the others have to keep their range.
 __device__ __forceinline__ bool in_range(float most, float low) { return most >= low && most <= 32768.f; }
+__device__ __forceinline__ int exponent(float v) { return __builtin_amdgcn_frexp_expf(v); }   // v < 2^exponent, at least half of it; 0 for 0
+__device__ __forceinline__ float power_of_two(float n) { return uniform(ldexpf(1.f, int(n))); }
+// Of scores that are to be multiplied with values of up to 2^16: below 2^-46 they add nothing to an output.
 __device__ __forceinline__ float to_range(float most) {
-    const int e = 14 - __builtin_amdgcn_frexp_expf(most);
-    return most > 0.f ? uniform(ldexpf(1.f, e < -100 ? -100 : e > 100 ? 100 : e)) : 1.f;
+    const int e = 14 - exponent(most);
+    return most > 0.f ? power_of_two(float(e < -126 ? -126 : e > 60 ? 60 : e)) : 1.f;
+}
+// Of the state, which is held under the power of two 2^now: what is to be added to `now` for a largest magnitude of 2^most (minus
+// infinity: nothing there).  2^now has bounds.  Beside values of zero a state decays without end, and a power that kept up with it would
+// overflow and meet those zeros; so from 2^-100 on a state fades, or where the `factor` of what is added is large by that much earlier.
+// At the other end all that a float holds is brought into range.
+__device__ __forceinline__ float change_of(float now, float most, float factor) {
+    if (most == -__builtin_inff()) return 0.f;
+    const float above = fmaxf(float(exponent(factor)), 0.f);
+    return uniform(fminf(fmaxf(14.f - ceilf(most), -126.f - now), fmaxf(100.f - above, -126.f) - now));
 }
 __device__ __forceinline__ float finite_magnitude(float v) { return fabsf(v) < __builtin_inff() ? fabsf(v) : 0.f; }
 // The largest finite magnitude in the wave's state.
@@ -295,7 +307,7 @@ __device__ __forceinline__ float8 half_of(const floatx16& v, int u) {
 }
 
 template <class T, int D, int WAVES, bool kOut>
-__global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2 : 1) void sweep_kernel(Sweeps a) {
+__global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && (WAVES == 4 || !kOut)) ? 2 : 1) void sweep_kernel(Sweeps a) {
     constexpr int kThreads = WAVES * 64, kTokens = kChunk<T>, kTiles = D / 32, kBlocks = kTokens / 32;
     typedef Tile<T, D> tile_d;
     typedef Tile<T, WAVES * 32> tile_e;
@@ -489,10 +501,14 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
                 for (int i = 0; i < kTiles; ++i) most = fmaxf(most, most8({half_of(x[i], 0), half_of(x[i], 1)}));
                 if (__any(most > 32768.f) || !__any(most >= 0x1p-8f)) {
                     most = most_finite(x);
-                    const float r = in_range(most, 0x1p-8f) ? 1.f : to_range(most);
-                    x_scale *= r;
+                    if (!in_range(most, 0x1p-8f)) {
+                        const float now = float(exponent(x_scale) - 1);
+                        const float change = fminf(change_of(now, most > 0.f ? float(exponent(most)) : -__builtin_inff(), factor_c), 126.f);
+                        const float r = power_of_two(change);
+                        x_scale = power_of_two(now + change);
 #pragma unroll
-                    for (int i = 0; i < kTiles; ++i) x[i] *= r;
+                        for (int i = 0; i < kTiles; ++i) x[i] *= r;
+                    }
                 }
             }
             // along the width: the rows against the state and against the chunk's other rows
@@ -620,12 +636,15 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && WAVES == 4) ? 2
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
                         most = fmaxf(most, finite_magnitude(float(values[kk][j])) * power(l, float(kTokens - 16 - 16 * kk)));
-                most = lanes_max<kWave>(most) * fabsf(factor_c) * x_scale;
-                const float larger = fmaxf(most, most_finite(x) * keep);
-                if (most > 32768.f || larger < 0x1p-3f) {
-                    const float r = to_range(larger);
-                    x_scale *= r;
-                    keep *= r;
+                // in exponents: products of these magnitudes may lie outside a float's range
+                most = lanes_max<kWave>(most) * __builtin_amdgcn_frexp_mantf(fabsf(factor_c));
+                const float now = float(exponent(x_scale) - 1), decay = l * (float(valid - 1) + lead), of_x = most_finite(x);
+                const float added = most > 0.f ? float(exponent(most) + exponent(factor_c)) + now : -__builtin_inff();
+                const float larger = fmaxf(added, of_x > 0.f ? float(exponent(of_x)) + decay : -__builtin_inff());
+                if (added > 15.f || larger <= -3.f) {
+                    const float change = uniform(fminf(change_of(now, larger, factor_c), floorf(126.f - decay)));
+                    x_scale = power_of_two(now + change);
+                    keep = decay > -126.f ? ldexpf(keep, int(change)) : __builtin_amdgcn_exp2f(decay + change);   // (0 below 2^-126)
                 }
             }
         }

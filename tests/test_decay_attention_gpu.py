@@ -464,3 +464,89 @@ def test_refusals():
     with pytest.raises(ValueError, match="state"):
         fl.decay_attention_step(q[:, 0], k[:, 0], v[:, 0], g, None)
     assert math.isfinite(float(f(q, k, v, g)[0].float().sum()))
+
+
+def _check_long(p, got, label=""):
+    """Like _check, for long walks with tokens of zeros, behind which little but decayed values is left.  A decay by e^-x is exp2 of a
+    product that is rounded to 32 bits a few times, 3 u x relative (x up to 104: what is smaller is below 2^-150), and an exp2 and a
+    product a chunk cost 4 u; one below 2^-126 is zero, which leaves less than 2^-110 out.  Operands of fp16 are held to 2^-25 at the
+    least: as parts of the state (as many as the head is wide) or as scores (64 a chunk), times another operand; in the state's
+    update, relative to the largest value of their chunk, 64 a chunk too.  Where no key is zero that value is in the state, whose
+    largest is then 1 or more before it decays; beside keys of zero it is not, and the bound is absolute."""
+    want, most = _definition(p), _definition(p, magnitudes=True)
+    dtype, (dk, dv) = p["q"].dtype, (p["q"].shape[-1], p["v"].shape[-1])
+    largest = max(float(p[name].abs().max()) for name in ("q", "k", "v", "do"))
+    unit, held = (UNIT[dtype] if dtype != torch.float32 else 0.0), (2.0 ** -25 if dtype == torch.float16 else 0.0)
+    decays = U32 * (64 + 312 + max(p["lengths"]) / 8 + 8)
+    beside = 64 * held * largest if bool((p["k"] == 0).all(-1).any()) else 0.0
+    for name, value in want.items():
+        if name in ("state", "d_initial"):
+            slack = (decays + (0 if unit == 0 else 2.0 ** -21)) * most[name] + ((0 if unit == 0 else 2.0 ** -21) + 64 * held * largest) * most[name].amax((-1, -2), keepdim=True) + (beside if name == "state" else 0.0)
+        else:
+            slack = (1.05 * unit + decays) * most[name] + held * largest * max(1.0, abs(p["scale"])) * (64 + max(dk, dv))
+        assert_within(got[name], value, slack + 2.0 ** -110, f"{label} {name}")
+
+
+_DECAYS = [0.2, 0.5, 0.75, 0.9, 0.97, 0.99]
+
+
+@pytest.mark.parametrize("name", ["v", "do", "k"])
+@pytest.mark.parametrize("whole", [False, True], ids=["few heads", "many heads"])
+@pytest.mark.parametrize("zeros,dtype", [(64, torch.float16), (130, torch.float16), (320, torch.float16), (1000, torch.float16), (1000, torch.bfloat16), (1000, torch.float32),
+                                         (8192, torch.float16)], ids=str)
+def test_tokens_of_zeros(zeros, dtype, whole, name):
+    """Padding, and tokens without a loss: the state decays beside them, far below anything that is added to it later."""
+    heads = 132 if whole else 6          # (more than 128: walked as a whole)
+    p = _problem(1, zeros + 140, heads=heads, kv_heads=heads, dk=16, dv=16, dtype=dtype, log_decay=[math.log(g) for g in _DECAYS] * (heads // 6), seed=zeros)
+    p[name][:, 70:70 + zeros] = 0        # ordinary tokens on both sides
+    _check_long(p, _own(p), f"{zeros} in the middle")
+    if zeros <= 1000:
+        p[name][:, 70:] = 0
+        _check_long(p, _own(p), f"{zeros} at the end")
+        p[name][:, :70 + zeros] = 0
+        _check_long(p, _own(p), "all")
+
+
+@pytest.mark.parametrize("dk,dv", [(72, 136), (128, 64), (200, 40)])
+def test_tokens_of_zeros_by_width(dk, dv):
+    p = _problem(2, 500, heads=6, kv_heads=2, dk=dk, dv=dv, dtype=torch.float16, log_decay=[math.log(g) for g in _DECAYS])
+    for name in ("v", "do", "k"):
+        bad = dict(p, **{name: p[name].clone()})
+        bad[name][0, 30:460] = 0
+        bad[name][1, 200:] = 0
+        _check_long(bad, _own(bad), name)
+
+
+@pytest.mark.parametrize("scale", [0.0, 2.0 ** -40, 2.0 ** 20])
+def test_tokens_of_zeros_under_other_scales(scale):
+    p = _problem(1, 500, heads=6, kv_heads=6, dk=16, dv=16, dtype=torch.float16, log_decay=[math.log(g) for g in _DECAYS], scale=scale)
+    if scale > 1:
+        p["q"] = (p["q"] * 2.0 ** -14).to(torch.float16)
+    for name in ("v", "do", "k"):
+        bad = dict(p, **{name: p[name].clone()})
+        bad[name][:, 60:440] = 0
+        got, want = _own(bad), _definition(bad)
+        for key, value in want.items():
+            assert not bool(torch.isnan(got[key]).any()), (name, key)
+            fits = value.abs() < 60000
+            assert bool(torch.isfinite(got[key][fits]).all()), (name, key)
+        if scale <= 1:
+            _check_long(bad, got, name)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_a_large_state_that_decays(dtype):
+    """An initial state of up to 2^112 and ordinary tokens: outputs are right where they fit their type, states throughout."""
+    p = _problem(1, 300, heads=6, kv_heads=6, dk=16, dv=16, dtype=dtype, log_decay=[math.log(g) for g in _DECAYS], train=False)
+    p["do"] = torch.zeros_like(p["v"])
+    p["d_state"] = None
+    p["state"] = p["state"] * 2.0 ** 110
+    got, want, most = _own(p), _definition(p), _definition(p, magnitudes=True)
+    fits = most["o"] < 60000
+    for name in ("o", "dq", "dk", "dv"):
+        assert not bool(torch.isnan(got[name]).any()), name
+    unit, held = (UNIT[dtype] if dtype != torch.float32 else 0.0), (2.0 ** -25 if dtype == torch.float16 else 0.0)
+    slack = (1.05 * unit + U32 * (64 + 312 + 50)) * most["o"] + held * 80 * 5
+    assert_within(torch.where(fits, got["o"], torch.zeros_like(got["o"])), torch.where(fits, want["o"], 0.0), torch.where(fits, slack, 0.0), "o")
+    slack = (U32 * (64 + 312 + 50) + 2.0 ** -21) * most["state"] + (2.0 ** -21 + 64 * held * 5) * most["state"].amax((-1, -2), keepdim=True)
+    assert_within(got["state"], want["state"], slack, "state")
