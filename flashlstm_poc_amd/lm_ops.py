@@ -89,6 +89,12 @@ def _written(t) -> None:
         torch.autograd.graph.increment_version(t)
 
 
+def _differentiated(*tensors) -> bool:
+    """Whether a call goes through autograd: one of these needs a gradient, or forward-mode derivatives are being taken.  A tensor that
+    carries such a derivative does not need a gradient and has an ordinary pointer; autograd refuses it, as the operators have none."""
+    return torch.autograd.forward_ad._current_level >= 0 or torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 def _ptr(t) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
@@ -203,7 +209,7 @@ class _LayerNormFunction(torch.autograd.Function):
 
 def layer_norm(x, weight=None, bias=None, *, eps: float = 1e-5, residual=None):
     """layer_norm_forward with autograd: y, or with a residual (y, total)."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight, bias)):
+    if _differentiated(x, residual, weight, bias):
         y, total = _LayerNormFunction.apply(x, residual, weight, bias, eps)
     else:
         y, total = layer_norm_forward(x, weight, bias, eps=eps, residual=residual)[:2]
@@ -395,7 +401,7 @@ class _DecayAttentionFunction(torch.autograd.Function):
 
 def decay_attention(q, k, v, log_decay, *, scale: Optional[float] = None, state=None, cu_seqlens=None) -> Tuple:
     """decay_attention_forward with autograd in q, k, v and state: (o, final state)."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, state)):
+    if _differentiated(q, k, v, state):
         return _DecayAttentionFunction.apply(q, k, v, state, log_decay, scale, cu_seqlens)
     return decay_attention_forward(q, k, v, log_decay, scale=scale, state=state, cu_seqlens=cu_seqlens)
 
@@ -511,6 +517,6 @@ class _DistillationFunction(torch.autograd.Function):
 
 def distillation_loss(logits, teacher_logits, teacher_index, *, temperature: float = 1.0):
     """distillation_forward's loss of every row, with autograd in logits (the teacher gets no gradient)."""
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if _differentiated(logits):
         return _DistillationFunction.apply(logits, teacher_logits, teacher_index, temperature)
     return distillation_forward(logits, teacher_logits, teacher_index, temperature=temperature)[0]
