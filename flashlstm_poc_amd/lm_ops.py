@@ -254,6 +254,12 @@ def _last_axis_contiguous(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _tokens_within_reach(t):
+    """The kernels form the offsets of a chunk's tokens in 32 bits, for distances below 2^23 elements: tensors with more between two tokens
+    (a transposed (tokens, sequences, ..) of very many features) are copied, sequence by sequence."""
+    return t.contiguous() if t.shape[-3] > 1 and t.stride(-3) >= 1 << 23 else t
+
+
 def _decay_shape(q, k, v, log_decay, scale, state, cu_seqlens, axes: int):
     """Checks q (.., heads, dk), k (.., kv_heads, dk) and v (.., kv_heads, dv) of `axes` axes, and what goes with them."""
     if not (_all_here(torch.float32, log_decay) and isinstance(q, torch.Tensor) and q.dtype in _DTYPES and _all_here(q.dtype, q, k, v)):
@@ -334,6 +340,7 @@ def decay_attention_forward(q, k, v, log_decay, *, scale: Optional[float] = None
     shape, states = _decay_shape(q, k, v, log_decay, scale, state, cu_seqlens, axes)
     q, k, v = (_last_axis_contiguous(t) for t in (q, k, v))
     o = _like_rows(q, states[1], states[3])
+    q, k, v = (_tokens_within_reach(t) for t in (q, k, v))
     final = torch.empty(states, device=q.device, dtype=torch.float32) if want_state else None
     workspace = _workspace(shape, 0, q.device)
     _check(_bind().flstm_decay_attention_forward(shape, _rows_of(q), _rows_of(k), _rows_of(v), _ptr(state), _rows_of(o),
@@ -355,6 +362,7 @@ def decay_attention_backward(do, q, k, v, log_decay, *, scale: Optional[float] =
     dq = _like_rows(q, *q.shape[-2:]) if want[0] else None
     dk = _like_rows(k, *k.shape[-2:]) if want[1] else None
     dv = _like_rows(v, *v.shape[-2:]) if want[2] else None
+    do, q, k, v = (_tokens_within_reach(t) for t in (do, q, k, v))
     d_initial = torch.empty(states, device=q.device, dtype=torch.float32) if want[3] else None
     workspace = _workspace(shape, 1, q.device)
     _check(_bind().flstm_decay_attention_backward(

@@ -550,3 +550,21 @@ def test_a_large_state_that_decays(dtype):
     assert_within(torch.where(fits, got["o"], torch.zeros_like(got["o"])), torch.where(fits, want["o"], 0.0), torch.where(fits, slack, 0.0), "o")
     slack = (U32 * (64 + 312 + 50) + 2.0 ** -21) * most["state"] + (2.0 ** -21 + 64 * held * 5) * most["state"].amax((-1, -2), keepdim=True)
     assert_within(got["state"], want["state"], slack, "state")
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_tokens_far_apart(packed):
+    """Tokens 2^23 elements apart and more, as of a (tokens, sequences, ..) tensor of very many features."""
+    p = _problem(2, 5, heads=4, kv_heads=2, dk=32, dv=40, dtype=torch.float16, lengths=[3, 2] if packed else None)
+    want = _own(p)
+    room = torch.zeros(5 * (1 << 23) + 4096, device="cuda", dtype=torch.float16)
+    for name in ("q", "k", "v", "do"):
+        t = p[name]
+        strides = (1 << 23, *t.stride()[1:]) if packed else (512, 1 << 23, *t.stride()[2:])
+        view = room.as_strided(t.shape, strides)
+        view.copy_(t)
+        got = _own(dict(p, **{name: view}))
+        for key in want:
+            assert torch.equal(want[key], got[key]), (name, key)
+        if not packed and name == "q":   # (outputs keep the memory order of q's rows)
+            assert got["o"].stride()[0] < got["o"].stride()[1] and got["dq"].stride()[0] < got["dq"].stride()[1]
