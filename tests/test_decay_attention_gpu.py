@@ -552,6 +552,32 @@ def test_a_large_state_that_decays(dtype):
     assert_within(got["state"], want["state"], slack, "state")
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("name", ["v", "k", "q", "do"])
+@pytest.mark.parametrize("length,at", [(150, 80), (150, 149), (1, 0), (65, 64), (600, 301)])
+def test_an_infinity_reaches_what_it_should(length, at, name, dtype):
+    """What an infinity of an input reaches by the definition is not finite, all else as it was.  (It may be NaN where the definition has
+    an infinity: values go into the state in parts, and heads are padded with zeros.)"""
+    p = _problem(1, length, dtype=dtype, dk=32, dv=48, seed=at)
+    most = _definition(p, magnitudes=True)
+    bad = dict(p, **{name: p[name].clone()})
+    bad[name][0, at, 0, 5], bad[name][0, at, 1, 7] = float("inf"), float("-inf")
+    got, want = _own(bad), _definition(bad)
+    unit = UNIT[dtype] if dtype != torch.float32 else 0.0
+    for key, value in want.items():
+        if key in ("state", "d_initial"):
+            slack = (64 * U32 + (0 if unit == 0 else 2.0 ** -21)) * most[key] + (0 if unit == 0 else 2.0 ** -21) * most[key].amax((-1, -2), keepdim=True)
+        else:
+            slack = (1.05 * unit + 64 * U32) * most[key]
+        numbers = torch.isfinite(value)
+        assert not bool(torch.isfinite(got[key][~numbers]).any()), (name, key)
+        assert_within(torch.where(numbers, got[key], torch.zeros_like(got[key])), torch.where(numbers, value, 0.0), slack, f"{name} {key}")
+    if name != "do" and length == 1:   # a single token's form keeps infinities as they are
+        state = p["state"].clone()
+        o = fl.decay_attention_step(bad["q"][:, 0], bad["k"][:, 0], bad["v"][:, 0], p["log_decay"], state)
+        assert torch.equal(torch.isinf(state), torch.isinf(want["state"])) and torch.equal(torch.isfinite(o), torch.isfinite(want["o"][:, 0]))
+
+
 @pytest.mark.parametrize("packed", [False, True])
 def test_tokens_far_apart(packed):
     """Tokens 2^23 elements apart and more, as of a (tokens, sequences, ..) tensor of very many features."""
