@@ -309,6 +309,11 @@ __device__ __forceinline__ float8 half_of(const floatx16& v, int u) {
 template <class T, int D, int WAVES, bool kOut>
 __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && (WAVES == 4 || !kOut)) ? 2 : 1) void sweep_kernel(Sweeps a) {
     constexpr int kThreads = WAVES * 64, kTokens = kChunk<T>, kTiles = D / 32, kBlocks = kTokens / 32;
+    // What is in 32 bits and becomes an operand of the outputs' products, the state that a token meets and the weighted scores, goes in
+    // in two parts of the narrower types (22 bits of fp16, 16 of bf16): an output is then as far from exact arithmetic as its one
+    // rounding.  In one part each it is 1.4 times as far (bf16 2.3e-3 instead of 1.66e-3, fp16 2.9e-4 instead of 2.07e-4, of the norm),
+    // and the sweeps with output take 3 to 12 % less time (16 x 2048 tokens of 16 heads of 128, bf16: 175 us instead of 189).
+    constexpr int kOperandParts = sizeof(T) == 2 ? 2 : 1;
     typedef Tile<T, D> tile_d;
     typedef Tile<T, WAVES * 32> tile_e;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -539,10 +544,14 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && (WAVES == 4 || 
                 __builtin_amdgcn_sched_barrier(0);
                 Operands then = now;
                 if (step + 1 < 2 * kTiles) then = operands(step + 1);
-                const frag xf = to_frag<T>(half_of(x[step / 2], step % 2));
+                const float8 state = half_of(x[step / 2], step % 2);
+                frag parts[kOperandParts];
+                parts[0] = to_frag<T>(state);
+                if constexpr (kOperandParts > 1) parts[1] = to_frag<T>(less<T>(state, parts[0]));
 #pragma unroll
                 for (int tb = 0; tb < kBlocks; ++tb) {
-                    o[tb] = mma(xf, now.q[tb], o[tb]);
+#pragma unroll
+                    for (const frag& part : parts) o[tb] = mma(part, now.q[tb], o[tb]);
 #pragma unroll
                     for (int sb = 0; sb <= tb; ++sb) scores[tb][sb] = mma(now.k[sb], now.q[tb], scores[tb][sb]);
                 }
@@ -595,10 +604,16 @@ __global__ __launch_bounds__(WAVES * 64, D <= 64 || (D == 128 && (WAVES == 4 || 
                 o[tb] *= factor_a * power(l, float(t < 0 ? 0 : t) + lead) * (w_scale / x_scale);
 #pragma unroll
                 for (int j = 0; j < 2 * (tb + 1); ++j) {
-                    frag weights = to_frag<T>(w[j]);
-                    // tokens behind the row's own: by bits, not a product with zero, for the score there may be anything
-                    if (j / 2 == tb) weights = __builtin_bit_cast(frag, __builtin_bit_cast(mask, weights) & *reinterpret_cast<const mask*>(causal(j % 2, lane)));
-                    o[tb] = mma(values[j], weights, o[tb]);
+                    asm volatile("" : "+v"(w[j]));   // (all weights first, then their parts: mixed, they need more registers than there are)
+                    frag parts[kOperandParts];
+                    parts[0] = to_frag<T>(w[j]);
+                    if constexpr (kOperandParts > 1) parts[1] = to_frag<T>(less<T>(w[j], parts[0]));
+#pragma unroll
+                    for (frag weights : parts) {
+                        // tokens behind the row's own: by bits, not a product with zero, for the score there may be anything
+                        if (j / 2 == tb) weights = __builtin_bit_cast(frag, __builtin_bit_cast(mask, weights) & *reinterpret_cast<const mask*>(causal(j % 2, lane)));
+                        o[tb] = mma(values[j], weights, o[tb]);
+                    }
                 }
                 if (w_scale != 1.f) o[tb] *= 1.f / w_scale;
                 if (tb == 0 && next_valid > 0) request_v(tid, next_valid);

@@ -594,3 +594,18 @@ def test_tokens_far_apart(packed):
             assert torch.equal(want[key], got[key]), (name, key)
         if not packed and name == "q":   # (outputs keep the memory order of q's rows)
             assert got["o"].stride()[0] < got["o"].stride()[1] and got["dq"].stride()[0] < got["dq"].stride()[1]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("sequences,length,lengths,kv_heads,dk,dv", [(2, 200, None, 2, 64, 64), (1, 130, None, 2, 128, 128), (1, 100, None, 1, 40, 65), (1, 90, None, 2, 256, 200),
+                                                                     (1, 70, None, 2, 128, 64), (1, 600, None, 1, 128, 128), (3, None, [300, 1, 64], 2, 72, 136)])
+def test_outputs_are_rounded_once(sequences, length, lengths, kv_heads, dk, dv, dtype):
+    """The narrower types' outputs are those of 32 bits, rounded: what is an operand on the way is held in two parts, which leaves 2^-18 of a
+    term at the most in bf16 (2^-22 in fp16, or 2^-25 times the other operand: a score's, 64 a chunk, or a part of the state's, one
+    for each of the head's width), in the state and in the scores."""
+    p = _problem(sequences, length, lengths=lengths, heads=2, kv_heads=kv_heads, dk=dk, dv=dv, dtype=dtype, seed=dk)
+    got, want, most = _own(p), _definition(p), _definition(p, magnitudes=True)
+    largest = max(float(p[name].abs().max()) for name in ("q", "k", "v", "do"))
+    for name in ("o", "dq", "dk", "dv"):
+        part = 2 * 2.0 ** -18 * most[name] if dtype == torch.bfloat16 else 2 * 2.0 ** -22 * most[name] + 2.0 ** -25 * largest * (64 + max(dk, dv))
+        assert_within(got[name], want[name], part + 64 * U32 * most[name], name)
