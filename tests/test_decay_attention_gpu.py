@@ -609,3 +609,24 @@ def test_outputs_are_rounded_once(sequences, length, lengths, kv_heads, dk, dv, 
     for name in ("o", "dq", "dk", "dv"):
         part = 2 * 2.0 ** -18 * most[name] if dtype == torch.bfloat16 else 2 * 2.0 ** -22 * most[name] + 2.0 ** -25 * largest * (64 + max(dk, dv))
         assert_within(got[name], want[name], part + 64 * U32 * most[name], name)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("small,large", [(1e-4, 1.0), (1.0, 100.0), (0.01, 300.0), (1.0, 1e4)])
+def test_magnitudes_of_what_fits(small, large, dtype):
+    """Large keys and small gradients: every output that fits its type is right, whatever the others do.  An operand of fp16 is held to 2^-17
+    of the largest beside it (2^-25 where that is 2^-8), and there are two: with terms up to four times a head's mean, less than 2^-13 of
+    the largest sum of terms in the head."""
+    p = _problem(1, 200, dtype=dtype, dk=64, dv=64, log_decay=[0.0, -0.02], with_state=False, scale=0.01)
+    p["do"] = (p["do"] * small).to(dtype)
+    p["k"] = (p["k"] * large).to(dtype)
+    got, want, most = _own(p), _definition(p), _definition(p, magnitudes=True)
+    for name, value in want.items():
+        fits = value.abs() < 60000
+        if name in ("state", "d_initial"):
+            slack = (64 * U32 + 2.0 ** -21) * most[name] + 2.0 ** -21 * most[name].amax((-1, -2), keepdim=True)
+        else:
+            slack = (1.05 * UNIT[dtype] + 64 * U32) * most[name] + (2.0 ** -13 * most[name].amax((1, 3), keepdim=True) if dtype == torch.float16 else 0.0)
+            assert not bool(torch.isnan(got[name]).any()), name
+        assert bool(fits.any()), name
+        assert_within(torch.where(fits, got[name], torch.zeros_like(got[name])), torch.where(fits, value, 0.0), torch.where(fits, slack, 0.0), name)
