@@ -103,13 +103,14 @@ class RecurrentStudent(torch.nn.Module):
     @torch.no_grad()
     def generate(self, prompt, count: int):
         """The `count` likeliest tokens behind prompt (T, B), one after the other -> (count, B)."""
+        out = torch.empty((count, prompt.shape[1]), device=prompt.device, dtype=torch.int64)
         logits, state = self(prompt)
-        token, out = logits[-1].argmax(-1), []
-        for _ in range(count):
-            out.append(token)
-            logits, state = self.step(token, state)
-            token = logits.argmax(-1)
-        return torch.stack(out)
+        logits = logits[-1]
+        for i in range(count):
+            if i > 0:
+                logits, state = self.step(out[i - 1], state)
+            out[i] = logits.argmax(-1)
+        return out
 
 
 def successor_teacher(vocabulary: int, top: int, seed: int = 0, device="cuda"):

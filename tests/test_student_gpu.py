@@ -41,3 +41,11 @@ def test_tokens_one_by_one_and_in_pieces():
 def test_refusals():
     with pytest.raises(ValueError, match="multiple"):
         RecurrentStudent(50, 100, 3)
+
+
+def test_no_tokens_asked_for():
+    student = RecurrentStudent(50, 64, 2)
+    prompt = torch.randint(0, 50, (4, 3), device="cuda")
+    one = student.generate(prompt, 1)
+    assert student.generate(prompt, 0).shape == (0, 3) and one.shape == (1, 3)
+    assert torch.equal(student.generate(prompt, 5)[:1], one)
