@@ -853,20 +853,25 @@ bool valid_shape(const flstm_decay_attention* p) {
 
 // Tokens a workgroup walks.  A walk over a whole sequence reads everything once, but few heads leave most of the chip idle; cut
 // into segments it reads keys and values twice, for what each segment adds to the state comes first.  Measured with heads of 128
-// x 128 (us, whole walks / segments): forward, 192 workgroups of 2048 tokens 162 / 200, 128 of them 156 / 135, 32 of 2100 packed tokens
-// on average (8192 the longest) 450 / 81, four of 4096 238 / 59; packed, 192 with up to 4096 tokens 240 / 207, since the longest
-// decides; both directions (three walks backward), 128 workgroups 365 / 448, 32 packed ones 905 / 254.
+// x 128, bf16 (us, whole walks / segments): forward, 192 workgroups of 2048 tokens 160 / 188, 128 of them 149 / 151, four of 4096
+// 275 / 54, four heads of eight packed sequences of 2530 tokens on average (8192 the longest) 540 / 92; packed, 192 workgroups with up to
+// 4096 tokens 276 / 227, since the longest decides; gradients (three walks), 128 workgroups of 2048 tokens 266 / 257, the four of 4096
+// 276 / 65, the packed eight 545 / 161.
 // Segments are as long as leaves 512 workgroups, which is two a CU and one round (256 where a workgroup's registers fill a CU):
-// 131072 tokens of 8 heads take 425 us in segments of 2048, 496 of 1024, 740 of 4096.  Of packed sequences, whose last segments are
-// not full, three quarters of one more each are reckoned with: 12 of them with 16 heads take 200 us so, 251 in
+// 131072 tokens of 8 heads, fp16, take 492 us in segments of 2048, 512 of 1024, 528 of 4096.  Of packed sequences, whose last segments are
+// not full, three quarters of one more each are reckoned with: 12 of them with 16 heads take 227 us so, 265 in
 // segments of 1408.
-// Segments shorter than 256 tokens come with fewer workgroups than that: more of them are states to be written, scanned and read for few
-// tokens, and backward there are three walks.  Up to 256 tokens a sequence is walked as a whole.  Segments of 64 tokens / of 256, both
-// directions: fp32, seven packed sequences of up to 200 tokens, 6 heads of 40 x 65, 118 / 195; one of 512, 16 heads of 128 x 128, 143 /
-// 251; bf16 100 / 119 for the latter.  (Four of 512 with 16 heads, bf16, gradients: 145 / 91; there segments stay at 256.)
+// Eight chunks are walked as a whole: three launches take as long.  512 tokens, bf16, whole walks / segments: 4 heads 41 / 42, 16 heads 42 /
+// 49, four sequences of 16 heads 43 / 58, gradients 39 / 44, 40 / 54, 43 / 82; of 1024 tokens 73 / 44, 74 / 51, 75 / 71 and 73 / 48, 73 /
+// 62, 78 / 130.  256 tokens of fp32, where a chunk has 32, are as many chunks (300 of 16 heads 86 / 62, gradients 86 / 63).
+// Segments shorter than 256 tokens come with fewer workgroups than 512: more of them are states to be written, scanned and read for few
+// tokens, and backward there are three walks.  Segments of 64 tokens / of 256, fp32, forward and gradients together: seven packed
+// sequences of up to 200 tokens, 6 heads of 40 x 65, 121 / 199; one of 512, 16 heads of 128 x 128, 147 / 256.  (Four of 512 with 16 heads,
+// bf16, gradients: 133 / 81.)
 size_t segment_of(const flstm_decay_attention* p, bool backward) {
     const size_t blocks = size_t(p->heads) * ceil_div(size_t(p->dv), 128), walks = p->sequences * blocks;
-    if (walks == 0 || p->tokens <= 256 || walks >= (backward ? 128 : p->cu_seqlens ? 256 : 129)) return kWhole;
+    const size_t chunk = p->dtype == FLSTM_OP_F32 ? kChunk<float> : kChunk<half_t>;
+    if (walks == 0 || p->tokens <= 8 * chunk || walks >= (backward ? 128 : p->cu_seqlens ? 256 : 129)) return kWhole;
     const size_t room = p->dk > 128 || p->dv > 128 ? 256 : 512;
     size_t segment;
     if (p->cu_seqlens) {

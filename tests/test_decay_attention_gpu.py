@@ -630,3 +630,11 @@ def test_magnitudes_of_what_fits(small, large, dtype):
             assert not bool(torch.isnan(got[name]).any()), name
         assert bool(fits.any()), name
         assert_within(torch.where(fits, got[name], torch.zeros_like(got[name])), torch.where(fits, value, 0.0), torch.where(fits, slack, 0.0), name)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("length", [256, 257, 449, 512, 513, 577])
+def test_around_eight_chunks(length, dtype):
+    """Where walks over whole sequences end and segments begin (512 tokens, 256 of fp32)."""
+    p = _problem(2, length, heads=2, kv_heads=1, dk=40, dv=72, dtype=dtype, seed=length)
+    _check(p, _own(p))
