@@ -10,15 +10,18 @@
 // A workgroup holds X of one head (128 columns of it at most) in its accumulators for a whole run of tokens, so that a token's rows
 // are read once, its output written once, and nothing else leaves the chip.  Each wave has 32 columns of X and forms the scores of
 // a chunk for itself: four times these products, and no exchange.  (Shared out through LDS, in tiles of 16 x 16 and with a third
-// barrier a chunk, they took the same time for heads of 128, 13 to 17 % more for heads of 64 and 6 % less for fp32.)  The layouts
+// barrier a chunk, they took the same time for heads of 128, 13 to 17 % more for heads of 64 and 6 % less for fp32, while the outputs'
+// operands were in one part.)  The layouts
 // are chosen so that no accumulator passes through LDS: in every product below the operand that was an accumulator before has its
 // contraction index where the accumulator rows lie (see `perm`).
 //
 // What bounds it is the chain of a chunk, not one unit: the next rows are requested under the products, written to LDS between two
-// barriers, multiplied, weighted, multiplied again.  A workgroup alone on its CU takes 8700 clocks for a chunk of 64 tokens of a
-// head of 128 x 128 (staging 1500, products with rows and state 2100, weights and outputs 1800, requests 1100, the state 1750; 2500
-// to 3000 of them MFMA), each of two 11900.  Measured, bf16 but for the second: 16 x 2048 tokens of 16 heads of 128 forward 175 us
-// (3.1 TB/s of rows), their gradients 400; 131072 tokens of 8 heads, fp16, 425; a copy reaches 5.1 TB/s.
+// barriers, multiplied, weighted, multiplied again.  A workgroup alone on its CU takes 10400 clocks for a chunk of 64 tokens of a
+// head of 128 x 128 (barrier and the rows' arrival 640, staging 1350, products with rows and state 2670, weights and outputs 2960,
+// requests 600, the state 2220; 3700 of them MFMA), each of two 13900.  Kernels alone, under the profiler, bf16 but for the second: 16 x 2048
+// tokens of 16 heads of 128 forward 209 us (2.6 TB/s of rows), their gradients 467; 131072 tokens of 8 heads, fp16, 143 for what segments
+// add, 15, and 338; a copy reaches 5.1 TB/s.  fp32: the matrix units are busy for 55 % of the forward pass (16 x 512 tokens of 16 heads,
+// 184 us) and 65 % of the gradients' (8192 tokens of 8 heads, 220 us); a third of that is scores, which each wave forms for itself.
 #include "lm_device.h"
 
 namespace flstm_hip {
@@ -777,8 +780,8 @@ template <class T> __global__ __launch_bounds__(256) void fold_kernel(Fold f) {
     }
 }
 
-// ---- single tokens: bound by reading and writing the state once (256 sequences of 16 heads of 128 x 128: 105 us, 5.1 TB/s, the rate
-// of a copy).  A workgroup has 64 columns of one state, a thread four of them of every 16th row.
+// ---- single tokens: bound by reading and writing the state once (256 sequences of 16 heads of 128 x 128, 268 MB of state: 93 us, 5.8
+// TB/s, where part of it is still in the cache behind the L2 from the token before; a copy reaches 5.1).  A workgroup has 64 columns of one state, a thread four of them of every 16th row.
 struct Step {
     Role q, k, v, out;
     int heads, d, e;

@@ -4,8 +4,8 @@
 // d_total and writes dx, a few operations a value.  A row therefore stays in registers from its one load to its store: L lanes
 // of a wave (or a whole workgroup, for rows of more than 2048) hold V vectors of eight values each.  The variance is summed over
 // the centred values, not as a difference of two moments, which costs a second reduction and no traffic.
-// Measured on 262144 rows of 1024 fp16 values with a residual: forward 389 us, 5.5 TB/s; backward with the parameters' gradients
-// 395 + 5 us, 5.4 TB/s (a copy reaches 5.1).  32 such rows take 4 us forward, a launch and two trips to memory.
+// Measured on 262144 rows of 1024 fp16 values with a residual, under the profiler: forward 397 us, 5.4 TB/s; backward with the parameters'
+// gradients 404 + 5 us, 5.3 TB/s (a copy reaches 5.1).  32 such rows take 4.3 us forward, a launch and two trips to memory.
 #include "lm_device.h"
 
 namespace flstm_hip {

@@ -59,10 +59,12 @@ int flstm_layer_norm_backward(size_t rows, size_t width, const void* dy, size_t 
  * more than a launch can have).  cu_seqlens must ascend from 0.  Bounds are clamped to 0 .. tokens, so that nothing
  * outside the tensors is touched whatever they are, but where they do not ascend outputs are not specified.  Tokens behind the last
  * bound get zeros.  An empty sequence's final state is its initial one.
- * What a NaN or an infinity of an input reaches by these formulas is not finite, and nothing else is changed by it.  Over more than one
- * token it may be a NaN where the formulas have an infinity: values are added to the state in parts and heads are padded with zeros.
- * fp16: a state is held under a power of two and fades below 2^-100; what is added to it is held to 2^-25 of the largest value (times
- * its decay to the chunk's end) in its chunk of 64 tokens, whatever keys it meets. */
+ * What a NaN or an infinity of an input reaches by these formulas is not finite, and nothing else is changed by it.  In all but
+ * flstm_decay_attention_step it may be a NaN where the formulas have an infinity: values are added to the state in parts and heads are
+ * padded with zeros.
+ * Outputs and gradients are those of 32 bits, rounded once.  fp16: a state is held under a power of two and fades below 2^-100; what is
+ * added to it (a value times its decay to the end of its chunk of 64 tokens) is held to 2^-22 of the largest of the chunk, whatever keys
+ * it meets, or of the state. */
 typedef struct {
     void* data;
     ptrdiff_t sequence, token, head;
