@@ -2,9 +2,9 @@
 residual stream, attention with a decaying state, and the distillation loss against a teacher's top logits.
 
 Each is there as plain functions (forward, backward, and what training or serving calls in one go) and with autograd, which has no
-forward-mode derivatives of them and says so.  torch is
-used for device memory, streams and autograd; every computation happens inside libflashlstm.so.  Work is enqueued on the
-current stream of the tensors' device, which has to be the current device, and not waited for.
+forward-mode derivatives of them and says so.  torch is used for device memory, streams and autograd; every computation happens
+inside libflashlstm.so.  Work is enqueued on the current stream of the tensors' device, which has to be the current device, and
+not waited for.
 """
 from __future__ import annotations
 
