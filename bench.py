@@ -96,7 +96,7 @@ def kernel_source_digest():
     import hashlib
     h = hashlib.sha256()
     d = os.path.join(ROOT, "flashlstm_poc_amd", "csrc")
-    others = ("decay_attention.hip", "distillation.hip", "layer_norm.hip", "lm_device.h")
+    others = ("beam_search.hip", "decay_attention.hip", "distillation.hip", "embedding.hip", "gated_recurrence.hip", "layer_norm.hip", "lm_device.h")
     for f in sorted(glob.glob(os.path.join(d, "*.hip")) + glob.glob(os.path.join(d, "*.h"))):
         if os.path.basename(f) in others:
             continue

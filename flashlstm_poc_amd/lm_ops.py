@@ -1,8 +1,9 @@
 """The operators around the recurrent layers of a language model (include/flashlstm/lm_ops.h) on torch tensors: layer norm on a
-residual stream, attention with a decaying state, and the distillation loss against a teacher's top logits.
+residual stream, attention with a decaying state, the distillation loss against a teacher's top logits, the embedding of tokens, a gated
+linear recurrence, and beam search.
 
-Each is there as plain functions (forward, backward, and what training or serving calls in one go) and with autograd, which has no
-forward-mode derivatives of them and says so.  torch is used for device memory, streams and autograd; every computation happens
+Each but the last is there as plain functions (forward, backward, and what training or serving calls in one go) and with autograd, which has
+no forward-mode derivatives of them and says so.  torch is used for device memory, streams and autograd; every computation happens
 inside libflashlstm.so.  Work is enqueued on the current stream of the tensors' device, which has to be the current device, and
 not waited for.
 """
@@ -43,6 +44,20 @@ def _bind() -> ctypes.CDLL:
         lib.flstm_distillation_workspace_bytes.argtypes = [problem]
         lib.flstm_distillation_workspace_bytes.restype = sz
         lib.flstm_distillation_train.argtypes = [problem, vp, sz, vp, vp, sz, vp, vp]
+        lib.flstm_embedding_forward.argtypes = [problem, vp, sz, i32, vp, i32, vp]
+        lib.flstm_embedding_workspace_bytes.argtypes = [problem]
+        lib.flstm_embedding_workspace_bytes.restype = sz
+        lib.flstm_embedding_backward.argtypes = [problem, vp, sz, i32, vp, i32, vp, vp]
+        lib.flstm_gated_recurrence_forward.argtypes = [shape, rows, rows, rows, vp, rows, vp, vp, vp, vp]
+        lib.flstm_gated_recurrence_backward.argtypes = [shape, rows, rows, rows, rows, vp, vp, rows, rows, rows, vp, vp, vp]
+        lib.flstm_gated_recurrence_step.argtypes = [shape, rows, rows, rows, rows, vp, vp]
+        for name in ("workspace_bytes", "saved_rows"):
+            getattr(lib, f"flstm_gated_recurrence_{name}").argtypes = [shape]
+            getattr(lib, f"flstm_gated_recurrence_{name}").restype = sz
+        lib.flstm_beam_select.argtypes = [problem, vp, vp, vp, vp, vp, vp]
+        lib.flstm_beam_select_workspace_bytes.argtypes = [problem]
+        lib.flstm_beam_select_workspace_bytes.restype = sz
+        lib.flstm_beam_reorder.argtypes = [sz, i32, vp, ctypes.c_char_p, i32, vp]
         _BOUND = lib
     return _BOUND
 
@@ -529,3 +544,343 @@ def distillation_loss(logits, teacher_logits, teacher_index, *, temperature: flo
     if _differentiated(logits):
         return _DistillationFunction.apply(logits, teacher_logits, teacher_index, temperature)
     return distillation_forward(logits, teacher_logits, teacher_index, temperature=temperature)[0]
+
+
+# ---- embedding of tokens
+
+_EMBEDDING = struct.Struct("@NNNPif0P")   # flstm_embedding
+
+
+def _indices(name: str, t) -> bool:
+    """Refuses what holds no int32 or int64 on the current device; returns whether it is int64."""
+    if not torch.is_tensor(t) or not t.is_cuda or t.get_device() != torch._C._cuda_getDevice():
+        raise ValueError(f"{name} must be a CUDA tensor on the current device")
+    if t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name} must be of type int32 or int64, not {t.dtype}")
+    return t.dtype == torch.int64
+
+
+def _op_dtype(name: str, dtype) -> int:
+    code = _DTYPES.get(dtype)
+    if code is None:
+        raise ValueError(f"unsupported {name} {dtype}: it must be float32, float16 or bfloat16")
+    return code
+
+
+def _scale(scale) -> float:
+    scale = float(scale)
+    if not abs(scale) <= 3.4028234663852886e38:
+        raise ValueError("scale must be a finite number")
+    return scale
+
+
+def embedding_forward(tokens, table, *, scale: float = 1.0, dtype=None):
+    """out[..., :] = scale * table[tokens[...]], rounded once to `dtype` (table's where None); zeros for a token outside the vocabulary (-1,
+    say).
+
+    tokens int32 / int64 of any shape, table (vocabulary, width) float32 / float16 / bfloat16.  Returns (*tokens.shape, width)."""
+    index_64, code = _indices("tokens", tokens), _device_tensor("table", table)
+    if table.dim() != 2 or table.shape[0] < 1:
+        raise ValueError(f"table must have shape (vocabulary, width): got {tuple(table.shape)}")
+    dtype = table.dtype if dtype is None else dtype
+    out_code, scale = _op_dtype("dtype", dtype), _scale(scale)
+    (vocabulary, width), tokens = table.shape, tokens.contiguous()
+    out = torch.empty((*tokens.shape, width), device=table.device, dtype=dtype)
+    if out.numel() == 0:
+        return out
+    rows = _rows(table)
+    if rows.stride(0) < width and vocabulary > 1:   # (rows that share memory)
+        rows = rows.contiguous()
+    problem = _EMBEDDING.pack(tokens.numel(), vocabulary, width, tokens.data_ptr(), index_64, scale)
+    _check(_bind().flstm_embedding_forward(problem, rows.data_ptr(), rows.stride(0), code, out.data_ptr(), out_code, _stream()),
+           "flstm_embedding_forward")
+    return out
+
+
+def embedding_backward(d_out, tokens, vocabulary: int, *, scale: float = 1.0, dtype=torch.float32):
+    """The table's gradient (vocabulary, width) of type `dtype` from that of embedding_forward's result, d_out (*tokens.shape, width): for each
+    token scale times the sum of its rows, zeros for tokens that do not occur."""
+    index_64, code = _indices("tokens", tokens), _device_tensor("d_out", d_out)
+    if d_out.dim() != tokens.dim() + 1 or d_out.shape[:-1] != tokens.shape:
+        raise ValueError(f"d_out must have shape {(*tokens.shape, 'width')}: got {tuple(d_out.shape)}")
+    if vocabulary < 1:
+        raise ValueError("vocabulary must be >= 1")
+    out_code, scale, width = _op_dtype("dtype", dtype), _scale(scale), d_out.shape[-1]
+    d_table = torch.empty((vocabulary, width), device=d_out.device, dtype=dtype)
+    if width == 0:
+        return d_table
+    tokens = tokens.contiguous()
+    rows = _rows(d_out) if d_out.numel() else d_out.reshape(0, width)
+    problem = _EMBEDDING.pack(tokens.numel(), vocabulary, width, tokens.data_ptr(), index_64, scale)
+    lib = _bind()
+    size = lib.flstm_embedding_workspace_bytes(problem)
+    workspace = torch.empty(size, device=d_out.device, dtype=torch.uint8) if size else None
+    _check(lib.flstm_embedding_backward(problem, rows.data_ptr(), rows.stride(0), code, d_table.data_ptr(), out_code, _ptr(workspace), _stream()),
+           "flstm_embedding_backward")
+    return d_table
+
+
+class _EmbeddingFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, tokens, scale, dtype):
+        ctx.save_for_backward(tokens)
+        ctx.vocabulary, ctx.scale, ctx.dtype = table.shape[0], scale, table.dtype
+        return embedding_forward(tokens, table, scale=scale, dtype=dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_out):
+        tokens, = ctx.saved_tensors
+        return embedding_backward(d_out, tokens, ctx.vocabulary, scale=ctx.scale, dtype=ctx.dtype), None, None, None
+
+
+def embedding(tokens, table, *, scale: float = 1.0, dtype=None):
+    """embedding_forward with autograd in table."""
+    if _differentiated(table):
+        return _EmbeddingFunction.apply(table, tokens, scale, dtype)
+    return embedding_forward(tokens, table, scale=scale, dtype=dtype)
+
+
+class Embedding(torch.nn.Module):
+    """Rows of a table of fp32 parameters, named and initialised as torch.nn.Embedding's, scaled, as activations of type `dtype`."""
+
+    def __init__(self, vocabulary: int, width: int, *, scale: float = 1.0, dtype=torch.float32, device="cuda"):
+        super().__init__()
+        if vocabulary < 1 or width < 1:
+            raise ValueError("vocabulary and width must be >= 1")
+        _op_dtype("dtype", dtype)
+        self.vocabulary, self.width, self.scale, self.dtype = int(vocabulary), int(width), _scale(scale), dtype
+        self.weight = torch.nn.Parameter(torch.empty((self.vocabulary, self.width), device=device, dtype=torch.float32))
+        torch.nn.init.normal_(self.weight)
+
+    def forward(self, tokens):
+        return embedding(tokens, self.weight, scale=self.scale, dtype=self.dtype)
+
+
+# ---- gated linear recurrence
+
+_RECURRENCE = struct.Struct("@NNPNi0P")   # flstm_recurrence
+
+
+def _recurrence(x, forget, gate, state, cu_seqlens, axes: int):
+    """Checks x, forget and gate (or None) of `axes` axes, the last of them the channels, and what goes with them."""
+    tensors = (x, forget) if gate is None else (x, forget, gate)
+    if not (isinstance(x, torch.Tensor) and x.dtype in _DTYPES and _all_here(x.dtype, *tensors)):
+        _device_tensor("x", x)
+        for name, t in (("forget", forget), ("gate", gate)):
+            if t is not None:
+                _device_tensor(name, t, x.dtype)
+    shape = x.shape
+    if len(shape) != axes:
+        raise ValueError(f"x must have {axes} axes, not {len(shape)}")
+    for name, t in (("forget", forget), ("gate", gate)):
+        if t is not None and t.shape != shape:
+            raise ValueError(f"{name} must have x's shape {tuple(shape)}: got {tuple(t.shape)}")
+    if cu_seqlens is not None:
+        _device_tensor_int("cu_seqlens", cu_seqlens)
+        if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1 or not cu_seqlens.is_contiguous():
+            raise ValueError("cu_seqlens must be a contiguous tensor of one more entry than there are sequences")
+        sequences, tokens = cu_seqlens.shape[0] - 1, shape[0]
+    else:
+        sequences, tokens = shape[0], shape[1] if axes == 3 else 1
+    states = (sequences, shape[-1])
+    _check_state("state", state, states)
+    return _RECURRENCE.pack(sequences, tokens, _ptr(cu_seqlens) or 0, shape[-1], _DTYPES[x.dtype]), states
+
+
+def _channel_rows(t, packed: bool = False):
+    """Where (sequences, tokens, width), packed (tokens, width), or for a single token (sequences, width), lies."""
+    if t is None:
+        return None
+    s = t.stride()
+    return _ROWS.pack(t.data_ptr(), 0 if packed else s[0], s[-2] if packed or len(s) == 3 else 0, 0)
+
+
+def _like_channels(x):
+    """An output in the memory order of x's rows."""
+    if x.dim() == 3 and x.stride(0) < x.stride(1) and x.shape[0] > 1:
+        return torch.empty((x.shape[1], x.shape[0], x.shape[2]), device=x.device, dtype=x.dtype).transpose(0, 1)
+    return torch.empty(x.shape, device=x.device, dtype=x.dtype)
+
+
+def _recurrence_workspace(shape: bytes, device):
+    size = _bind().flstm_gated_recurrence_workspace_bytes(shape)
+    return torch.empty(size, device=device, dtype=torch.uint8) if size else None
+
+
+def gated_recurrence_forward(x, forget, gate=None, *, state=None, cu_seqlens=None, want_state: bool = True, want_saved: bool = True) -> Tuple:
+    """c_t = f_t c_{t-1} + (1 - f_t) x_t with f = sigmoid(forget), y_t = c_t or, with a gate, sigmoid(gate_t) c_t, for every channel of every sequence.
+
+    x, forget, gate (sequences, tokens, width) float32 / float16 / bfloat16, of any strides (parts of one projection, a transposed
+    (tokens, sequences, width)).  Or packed, (tokens, width), with cu_seqlens (sequences + 1,) int32, from 0 on.  state (sequences, width)
+    float32: the state in front of the first tokens (None: zeros).
+    Returns (y, state behind the last tokens, saved), the latter two None where not wanted; gated_recurrence_backward takes saved."""
+    packed = cu_seqlens is not None
+    shape, states = _recurrence(x, forget, gate, state, cu_seqlens, 2 if packed else 3)
+    x, forget = _last_axis_contiguous(x), _last_axis_contiguous(forget)
+    gate = None if gate is None else _last_axis_contiguous(gate)
+    y, lib = _like_channels(x), _bind()
+    final = torch.empty(states, device=x.device, dtype=torch.float32) if want_state else None
+    saved = torch.empty((lib.flstm_gated_recurrence_saved_rows(shape), states[1]), device=x.device, dtype=torch.float32) if want_saved else None
+    workspace = _recurrence_workspace(shape, x.device)
+    _check(lib.flstm_gated_recurrence_forward(shape, _channel_rows(x, packed), _channel_rows(forget, packed), _channel_rows(gate, packed), _ptr(state),
+                                              _channel_rows(y, packed), _ptr(final), _ptr(saved), _ptr(workspace), _stream()),
+           "flstm_gated_recurrence_forward")
+    return y, final, saved
+
+
+def gated_recurrence_backward(dy, x, forget, gate, saved, *, d_state=None, cu_seqlens=None, want=(True, True, True, True)) -> Tuple:
+    """Gradients (dx, dforget, dgate, d_initial_state) of gated_recurrence_forward from those of y and of the final state (None: zeros); `want`
+    tells which (None for the others, and for dgate without a gate).  saved: what the forward pass returned."""
+    packed = cu_seqlens is not None
+    shape, states = _recurrence(x, forget, gate, d_state, cu_seqlens, 2 if packed else 3)
+    _device_tensor("dy", dy, x.dtype)
+    if dy.shape != x.shape:
+        raise ValueError(f"dy must have x's shape {tuple(x.shape)}: got {tuple(dy.shape)}")
+    lib = _bind()
+    _check_state("saved", saved, (lib.flstm_gated_recurrence_saved_rows(shape), states[1]))
+    if saved is None:
+        raise ValueError("saved must be what the forward pass returned")
+    dy, x, forget = (_last_axis_contiguous(t) for t in (dy, x, forget))
+    gate = None if gate is None else _last_axis_contiguous(gate)
+    dx = _like_channels(x) if want[0] else None
+    dforget = _like_channels(x) if want[1] else None
+    dgate = _like_channels(x) if want[2] and gate is not None else None
+    d_initial = torch.empty(states, device=x.device, dtype=torch.float32) if want[3] else None
+    workspace = _recurrence_workspace(shape, x.device)
+    _check(lib.flstm_gated_recurrence_backward(
+        shape, _channel_rows(dy, packed), _channel_rows(x, packed), _channel_rows(forget, packed), _channel_rows(gate, packed), saved.data_ptr(),
+        _ptr(d_state), _channel_rows(dx, packed), _channel_rows(dforget, packed), _channel_rows(dgate, packed), _ptr(d_initial), _ptr(workspace),
+        _stream()), "flstm_gated_recurrence_backward")
+    return dx, dforget, dgate, d_initial
+
+
+def gated_recurrence_step(x, forget, state, gate=None):
+    """One token of every sequence: x, forget, gate (sequences, width); `state` (sequences, width) float32 is updated in place.  Returns y.
+    No autograd."""
+    if state is None:
+        raise ValueError("state must be a tensor: it is updated in place")
+    shape, states = _recurrence(x, forget, gate, state, None, 2)
+    x, forget = _last_axis_contiguous(x), _last_axis_contiguous(forget)
+    gate = None if gate is None else _last_axis_contiguous(gate)
+    y = torch.empty(states, device=x.device, dtype=x.dtype)
+    _check(_bind().flstm_gated_recurrence_step(shape, _channel_rows(x), _channel_rows(forget), _channel_rows(gate), _channel_rows(y), state.data_ptr(),
+                                               _stream()), "flstm_gated_recurrence_step")
+    _written(state)
+    return y
+
+
+class _GatedRecurrenceFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, forget, gate, state, cu_seqlens):
+        y, final, saved = gated_recurrence_forward(x, forget, gate, state=state, cu_seqlens=cu_seqlens)
+        ctx.save_for_backward(x, forget, gate, saved, cu_seqlens)
+        ctx.set_materialize_grads(False)
+        return y, final
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, d_final):
+        x, forget, gate, saved, cu_seqlens = ctx.saved_tensors
+        if dy is None:
+            dy = torch.zeros(x.shape, device=x.device, dtype=x.dtype)
+        if d_final is not None:
+            d_final = d_final.contiguous()
+        grads = gated_recurrence_backward(dy, x, forget, gate, saved, d_state=d_final, cu_seqlens=cu_seqlens, want=ctx.needs_input_grad[:4])
+        return (*grads, None)
+
+
+def gated_recurrence(x, forget, gate=None, *, state=None, cu_seqlens=None) -> Tuple:
+    """gated_recurrence_forward with autograd in x, forget, gate and state: (y, final state)."""
+    if _differentiated(x, forget, gate, state):
+        return _GatedRecurrenceFunction.apply(x, forget, gate, state, cu_seqlens)
+    return gated_recurrence_forward(x, forget, gate, state=state, cu_seqlens=cu_seqlens, want_saved=False)[:2]
+
+
+# ---- beam search
+
+_BEAMS = struct.Struct("@NiiNPNiPPq")   # flstm_beams
+_BEAM_STATE = struct.Struct("@PNN")
+_MAX_BEAMS, _MAX_STATES = 32, 16
+
+
+def beam_select(logits, scores, *, beams: Optional[int] = None, end: Optional[int] = None, finished=None) -> Tuple:
+    """The best continuations of every sequence's hypotheses by one token, by scores + log_softmax(logits), the best first and of equal ones
+    that of the lower hypothesis and token.
+
+    logits (sequences, hypotheses, vocabulary) float32 / float16 / bfloat16, scores (sequences, hypotheses) float32 (minus infinity: no
+    hypothesis).  beams: how many are kept, as many as there are where None; up to 32 of both.  end: the token that ends a hypothesis;
+    finished (sequences, hypotheses) bool: those that are, which stay as they are, with `end` as their token.
+    Returns (scores, parents, tokens, finished), (sequences, beams) of float32, int64, int64 and bool (None without `end`).  Logits of minus
+    infinity and NaN are no continuations; where there are too few, scores are minus infinity and tokens -1.  No autograd."""
+    code = _device_tensor("logits", logits)
+    if logits.dim() != 3 or logits.shape[2] < 1:
+        raise ValueError(f"logits must have shape (sequences, hypotheses, vocabulary): got {tuple(logits.shape)}")
+    sequences, hypotheses, vocabulary = logits.shape
+    keep = hypotheses if beams is None else int(beams)
+    if not (1 <= hypotheses <= _MAX_BEAMS and 1 <= keep <= _MAX_BEAMS):
+        raise ValueError(f"between 1 and {_MAX_BEAMS} hypotheses and beams: got {hypotheses} and {keep}")
+    _device_tensor("scores", scores, torch.float32)
+    if scores.shape != (sequences, hypotheses):
+        raise ValueError(f"scores must have shape {(sequences, hypotheses)}: got {tuple(scores.shape)}")
+    if end is not None and not 0 <= end < vocabulary:
+        raise ValueError(f"end must lie in the vocabulary: got {end}")
+    if finished is not None:
+        if end is None:
+            raise ValueError("finished hypotheses need an `end`")
+        if not torch.is_tensor(finished) or finished.device != logits.device or finished.dtype != torch.bool:
+            raise ValueError("finished must be a bool tensor on the device of logits")
+        if finished.shape != (sequences, hypotheses):
+            raise ValueError(f"finished must have shape {(sequences, hypotheses)}: got {tuple(finished.shape)}")
+        finished = finished.contiguous()
+    scores = scores.contiguous()
+    rows = _rows(logits) if logits.numel() else logits
+    ld = rows.stride(0) if sequences * hypotheses > 1 else vocabulary
+    if ld < vocabulary:   # (rows that share memory)
+        rows, ld = rows.contiguous(), vocabulary
+    shape, dev = (sequences, keep), logits.device
+    out_scores = torch.empty(shape, device=dev, dtype=torch.float32)
+    parents, tokens = torch.empty((2, *shape), device=dev, dtype=torch.int64).unbind(0)
+    out_finished = None if end is None else torch.empty(shape, device=dev, dtype=torch.bool)
+    problem = _BEAMS.pack(sequences, hypotheses, keep, vocabulary, rows.data_ptr(), ld, code, scores.data_ptr(), _ptr(finished) or 0,
+                          -1 if end is None else end)
+    lib = _bind()
+    workspace = torch.empty(lib.flstm_beam_select_workspace_bytes(problem), device=dev, dtype=torch.uint8)
+    _check(lib.flstm_beam_select(problem, out_scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(), _ptr(out_finished), workspace.data_ptr(),
+                                 _stream()), "flstm_beam_select")
+    return out_scores, parents, tokens, out_finished
+
+
+def beam_reorder(parents, *states) -> None:
+    """Hypothesis b of sequence s becomes, in every one of `states`, what hypothesis parents[s, b] was, in place; rows that stay are not touched.
+
+    parents (sequences, hypotheses) int64, as beam_select returns them; up to 32 hypotheses; one outside them leaves its row as it is.  states: tensors
+    of any type, (sequences * hypotheses, ..) or (sequences, hypotheses, ..), with contiguous rows.  No autograd."""
+    if not torch.is_tensor(parents) or not parents.is_cuda or parents.get_device() != torch._C._cuda_getDevice() or parents.dtype != torch.int64:
+        raise ValueError("parents must be an int64 CUDA tensor on the current device")
+    if parents.dim() != 2 or not 1 <= parents.shape[1] <= _MAX_BEAMS:
+        raise ValueError(f"parents must have shape (sequences, hypotheses), of 1 to {_MAX_BEAMS}: got {tuple(parents.shape)}")
+    sequences, hypotheses = parents.shape
+    packed = []
+    for i, t in enumerate(states):
+        if not torch.is_tensor(t) or t.get_device() != parents.get_device():
+            raise ValueError(f"state {i} must be a CUDA tensor on the device of parents")
+        of = t.shape
+        if of[:1] == (sequences * hypotheses,):
+            stride, row = t.stride(0), t.shape[1:]
+        elif of[:2] == (sequences, hypotheses) and (sequences == 1 or hypotheses == 1 or t.stride(0) == hypotheses * t.stride(1)):
+            stride, row = t.stride(0) if hypotheses == 1 else t.stride(1), t.shape[2:]
+        else:
+            raise ValueError(f"state {i} must have {sequences} x {hypotheses} rows, evenly spaced: got shape {tuple(of)}")
+        size = row.numel()
+        if size and sequences and not (t[0, 0] if len(of) - len(row) == 2 else t[0]).is_contiguous() or sequences * hypotheses > 1 and stride < size:
+            raise ValueError(f"state {i} must have contiguous rows of its own")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"state {i} needs a gradient: it would be changed in place")
+        packed.append(_BEAM_STATE.pack(t.data_ptr(), max(stride, size) * t.element_size(), size * t.element_size()))
+    parents = parents.contiguous()
+    for at in range(0, len(packed), _MAX_STATES):
+        some = packed[at:at + _MAX_STATES]
+        _check(_bind().flstm_beam_reorder(sequences, hypotheses, parents.data_ptr(), b"".join(some), len(some), _stream()), "flstm_beam_reorder")
+    for t in states:
+        _written(t)

@@ -1,5 +1,6 @@
 /* Operators around the recurrent layers of a language model, for MI355X (gfx950): layer norm on a residual stream, attention
- * whose memory is a decaying state of fixed size, and the distillation loss against a teacher's top logits.
+ * whose memory is a decaying state of fixed size, the distillation loss against a teacher's top logits, the embedding of tokens,
+ * a gated linear recurrence, and beam search.
  * They have no counterpart in the reference, which is an LSTM layer alone.
  *
  * All pointers are device pointers.  Every function only enqueues work on `stream`: it allocates nothing, waits for nothing and
@@ -130,6 +131,107 @@ int flstm_distillation_backward(const flstm_distillation* problem, const float* 
 size_t flstm_distillation_workspace_bytes(const flstm_distillation* problem);
 int flstm_distillation_train(const flstm_distillation* problem, const float* d_loss, size_t d_stride, float* loss,
                              void* dlogits, size_t ldd, void* workspace, void* stream);
+
+/* ---- embedding of tokens
+ *
+ * out[i] = scale * table[index[i]], in 32 bits, rounded to out's type once; a token outside 0 .. vocabulary - 1 (-1, say) gives a row of
+ * zeros and has no gradient.  index: int32, or int64 where index_64 is not 0, contiguous.  Rows of table are ld elements apart, out is
+ * contiguous.  vocabulary and tokens are below 2^31, width below 2^24.
+ *
+ * Backward, of the gradient d_out of out (rows ldd elements apart):
+ *   d_table[v] = scale * sum over i with index[i] = v of d_out[i]
+ * in the order of i within a chunk of the sorted tokens and chunk behind chunk, in 32 bits, rounded to d_table's type once.  Every row of
+ * d_table (contiguous) is written, those of tokens that do not occur with zeros.  `workspace`: flstm_embedding_workspace_bytes()
+ * bytes, 16-byte aligned (null where that is 0). */
+typedef struct {
+    size_t tokens, vocabulary, width;
+    const void* index;
+    int index_64;
+    float scale;
+} flstm_embedding;
+
+int flstm_embedding_forward(const flstm_embedding* problem, const void* table, size_t ld, flstm_op_dtype table_dtype, void* out,
+                            flstm_op_dtype dtype, void* stream);
+size_t flstm_embedding_workspace_bytes(const flstm_embedding* problem);
+int flstm_embedding_backward(const flstm_embedding* problem, const void* d_out, size_t ldd, flstm_op_dtype dtype, void* d_table,
+                             flstm_op_dtype table_dtype, void* workspace, void* stream);
+
+/* ---- gated linear recurrence
+ *
+ * For every sequence and each of `width` channels, over the sequence's tokens t, with f = sigmoid(forget):
+ *   c_t = f_t c_{t-1} + (1 - f_t) x_t   (c before the first token = state_in or zeros)
+ *   y_t = c_t, or with an output gate sigmoid(gate_t) c_t
+ * States are contiguous fp32 (sequences, width); sums and states are held in 32 bits, y is rounded once.
+ *
+ * A tensor's element (sequence, token, channel) lies at data + sequence * .sequence + token * .token + channel elements (.head is not read).
+ * With cu_seqlens (sequences + 1 int32 on the device) sequences are packed along the token axis, as in flstm_decay_attention: bounds must
+ * ascend from 0, are clamped to 0 .. tokens, and tokens behind the last bound get zeros.  An empty sequence's final state is its
+ * initial one.
+ * What a NaN or an infinity of an input reaches by these formulas is not finite, and nothing else is changed by it; it may be a NaN where
+ * the formulas have an infinity.  A difference c - x that leaves the range of 32 bits counts as infinite, and with 16-bit
+ * tensors a sigmoid below 2^-126 as zero.
+ *
+ * Backward, of the gradients d_y of y and d_state_out of the state behind the last tokens (null: zeros):
+ *   G_t = sigmoid(gate_t) d_y_t + f_{t+1} G_{t+1}   (G behind the last token, times f, is d_state_out)
+ *   dx = (1 - f) G;  dforget = G (c_{t-1} - x) f (1 - f);  dgate = d_y c sigmoid(gate) (1 - sigmoid(gate));  d_state_in = f_1 G_1
+ * from x, forget, gate and `saved`, the states in front of every 16th token of a sequence, which the forward pass left:
+ * flstm_gated_recurrence_saved_rows() rows of `width` fp32.  Each gradient may be null. */
+typedef struct {
+    size_t sequences, tokens;
+    const int* cu_seqlens;
+    size_t width;
+    flstm_op_dtype dtype;
+} flstm_recurrence;
+
+/* gate (or its data), state_in, state_out and saved may be null; state_in and state_out must not be one buffer, and y must not lie in an input.
+ * `workspace`: flstm_gated_recurrence_workspace_bytes() bytes, 16-byte aligned (null where that is 0), forward and backward. */
+int flstm_gated_recurrence_forward(const flstm_recurrence* shape, const flstm_rows* x, const flstm_rows* forget, const flstm_rows* gate,
+                                   const float* state_in, const flstm_rows* y, float* state_out, float* saved, void* workspace, void* stream);
+int flstm_gated_recurrence_backward(const flstm_recurrence* shape, const flstm_rows* d_y, const flstm_rows* x, const flstm_rows* forget,
+                                    const flstm_rows* gate, const float* saved, const float* d_state_out, const flstm_rows* dx,
+                                    const flstm_rows* dforget, const flstm_rows* dgate, float* d_state_in, void* workspace, void* stream);
+size_t flstm_gated_recurrence_workspace_bytes(const flstm_recurrence* shape);
+size_t flstm_gated_recurrence_saved_rows(const flstm_recurrence* shape);
+/* One token of every sequence (shape->tokens, cu_seqlens and .token are not read), the state updated in place. */
+int flstm_gated_recurrence_step(const flstm_recurrence* shape, const flstm_rows* x, const flstm_rows* forget, const flstm_rows* gate,
+                                const flstm_rows* y, float* state, void* stream);
+
+/* ---- beam search
+ *
+ * Each sequence has `beams` hypotheses with a score (the logarithm of a probability; minus infinity: none).  Their continuations by a token j,
+ *   scores[b] + logits[b][j] - log of the sum of exp(logits[b]),
+ * are ordered, the larger first and of equal ones that with the lower b * vocabulary + j, and the first `keep` returned: score, parent (b)
+ * and token.  A hypothesis that is finished (`finished` not null and not 0) has one continuation, the token `end` with its score as it is; its
+ * logits are not read.  Logits of minus infinity and NaN are no continuations; plus infinity counts as the largest number of fp32.  Where
+ * there are fewer than `keep`, the places behind them get the score minus infinity, the token -1 and the place itself as parent (0 from
+ * `beams` on).  A returned hypothesis is finished if its token is `end` or -1.
+ * Scores are compared in 64 bits and returned in 32.  Row (s, b) of the logits begins (s * beams + b) * ld elements behind the first.
+ * 1 <= beams, keep <= 32, vocabulary below 2^31 - 65536.  Results must not lie in the inputs.
+ * `workspace`: flstm_beam_select_workspace_bytes() bytes, 16-byte aligned. */
+typedef struct {
+    size_t sequences;
+    int beams, keep;
+    size_t vocabulary;
+    const void* logits;
+    size_t ld;
+    flstm_op_dtype dtype;
+    const float* scores;
+    const unsigned char* finished;
+    long long end;
+} flstm_beams;
+
+size_t flstm_beam_select_workspace_bytes(const flstm_beams* problem);
+/* `finished` (of the results) may be null. */
+int flstm_beam_select(const flstm_beams* problem, float* scores, long long* parents, long long* tokens, unsigned char* finished,
+                      void* workspace, void* stream);
+
+/* Row (s, b) of each of `count` (at most 16) tensors becomes what row (s, parents[s][b]) was, in place.  Rows of `bytes` bytes begin
+ * (s * beams + b) * stride bytes behind data; 1 <= beams <= 32.  A parent outside 0 .. beams - 1 leaves its row as it is. */
+typedef struct {
+    void* data;
+    size_t stride, bytes;
+} flstm_beam_state;
+int flstm_beam_reorder(size_t sequences, int beams, const long long* parents, const flstm_beam_state* states, int count, void* stream);
 
 #ifdef __cplusplus
 }
