@@ -1,11 +1,12 @@
 // Beam search (lm_ops.h): the best continuations of every sequence's beams, and the beams' states moved behind them.
 //
 // The selection is bound by one reading of the logits.  A workgroup has a part of a row: the part's largest logit, the sum of its
-// exponentials, and its best entries, all from registers.  What takes part in the ordering are whole numbers, the logit's order
-// above and the place's complement below, so that no two are equal and equal logits come lowest place first; the k-th best of the
-// threads' own best entries is a bound that at least k entries reach, and only the k threads in front of it can hold others that
-// do.  A second kernel puts the parts together: the rows' logarithms, and the candidates' values in 64 bits, so that which of two
-// is larger does not depend on a rounding to 32.
+// exponentials, and its `keep` best entries, all from registers.  Its threads form at least `keep` groups; the smallest of the
+// groups' largest logits is a bound that `keep` entries reach and few others do (20 of 8192 random ones for 8, 110 for 32), so that what
+// is ordered is a short list.  Ordered are whole numbers, the logit's order above and the place's complement below: no two are equal,
+// and equal logits come lowest place first.  Of very many logits that are equal to the bound the lowest
+// places are listed, bounded the same way; where even that is too long, the best are taken out one by one.  A second kernel puts the parts together: the rows' logarithms, and the continuations' values in 64
+// bits, so that which of two is larger does not depend on a rounding to 32.
 #include "lm_device.h"
 
 namespace flstm_hip {
@@ -14,13 +15,15 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxKeep = 32, kMaxBeams = 32;
 constexpr int kVectors = 4, kTile = kThreads * kVectors * 8;   // logits a workgroup holds at a time
-constexpr size_t kMaxParts = 64;
+constexpr size_t kMaxParts = 64;   // one for each lane of a wave
+constexpr int kList = 1024;        // entries that are ordered at once
 constexpr float kLowest = -3.4028234663852886e38f, kHighest = 3.4028234663852886e38f;
 
 struct Select {
     size_t sequences, ld;
     int beams, keep, parts;
-    unsigned vocabulary, part;      // part: logits, a multiple of kTile
+    unsigned vocabulary, part;      // part: logits
+    int groups;                     // of threads, 4 to 32, a power of two, no fewer than `keep`
     const void* logits;
     const float* scores;
     const unsigned char* finished;  // or null
@@ -41,119 +44,194 @@ __device__ __forceinline__ unsigned order_of(float z) {
 __device__ __forceinline__ float logit_of(unsigned o) { return __builtin_bit_cast(float, o ^ (o >> 31 ? 0x80000000u : 0xffffffffu)); }
 __device__ __forceinline__ u64 key_of(float z, unsigned place) { return z > -__builtin_inff() ? u64(order_of(z)) << 32 | ~place : 0; }
 
-// A candidate of a sequence: its value as a whole number that orders alike (0: none), and its place among the sequence's.
-struct Candidate {
-    u64 order, place;
-};
-__device__ __forceinline__ bool ahead(u64 x, u64 y) { return x > y; }
-__device__ __forceinline__ bool ahead(const Candidate& x, const Candidate& y) { return x.order > y.order || (x.order == y.order && x.place < y.place); }
-__device__ __forceinline__ u64 better(u64 x, u64 y) { return x > y ? x : y; }
-__device__ __forceinline__ Candidate better(const Candidate& x, const Candidate& y) {
-    const bool first = ahead(x, y);
-    return Candidate{first ? x.order : y.order, first ? x.place : y.place};
-}
-__device__ __forceinline__ bool exists(u64 x) { return x != 0; }
-__device__ __forceinline__ bool exists(const Candidate& x) { return x.order != 0; }
-
-// The `keep` best of `best` (in LDS, best first, none behind the last) and of all threads' v[], no two of which are equal:
-// afterwards in `best`.
-template <class K, int N> struct Scratch {
-    K heads[kThreads + kMaxKeep];
-    K list[kMaxKeep * N + kMaxKeep];
-    K bound;
-    int count;
-};
-template <class K, int N> __device__ __forceinline__ void take_best(Scratch<K, N>& s, K* best, int keep, const K (&v)[N]) {
-    const int tid = threadIdx.x, all = kThreads + keep;
-    K own = v[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) own = better(own, v[i]);
-    __syncthreads();   // (`best` is there, and the last call's readers are done)
-    s.heads[tid] = own;
-    if (tid < keep) s.heads[kThreads + tid] = best[tid];
-    if (tid == 0) { s.bound = K{}; s.count = 0; }
-    __syncthreads();
-    const auto ranked = [&](const K& key) {
-        int rank = 0;
-        for (int i = 0; i < all; ++i) rank += ahead(s.heads[i], key);
-        if (exists(key) && rank == keep - 1) s.bound = key;
-    };
-    ranked(own);
-    if (tid < keep) ranked(best[tid]);
-    __syncthreads();
-    const K bound = s.bound;   // at most `keep` threads' heads are not behind it
-    const auto offer = [&](const K& key) {
-        if (exists(key) && !ahead(bound, key)) s.list[atomicAdd(&s.count, 1)] = key;
-    };
-    if (!ahead(bound, own))
-#pragma unroll
-        for (int i = 0; i < N; ++i) offer(v[i]);
-    if (tid < keep) offer(best[tid]);
-    __syncthreads();
-    const int count = s.count;
-    if (tid < keep && tid >= count) best[tid] = K{};
-    for (int i = tid; i < count; i += kThreads) {
-        const K key = s.list[i];
-        int rank = 0;
-        for (int j = 0; j < count; ++j) rank += ahead(s.list[j], key);
-        if (rank < keep) best[rank] = key;
+// A value folded over the lanes l, l + groups, l + 2 groups, .. of a wave.
+template <class Op> __device__ __forceinline__ float groups_fold(float v, int groups, Op op) {
+    unsigned u = __builtin_bit_cast(unsigned, v);
+    const auto across = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    v = op(__builtin_bit_cast(float, unsigned(across[0])), __builtin_bit_cast(float, unsigned(across[1])));
+    if (groups <= 16) {
+        u = __builtin_bit_cast(unsigned, v);
+        const auto rows = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        v = op(__builtin_bit_cast(float, unsigned(rows[0])), __builtin_bit_cast(float, unsigned(rows[1])));
     }
-}
-
-template <class Op> __device__ __forceinline__ float all_threads(float v, float* scratch, Op op) {
-    v = lanes_fold<kWave>(v, op);
-    __syncthreads();   // (the last one's readers are done)
-    if (threadIdx.x % kWave == 0) scratch[threadIdx.x / kWave] = v;
-    __syncthreads();
-    v = scratch[0];
-#pragma unroll
-    for (int w = 1; w < kThreads / kWave; ++w) v = op(v, scratch[w]);
+    if (groups <= 8) v = op(v, lane_moved<0x128>(v));   // row_ror 8
+    if (groups <= 4) v = op(v, lane_moved<0x124>(v));   // row_ror 4
     return v;
 }
 
+// A logit as a number: minus infinity for a NaN, the largest finite one for infinity.
+__device__ __forceinline__ float number(float x) { return x > -__builtin_inff() ? fminf(x, kHighest) : -__builtin_inff(); }
+
+// The largest of the workgroup's, in all threads.
+__device__ __forceinline__ u64 all_largest(u64 v, u64* scratch) {
+#pragma unroll
+    for (int d = kWave / 2; d > 0; d /= 2) {
+        const u64 other = __shfl_xor(v, d);
+        v = other > v ? other : v;
+    }
+    __syncthreads();
+    if (threadIdx.x % kWave == 0) scratch[threadIdx.x / kWave] = v;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kThreads / kWave; ++w) v = scratch[w] > v ? scratch[w] : v;
+    return v;
+}
+
+// The list again where very many logits are equal to the bound (those that a mask left at its type's lowest value, say): of these, those up to
+// a place that the first ones of all groups reach.  Returns how many there are then.
+template <class T> __device__ int fewer(const T* z, unsigned base, unsigned end, float bound, u64 before, int groups, u64* list,
+                                        float (*heads)[kMaxKeep], int& count) {
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+    const unsigned stop = end - base < unsigned(kTile) ? end - base : kTile;
+    float first = __builtin_inff();
+    for (unsigned c = tid; c < stop; c += kThreads) {
+        const float x = number(float(z[base + c]));
+        if (x >= bound) first = fminf(first, x > bound ? -1.f : float(c));   // (a group with one above it needs no equal one)
+    }
+    first = groups_fold(first, groups, [](float x, float y) { return fminf(x, y); });
+    __syncthreads();   // (the readers of `count` and `heads` are done)
+    if (lane < groups) heads[wave][lane] = first;
+    if (tid == 0) count = 0;
+    __syncthreads();
+    first = heads[0][lane % groups];
+    for (int w = 1; w < kThreads / kWave; ++w) first = fminf(first, heads[w][lane % groups]);
+    const float place = lanes_max<kWave>(first);
+    const auto offer = [&](u64 key) {
+        const int at = atomicAdd(&count, 1);
+        if (at < kList) list[at] = key;
+    };
+    for (unsigned c = tid; c < stop; c += kThreads) {
+        const float x = number(float(z[base + c]));
+        if (x > bound || (x == bound && float(c) <= place)) offer(key_of(x, base + c));
+    }
+    if (before) offer(before);
+    __syncthreads();
+    return count;
+}
+
 template <class T> __global__ __launch_bounds__(kThreads) void part_kernel(Select a) {
-    __shared__ Scratch<u64, kVectors * 8> scratch;
-    __shared__ u64 best[kMaxKeep];
-    __shared__ float waves[kThreads / kWave];
+    __shared__ u64 list[kList], best[kMaxKeep], largest[kThreads / kWave];
+    __shared__ float heads[kThreads / kWave][kMaxKeep], waves[kThreads / kWave];
+    __shared__ int count;
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
     const size_t block = a.first + blockIdx.x, row = block / unsigned(a.parts);
     const unsigned part = unsigned(block - row * unsigned(a.parts)), begin = part * a.part;
     const unsigned end = a.vocabulary - begin < a.part ? a.vocabulary : begin + a.part;
-    if (!(a.scores[row] > -__builtin_inff()) || (a.finished && a.finished[row])) return;   // (its candidates are not read)
+    if (!(a.scores[row] > -__builtin_inff()) || (a.finished && a.finished[row])) return;   // (its continuations are not read)
     const T* z = static_cast<const T*>(a.logits) + row * a.ld;
-    if (int(threadIdx.x) < a.keep) best[threadIdx.x] = 0;
+    if (tid < a.keep) best[tid] = 0;
     float most = kLowest, sum = 0.f;
     for (unsigned base = begin; base < end; base += kTile) {
-        float8 v[kVectors];
-        float m = most;
+        typename Vec8<T>::type v[kVectors];   // as they come: converted three times, in half the registers
+        float m = -__builtin_inff();
 #pragma unroll
         for (int j = 0; j < kVectors; ++j) {
-            const unsigned c = base + (j * kThreads + threadIdx.x) * 8;
-            const int n = c < end ? (end - c < 8 ? int(end - c) : 8) : 0;
-            v[j] = load8(z + c, n);
+            const unsigned c = base + (j * kThreads + tid) * 8;
+            if (c + 8 <= end) {
+                __builtin_memcpy(&v[j], __builtin_assume_aligned(z + c, sizeof(T)), sizeof(v[j]));
+            } else {
+                float8 w = load8(z + c, c < end ? int(end - c) : 0);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                v[j][i] = i < n && v[j][i] > -__builtin_inff() ? fminf(v[j][i], kHighest) : -__builtin_inff();   // (NaN: minus infinity)
-                m = fmaxf(m, v[j][i]);
+                for (int i = 0; i < 8; ++i) w[i] = c + i < end ? w[i] : -__builtin_inff();
+                v[j] = __builtin_convertvector(w, typename Vec8<T>::type);
             }
         }
+#pragma unroll
+        for (int j = 0; j < kVectors; ++j) {
+            asm volatile("" : "+v"(v[j]));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = fmaxf(m, float(v[j][i]));   // (a NaN is no one's maximum)
+        }
+        m = groups_fold(fminf(m, kHighest), a.groups, [](float x, float y) { return fmaxf(x, y); });
+        if (lane < a.groups) heads[wave][lane] = m;
+        if (tid == 0) count = 0;
+        __syncthreads();   // (`best` is there)
+        m = heads[0][lane % a.groups];
+#pragma unroll
+        for (int w = 1; w < kThreads / kWave; ++w) m = fmaxf(m, heads[w][lane % a.groups]);
+        float bound = lanes_fold<kWave>(m, [](float x, float y) { return fminf(x, y); });
+        bound = fmaxf(bound, kLowest);   // (minus infinity is no continuation)
+        if (base > begin && best[a.keep - 1]) bound = fmaxf(bound, logit_of(unsigned(best[a.keep - 1] >> 32)));
+        m = fmaxf(most, lanes_max<kWave>(m));
         sum *= __builtin_amdgcn_exp2f((most - m) * 1.4426950408889634f);
         most = m;
-        u64 keys[kVectors * 8];
+        float more = 0.f;
 #pragma unroll
-        for (int j = 0; j < kVectors; ++j)
+        for (int j = 0; j < kVectors; ++j) {
+            asm volatile("" : "+v"(v[j]));
+            float reach = -__builtin_inff();
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                sum += __builtin_amdgcn_exp2f((v[j][i] - most) * 1.4426950408889634f);
-                keys[j * 8 + i] = key_of(v[j][i], base + (j * kThreads + threadIdx.x) * 8 + i);
+                const float d = float(v[j][i]) - most;
+                more += __builtin_amdgcn_exp2f(d * 1.4426950408889634f);
+                reach = fmaxf(reach, d);
             }
-        take_best(scratch, best, a.keep, keys);
+            if (reach >= bound - most)   // (rounding keeps the order)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float x = number(float(v[j][i]));
+                    if (x >= bound) {
+                        const int at = atomicAdd(&count, 1);
+                        if (at < kList) list[at] = key_of(x, base + (j * kThreads + tid) * 8 + i);
+                    }
+                }
+        }
+        if (!(more < __builtin_inff())) {   // a NaN or an infinity among them: once more, without
+            more = 0.f;
+            for (int i = 0; i < kVectors * 8; ++i) {
+                const unsigned c = base + (i / 8 * kThreads + tid) * 8 + i % 8;
+                if (c < end) more += __builtin_amdgcn_exp2f((number(float(z[c])) - most) * 1.4426950408889634f);
+            }
+        }
+        sum += more;
+        if (base + kTile >= end) {
+            sum = lanes_sum<kWave>(sum);
+            if (lane == 0) waves[wave] = sum;
+        }
+        const u64 before = tid < a.keep ? best[tid] : 0;   // of the tiles in front
+        if (before) {
+            const int at = atomicAdd(&count, 1);
+            if (at < kList) list[at] = before;
+        }
+        __syncthreads();
+        int some = count;
+        if (some > kList) some = fewer(z, base, end, bound, before, a.groups, list, heads, count);
+        if (some <= kList) {
+            if (tid < a.keep && tid >= some) best[tid] = 0;
+            for (int i = tid; i < some; i += kThreads) {
+                const u64 key = list[i];
+                int rank = 0;
+                for (int j = 0; j < some; ++j) rank += list[j] > key;
+                if (rank < a.keep) best[rank] = key;
+            }
+        } else {
+            u64 last = ~u64(0);
+            for (int r = 0; r < a.keep; ++r) {
+                u64 key = before < last ? before : 0;
+                for (unsigned c = base + tid; c < end && c < base + kTile; c += kThreads) {
+                    const u64 k = key_of(number(float(z[c])), c);
+                    key = k < last && k > key ? k : key;
+                }
+                last = all_largest(key, largest);
+                if (tid == 0) best[r] = last;
+            }
+        }
+        __syncthreads();
     }
-    const float m = all_threads(most, waves, [](float x, float y) { return fmaxf(x, y); });
-    const float s = all_threads(sum * __builtin_amdgcn_exp2f((most - m) * 1.4426950408889634f), waves, [](float x, float y) { return x + y; });
-    if (threadIdx.x == 0) a.sums[block] = float2{m, s};
-    if (int(threadIdx.x) < a.keep) a.best[block * a.keep + threadIdx.x] = best[threadIdx.x];
+    if (tid == 0) {
+        float s = waves[0];
+#pragma unroll
+        for (int w = 1; w < kThreads / kWave; ++w) s += waves[w];
+        a.sums[block] = float2{most, s};
+    }
+    if (tid < a.keep) a.best[block * a.keep + tid] = best[tid];
 }
 
+// A continuation of a sequence: its value as a whole number that orders alike (0: none), and its place among the sequence's.
+struct Candidate {
+    u64 order, place;
+};
+__device__ __forceinline__ bool ahead(const Candidate& x, const Candidate& y) { return x.order > y.order || (x.order == y.order && x.place < y.place); }
 __device__ __forceinline__ u64 order_of(double v) {
     const u64 u = __builtin_bit_cast(u64, v);
     return u ^ (u64(static_cast<long long>(u) >> 63) | u64(1) << 63);
@@ -161,47 +239,94 @@ __device__ __forceinline__ u64 order_of(double v) {
 __device__ __forceinline__ double value_of(u64 o) { return __builtin_bit_cast(double, o ^ (o >> 63 ? u64(1) << 63 : ~u64(0))); }
 
 __global__ __launch_bounds__(kThreads) void join_kernel(Select a) {
-    constexpr int kEach = 16;
-    __shared__ Scratch<Candidate, kEach> scratch;
-    __shared__ Candidate best[kMaxKeep];
-    __shared__ double most[kMaxBeams], log_sum[kMaxBeams];
+    __shared__ Candidate list[kList], best[kMaxKeep];
+    __shared__ u64 heads[kThreads / kWave][kMaxKeep], largest[kThreads / kWave];
+    __shared__ double most[kMaxBeams], rest[kMaxBeams];   // a row's largest logit; what its difference to one is off by
+    __shared__ int state[kMaxBeams];        // of a hypothesis: 0 none, 1 alive, 2 finished
+    __shared__ int count;
     const size_t sequence = a.first + blockIdx.x, row0 = sequence * a.beams;
-    const int tid = threadIdx.x;
-    const auto done = [&](int b) { return a.finished && a.finished[row0 + b]; };
-    if (tid < a.beams && a.scores[row0 + tid] > -__builtin_inff() && !done(tid)) {
-        const float2* sums = a.sums + (row0 + tid) * a.parts;
-        float m = kLowest;
-        for (int p = 0; p < a.parts; ++p) m = fmaxf(m, sums[p].x);
-        double s = 0;
-        for (int p = 0; p < a.parts; ++p) s += double(sums[p].y) * exp(double(sums[p].x) - double(m));
-        most[tid] = m;
-        log_sum[tid] = log(s);
-    }
-    __syncthreads();
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
     const int per = a.parts * a.keep, all = a.beams * per;
+    for (int b = wave; b < a.beams; b += kThreads / kWave) {
+        const float score = a.scores[row0 + b];
+        const bool done = a.finished && a.finished[row0 + b], alive = score > -__builtin_inff() && !done;
+        float2 p{kLowest, 0.f};
+        if (alive && lane < a.parts) p = a.sums[(row0 + b) * a.parts + lane];
+        const float m = lanes_max<kWave>(p.x), s = lanes_sum<kWave>(p.y * __builtin_amdgcn_exp2f((p.x - m) * 1.4426950408889634f));
+        if (lane == 0) {
+            most[b] = m;
+            rest[b] = done ? double(score) : double(score) - log(double(s));
+            state[b] = !(score > -__builtin_inff()) ? 0 : done ? 2 : 1;
+        }
+    }
+    if (tid < a.keep) best[tid] = Candidate{0, 0};
+    if (tid == 0) count = 0;
+    __syncthreads();
     const auto candidate = [&](int i) {
         const int b = i / per;
-        const float score = a.scores[row0 + b];
-        if (!(score > -__builtin_inff())) return Candidate{0, 0};
-        if (done(b)) return i == b * per ? Candidate{order_of(double(score)), u64(b) * a.vocabulary + u64(a.end)} : Candidate{0, 0};
-        const u64 key = a.best[row0 * per + i];
-        if (key == 0) return Candidate{0, 0};
-        return Candidate{order_of(double(logit_of(unsigned(key >> 32))) - most[b] - log_sum[b] + double(score)), u64(b) * a.vocabulary + unsigned(~key)};
+        const u64 row = u64(b) * a.vocabulary;
+        if (state[b] == 2) return i == b * per ? Candidate{order_of(rest[b]), row + u64(a.end)} : Candidate{0, 0};
+        const u64 key = state[b] == 1 ? a.best[row0 * per + i] : 0;
+        return key ? Candidate{order_of(double(logit_of(unsigned(key >> 32))) - most[b] + rest[b]), row + unsigned(~key)} : Candidate{0, 0};
     };
-    if (tid < a.keep) best[tid] = Candidate{0, 0};
-    for (int base = 0; base < all; base += kThreads * kEach) {
-        Candidate v[kEach];
+    u64 head = 0;
+    const Candidate own = tid < all ? candidate(tid) : Candidate{0, 0};   // (most calls have no more)
+    head = own.order;
+    for (int i = tid + kThreads; i < all; i += kThreads) {
+        const u64 o = candidate(i).order;
+        head = o > head ? o : head;
+    }
+    for (int d = kWave / 2; d >= a.groups; d /= 2) {
+        const u64 other = __shfl_xor(head, d);
+        head = other > head ? other : head;
+    }
+    if (lane < a.groups) heads[wave][lane] = head;
+    __syncthreads();
+    u64 bound = heads[0][lane % a.groups];
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-            const int i = base + j * kThreads + tid;
-            v[j] = i < all ? candidate(i) : Candidate{0, 0};
+    for (int w = 1; w < kThreads / kWave; ++w) bound = heads[w][lane % a.groups] > bound ? heads[w][lane % a.groups] : bound;
+    for (int d = a.groups / 2; d > 0; d /= 2) {
+        const u64 other = __shfl_xor(bound, d);
+        bound = other < bound ? other : bound;
+    }
+    const auto offer = [&](const Candidate& c) {
+        if (c.order && c.order >= bound) {
+            const int at = atomicAdd(&count, 1);
+            if (at < kList) list[at] = c;
         }
-        take_best(scratch, best, a.keep, v);
+    };
+    offer(own);
+    for (int i = tid + kThreads; i < all; i += kThreads) offer(candidate(i));
+    __syncthreads();
+    const int some = count;
+    if (some <= kList) {
+        for (int i = tid; i < some; i += kThreads) {
+            const Candidate c = list[i];
+            int rank = 0;
+            for (int j = 0; j < some; ++j) rank += ahead(list[j], c);
+            if (rank < a.keep) best[rank] = c;
+        }
+    } else {
+        u64 last = ~u64(0), last_place = 0;
+        for (int r = 0; r < a.keep; ++r) {   // the largest value behind the last one, and the lowest place that has it
+            u64 o = 0, place = ~u64(0);
+            for (int i = tid; i < all; i += kThreads) {
+                const Candidate c = candidate(i);
+                if (c.order && (c.order < last || (c.order == last && c.place > last_place)) && (c.order > o || (c.order == o && c.place < place))) {
+                    o = c.order;
+                    place = c.place;
+                }
+            }
+            last = all_largest(o, largest);
+            last_place = ~all_largest(o == last ? ~place : 0, largest);
+            if (tid == 0 && last) best[r] = Candidate{last, last_place};
+            if (!last) break;
+        }
     }
     __syncthreads();
     if (tid >= a.keep) return;
     const Candidate c = best[tid];
-    const bool there = exists(c);
+    const bool there = c.order != 0;
     const u64 b = c.place / a.vocabulary;
     const long long token = there ? (long long)(c.place - b * a.vocabulary) : -1;
     const size_t o = sequence * a.keep + tid;
@@ -278,7 +403,11 @@ bool valid(const flstm_beams* p) {
            p->keep <= kMaxKeep && p->vocabulary >= 1 && p->vocabulary < (size_t(1) << 31) - 65536 && p->ld >= p->vocabulary &&
            (!p->finished || (p->end >= 0 && p->end < (long long)p->vocabulary)) && (p->sequences == 0 || (p->logits && p->scores));
 }
-size_t part_of(const flstm_beams* p) { return round_up(ceil_div(p->vocabulary, kMaxParts), kTile); }
+// Rows in parts of about one size, none above kTile as long as kMaxParts are enough.
+size_t part_of(const flstm_beams* p) {
+    const size_t parts = ceil_div(p->vocabulary, kTile);
+    return round_up(ceil_div(p->vocabulary, parts < kMaxParts ? parts : kMaxParts), 64);
+}
 size_t parts_of(const flstm_beams* p) { return ceil_div(p->vocabulary, part_of(p)); }
 size_t best_bytes(const flstm_beams* p) { return round_up(p->sequences * p->beams * parts_of(p) * p->keep * sizeof(u64), 16); }
 
@@ -299,6 +428,8 @@ extern "C" int flstm_beam_select(const flstm_beams* p, float* scores, long long*
     Select a{};
     a.sequences = p->sequences; a.ld = p->ld; a.beams = p->beams; a.keep = p->keep; a.vocabulary = unsigned(p->vocabulary);
     a.part = unsigned(part_of(p)); a.parts = int(parts_of(p)); a.logits = p->logits; a.scores = p->scores; a.finished = p->finished;
+    a.groups = 4;
+    while (a.groups < a.keep) a.groups *= 2;
     a.end = p->end; a.best = static_cast<u64*>(workspace); a.sums = reinterpret_cast<float2*>(static_cast<char*>(workspace) + best_bytes(p));
     a.out_scores = scores; a.out_parents = parents; a.out_tokens = tokens; a.out_finished = finished;
     const size_t blocks = p->sequences * p->beams * a.parts;

@@ -1,17 +1,19 @@
 // Embedding of tokens with a scale, and its gradient by sorted tokens (lm_ops.h).
 //
 // Both are bound by memory.  The lookup copies rows; a thread takes vectors of eight, whatever the width, so that no lane idles where
-// a row is no multiple of a wave.  The gradient sorts the tokens with their positions (stable, eight to ten bits of the token at a
-// time), after which the rows of one token lie behind one another: chunks of the sorted list are summed in registers, in the order of the
-// positions, and written once where a token's rows end.  What crosses a chunk's border is left as partial sums that a last
-// kernel adds up in order.  No atomics on values: the result depends on tokens and sizes alone.
+// a row is no multiple of a wave.  The gradient sorts the tokens with their positions, stable, after which the rows of one token lie behind one
+// another: chunks of the sorted list are summed in registers, in the order of the positions, and written once where a token's rows end.  What
+// crosses a chunk's border is put together in LDS by the workgroup, whose chunks follow each other, and what crosses the workgroup's is left as partial
+// sums that a last kernel adds up in order.  No atomics on values: the result depends on tokens and sizes alone.
+// Few tokens are sorted by counting for each how many come in front of it, in one launch; many in stable passes over eight to ten bits.
+#include <type_traits>
+
 #include "lm_device.h"
 
 namespace flstm_hip {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kChunk = 32;   // sorted positions a thread sums
 
 struct Tokens {
     size_t count;
@@ -25,30 +27,106 @@ __device__ __forceinline__ unsigned token_at(const Tokens& t, size_t i) {
     return v >= 0 && v < (long long)t.vocabulary ? unsigned(v) : t.vocabulary;
 }
 
+// Vector v of a row: eight columns from the returned one on, which the last two vectors of a width that is no multiple of eight have in part in
+// common; what is common is computed and written twice, alike.  So no lane has a branch of its own, behind which its loads would be waited for one
+// by one.  Rows of less than eight columns (kNarrow) are one vector.
+template <bool kNarrow> __device__ __forceinline__ size_t column(size_t v, size_t width) {
+    return kNarrow ? 0 : v * 8 + 8 <= width ? v * 8 : width - 8;
+}
+template <bool kNarrow, bool kPassing, class T> __device__ __forceinline__ float8 load_vector(const T* p, size_t width) {
+    typedef typename Vec8<T>::type __attribute__((aligned(sizeof(T)))) U;
+    if constexpr (kNarrow) return load8(p, int(width));
+    else if constexpr (kPassing) return __builtin_convertvector(__builtin_nontemporal_load(reinterpret_cast<const U*>(p)), float8);
+    else return load8(p);
+}
+template <bool kPassing, class V, class T> __device__ __forceinline__ void store_any(T* p, V v) {
+    typedef V __attribute__((aligned(sizeof(T)))) U;
+    if constexpr (kPassing) __builtin_nontemporal_store(v, reinterpret_cast<U*>(p));
+    else *reinterpret_cast<U*>(p) = v;
+}
+template <bool kNarrow, bool kPassing, class T> __device__ __forceinline__ void store_vector(T* p, float8 v, size_t width) {
+    if constexpr (kNarrow) store8(p, v, int(width));
+    else store_any<kPassing>(p, __builtin_convertvector(v, typename Vec8<T>::type));
+}
+// Beyond what the L2s hold, looked-up rows and rows of zeros are written past them, and what the gradient sums is read past them (kPassing):
+// 65536 rows of 1024 fp16 are looked up in 39 us instead of 48, and their gradient's 50001 rows of 1024 fp32 take 65 instead of 80.
+constexpr size_t kMostKept = size_t(32) << 20;   // bytes
+
 // ---- the lookup
+
+constexpr int kLookups = 2;   // vectors a thread has on their way
 
 struct Lookup {
     Tokens t;
-    unsigned vectors;   // a row
-    size_t first, items, width, ld;
+    unsigned vectors, items;   // a row; a launch
+    size_t first, width, ld;   // first: the launch's first row
     const void* table;
     void* out;
     float scale;
 };
 
-template <class From, class To> __global__ __launch_bounds__(kThreads) void lookup_kernel(Lookup a) {
-    const size_t item = a.first + size_t(blockIdx.x) * kThreads + threadIdx.x;
-    if (item >= a.items) return;
-    const size_t row = item / a.vectors;
-    const size_t c = (item - row * a.vectors) * 8;
-    const unsigned token = token_at(a.t, row);
-    const int n = a.width - c < 8 ? int(a.width - c) : 8;
-    float8 v = 0.f;
-    if (token < a.t.vocabulary) v = a.scale * load8(static_cast<const From*>(a.table) + token * a.ld + c, n);
-    store8(static_cast<To*>(a.out) + row * a.width + c, v, n);
+template <class From, class To, bool kNarrow, bool kPassing> __global__ __launch_bounds__(kThreads) void lookup_kernel(Lookup a) {
+    unsigned token[kLookups];
+    To* out[kLookups];
+    float8 v[kLookups];
+    const unsigned item = blockIdx.x * (kThreads * kLookups) + threadIdx.x;
+    const auto there = [&](int j) { return item + j * kThreads < a.items; };
+#pragma unroll
+    for (int j = 0; j < kLookups; ++j) {
+        const unsigned i = there(j) ? item + j * kThreads : 0, r = i / a.vectors;
+        const size_t row = a.first + r, c = column<kNarrow>(i - r * a.vectors, a.width);
+        token[j] = token_at(a.t, row);
+        out[j] = static_cast<To*>(a.out) + row * a.width + c;
+        v[j] = load_vector<kNarrow, false>(static_cast<const From*>(a.table) + (token[j] < a.t.vocabulary ? token[j] : 0) * a.ld + c, a.width);
+    }
+#pragma unroll
+    for (int j = 0; j < kLookups; ++j) {
+        const float8 zero = 0.f;
+        if (there(j)) store_vector<kNarrow, kPassing>(out[j], token[j] < a.t.vocabulary ? a.scale * v[j] : zero, a.width);
+    }
 }
 
-// ---- sorting: one stable pass over some bits of the token.  A workgroup has a tile of consecutive entries, each of its waves a
+// ---- sorting few tokens: an entry's place is the number of those in front of it.  A workgroup has 64 entries, each of its waves a
+// part of all others.
+
+constexpr int kRankThreads = 1024, kRankWaves = kRankThreads / kWave;
+constexpr size_t kMostRanked = 8192;
+
+__global__ __launch_bounds__(kRankThreads) void rank_kernel(Tokens t, unsigned* keys_out, unsigned* at_out) {
+    extern __shared__ unsigned keys[];   // all of them, rounded up to whole fours a wave, and kRankWaves rows of kWave counts
+    const unsigned count = unsigned(t.count), part = (count + kRankWaves * 4 - 1) / (kRankWaves * 4) * 4, whole = part * kRankWaves;
+    unsigned* counts = keys + whole;
+    for (unsigned i = threadIdx.x; i < whole; i += kRankThreads) keys[i] = i < count ? token_at(t, i) : ~0u;   // (behind all others)
+    __syncthreads();
+    const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave, first = blockIdx.x * kWave, i = first + lane;
+    const unsigned key = i < whole ? keys[i] : ~0u, from = wave * part, to = from + part;
+    unsigned rank = 0;
+    typedef unsigned uint4v __attribute__((ext_vector_type(4)));
+    const auto among = [&](unsigned begin, unsigned end, auto&& ahead) {
+        if (begin < from) begin = from;
+        if (end > to) end = to;
+#pragma unroll 4
+        for (unsigned j = begin; j < end; j += 4) {
+            const uint4v k = *reinterpret_cast<const uint4v*>(keys + j);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) rank += ahead(k[e], j + e);
+        }
+    };
+    among(0, first, [&](unsigned k, unsigned) { return k <= key; });
+    among(first, first + kWave, [&](unsigned k, unsigned j) { return k < key || (k == key && j < i); });
+    among(first + kWave, whole, [&](unsigned k, unsigned) { return k < key; });
+    counts[wave * kWave + lane] = rank;
+    __syncthreads();
+    if (wave == 0 && i < count) {
+        rank = 0;
+#pragma unroll
+        for (int w = 0; w < kRankWaves; ++w) rank += counts[w * kWave + lane];
+        keys_out[rank] = key;
+        at_out[rank] = i;
+    }
+}
+
+// ---- sorting many tokens: one stable pass over some bits of the token.  A workgroup has a tile of consecutive entries, each of its waves a
 // consecutive part of that, 64 entries at a time in order.
 
 constexpr int kSortThreads = 512, kSortWaves = kSortThreads / kWave, kMaxBits = 10;
@@ -74,7 +152,7 @@ __global__ __launch_bounds__(kSortThreads) void count_kernel(SortPass a) {
 
 __global__ __launch_bounds__(kSortThreads) void scatter_kernel(SortPass a) {
     __shared__ unsigned place[kSortWaves][1 << kMaxBits];   // counts of each wave's part, then where its next entry goes
-    __shared__ unsigned sums[kSortThreads];
+    __shared__ unsigned sums[kSortWaves];
     const unsigned bins = 1u << a.bits, wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
     const unsigned begin = blockIdx.x * a.tile, end = a.count - begin < a.tile ? a.count : begin + a.tile;
     const unsigned part = a.tile / kSortWaves, from = begin + wave * part;
@@ -88,23 +166,27 @@ __global__ __launch_bounds__(kSortThreads) void scatter_kernel(SortPass a) {
     for (unsigned j = 0; j < (1 << kMaxBits) / kSortThreads; ++j) {
         before[j] = total[j] = 0;
         const unsigned b = threadIdx.x * per + j;
-        if (j < per && b < bins)
+        if (j < per && b < bins) {
+            const unsigned* n = a.counts + b;
+#pragma unroll 16
             for (unsigned tile = 0; tile < a.tiles; ++tile) {
-                const unsigned n = a.counts[size_t(tile) * bins + b];
-                total[j] += n;
-                before[j] += tile < blockIdx.x ? n : 0;
+                const unsigned v = n[size_t(tile) * bins];
+                total[j] += v;
+                before[j] += tile < blockIdx.x ? v : 0;
             }
+        }
         all += total[j];
     }
-    sums[threadIdx.x] = all;
-    __syncthreads();
-    for (unsigned d = 1; d < kSortThreads; d *= 2) {
-        const unsigned v = threadIdx.x >= d ? sums[threadIdx.x - d] : 0;
-        __syncthreads();
-        sums[threadIdx.x] += v;
-        __syncthreads();
+    unsigned at = all;   // the sum over the threads up to this one
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+        const unsigned v = __shfl_up(at, d);
+        at += int(lane) >= d ? v : 0;
     }
-    unsigned at = sums[threadIdx.x] - all;
+    if (lane == kWave - 1) sums[wave] = at;
+    __syncthreads();
+    at -= all;
+    for (unsigned w = 0; w < wave; ++w) at += sums[w];
 #pragma unroll
     for (unsigned j = 0; j < (1 << kMaxBits) / kSortThreads; ++j) {
         const unsigned b = threadIdx.x * per + j;
@@ -147,85 +229,170 @@ __global__ __launch_bounds__(kSortThreads) void scatter_kernel(SortPass a) {
 // ---- the gradient from sorted tokens
 
 struct Sums {
-    unsigned count, vocabulary, vectors, chunks;
+    unsigned count, vocabulary, vectors, groups, slabs;   // groups: of kThreads / LANES chunks; slabs: of LANES vectors
+    int chunk;                                            // entries
     size_t width, ldd;
     const unsigned *keys, *at;
     const void* d_out;
     void* d_table;
-    float* partials;   // [chunk][entries of a token that began before; of one that goes on behind][width]
+    float* partials;   // [group][entries of a token that began before; of one that goes on behind][width]
     float scale;
     unsigned sum_blocks;
 };
 
-constexpr int kZeroRows = 64;   // rows of the table that a workgroup looks for among the tokens
+constexpr int kMaxChunk = 32, kZeroRows = 64;   // rows of the table that a workgroup looks for among the tokens
 
-template <class From, class To> __global__ __launch_bounds__(kThreads) void sum_kernel(Sums a) {
-    if (blockIdx.x >= a.sum_blocks) {   // rows without a token
-        __shared__ int empty[kZeroRows];
-        const size_t row0 = size_t(blockIdx.x - a.sum_blocks) * kZeroRows;
-        if (threadIdx.x < kZeroRows) {
-            const unsigned row = unsigned(row0) + threadIdx.x;
-            unsigned lo = 0, hi = a.count;   // the first entry whose token is not below the row
-            while (lo < hi) {
-                const unsigned mid = lo + (hi - lo) / 2;
-                if (a.keys[mid] < row) lo = mid + 1; else hi = mid;
-            }
-            empty[threadIdx.x] = row < a.vocabulary && (lo == a.count || a.keys[lo] != row);
-        }
-        __syncthreads();
-        const float8 zero = 0.f;
-        for (unsigned i = threadIdx.x; i < kZeroRows * a.vectors; i += kThreads) {
-            const unsigned r = i / a.vectors;
-            const size_t c = size_t(i - r * a.vectors) * 8;
-            if (empty[r]) store8(static_cast<To*>(a.d_table) + (row0 + r) * a.width + c, zero, a.width - c < 8 ? int(a.width - c) : 8);
-        }
-        return;
+template <class To, bool kNarrow, bool kPassing> __device__ __forceinline__ void zero_rows(const Sums& a, size_t row0) {
+    __shared__ int empty[kZeroRows];
+    // the entries of these rows, [lo, hi): all threads look at as many places at a time
+    unsigned lo = 0, hi = a.count, lo_end = a.count, hi_begin = 0;
+    const unsigned row1 = row0 + kZeroRows < a.vocabulary ? unsigned(row0) + kZeroRows : a.vocabulary;
+    if (threadIdx.x < kZeroRows) empty[threadIdx.x] = 1;
+    while (lo < lo_end || hi_begin < hi) {   // the first entry not below row0 lies in [lo, lo_end], the first not below row1 in [hi_begin, hi]
+        const unsigned step = (lo_end - lo) / kThreads + 1, step1 = (hi - hi_begin) / kThreads + 1;
+        const unsigned i = lo + threadIdx.x * step, i1 = hi_begin + threadIdx.x * step1;
+        const unsigned key = i < lo_end ? a.keys[i] : ~0u, key1 = i1 < hi ? a.keys[i1] : ~0u;
+        const unsigned below = __syncthreads_count(key < row0), below1 = __syncthreads_count(key1 < row1);
+        const unsigned end = lo + below * step, end1 = hi_begin + below1 * step1;
+        lo = below ? end - step + 1 : lo;
+        lo_end = below == 0 ? lo : end < lo_end ? end : lo_end;
+        hi_begin = below1 ? end1 - step1 + 1 : hi_begin;
+        hi = below1 == 0 ? hi_begin : end1 < hi ? end1 : hi;
     }
-    const size_t item = size_t(blockIdx.x) * kThreads + threadIdx.x;
-    const unsigned chunk = unsigned(item / a.vectors);
-    if (chunk >= a.chunks) return;
-    const size_t c = (item - size_t(chunk) * a.vectors) * 8;
-    const int n = a.width - c < 8 ? int(a.width - c) : 8;
-    const unsigned begin = chunk * kChunk, end = a.count - begin < kChunk ? a.count : begin + kChunk;
-    const From* d = static_cast<const From*>(a.d_out) + c;
-    To* out = static_cast<To*>(a.d_table) + c;
-    float* partial = a.partials + size_t(chunk) * 2 * a.width + c;
-    unsigned token = a.keys[begin];
-    bool began = begin == 0 || a.keys[begin - 1] != token;   // the token's entries begin in this chunk
-    float8 sum = 0.f;
-    for (unsigned i = begin; i < end; ++i) {
-        const unsigned next = a.keys[i];
-        if (next != token) {
-            if (began) store8(out + size_t(token) * a.width, a.scale * sum, n);
-            else store8(partial, sum, n);
-            began = true;
-            token = next;
-            sum = 0.f;
+    if (hi - lo <= 4 * kThreads) {
+        for (unsigned i = lo + threadIdx.x; i < hi; i += kThreads) empty[a.keys[i] - unsigned(row0)] = 0;
+    } else if (threadIdx.x < kZeroRows && row0 + threadIdx.x < row1) {
+        const unsigned row = unsigned(row0) + threadIdx.x;
+        unsigned first = lo, end = hi;
+        while (first < end) {
+            const unsigned mid = first + (end - first) / 2;
+            if (a.keys[mid] < row) first = mid + 1; else end = mid;
         }
-        if (token >= a.vocabulary) return;
-        sum += load8(d + a.at[i] * a.ldd, n);
+        empty[threadIdx.x] = first == hi || a.keys[first] != row;
     }
-    const bool ends = end == a.count || a.keys[end] != token;
-    if (began && ends) store8(out + size_t(token) * a.width, a.scale * sum, n);
-    else store8(partial + (began ? a.width : 0), sum, n);
+    __syncthreads();
+    // a wave a row, sixteen bytes a lane and store
+    constexpr int kPiece = 16 / int(sizeof(To));
+    typedef To Piece __attribute__((ext_vector_type(kPiece)));
+    const Piece zero = To(0.f);
+    for (unsigned r = threadIdx.x / kWave; r < row1 - unsigned(row0); r += kThreads / kWave) {
+        if (!empty[r]) continue;
+        To* out = static_cast<To*>(a.d_table) + (row0 + r) * a.width;
+        if constexpr (kNarrow) {
+            if (threadIdx.x % kWave < a.width) out[threadIdx.x % kWave] = To(0.f);
+        } else {
+            for (size_t i = threadIdx.x % kWave * kPiece; i < a.width; i += kWave * kPiece)
+                store_any<kPassing>(out + (i + kPiece <= a.width ? i : a.width - kPiece), zero);
+        }
+    }
 }
 
-// What each token's entries left in more than one chunk: the chunk that they begin in adds them up.
-template <class To> __global__ __launch_bounds__(kThreads) void join_kernel(Sums a) {
+// A thread sums the entries of one chunk in one vector of columns; kThreads / LANES chunks behind one another and LANES vectors beside one
+// another are a workgroup's.
+template <class From, class To, int LANES, bool kNarrow, bool kPassing> __global__ __launch_bounds__(kThreads) void sum_kernel(Sums a) {
+    constexpr int kChunks = kThreads / LANES, kRows = sizeof(From) == 2 ? 8 : 4;   // rows on their way to a thread
+    if (blockIdx.x >= a.sum_blocks) return zero_rows<To, kNarrow, kPassing>(a, size_t(blockIdx.x - a.sum_blocks) * kZeroRows);
+    __shared__ unsigned keys[kChunks * kMaxChunk + 2], at[kChunks * kMaxChunk];   // keys: with those in front of and behind the workgroup's
+    __shared__ float8 heads[kChunks][LANES], tails[kChunks][LANES];
+    const unsigned group = blockIdx.x / a.slabs, slab = blockIdx.x - group * a.slabs;
+    const int size = kChunks * a.chunk, tid = threadIdx.x, chunk = tid / LANES;
+    int lane = tid % LANES;
+    const unsigned begin = group * size;
+    const int here = a.count - begin < unsigned(size) ? int(a.count - begin) : size;
+    constexpr unsigned kNone = ~0u;   // no token, and not the one behind the vocabulary
+    for (int i = tid; i < size + 2; i += kThreads) keys[i] = i <= here + 1 && (i > 0 || group > 0) && begin + i - 1 < a.count ? a.keys[begin + i - 1] : kNone;
+    for (int i = tid; i < size; i += kThreads) at[i] = a.at[i < here ? begin + i : begin];   // (any row, where there is none)
+    __syncthreads();
+    if (slab * LANES + lane >= a.vectors) lane = a.vectors - 1 - slab * LANES;   // (a slab's last lanes do the last one's work again)
+    const size_t c = column<kNarrow>(slab * LANES + lane, a.width);
+    const From* d = static_cast<const From*>(a.d_out) + c;
+    To* out = static_cast<To*>(a.d_table) + c;
+    const auto put = [&](unsigned row, float8 v) { store_vector<kNarrow, false>(out + size_t(row) * a.width, a.scale * v, a.width); };
+    const unsigned* key = keys + 1;
+    const int from = chunk * a.chunk, to = from + a.chunk;
+    unsigned token = key[from];
+    float8 sum = 0.f;
+    bool began = key[from - 1] != token;   // the token's entries begin in this chunk
+    for (int i = from; i < to; i += kRows) {
+        float8 row[kRows];
+        unsigned next[kRows];
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+            next[r] = key[i + r];
+            row[r] = load_vector<kNarrow, kPassing>(d + at[i + r] * a.ldd, a.width);
+        }
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+            if (next[r] != token) {
+                if (!began) heads[chunk][lane] = sum;
+                else if (token < a.vocabulary) put(token, sum);
+                began = true;
+                token = next[r];
+                sum = 0.f;
+            }
+            sum += row[r];
+        }
+    }
+    if (began && key[to] != token) {
+        if (token < a.vocabulary) put(token, sum);
+    } else if (began) {
+        tails[chunk][lane] = sum;
+    } else {
+        heads[chunk][lane] = sum;
+    }
+    __syncthreads();
+    // what crosses the chunks' borders, in order
+    if (chunk > 0) return;
+    sum = 0.f;
+    began = false;
+    float* partial = a.partials + size_t(group) * 2 * a.width + c;
+#pragma unroll 4
+    for (int k = 0; k < kChunks; ++k) {
+        const int first = k * a.chunk, last = first + a.chunk - 1;
+        const unsigned front = key[first - 1], head = key[first], tail = key[last], behind = key[last + 1];
+        const float8 of_head = heads[k][lane], of_tail = tails[k][lane];
+        const bool enters = head < a.vocabulary && front == head, leaves = tail < a.vocabulary && behind == tail, whole = enters && head == tail;
+        if (enters) sum += of_head;
+        if (enters && !(whole && leaves)) {
+            if (began) put(head, sum);
+            else store_vector<kNarrow, false>(partial, sum, a.width);
+        }
+        if (leaves && !whole) {
+            sum = of_tail;
+            began = true;
+        }
+    }
+    const unsigned tail = key[size - 1];
+    if (tail < a.vocabulary && key[size] == tail) store_vector<kNarrow, false>(partial + (began ? a.width : 0), sum, a.width);
+}
+
+// What each token's entries left in more than one group: the group that they begin in adds them up.
+template <class To, bool kNarrow> __global__ __launch_bounds__(kThreads) void join_kernel(Sums a, unsigned size) {
     const size_t item = size_t(blockIdx.x) * kThreads + threadIdx.x;
-    unsigned chunk = unsigned(item / a.vectors);
-    if (chunk + 1 >= a.chunks) return;   // (the last one's end)
-    const size_t c = (item - size_t(chunk) * a.vectors) * 8;
-    const int n = a.width - c < 8 ? int(a.width - c) : 8;
-    const unsigned begin = chunk * kChunk, last = begin + kChunk - 1, token = a.keys[last];
-    if (token >= a.vocabulary || a.keys[last + 1] != token || (begin > 0 && a.keys[begin - 1] == token && a.keys[begin] == token)) return;
+    unsigned group = unsigned(item / a.vectors);
+    if (group + 1 >= a.groups) return;
+    const size_t c = column<kNarrow>(item - size_t(group) * a.vectors, a.width);
+    const unsigned begin = group * size, last = begin + size - 1, token = a.keys[last];
+    if (token >= a.vocabulary || a.keys[last + 1] != token || (begin > 0 && a.keys[begin - 1] == token)) return;
     const float* partial = a.partials + c;
-    float8 sum = load8(partial + (size_t(chunk) * 2 + 1) * a.width, n);
-    do {
-        ++chunk;
-        sum += load8(partial + size_t(chunk) * 2 * a.width, n);
-    } while (chunk + 1 < a.chunks && a.keys[chunk * kChunk + kChunk] == token);
-    store8(static_cast<To*>(a.d_table) + size_t(token) * a.width + c, a.scale * sum, n);
+    float8 sum = load_vector<kNarrow, false>(partial + (size_t(group) * 2 + 1) * a.width, a.width);
+    constexpr int kAhead = 8;
+    for (bool more = true; more;) {
+        float8 v[kAhead];
+        bool there[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const unsigned g = group + 1 + j < a.groups ? group + 1 + j : a.groups - 1;
+            there[j] = group + 1 + j < a.groups && a.keys[g * size] == token;
+            v[j] = load_vector<kNarrow, false>(partial + size_t(g) * 2 * a.width, a.width);
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+            if (there[j]) sum += v[j];
+        more = there[kAhead - 1];
+        group += kAhead;
+    }
+    store_vector<kNarrow, false>(static_cast<To*>(a.d_table) + size_t(token) * a.width + c, a.scale * sum, a.width);
 }
 
 // ---- host side
@@ -248,18 +415,36 @@ SortPlan sort_plan(const flstm_embedding* p) {
     SortPlan s;
     s.passes = (bits + kMaxBits - 1) / kMaxBits;
     s.bits = (bits + s.passes - 1) / s.passes;
-    const size_t tile = round_up(ceil_div(p->tokens, 256), kSortThreads);
-    s.tile = unsigned(tile < 2048 ? 2048 : tile);
+    const size_t tile = round_up(ceil_div(p->tokens, 128), kSortThreads);
+    s.tile = unsigned(tile < 1024 ? 1024 : tile);
     s.tiles = unsigned(ceil_div(p->tokens, s.tile));
     return s;
 }
+bool ranked(const flstm_embedding* p) { return p->tokens <= kMostRanked; }
+
+// Lanes beside one another for a row's vectors, and entries a thread sums: as many as leave enough workgroups.
+struct SumPlan {
+    int lanes, chunk;
+    unsigned groups, slabs;
+    size_t size() const { return size_t(kThreads / lanes) * chunk; }
+};
+SumPlan sum_plan(const flstm_embedding* p) {
+    const size_t vectors = ceil_div(p->width, 8);
+    SumPlan s;
+    s.lanes = vectors <= 4 ? 4 : round_up(vectors, 8) * 10 <= round_up(vectors, 16) * 9 ? 8 : 16;
+    s.slabs = unsigned(ceil_div(vectors, s.lanes));
+    for (s.chunk = kMaxChunk; s.chunk > 8 && ceil_div(p->tokens, s.size()) * s.slabs < 512;) s.chunk /= 2;
+    s.groups = unsigned(ceil_div(p->tokens, s.size()));
+    return s;
+}
 struct Room {   // of the workspace, in bytes
-    size_t list, counts, partials;
-    size_t all() const { return 4 * list + counts + partials; }
+    size_t list, lists, counts, partials;
+    size_t all() const { return lists * list + counts + partials; }
 };
 Room room_of(const flstm_embedding* p) {
     const SortPlan s = sort_plan(p);
-    return Room{round_up(p->tokens * 4, 16), round_up((size_t(s.tiles) << s.bits) * 4, 16), round_up(ceil_div(p->tokens, kChunk) * 2 * p->width * 4, 16)};
+    return Room{round_up(p->tokens * 4, 16), size_t(ranked(p) ? 2 : 4), ranked(p) ? 0 : round_up((size_t(s.tiles) << s.bits) * 4, 16),
+                round_up(size_t(sum_plan(p).groups) * 2 * p->width * 4, 16)};
 }
 
 }  // namespace
@@ -273,13 +458,17 @@ extern "C" int flstm_embedding_forward(const flstm_embedding* p, const void* tab
     if (p->tokens == 0 || p->width == 0) return 0;
     if (!table || !out) return FLSTM_E_INVALID;
     Lookup a{tokens_of(p), unsigned(ceil_div(p->width, 8)), 0, 0, p->width, ld, table, out, p->scale};
-    a.items = p->tokens * a.vectors;
     return with_type(table_dtype, [&](auto from) {
         return with_type(dtype, [&](auto to) {
-            constexpr size_t kMost = size_t(1) << 31;   // threads a launch
-            for (a.first = 0; a.first < a.items; a.first += kMost) {
-                const size_t some = a.items - a.first < kMost ? a.items - a.first : kMost;
-                lookup_kernel<decltype(from), decltype(to)><<<unsigned(ceil_div(some, kThreads)), kThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
+            const size_t most = (size_t(1) << 31) / a.vectors;   // rows a launch
+            const bool passing = p->tokens * p->width * sizeof(to) > kMostKept;
+            for (a.first = 0; a.first < p->tokens; a.first += most) {
+                a.items = unsigned((p->tokens - a.first < most ? p->tokens - a.first : most) * a.vectors);
+                const unsigned grid = unsigned(ceil_div(a.items, kThreads * kLookups));
+                hipStream_t s = static_cast<hipStream_t>(stream);
+                if (p->width < 8) lookup_kernel<decltype(from), decltype(to), true, false><<<grid, kThreads, 0, s>>>(a);
+                else if (passing) lookup_kernel<decltype(from), decltype(to), false, true><<<grid, kThreads, 0, s>>>(a);
+                else lookup_kernel<decltype(from), decltype(to), false, false><<<grid, kThreads, 0, s>>>(a);
                 if (const int rc = launched()) return rc;
             }
             return 0;
@@ -295,40 +484,60 @@ extern "C" int flstm_embedding_backward(const flstm_embedding* p, const void* d_
     if (p->width == 0) return 0;
     if (!d_table || (p->tokens > 0 && (!d_out || !workspace))) return FLSTM_E_INVALID;
     hipStream_t s = static_cast<hipStream_t>(stream);
+    const SumPlan plan = sum_plan(p);
     Sums a{};
     a.count = unsigned(p->tokens); a.vocabulary = unsigned(p->vocabulary); a.vectors = unsigned(ceil_div(p->width, 8));
-    a.chunks = unsigned(ceil_div(p->tokens, kChunk)); a.width = p->width; a.ldd = ldd; a.d_out = d_out; a.d_table = d_table; a.scale = p->scale;
-    const size_t sums = ceil_div(size_t(a.chunks) * a.vectors, kThreads), zeros = ceil_div(p->vocabulary, kZeroRows);
-    if (sums + zeros > (size_t(1) << 31) / kThreads * 2 - 1) return FLSTM_E_TOO_LARGE;
+    a.groups = plan.groups; a.slabs = plan.slabs; a.chunk = plan.chunk;
+    a.width = p->width; a.ldd = ldd; a.d_out = d_out; a.d_table = d_table; a.scale = p->scale;
+    const size_t sums = size_t(a.groups) * a.slabs, zeros = ceil_div(p->vocabulary, kZeroRows), joins = ceil_div(size_t(a.groups) * a.vectors, kThreads);
+    if (sums + zeros > 0xffffffffu / kThreads || joins > 0xffffffffu / kThreads) return FLSTM_E_TOO_LARGE;
     if (p->tokens > 0) {
-        const SortPlan plan = sort_plan(p);
         const Room room = room_of(p);
         char* at = static_cast<char*>(workspace);
-        unsigned* lists[2][2];
-        for (auto& pair : lists)
-            for (auto& list : pair) {
-                list = reinterpret_cast<unsigned*>(at);
-                at += room.list;
+        unsigned* lists[2][2] = {};
+        for (size_t i = 0; i < room.lists; ++i, at += room.list) lists[i / 2][i % 2] = reinterpret_cast<unsigned*>(at);
+        int last = 0;
+        if (ranked(p)) {
+            const size_t lds = (round_up(p->tokens, kRankWaves * 4) + kRankThreads) * 4;
+            rank_kernel<<<unsigned(ceil_div(p->tokens, kWave)), kRankThreads, lds, s>>>(tokens_of(p), lists[0][0], lists[0][1]);
+        } else {
+            const SortPlan sort = sort_plan(p);
+            SortPass pass{tokens_of(p), a.count, sort.tile, sort.tiles, 0, sort.bits, 1, nullptr, nullptr, nullptr, nullptr, reinterpret_cast<unsigned*>(at)};
+            for (int i = 0; i < sort.passes; ++i) {
+                last = i % 2;
+                pass.shift = i * sort.bits;
+                pass.first = i == 0;
+                pass.keys_in = lists[1 - last][0]; pass.at_in = lists[1 - last][1];
+                pass.keys_out = lists[last][0]; pass.at_out = lists[last][1];
+                count_kernel<<<sort.tiles, kSortThreads, 0, s>>>(pass);
+                scatter_kernel<<<sort.tiles, kSortThreads, 0, s>>>(pass);
             }
-        SortPass pass{tokens_of(p), a.count, plan.tile, plan.tiles, 0, plan.bits, 1, nullptr, nullptr, nullptr, nullptr, reinterpret_cast<unsigned*>(at)};
-        a.partials = reinterpret_cast<float*>(at + room.counts);
-        for (int i = 0; i < plan.passes; ++i) {
-            pass.shift = i * plan.bits;
-            pass.first = i == 0;
-            pass.keys_in = lists[(i + 1) % 2][0]; pass.at_in = lists[(i + 1) % 2][1];
-            pass.keys_out = lists[i % 2][0]; pass.at_out = lists[i % 2][1];
-            count_kernel<<<plan.tiles, kSortThreads, 0, s>>>(pass);
-            scatter_kernel<<<plan.tiles, kSortThreads, 0, s>>>(pass);
-            if (const int rc = launched()) return rc;
         }
-        a.keys = lists[(plan.passes + 1) % 2][0]; a.at = lists[(plan.passes + 1) % 2][1];
+        if (const int rc = launched()) return rc;
+        a.keys = lists[last][0]; a.at = lists[last][1];
+        a.partials = reinterpret_cast<float*>(at + room.counts);
     }
     a.sum_blocks = unsigned(sums);
     return with_type(dtype, [&](auto from) {
         return with_type(table_dtype, [&](auto to) {
-            sum_kernel<decltype(from), decltype(to)><<<unsigned(sums + zeros), kThreads, 0, s>>>(a);
+            typedef decltype(from) From;
+            typedef decltype(to) To;
+            const unsigned grid = unsigned(sums + zeros);
+            const bool passing = p->vocabulary * p->width * sizeof(to) > kMostKept || p->tokens * p->width * sizeof(from) > kMostKept;
+            const auto sum = [&](auto lanes) {
+                constexpr int kLanes = decltype(lanes)::value;
+                if (passing) sum_kernel<From, To, kLanes, false, true><<<grid, kThreads, 0, s>>>(a);
+                else sum_kernel<From, To, kLanes, false, false><<<grid, kThreads, 0, s>>>(a);
+            };
+            if (plan.lanes == 16) sum(std::integral_constant<int, 16>());
+            else if (plan.lanes == 8) sum(std::integral_constant<int, 8>());
+            else if (p->width >= 8) sum(std::integral_constant<int, 4>());
+            else sum_kernel<From, To, 4, true, false><<<grid, kThreads, 0, s>>>(a);
             if (const int rc = launched()) return rc;
-            if (a.chunks > 1) join_kernel<decltype(to)><<<unsigned(sums), kThreads, 0, s>>>(a);
+            if (a.groups > 1) {
+                if (p->width >= 8) join_kernel<To, false><<<unsigned(joins), kThreads, 0, s>>>(a, unsigned(plan.size()));
+                else join_kernel<To, true><<<unsigned(joins), kThreads, 0, s>>>(a, unsigned(plan.size()));
+            }
             return launched();
         });
     });

@@ -131,6 +131,17 @@ def test_masks(dtype):
     assert not bool((got[1][0] == 1).any()) and bool(got[0].isfinite().all())
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_few_allowed_among_many_equal(dtype):
+    """Masks that leave logits where the threads' groups do not all find one, with everything else at one value."""
+    for vocabulary, low in ((8192, torch.finfo(dtype).min), (30000, 0.0), (1100001, -7.0)):
+        for allowed in (slice(0, 1), slice(5000, 5003), slice(0, None, 16), slice(8, None, 4096), slice(1, None, 2)):
+            p = _problem(2, 2, vocabulary, dtype, seed=15, finished=0)
+            masked = torch.full_like(p["logits"], low)
+            masked[..., allowed] = p["logits"][..., allowed] + 20
+            _check({**p, "logits": masked}, f"{allowed} of {vocabulary}", beams=11)
+
+
 def test_all_finished():
     p = _problem(3, 4, 800, seed=11, finished=2)
     p["logits"][:] = float("nan")
