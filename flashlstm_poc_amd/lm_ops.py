@@ -51,9 +51,10 @@ def _bind() -> ctypes.CDLL:
         lib.flstm_gated_recurrence_forward.argtypes = [shape, rows, rows, rows, vp, rows, vp, vp, vp, vp]
         lib.flstm_gated_recurrence_backward.argtypes = [shape, rows, rows, rows, rows, vp, vp, rows, rows, rows, vp, vp, vp]
         lib.flstm_gated_recurrence_step.argtypes = [shape, rows, rows, rows, rows, vp, vp]
-        for name in ("workspace_bytes", "saved_rows"):
-            getattr(lib, f"flstm_gated_recurrence_{name}").argtypes = [shape]
-            getattr(lib, f"flstm_gated_recurrence_{name}").restype = sz
+        lib.flstm_gated_recurrence_workspace_bytes.argtypes = [shape, i32]
+        lib.flstm_gated_recurrence_workspace_bytes.restype = sz
+        lib.flstm_gated_recurrence_saved_rows.argtypes = [shape]
+        lib.flstm_gated_recurrence_saved_rows.restype = sz
         lib.flstm_beam_select.argtypes = [problem, vp, vp, vp, vp, vp, vp]
         lib.flstm_beam_select_workspace_bytes.argtypes = [problem]
         lib.flstm_beam_select_workspace_bytes.restype = sz
@@ -703,8 +704,8 @@ def _like_channels(x):
     return torch.empty(x.shape, device=x.device, dtype=x.dtype)
 
 
-def _recurrence_workspace(shape: bytes, device):
-    size = _bind().flstm_gated_recurrence_workspace_bytes(shape)
+def _recurrence_workspace(shape: bytes, backward: int, device):
+    size = _bind().flstm_gated_recurrence_workspace_bytes(shape, backward)
     return torch.empty(size, device=device, dtype=torch.uint8) if size else None
 
 
@@ -722,7 +723,7 @@ def gated_recurrence_forward(x, forget, gate=None, *, state=None, cu_seqlens=Non
     y, lib = _like_channels(x), _bind()
     final = torch.empty(states, device=x.device, dtype=torch.float32) if want_state else None
     saved = torch.empty((lib.flstm_gated_recurrence_saved_rows(shape), states[1]), device=x.device, dtype=torch.float32) if want_saved else None
-    workspace = _recurrence_workspace(shape, x.device)
+    workspace = _recurrence_workspace(shape, 0, x.device)
     _check(lib.flstm_gated_recurrence_forward(shape, _channel_rows(x, packed), _channel_rows(forget, packed), _channel_rows(gate, packed), _ptr(state),
                                               _channel_rows(y, packed), _ptr(final), _ptr(saved), _ptr(workspace), _stream()),
            "flstm_gated_recurrence_forward")
@@ -747,7 +748,7 @@ def gated_recurrence_backward(dy, x, forget, gate, saved, *, d_state=None, cu_se
     dforget = _like_channels(x) if want[1] else None
     dgate = _like_channels(x) if want[2] and gate is not None else None
     d_initial = torch.empty(states, device=x.device, dtype=torch.float32) if want[3] else None
-    workspace = _recurrence_workspace(shape, x.device)
+    workspace = _recurrence_workspace(shape, 1, x.device)
     _check(lib.flstm_gated_recurrence_backward(
         shape, _channel_rows(dy, packed), _channel_rows(x, packed), _channel_rows(forget, packed), _channel_rows(gate, packed), saved.data_ptr(),
         _ptr(d_state), _channel_rows(dx, packed), _channel_rows(dforget, packed), _channel_rows(dgate, packed), _ptr(d_initial), _ptr(workspace),

@@ -184,13 +184,13 @@ typedef struct {
 } flstm_recurrence;
 
 /* gate (or its data), state_in, state_out and saved may be null; state_in and state_out must not be one buffer, and y must not lie in an input.
- * `workspace`: flstm_gated_recurrence_workspace_bytes() bytes, 16-byte aligned (null where that is 0), forward and backward. */
+ * `workspace`: flstm_gated_recurrence_workspace_bytes(shape, backward) bytes, 16-byte aligned (null where that is 0). */
 int flstm_gated_recurrence_forward(const flstm_recurrence* shape, const flstm_rows* x, const flstm_rows* forget, const flstm_rows* gate,
                                    const float* state_in, const flstm_rows* y, float* state_out, float* saved, void* workspace, void* stream);
 int flstm_gated_recurrence_backward(const flstm_recurrence* shape, const flstm_rows* d_y, const flstm_rows* x, const flstm_rows* forget,
                                     const flstm_rows* gate, const float* saved, const float* d_state_out, const flstm_rows* dx,
                                     const flstm_rows* dforget, const flstm_rows* dgate, float* d_state_in, void* workspace, void* stream);
-size_t flstm_gated_recurrence_workspace_bytes(const flstm_recurrence* shape);
+size_t flstm_gated_recurrence_workspace_bytes(const flstm_recurrence* shape, int backward);
 size_t flstm_gated_recurrence_saved_rows(const flstm_recurrence* shape);
 /* One token of every sequence (shape->tokens, cu_seqlens and .token are not read), the state updated in place. */
 int flstm_gated_recurrence_step(const flstm_recurrence* shape, const flstm_rows* x, const flstm_rows* forget, const flstm_rows* gate,

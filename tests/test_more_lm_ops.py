@@ -42,9 +42,9 @@ def test_gated_recurrence_refuses_before_device_work():
     backward = lambda s=shape(), dy=rows(), x=rows(), g=None, saved=SOME, dg=None: lib.flstm_gated_recurrence_backward(
         s, dy, x, rows(), g, saved, None, rows(), rows(), dg, None, None, None)
     step = lambda s=shape(), x=rows(), y=rows(), state=SOME: lib.flstm_gated_recurrence_step(s, x, rows(), None, y, state, None)
-    for change in (dict(dtype=3), dict(dtype=-1), dict(sequences=1 << 31), dict(tokens=1 << 39), dict(width=1 << 31), dict(cu_seqlens=4096, tokens=1 << 31)):
+    for change in (dict(dtype=3), dict(dtype=-1), dict(sequences=1 << 31), dict(tokens=1 << 39), dict(width=1 << 28), dict(cu_seqlens=4096, tokens=1 << 31)):
         assert forward(shape(**change)) == 1 and backward(shape(**change)) == 1 and step(shape(**change)) == 1, change
-        assert lib.flstm_gated_recurrence_workspace_bytes(shape(**change)) == 0 and lib.flstm_gated_recurrence_saved_rows(shape(**change)) == 0
+        assert lib.flstm_gated_recurrence_workspace_bytes(shape(**change), 0) == 0 and lib.flstm_gated_recurrence_saved_rows(shape(**change)) == 0
     assert forward(None) == 1 and forward(x=None) == 1 and forward(u=rows(None)) == 1 and forward(y=rows(None)) == 1
     assert forward(shape(sequences=1, tokens=1 << 20)) == 1     # no workspace
     assert backward(None) == 1 and backward(dy=None) == 1 and backward(x=rows(None)) == 1 and backward(saved=None) == 1 and backward(dg=rows()) == 1
