@@ -17,7 +17,7 @@ constexpr int kMaxKeep = 32, kMaxBeams = 32;
 constexpr int kVectors = 4, kTile = kThreads * kVectors * 8;   // logits a workgroup holds at a time
 constexpr size_t kMaxParts = 64;   // one for each lane of a wave
 constexpr int kList = 1024;        // entries that are ordered at once
-constexpr float kLowest = -3.4028234663852886e38f, kHighest = 3.4028234663852886e38f;
+constexpr float kLog2e = 1.4426950408889634f, kLowest = -3.4028234663852886e38f, kHighest = 3.4028234663852886e38f;
 
 struct Select {
     size_t sequences, ld;
@@ -124,17 +124,30 @@ template <class T> __global__ __launch_bounds__(kThreads) void part_kernel(Selec
     for (unsigned base = begin; base < end; base += kTile) {
         typename Vec8<T>::type v[kVectors];   // as they come: converted three times, in half the registers
         float m = -__builtin_inff();
-#pragma unroll
-        for (int j = 0; j < kVectors; ++j) {
+        const auto place_of = [&](int j) {   // of a vector's first entry
             const unsigned c = base + (j * kThreads + tid) * 8;
-            if (c + 8 <= end) {
-                __builtin_memcpy(&v[j], __builtin_assume_aligned(z + c, sizeof(T)), sizeof(v[j]));
-            } else {
-                float8 w = load8(z + c, c < end ? int(end - c) : 0);
+            return c + 8 > end && a.vocabulary >= 8 ? end - 8 : c;
+        };
+        // All vectors are requested without a branch, behind which they would be waited for one by one: the last one of the part from where it ends, and what is
+        // not this thread's of it taken out.  (Rows of less than a vector: piece by piece.)
+        if (a.vocabulary >= 8) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) w[i] = c + i < end ? w[i] : -__builtin_inff();
-                v[j] = __builtin_convertvector(w, typename Vec8<T>::type);
+            for (int j = 0; j < kVectors; ++j) {
+                __builtin_memcpy(&v[j], __builtin_assume_aligned(z + place_of(j), sizeof(T)), sizeof(v[j]));
             }
+#pragma unroll
+            for (int j = 0; j < kVectors; ++j) {
+                const unsigned c = base + (j * kThreads + tid) * 8;
+                if (c + 8 > end)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[j][i] = c < end && place_of(j) + i >= c ? v[j][i] : T(-__builtin_inff());
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < kVectors; ++j) v[j] = T(-__builtin_inff());
+            if (tid == 0)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[0][i] = unsigned(i) < end ? z[i] : v[0][i];
         }
 #pragma unroll
         for (int j = 0; j < kVectors; ++j) {
@@ -153,34 +166,40 @@ template <class T> __global__ __launch_bounds__(kThreads) void part_kernel(Selec
         bound = fmaxf(bound, kLowest);   // (minus infinity is no continuation)
         if (base > begin && best[a.keep - 1]) bound = fmaxf(bound, logit_of(unsigned(best[a.keep - 1] >> 32)));
         m = fmaxf(most, lanes_max<kWave>(m));
-        sum *= __builtin_amdgcn_exp2f((most - m) * 1.4426950408889634f);
+        sum *= __builtin_amdgcn_exp2f((most - m) * kLog2e);
         most = m;
+        // exponents as one operation each, z log2(e) - shift; what the rounding of shift is off by is put right behind the sum
+        const float shift = most * kLog2e;
+        const float reached = __builtin_fmaf(bound, kLog2e, -shift);   // (rounding keeps the order)
         float more = 0.f;
 #pragma unroll
         for (int j = 0; j < kVectors; ++j) {
             asm volatile("" : "+v"(v[j]));
-            float reach = -__builtin_inff();
+            float d[8], reach = -__builtin_inff();
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float d = float(v[j][i]) - most;
-                more += __builtin_amdgcn_exp2f(d * 1.4426950408889634f);
-                reach = fmaxf(reach, d);
+                d[i] = __builtin_fmaf(float(v[j][i]), kLog2e, -shift);
+                more += __builtin_amdgcn_exp2f(d[i]);
+                reach = fmaxf(reach, d[i]);
             }
-            if (reach >= bound - most)   // (rounding keeps the order)
+            if (!(reach < reached))   // (a thread's eight hardly ever hold one that does, a wave's mostly)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float x = number(float(v[j][i]));
-                    if (x >= bound) {
-                        const int at = atomicAdd(&count, 1);
-                        if (at < kList) list[at] = key_of(x, base + (j * kThreads + tid) * 8 + i);
+                for (int i = 0; i < 8; ++i)
+                    if (!(d[i] < reached)) {
+                        const float x = number(float(v[j][i]));
+                        if (x >= bound) {
+                            const int at = atomicAdd(&count, 1);
+                            if (at < kList) list[at] = key_of(x, place_of(j) + i);
+                        }
                     }
-                }
         }
-        if (!(more < __builtin_inff())) {   // a NaN or an infinity among them: once more, without
+        if (more < __builtin_inff() && fabsf(shift) < __builtin_inff()) {
+            more *= __builtin_amdgcn_exp2f(-__builtin_fmaf(most, kLog2e, -shift));
+        } else {   // a NaN or an infinity among them, or exponents that are none: once more, number by number
             more = 0.f;
             for (int i = 0; i < kVectors * 8; ++i) {
                 const unsigned c = base + (i / 8 * kThreads + tid) * 8 + i % 8;
-                if (c < end) more += __builtin_amdgcn_exp2f((number(float(z[c])) - most) * 1.4426950408889634f);
+                if (c < end) more += __builtin_amdgcn_exp2f((number(float(z[c])) - most) * kLog2e);
             }
         }
         sum += more;
@@ -252,7 +271,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Select a) {
         const bool done = a.finished && a.finished[row0 + b], alive = score > -__builtin_inff() && !done;
         float2 p{kLowest, 0.f};
         if (alive && lane < a.parts) p = a.sums[(row0 + b) * a.parts + lane];
-        const float m = lanes_max<kWave>(p.x), s = lanes_sum<kWave>(p.y * __builtin_amdgcn_exp2f((p.x - m) * 1.4426950408889634f));
+        const float m = lanes_max<kWave>(p.x), s = lanes_sum<kWave>(p.y * __builtin_amdgcn_exp2f((p.x - m) * kLog2e));
         if (lane == 0) {
             most[b] = m;
             rest[b] = done ? double(score) : double(score) - log(double(s));

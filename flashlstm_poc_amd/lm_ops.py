@@ -814,14 +814,15 @@ def beam_select(logits, scores, *, beams: Optional[int] = None, end: Optional[in
     finished (sequences, hypotheses) bool: those that are, which stay as they are, with `end` as their token.
     Returns (scores, parents, tokens, finished), (sequences, beams) of float32, int64, int64 and bool (None without `end`).  Logits of minus
     infinity and NaN are no continuations; where there are too few, scores are minus infinity and tokens -1.  No autograd."""
-    code = _device_tensor("logits", logits)
-    if logits.dim() != 3 or logits.shape[2] < 1:
-        raise ValueError(f"logits must have shape (sequences, hypotheses, vocabulary): got {tuple(logits.shape)}")
-    sequences, hypotheses, vocabulary = logits.shape
+    code, of = _device_tensor("logits", logits), logits.shape
+    if len(of) != 3 or of[2] < 1:
+        raise ValueError(f"logits must have shape (sequences, hypotheses, vocabulary): got {tuple(of)}")
+    sequences, hypotheses, vocabulary = of
     keep = hypotheses if beams is None else int(beams)
     if not (1 <= hypotheses <= _MAX_BEAMS and 1 <= keep <= _MAX_BEAMS):
         raise ValueError(f"between 1 and {_MAX_BEAMS} hypotheses and beams: got {hypotheses} and {keep}")
-    _device_tensor("scores", scores, torch.float32)
+    if not _all_here(torch.float32, scores):
+        _device_tensor("scores", scores, torch.float32)
     if scores.shape != (sequences, hypotheses):
         raise ValueError(f"scores must have shape {(sequences, hypotheses)}: got {tuple(scores.shape)}")
     if end is not None and not 0 <= end < vocabulary:
@@ -829,16 +830,18 @@ def beam_select(logits, scores, *, beams: Optional[int] = None, end: Optional[in
     if finished is not None:
         if end is None:
             raise ValueError("finished hypotheses need an `end`")
-        if not torch.is_tensor(finished) or finished.device != logits.device or finished.dtype != torch.bool:
+        if not _all_here(torch.bool, finished):
             raise ValueError("finished must be a bool tensor on the device of logits")
         if finished.shape != (sequences, hypotheses):
             raise ValueError(f"finished must have shape {(sequences, hypotheses)}: got {tuple(finished.shape)}")
         finished = finished.contiguous()
     scores = scores.contiguous()
-    rows = _rows(logits) if logits.numel() else logits
-    ld = rows.stride(0) if sequences * hypotheses > 1 else vocabulary
-    if ld < vocabulary:   # (rows that share memory)
-        rows, ld = rows.contiguous(), vocabulary
+    rows, ld = logits, vocabulary
+    if not logits.is_contiguous():
+        rows = _rows(logits)
+        ld = rows.stride(0) if sequences * hypotheses > 1 else vocabulary
+        if ld < vocabulary:   # (rows that share memory)
+            rows, ld = rows.contiguous(), vocabulary
     shape, dev = (sequences, keep), logits.device
     out_scores = torch.empty(shape, device=dev, dtype=torch.float32)
     parents, tokens = torch.empty((2, *shape), device=dev, dtype=torch.int64).unbind(0)
@@ -862,26 +865,30 @@ def beam_reorder(parents, *states) -> None:
     if parents.dim() != 2 or not 1 <= parents.shape[1] <= _MAX_BEAMS:
         raise ValueError(f"parents must have shape (sequences, hypotheses), of 1 to {_MAX_BEAMS}: got {tuple(parents.shape)}")
     sequences, hypotheses = parents.shape
-    packed = []
+    rows, device, packed = sequences * hypotheses, parents.get_device(), []
     for i, t in enumerate(states):
-        if not torch.is_tensor(t) or t.get_device() != parents.get_device():
+        if not isinstance(t, torch.Tensor) or t.get_device() != device:
             raise ValueError(f"state {i} must be a CUDA tensor on the device of parents")
-        of = t.shape
-        if of[:1] == (sequences * hypotheses,):
-            stride, row = t.stride(0), t.shape[1:]
-        elif of[:2] == (sequences, hypotheses) and (sequences == 1 or hypotheses == 1 or t.stride(0) == hypotheses * t.stride(1)):
-            stride, row = t.stride(0) if hypotheses == 1 else t.stride(1), t.shape[2:]
+        of, strides = t.shape, t.stride()
+        if of[:1] == (rows,):
+            axes, stride = 1, strides[0]
+        elif of[:2] == (sequences, hypotheses) and (sequences == 1 or hypotheses == 1 or strides[0] == hypotheses * strides[1]):
+            axes, stride = 2, strides[0] if hypotheses == 1 else strides[1]
         else:
             raise ValueError(f"state {i} must have {sequences} x {hypotheses} rows, evenly spaced: got shape {tuple(of)}")
-        size = row.numel()
-        if size and sequences and not (t[0, 0] if len(of) - len(row) == 2 else t[0]).is_contiguous() or sequences * hypotheses > 1 and stride < size:
+        size, whole = 1, True
+        for n, s in zip(of[:axes - 1:-1], strides[:axes - 1:-1]):
+            whole = whole and (n == 1 or s == size)
+            size *= n
+        if rows and size and (not whole or rows > 1 and stride < size):
             raise ValueError(f"state {i} must have contiguous rows of its own")
         if t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"state {i} needs a gradient: it would be changed in place")
-        packed.append(_BEAM_STATE.pack(t.data_ptr(), max(stride, size) * t.element_size(), size * t.element_size()))
-    parents = parents.contiguous()
+        element = t.element_size()
+        packed.append(_BEAM_STATE.pack(t.data_ptr(), max(stride, size) * element, size * element))
+    parents, lib = parents.contiguous(), _bind()
     for at in range(0, len(packed), _MAX_STATES):
         some = packed[at:at + _MAX_STATES]
-        _check(_bind().flstm_beam_reorder(sequences, hypotheses, parents.data_ptr(), b"".join(some), len(some), _stream()), "flstm_beam_reorder")
+        _check(lib.flstm_beam_reorder(sequences, hypotheses, parents.data_ptr(), b"".join(some), len(some), _stream()), "flstm_beam_reorder")
     for t in states:
         _written(t)
