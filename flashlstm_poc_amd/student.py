@@ -1,12 +1,12 @@
 """A small recurrent language model of this library's parts, distilled from a teacher's top logits and run token by token.
 
-RecurrentStudent is a residual stream with, in every layer, a norm and an LSTM, a norm and attention with a decaying state, and
-at the end a norm and the logits.  Both mixers carry a state of fixed size, so that a token costs the same however long the text
-in front of it is.  `python -m flashlstm_poc_amd.student` trains one against a teacher that knows which tokens may follow which,
-then continues a prompt token by token.
+RecurrentStudent is a residual stream with, in every layer, a norm and an LSTM or a gated linear recurrence, a norm and attention with a
+decaying state, and at the end a norm and the logits.  All mixers carry a state of fixed size, so that a token costs the same however long
+the text in front of it is.  `python -m flashlstm_poc_amd.student` trains one against a teacher that knows which tokens may follow which,
+then continues a prompt token by token, the likeliest one each or with beams.
 
-The reference has no language model; this runs layer_norm, decay_attention, decay_attention_step and distillation_train /
-distillation_loss together with StackedLSTM as a user's program would.
+The reference has no language model; this runs embedding, layer_norm, decay_attention, decay_attention_step, gated_recurrence,
+gated_recurrence_step, beam_select, beam_reorder and distillation_train / distillation_loss together with StackedLSTM as a user's program would.
 """
 from __future__ import annotations
 
@@ -15,28 +15,38 @@ from typing import List, NamedTuple, Optional, Tuple
 
 import torch
 
-from .lm_ops import LayerNorm, decay_attention, decay_attention_step, distillation_loss
+from .lm_ops import (Embedding, LayerNorm, beam_reorder, beam_select, decay_attention, decay_attention_step, distillation_loss, gated_recurrence,
+                     gated_recurrence_step)
 from .stack import StackedLSTM
 
 
 class LayerState(NamedTuple):
-    """What a layer carries from token to token: the LSTM's h and c (1, B, width) and the attention's (B, heads, d, d)."""
-    h: torch.Tensor
+    """What a layer carries from token to token: the LSTM's h and c (1, B, width), or None and the gated recurrence's (B, width), and the
+    attention's (B, heads, d, d)."""
+    h: Optional[torch.Tensor]
     c: torch.Tensor
     memory: torch.Tensor
 
 
 class RecurrentLayer(torch.nn.Module):
-    """Norm, LSTM, norm, attention with a decaying state; each reads the residual stream and returns what is to be added to it, which
-    the next norm does."""
+    """Norm, LSTM (or, `recurrence` "gated", a gated linear recurrence), norm, attention with a decaying state; each reads the residual
+    stream and returns what is to be added to it, which the next norm does."""
 
-    def __init__(self, width: int, heads: int, device="cuda"):
+    def __init__(self, width: int, heads: int, device="cuda", recurrence: str = "lstm"):
         super().__init__()
+        if recurrence not in ("lstm", "gated"):
+            raise ValueError(f"recurrence must be 'lstm' or 'gated', not {recurrence!r}")
         if heads < 1 or width % heads != 0:
             raise ValueError(f"width ({width}) must be a multiple of the number of heads ({heads})")
         self.heads = heads
         self.norm_lstm, self.norm_attention = LayerNorm(width, device=device), LayerNorm(width, device=device)
-        self.lstm = StackedLSTM(width, width, 1, device=device)
+        self.gated = recurrence == "gated"
+        if self.gated:
+            self.gates = torch.nn.Linear(width, 3 * width, device=device)     # values, forget gates, output gates
+            with torch.no_grad():   # memories of 2 to some 150 tokens
+                self.gates.bias[width:2 * width] = torch.linspace(0, 5, width, device=device)
+        else:
+            self.lstm = StackedLSTM(width, width, 1, device=device)
         self.qkv = torch.nn.Linear(width, 3 * width, bias=False, device=device)
         self.out = torch.nn.Linear(width, width, bias=False, device=device)
         # memories of 2 to 2^8 tokens, longer from head to head
@@ -50,19 +60,31 @@ class RecurrentLayer(torch.nn.Module):
     def _join(self, o):
         return torch.nn.functional.linear(o.flatten(-2), self.out.weight.to(o.dtype))
 
+    def _gates(self, y):
+        return torch.nn.functional.linear(y, self.gates.weight.to(y.dtype), self.gates.bias.to(y.dtype)).chunk(3, -1)
+
     def forward(self, stream, added, state: Optional[LayerState]):
         """stream, added (T, B, width) fp16, added None in front of the first layer -> stream, added, LayerState."""
         y, stream = (self.norm_lstm(stream), stream) if added is None else self.norm_lstm(stream, added)
-        added, (h, c) = self.lstm(y, None if state is None else (state.h, state.c))
+        if self.gated:
+            x, forget, gate = (t.transpose(0, 1) for t in self._gates(y))     # (B, T, width), as they lie
+            added, c = gated_recurrence(x, forget, gate, state=None if state is None else state.c)
+            added, h = added.transpose(0, 1), None
+        else:
+            added, (h, c) = self.lstm(y, None if state is None else (state.h, state.c))
         y, stream = self.norm_attention(stream, added)
         q, k, v = (t.transpose(0, 1) for t in self._heads(y))     # (B, T, heads, d), as they lie
         o, memory = decay_attention(q, k, v, self.log_decay, state=None if state is None else state.memory)
         return stream, self._join(o.transpose(0, 1)), LayerState(h, c, memory)
 
     def step(self, stream, added, state: LayerState):
-        """The same for one token, stream and added (1, B, width); state.memory is updated in place."""
+        """The same for one token, stream and added (1, B, width); state.memory and a gated recurrence's c are updated in place."""
         y, stream = (self.norm_lstm(stream), stream) if added is None else self.norm_lstm(stream, added)
-        added, (h, c) = self.lstm(y, (state.h, state.c))
+        if self.gated:
+            x, forget, gate = self._gates(y[0])
+            added, h, c = gated_recurrence_step(x, forget, state.c, gate)[None], None, state.c
+        else:
+            added, (h, c) = self.lstm(y, (state.h, state.c))
         y, stream = self.norm_attention(stream, added)
         q, k, v = self._heads(y[0])
         o = decay_attention_step(q, k, v, self.log_decay, state.memory)
@@ -72,10 +94,10 @@ class RecurrentLayer(torch.nn.Module):
 class RecurrentStudent(torch.nn.Module):
     """Tokens (T, B) -> logits (T, B, vocabulary) fp16; parameters fp32, activations fp16."""
 
-    def __init__(self, vocabulary: int, width: int, heads: int, layers: int = 1, device="cuda"):
+    def __init__(self, vocabulary: int, width: int, heads: int, layers: int = 1, device="cuda", recurrence: str = "lstm"):
         super().__init__()
-        self.embedding = torch.nn.Embedding(vocabulary, width, device=device)
-        self.layers = torch.nn.ModuleList(RecurrentLayer(width, heads, device) for _ in range(layers))
+        self.embedding = Embedding(vocabulary, width, dtype=torch.float16, device=device)
+        self.layers = torch.nn.ModuleList(RecurrentLayer(width, heads, device, recurrence) for _ in range(layers))
         self.norm = LayerNorm(width, device=device)
         self.head = torch.nn.Linear(width, vocabulary, bias=False, device=device)
 
@@ -85,7 +107,7 @@ class RecurrentStudent(torch.nn.Module):
 
     def forward(self, tokens, state: Optional[List[LayerState]] = None) -> Tuple:
         """A prompt or a training batch from `state` (None: the beginning) -> logits of all positions, state behind them."""
-        stream, added, out = self.embedding(tokens).half(), None, []
+        stream, added, out = self.embedding(tokens), None, []
         for i, layer in enumerate(self.layers):
             stream, added, after = layer(stream, added, None if state is None else state[i])
             out.append(after)
@@ -93,8 +115,9 @@ class RecurrentStudent(torch.nn.Module):
 
     @torch.no_grad()
     def step(self, tokens, state: List[LayerState]) -> Tuple:
-        """One token of every sequence, tokens (B,) -> logits (B, vocabulary), state; the memories in `state` are updated in place."""
-        stream, added, out = self.embedding(tokens)[None].half(), None, []
+        """One token of every sequence, tokens (B,) -> logits (B, vocabulary), state; the memories in `state` (and gated recurrences' c) are updated
+        in place."""
+        stream, added, out = self.embedding(tokens)[None], None, []
         for layer, before in zip(self.layers, state):
             stream, added, after = layer.step(stream, added, before)
             out.append(after)
@@ -111,6 +134,26 @@ class RecurrentStudent(torch.nn.Module):
                 logits, state = self.step(out[i - 1], state)
             out[i] = logits.argmax(-1)
         return out
+
+    @torch.no_grad()
+    def search(self, prompt, count: int, beams: int, end: Optional[int] = None) -> Tuple:
+        """Continues prompt (T, B) by `count` tokens, of which `beams` ways are followed at a time; a way ends with the token `end`, which fills its
+        rest.  Returns the ways found, best first, as tokens (B, beams, count), -1 where there were fewer, and the logarithms of their
+        probabilities (B, beams)."""
+        batch, device = prompt.shape[1], prompt.device
+        found = torch.full((batch * beams, count), -1, device=device, dtype=torch.int64)
+        if count == 0:
+            return found.view(batch, beams, 0), torch.zeros((batch, beams), device=device)
+        logits, state = self(prompt)
+        scores, _, tokens, finished = beam_select(logits[-1, :, None], torch.zeros((batch, 1), device=device), beams=beams, end=end)
+        state = [LayerState(*(t if t is None else t.repeat_interleave(beams, t.dim() - 2 if t.dim() < 4 else 0) for t in layer)) for layer in state]
+        found[:, 0] = tokens.flatten()
+        for i in range(1, count):
+            logits, state = self.step(tokens.flatten(), state)
+            scores, parents, tokens, finished = beam_select(logits.view(batch, beams, -1), scores, end=end, finished=finished)
+            beam_reorder(parents, found, *(t if t.dim() != 3 else t[0] for layer in state for t in layer if t is not None))
+            found[:, i] = tokens.flatten()
+        return found.view(batch, beams, count), scores
 
 
 def successor_teacher(vocabulary: int, top: int, seed: int = 0, device="cuda"):
@@ -159,9 +202,11 @@ def main() -> None:
     ap.add_argument("--steps", type=int, default=200)
     ap.add_argument("--length", type=int, default=64)
     ap.add_argument("--batch", type=int, default=32)
+    ap.add_argument("--recurrence", choices=("lstm", "gated"), default="lstm")
+    ap.add_argument("--beams", type=int, default=0, help="continue the prompt with a search too")
     a = ap.parse_args()
     torch.manual_seed(0)
-    student = RecurrentStudent(a.vocabulary, a.width, a.heads, a.layers)
+    student = RecurrentStudent(a.vocabulary, a.width, a.heads, a.layers, recurrence=a.recurrence)
     teacher = successor_teacher(a.vocabulary, a.top)
     train(student, teacher, a.steps, length=a.length, batch=a.batch, report=lambda s, v: print(f"step {s:5d}  loss {v:.4f}", flush=True))
     prompt = torch.randint(0, a.vocabulary, (8, 4), device="cuda")
@@ -169,6 +214,9 @@ def main() -> None:
     follows = torch.cat([prompt[-1:], out])
     right = (teacher[1][follows[:-1].long(), 0] == follows[1:]).float().mean()
     print(f"tokens that are the teacher's first choice: {100 * float(right):.0f} %")
+    if a.beams:
+        found, scores = student.search(prompt, 16, a.beams)
+        print(f"search of {a.beams} beams: mean log probability {float(scores[:, 0].mean()):.3f}, first way {found[0, 0].tolist()}")
 
 
 if __name__ == "__main__":
