@@ -86,13 +86,37 @@ template <class From, class To, bool kNarrow, bool kPassing> __global__ __launch
     }
 }
 
+// ---- zeros for the whole gradient, of which the tokens' rows are written afterwards.  Sorting leaves most of the chip idle: each of its launches has
+// workgroups behind its own that clear a share of the table meanwhile.  (Clearing only what has no token, beside the sums, is a third fewer bytes and a search
+// for every row, and takes 89 us instead of 87 for sorting 65536 tokens and the sums of 1024 fp16 over 50001 fp32 rows.)
+
+struct Zeros {
+    char* at;
+    size_t bytes;          // of the launch's share
+    unsigned first;        // the launch's first workgroup for this
+};
+constexpr size_t kZeroBytes = 65536;   // a workgroup
+
+template <bool kPassing> __device__ __forceinline__ void clear_share(const Zeros& z) {
+    const size_t begin = size_t(blockIdx.x - z.first) * kZeroBytes, end = z.bytes - begin < kZeroBytes ? z.bytes : begin + kZeroBytes;
+    typedef unsigned Piece __attribute__((ext_vector_type(4)));
+    const Piece zero = 0u;
+    if (z.bytes < sizeof(Piece)) {
+        if (threadIdx.x < z.bytes / 2) reinterpret_cast<short*>(z.at)[threadIdx.x] = 0;
+        return;
+    }
+    for (size_t i = begin + threadIdx.x * sizeof(Piece); i < end; i += blockDim.x * sizeof(Piece))
+        store_any<kPassing>(reinterpret_cast<short*>(z.at + (i + sizeof(Piece) <= z.bytes ? i : z.bytes - sizeof(Piece))), zero);
+}
+
 // ---- sorting few tokens: an entry's place is the number of those in front of it.  A workgroup has 64 entries, each of its waves a
 // part of all others.
 
 constexpr int kRankThreads = 1024, kRankWaves = kRankThreads / kWave;
 constexpr size_t kMostRanked = 8192;
 
-__global__ __launch_bounds__(kRankThreads) void rank_kernel(Tokens t, unsigned* keys_out, unsigned* at_out) {
+template <bool kPassing> __global__ __launch_bounds__(kRankThreads) void rank_kernel(Tokens t, unsigned* keys_out, unsigned* at_out, Zeros zeros) {
+    if (blockIdx.x >= zeros.first) return clear_share<kPassing>(zeros);
     extern __shared__ unsigned keys[];   // all of them, rounded up to whole fours a wave, and kRankWaves rows of kWave counts
     const unsigned count = unsigned(t.count), part = (count + kRankWaves * 4 - 1) / (kRankWaves * 4) * 4, whole = part * kRankWaves;
     unsigned* counts = keys + whole;
@@ -140,7 +164,8 @@ struct SortPass {
 };
 __device__ __forceinline__ unsigned key_at(const SortPass& a, unsigned i) { return a.first ? token_at(a.t, i) : a.keys_in[i]; }
 
-__global__ __launch_bounds__(kSortThreads) void count_kernel(SortPass a) {
+template <bool kPassing> __global__ __launch_bounds__(kSortThreads) void count_kernel(SortPass a, Zeros zeros) {
+    if (blockIdx.x >= zeros.first) return clear_share<kPassing>(zeros);
     __shared__ unsigned counts[1 << kMaxBits];
     const unsigned bins = 1u << a.bits, begin = blockIdx.x * a.tile, end = a.count - begin < a.tile ? a.count : begin + a.tile;
     for (unsigned b = threadIdx.x; b < bins; b += kSortThreads) counts[b] = 0;
@@ -150,7 +175,8 @@ __global__ __launch_bounds__(kSortThreads) void count_kernel(SortPass a) {
     for (unsigned b = threadIdx.x; b < bins; b += kSortThreads) a.counts[size_t(blockIdx.x) * bins + b] = counts[b];
 }
 
-__global__ __launch_bounds__(kSortThreads) void scatter_kernel(SortPass a) {
+template <bool kPassing> __global__ __launch_bounds__(kSortThreads) void scatter_kernel(SortPass a, Zeros zeros) {
+    if (blockIdx.x >= zeros.first) return clear_share<kPassing>(zeros);
     __shared__ unsigned place[kSortWaves][1 << kMaxBits];   // counts of each wave's part, then where its next entry goes
     __shared__ unsigned sums[kSortWaves];
     const unsigned bins = 1u << a.bits, wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
@@ -167,12 +193,17 @@ __global__ __launch_bounds__(kSortThreads) void scatter_kernel(SortPass a) {
         before[j] = total[j] = 0;
         const unsigned b = threadIdx.x * per + j;
         if (j < per && b < bins) {
-            const unsigned* n = a.counts + b;
-#pragma unroll 16
-            for (unsigned tile = 0; tile < a.tiles; ++tile) {
-                const unsigned v = n[size_t(tile) * bins];
-                total[j] += v;
-                before[j] += tile < blockIdx.x ? v : 0;
+            constexpr unsigned kAhead = 16;   // on their way together
+            for (unsigned first = 0; first < a.tiles; first += kAhead) {
+                unsigned n[kAhead];
+#pragma unroll
+                for (unsigned k = 0; k < kAhead; ++k) n[k] = a.counts[size_t(first + k < a.tiles ? first + k : first) * bins + b];
+#pragma unroll
+                for (unsigned k = 0; k < kAhead; ++k) {
+                    const unsigned v = first + k < a.tiles ? n[k] : 0;
+                    total[j] += v;
+                    before[j] += first + k < blockIdx.x ? v : 0;
+                }
             }
         }
         all += total[j];
@@ -237,61 +268,14 @@ struct Sums {
     void* d_table;
     float* partials;   // [group][entries of a token that began before; of one that goes on behind][width]
     float scale;
-    unsigned sum_blocks;
 };
 
-constexpr int kMaxChunk = 32, kZeroRows = 64;   // rows of the table that a workgroup looks for among the tokens
-
-template <class To, bool kNarrow, bool kPassing> __device__ __forceinline__ void zero_rows(const Sums& a, size_t row0) {
-    __shared__ int empty[kZeroRows];
-    // the entries of these rows, [lo, hi): all threads look at as many places at a time
-    unsigned lo = 0, hi = a.count, lo_end = a.count, hi_begin = 0;
-    const unsigned row1 = row0 + kZeroRows < a.vocabulary ? unsigned(row0) + kZeroRows : a.vocabulary;
-    if (threadIdx.x < kZeroRows) empty[threadIdx.x] = 1;
-    while (lo < lo_end || hi_begin < hi) {   // the first entry not below row0 lies in [lo, lo_end], the first not below row1 in [hi_begin, hi]
-        const unsigned step = (lo_end - lo) / kThreads + 1, step1 = (hi - hi_begin) / kThreads + 1;
-        const unsigned i = lo + threadIdx.x * step, i1 = hi_begin + threadIdx.x * step1;
-        const unsigned key = i < lo_end ? a.keys[i] : ~0u, key1 = i1 < hi ? a.keys[i1] : ~0u;
-        const unsigned below = __syncthreads_count(key < row0), below1 = __syncthreads_count(key1 < row1);
-        const unsigned end = lo + below * step, end1 = hi_begin + below1 * step1;
-        lo = below ? end - step + 1 : lo;
-        lo_end = below == 0 ? lo : end < lo_end ? end : lo_end;
-        hi_begin = below1 ? end1 - step1 + 1 : hi_begin;
-        hi = below1 == 0 ? hi_begin : end1 < hi ? end1 : hi;
-    }
-    if (hi - lo <= 4 * kThreads) {
-        for (unsigned i = lo + threadIdx.x; i < hi; i += kThreads) empty[a.keys[i] - unsigned(row0)] = 0;
-    } else if (threadIdx.x < kZeroRows && row0 + threadIdx.x < row1) {
-        const unsigned row = unsigned(row0) + threadIdx.x;
-        unsigned first = lo, end = hi;
-        while (first < end) {
-            const unsigned mid = first + (end - first) / 2;
-            if (a.keys[mid] < row) first = mid + 1; else end = mid;
-        }
-        empty[threadIdx.x] = first == hi || a.keys[first] != row;
-    }
-    __syncthreads();
-    // a wave a row, sixteen bytes a lane and store
-    constexpr int kPiece = 16 / int(sizeof(To));
-    typedef To Piece __attribute__((ext_vector_type(kPiece)));
-    const Piece zero = To(0.f);
-    for (unsigned r = threadIdx.x / kWave; r < row1 - unsigned(row0); r += kThreads / kWave) {
-        if (!empty[r]) continue;
-        To* out = static_cast<To*>(a.d_table) + (row0 + r) * a.width;
-        if constexpr (kNarrow) {
-            if (threadIdx.x % kWave < a.width) out[threadIdx.x % kWave] = To(0.f);
-        } else {
-            for (size_t i = threadIdx.x % kWave * kPiece; i < a.width; i += kWave * kPiece)
-                store_any<kPassing>(out + (i + kPiece <= a.width ? i : a.width - kPiece), zero);
-        }
-    }
-}
+constexpr int kMaxChunk = 32;
 
 // A thread sums the entries of one chunk in one vector of columns; kThreads / LANES chunks behind one another and LANES vectors beside one
 // another are a workgroup's.
 template <class From, class To, int LANES, bool kNarrow, bool kPassing> __global__ __launch_bounds__(kThreads) void sum_kernel(Sums a) {
     constexpr int kChunks = kThreads / LANES, kRows = sizeof(From) == 2 ? 8 : 4;   // rows on their way to a thread
-    if (blockIdx.x >= a.sum_blocks) return zero_rows<To, kNarrow, kPassing>(a, size_t(blockIdx.x - a.sum_blocks) * kZeroRows);
     __shared__ unsigned keys[kChunks * kMaxChunk + 2], at[kChunks * kMaxChunk];   // keys: with those in front of and behind the workgroup's
     __shared__ float8 heads[kChunks][LANES], tails[kChunks][LANES];
     const unsigned group = blockIdx.x / a.slabs, slab = blockIdx.x - group * a.slabs;
@@ -431,7 +415,7 @@ struct SumPlan {
 SumPlan sum_plan(const flstm_embedding* p) {
     const size_t vectors = ceil_div(p->width, 8);
     SumPlan s;
-    s.lanes = vectors <= 4 ? 4 : round_up(vectors, 8) * 10 <= round_up(vectors, 16) * 9 ? 8 : 16;
+    s.lanes = vectors <= 4 ? 4 : vectors <= 8 ? 8 : 16;
     s.slabs = unsigned(ceil_div(vectors, s.lanes));
     for (s.chunk = kMaxChunk; s.chunk > 8 && ceil_div(p->tokens, s.size()) * s.slabs < 512;) s.chunk /= 2;
     s.groups = unsigned(ceil_div(p->tokens, s.size()));
@@ -489,44 +473,58 @@ extern "C" int flstm_embedding_backward(const flstm_embedding* p, const void* d_
     a.count = unsigned(p->tokens); a.vocabulary = unsigned(p->vocabulary); a.vectors = unsigned(ceil_div(p->width, 8));
     a.groups = plan.groups; a.slabs = plan.slabs; a.chunk = plan.chunk;
     a.width = p->width; a.ldd = ldd; a.d_out = d_out; a.d_table = d_table; a.scale = p->scale;
-    const size_t sums = size_t(a.groups) * a.slabs, zeros = ceil_div(p->vocabulary, kZeroRows), joins = ceil_div(size_t(a.groups) * a.vectors, kThreads);
-    if (sums + zeros > 0xffffffffu / kThreads || joins > 0xffffffffu / kThreads) return FLSTM_E_TOO_LARGE;
-    if (p->tokens > 0) {
-        const Room room = room_of(p);
-        char* at = static_cast<char*>(workspace);
-        unsigned* lists[2][2] = {};
-        for (size_t i = 0; i < room.lists; ++i, at += room.list) lists[i / 2][i % 2] = reinterpret_cast<unsigned*>(at);
-        int last = 0;
-        if (ranked(p)) {
-            const size_t lds = (round_up(p->tokens, kRankWaves * 4) + kRankThreads) * 4;
-            rank_kernel<<<unsigned(ceil_div(p->tokens, kWave)), kRankThreads, lds, s>>>(tokens_of(p), lists[0][0], lists[0][1]);
-        } else {
-            const SortPlan sort = sort_plan(p);
-            SortPass pass{tokens_of(p), a.count, sort.tile, sort.tiles, 0, sort.bits, 1, nullptr, nullptr, nullptr, nullptr, reinterpret_cast<unsigned*>(at)};
-            for (int i = 0; i < sort.passes; ++i) {
-                last = i % 2;
-                pass.shift = i * sort.bits;
-                pass.first = i == 0;
-                pass.keys_in = lists[1 - last][0]; pass.at_in = lists[1 - last][1];
-                pass.keys_out = lists[last][0]; pass.at_out = lists[last][1];
-                count_kernel<<<sort.tiles, kSortThreads, 0, s>>>(pass);
-                scatter_kernel<<<sort.tiles, kSortThreads, 0, s>>>(pass);
-            }
+    const size_t sums = size_t(a.groups) * a.slabs, joins = ceil_div(size_t(a.groups) * a.vectors, kThreads);
+    const size_t size = table_dtype == FLSTM_OP_F32 ? 4 : 2, bytes = p->vocabulary * p->width * size;
+    const bool passing = bytes > kMostKept;
+    const SortPlan sort = sort_plan(p);
+    const int launches = ranked(p) ? 1 : 2 * sort.passes;
+    const size_t share = round_up(ceil_div(bytes, launches), kZeroBytes);   // that each clears
+    if (sums > 0xffffffffu / kThreads || joins > 0xffffffffu / kThreads || share / kZeroBytes + kMostRanked > 0xffffffffu / kRankThreads) return FLSTM_E_TOO_LARGE;
+    int launch = 0;
+    const auto zeros_behind = [&](unsigned blocks, unsigned& grid) {
+        const size_t from = share * launch++, some = from >= bytes ? 0 : bytes - from < share ? bytes - from : share;
+        grid = blocks + unsigned(ceil_div(some, kZeroBytes));
+        return Zeros{static_cast<char*>(d_table) + from, some, blocks};
+    };
+    const Room room = room_of(p);
+    char* at = static_cast<char*>(workspace);
+    unsigned* lists[2][2] = {};
+    for (size_t i = 0; i < room.lists; ++i, at += room.list) lists[i / 2][i % 2] = reinterpret_cast<unsigned*>(at);
+    int last = 0;
+    unsigned grid;
+    if (ranked(p)) {
+        const size_t lds = (round_up(p->tokens, kRankWaves * 4) + kRankThreads) * 4;
+        const Zeros zeros = zeros_behind(unsigned(ceil_div(p->tokens, kWave)), grid);
+        if (passing) rank_kernel<true><<<grid, kRankThreads, lds, s>>>(tokens_of(p), lists[0][0], lists[0][1], zeros);
+        else rank_kernel<false><<<grid, kRankThreads, lds, s>>>(tokens_of(p), lists[0][0], lists[0][1], zeros);
+    } else {
+        SortPass pass{tokens_of(p), a.count, sort.tile, sort.tiles, 0, sort.bits, 1, nullptr, nullptr, nullptr, nullptr, reinterpret_cast<unsigned*>(at)};
+        for (int i = 0; i < sort.passes; ++i) {
+            last = i % 2;
+            pass.shift = i * sort.bits;
+            pass.first = i == 0;
+            pass.keys_in = lists[1 - last][0]; pass.at_in = lists[1 - last][1];
+            pass.keys_out = lists[last][0]; pass.at_out = lists[last][1];
+            Zeros zeros = zeros_behind(sort.tiles, grid);
+            if (passing) count_kernel<true><<<grid, kSortThreads, 0, s>>>(pass, zeros);
+            else count_kernel<false><<<grid, kSortThreads, 0, s>>>(pass, zeros);
+            zeros = zeros_behind(sort.tiles, grid);
+            if (passing) scatter_kernel<true><<<grid, kSortThreads, 0, s>>>(pass, zeros);
+            else scatter_kernel<false><<<grid, kSortThreads, 0, s>>>(pass, zeros);
         }
-        if (const int rc = launched()) return rc;
-        a.keys = lists[last][0]; a.at = lists[last][1];
-        a.partials = reinterpret_cast<float*>(at + room.counts);
     }
-    a.sum_blocks = unsigned(sums);
+    if (const int rc = launched()) return rc;
+    if (p->tokens == 0) return 0;
+    a.keys = lists[last][0]; a.at = lists[last][1];
+    a.partials = reinterpret_cast<float*>(at + room.counts);
     return with_type(dtype, [&](auto from) {
         return with_type(table_dtype, [&](auto to) {
             typedef decltype(from) From;
             typedef decltype(to) To;
-            const unsigned grid = unsigned(sums + zeros);
-            const bool passing = p->vocabulary * p->width * sizeof(to) > kMostKept || p->tokens * p->width * sizeof(from) > kMostKept;
+            const unsigned grid = unsigned(sums);
             const auto sum = [&](auto lanes) {
                 constexpr int kLanes = decltype(lanes)::value;
-                if (passing) sum_kernel<From, To, kLanes, false, true><<<grid, kThreads, 0, s>>>(a);
+                if (p->tokens * p->width * sizeof(From) > kMostKept) sum_kernel<From, To, kLanes, false, true><<<grid, kThreads, 0, s>>>(a);
                 else sum_kernel<From, To, kLanes, false, false><<<grid, kThreads, 0, s>>>(a);
             };
             if (plan.lanes == 16) sum(std::integral_constant<int, 16>());
