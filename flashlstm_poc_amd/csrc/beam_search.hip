@@ -33,7 +33,7 @@ struct Select {
     float* out_scores;
     long long *out_parents, *out_tokens;
     unsigned char* out_finished;
-    size_t first;                   // the launch's first workgroup
+    size_t first;                   // the launch's first row, or sequence
 };
 
 // A logit as a whole number that orders alike; 0 for what is no candidate.
@@ -79,8 +79,7 @@ __device__ __forceinline__ u64 all_largest(u64 v, u64* scratch) {
 
 // The list again where very many logits are equal to the bound (those that a mask left at its type's lowest value, say): of these, those up to
 // a place that the first ones of all groups reach.  Returns how many there are then.
-template <class T> __device__ int fewer(const T* z, unsigned base, unsigned end, float bound, u64 before, int groups, u64* list,
-                                        float (*heads)[kMaxKeep], int& count) {
+template <class T> __device__ int fewer(const T* z, unsigned base, unsigned end, float bound, int groups, unsigned* places, float (*heads)[kMaxKeep], int& count) {
     const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
     const unsigned stop = end - base < unsigned(kTile) ? end - base : kTile;
     float first = __builtin_inff();
@@ -96,30 +95,28 @@ template <class T> __device__ int fewer(const T* z, unsigned base, unsigned end,
     first = heads[0][lane % groups];
     for (int w = 1; w < kThreads / kWave; ++w) first = fminf(first, heads[w][lane % groups]);
     const float place = lanes_max<kWave>(first);
-    const auto offer = [&](u64 key) {
-        const int at = atomicAdd(&count, 1);
-        if (at < kList) list[at] = key;
-    };
     for (unsigned c = tid; c < stop; c += kThreads) {
         const float x = number(float(z[base + c]));
-        if (x > bound || (x == bound && float(c) <= place)) offer(key_of(x, base + c));
+        if (x > bound || (x == bound && float(c) <= place)) {
+            const int at = atomicAdd(&count, 1);
+            if (at < kList) places[at] = base + c;
+        }
     }
-    if (before) offer(before);
     __syncthreads();
     return count;
 }
 
 template <class T> __global__ __launch_bounds__(kThreads) void part_kernel(Select a) {
-    __shared__ u64 list[kList], best[kMaxKeep], largest[kThreads / kWave];
+    __shared__ u64 list[kList + kMaxKeep], best[kMaxKeep], largest[kThreads / kWave];
+    __shared__ unsigned places[kList];
     __shared__ float heads[kThreads / kWave][kMaxKeep], waves[kThreads / kWave];
     __shared__ int count;
     const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-    const size_t block = a.first + blockIdx.x, row = block / unsigned(a.parts);
-    const unsigned part = unsigned(block - row * unsigned(a.parts)), begin = part * a.part;
+    const unsigned in_launch = blockIdx.x / unsigned(a.parts), part = blockIdx.x - in_launch * unsigned(a.parts), begin = part * a.part;
+    const size_t row = a.first + in_launch, block = row * unsigned(a.parts) + part;
     const unsigned end = a.vocabulary - begin < a.part ? a.vocabulary : begin + a.part;
     if (!(a.scores[row] > -__builtin_inff()) || (a.finished && a.finished[row])) return;   // (its continuations are not read)
     const T* z = static_cast<const T*>(a.logits) + row * a.ld;
-    if (tid < a.keep) best[tid] = 0;
     float most = kLowest, sum = 0.f;
     for (unsigned base = begin; base < end; base += kTile) {
         typename Vec8<T>::type v[kVectors];   // as they come: converted three times, in half the registers
@@ -158,7 +155,7 @@ template <class T> __global__ __launch_bounds__(kThreads) void part_kernel(Selec
         m = groups_fold(fminf(m, kHighest), a.groups, [](float x, float y) { return fmaxf(x, y); });
         if (lane < a.groups) heads[wave][lane] = m;
         if (tid == 0) count = 0;
-        __syncthreads();   // (`best` is there)
+        __syncthreads();
         m = heads[0][lane % a.groups];
 #pragma unroll
         for (int w = 1; w < kThreads / kWave; ++w) m = fmaxf(m, heads[w][lane % a.groups]);
@@ -172,26 +169,28 @@ template <class T> __global__ __launch_bounds__(kThreads) void part_kernel(Selec
         const float shift = most * kLog2e;
         const float reached = __builtin_fmaf(bound, kLog2e, -shift);   // (rounding keeps the order)
         float more = 0.f;
+        unsigned reach = 0;   // a bit for each of this thread's entries: which reach the bound
 #pragma unroll
         for (int j = 0; j < kVectors; ++j) {
             asm volatile("" : "+v"(v[j]));
-            float d[8], reach = -__builtin_inff();
+            float d[8], largest_d = -__builtin_inff();
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 d[i] = __builtin_fmaf(float(v[j][i]), kLog2e, -shift);
                 more += __builtin_amdgcn_exp2f(d[i]);
-                reach = fmaxf(reach, d[i]);
+                largest_d = fmaxf(largest_d, d[i]);
             }
-            if (!(reach < reached))   // (a thread's eight hardly ever hold one that does, a wave's mostly)
+            if (!(largest_d < reached)) {   // (a thread's eight hardly ever hold one that does, a wave's mostly)
+                unsigned bits = 0;
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (!(d[i] < reached)) {
-                        const float x = number(float(v[j][i]));
-                        if (x >= bound) {
-                            const int at = atomicAdd(&count, 1);
-                            if (at < kList) list[at] = key_of(x, place_of(j) + i);
-                        }
-                    }
+                for (int i = 7; i >= 0; --i) bits = bits + bits + unsigned(!(d[i] < reached));
+                reach |= bits << j * 8;
+            }
+        }
+        while (reach) {
+            const int e = __ffs(int(reach)) - 1, at = atomicAdd(&count, 1);
+            reach &= reach - 1;
+            if (at < kList) places[at] = place_of(e / 8) + e % 8;
         }
         if (more < __builtin_inff() && fabsf(shift) < __builtin_inff()) {
             more *= __builtin_amdgcn_exp2f(-__builtin_fmaf(most, kLog2e, -shift));
@@ -207,21 +206,24 @@ template <class T> __global__ __launch_bounds__(kThreads) void part_kernel(Selec
             sum = lanes_sum<kWave>(sum);
             if (lane == 0) waves[wave] = sum;
         }
-        const u64 before = tid < a.keep ? best[tid] : 0;   // of the tiles in front
-        if (before) {
-            const int at = atomicAdd(&count, 1);
-            if (at < kList) list[at] = before;
-        }
+        const u64 before = base > begin && tid < a.keep ? best[tid] : 0;   // of the tiles in front
         __syncthreads();
         int some = count;
-        if (some > kList) some = fewer(z, base, end, bound, before, a.groups, list, heads, count);
+        if (some > kList) some = fewer(z, base, end, bound, a.groups, places, heads, count);
         if (some <= kList) {
-            if (tid < a.keep && tid >= some) best[tid] = 0;
+            for (int i = tid; i < some; i += kThreads) list[i] = key_of(number(float(z[places[i]])), places[i]);
+            if (base > begin) {
+                if (tid < a.keep) list[some + tid] = before;
+                some += a.keep;
+            }
+            if (tid < a.keep) best[tid] = 0;
+            __syncthreads();
             for (int i = tid; i < some; i += kThreads) {
                 const u64 key = list[i];
                 int rank = 0;
+#pragma unroll 8
                 for (int j = 0; j < some; ++j) rank += list[j] > key;
-                if (rank < a.keep) best[rank] = key;
+                if (rank < a.keep && key) best[rank] = key;
             }
         } else {
             u64 last = ~u64(0);
@@ -265,7 +267,19 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Select a) {
     __shared__ int count;
     const size_t sequence = a.first + blockIdx.x, row0 = sequence * a.beams;
     const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-    const int per = a.parts * a.keep, all = a.beams * per;
+    // The best of all parts first, then the second, and so on: so each group of threads has some of the first, and its bound is close where parts are
+    // alike.  Where a part holds all of the best, the last of its entries is one that is closer; the larger of the two counts.
+    const int lists = a.beams * a.parts, all = lists * a.keep;
+    const float by_lists = 1.f / float(lists), by_parts = 1.f / float(a.parts);
+    const auto quotient = [](int i, float inverse) { return int((float(i) + 0.5f) * inverse); };   // (of numbers below 2^17: half a step is more than any error)
+    const auto key_at = [&](int i) {
+        const int rank = quotient(i, by_lists);
+        return a.best[(row0 * a.parts + (i - rank * lists)) * a.keep + rank];
+    };
+    constexpr int kHeld = 8;   // of a thread's continuations, requested at once
+    u64 held[kHeld];
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) held[j] = tid + j * kThreads < all ? key_at(tid + j * kThreads) : 0;
     for (int b = wave; b < a.beams; b += kThreads / kWave) {
         const float score = a.scores[row0 + b];
         const bool done = a.finished && a.finished[row0 + b], alive = score > -__builtin_inff() && !done;
@@ -281,20 +295,31 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Select a) {
     if (tid < a.keep) best[tid] = Candidate{0, 0};
     if (tid == 0) count = 0;
     __syncthreads();
-    const auto candidate = [&](int i) {
-        const int b = i / per;
+    const auto candidate_of = [&](int i, u64 key) {
+        const int rank = quotient(i, by_lists), b = quotient(i - rank * lists, by_parts);
         const u64 row = u64(b) * a.vocabulary;
-        if (state[b] == 2) return i == b * per ? Candidate{order_of(rest[b]), row + u64(a.end)} : Candidate{0, 0};
-        const u64 key = state[b] == 1 ? a.best[row0 * per + i] : 0;
-        return key ? Candidate{order_of(double(logit_of(unsigned(key >> 32))) - most[b] + rest[b]), row + unsigned(~key)} : Candidate{0, 0};
+        if (state[b] == 2) return i == b * a.parts ? Candidate{order_of(rest[b]), row + u64(a.end)} : Candidate{0, 0};
+        return key && state[b] == 1 ? Candidate{order_of(double(logit_of(unsigned(key >> 32))) - most[b] + rest[b]), row + unsigned(~key)} : Candidate{0, 0};
     };
-    u64 head = 0;
-    const Candidate own = tid < all ? candidate(tid) : Candidate{0, 0};   // (most calls have no more)
-    head = own.order;
-    for (int i = tid + kThreads; i < all; i += kThreads) {
-        const u64 o = candidate(i).order;
+    const auto candidate = [&](int i) { return candidate_of(i, key_at(i)); };
+    u64 head = 0, end_of_list = 0, orders[kHeld];
+    const auto heads_of = [&](int i, u64 o) {
         head = o > head ? o : head;
+        if (i >= all - lists) end_of_list = o > end_of_list ? o : end_of_list;
+    };
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+        const int i = tid + j * kThreads;
+        orders[j] = i < all ? candidate_of(i, held[j]).order : 0;
+        heads_of(i, orders[j]);
     }
+    for (int i = tid + kHeld * kThreads; i < all; i += kThreads) heads_of(i, candidate(i).order);
+#pragma unroll
+    for (int d = kWave / 2; d > 0; d /= 2) {
+        const u64 other = __shfl_xor(end_of_list, d);
+        end_of_list = other > end_of_list ? other : end_of_list;
+    }
+    if (lane == 0) largest[wave] = end_of_list;
     for (int d = kWave / 2; d >= a.groups; d /= 2) {
         const u64 other = __shfl_xor(head, d);
         head = other > head ? other : head;
@@ -308,20 +333,25 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Select a) {
         const u64 other = __shfl_xor(bound, d);
         bound = other < bound ? other : bound;
     }
+#pragma unroll
+    for (int w = 0; w < kThreads / kWave; ++w) bound = largest[w] > bound ? largest[w] : bound;
     const auto offer = [&](const Candidate& c) {
         if (c.order && c.order >= bound) {
             const int at = atomicAdd(&count, 1);
             if (at < kList) list[at] = c;
         }
     };
-    offer(own);
-    for (int i = tid + kThreads; i < all; i += kThreads) offer(candidate(i));
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j)
+        if (orders[j] && orders[j] >= bound) offer(candidate_of(tid + j * kThreads, held[j]));
+    for (int i = tid + kHeld * kThreads; i < all; i += kThreads) offer(candidate(i));
     __syncthreads();
     const int some = count;
     if (some <= kList) {
         for (int i = tid; i < some; i += kThreads) {
             const Candidate c = list[i];
             int rank = 0;
+#pragma unroll 8
             for (int j = 0; j < some; ++j) rank += ahead(list[j], c);
             if (rank < a.keep) best[rank] = c;
         }
@@ -362,7 +392,7 @@ struct State {
     char* data;
     size_t stride, bytes;
     unsigned slabs;      // workgroups a sequence
-    size_t first;        // its first workgroup
+    unsigned first;      // its first workgroup
 };
 struct Reorder {
     const long long* parents;
@@ -381,9 +411,9 @@ template <int B> __global__ __launch_bounds__(kThreads) void reorder_kernel(Reor
     int i = 0;
     while (i + 1 < a.count && a.states[i + 1].first <= blockIdx.x) ++i;
     const State& s = a.states[i];
-    const size_t block = blockIdx.x - s.first, sequence = block / s.slabs;
-    const size_t at = ((block - sequence * s.slabs) * kThreads + threadIdx.x) * 16;
-    const long long* parents = a.parents + sequence * a.beams;
+    const unsigned block = blockIdx.x - s.first, sequence = block / s.slabs;
+    const size_t at = (size_t(block - sequence * s.slabs) * kThreads + threadIdx.x) * 16;
+    const long long* parents = a.parents + size_t(sequence) * a.beams;
     int from[B];
 #pragma unroll
     for (int b = 0; b < B; ++b) {
@@ -391,7 +421,7 @@ template <int B> __global__ __launch_bounds__(kThreads) void reorder_kernel(Reor
         from[b] = p >= 0 && p < a.beams ? int(p) : b;
     }
     if (at >= s.bytes) return;
-    char* row = s.data + sequence * a.beams * s.stride + at;
+    char* row = s.data + size_t(sequence) * a.beams * s.stride + at;
     if (s.bytes - at >= 16) {
         floatx4 v[B];
 #pragma unroll
@@ -451,10 +481,10 @@ extern "C" int flstm_beam_select(const flstm_beams* p, float* scores, long long*
     while (a.groups < a.keep) a.groups *= 2;
     a.end = p->end; a.best = static_cast<u64*>(workspace); a.sums = reinterpret_cast<float2*>(static_cast<char*>(workspace) + best_bytes(p));
     a.out_scores = scores; a.out_parents = parents; a.out_tokens = tokens; a.out_finished = finished;
-    const size_t blocks = p->sequences * p->beams * a.parts;
+    const size_t rows = p->sequences * p->beams, most = kMostBlocks / a.parts;   // rows a launch
     hipStream_t s = static_cast<hipStream_t>(stream);
-    for (a.first = 0; a.first < blocks; a.first += kMostBlocks) {
-        const unsigned some = unsigned(blocks - a.first < kMostBlocks ? blocks - a.first : kMostBlocks);
+    for (a.first = 0; a.first < rows; a.first += most) {
+        const unsigned some = unsigned((rows - a.first < most ? rows - a.first : most) * a.parts);
         const int rc = with_type(p->dtype, [&](auto zero) {
             part_kernel<decltype(zero)><<<some, kThreads, 0, s>>>(a);
             return launched();
@@ -480,10 +510,10 @@ extern "C" int flstm_beam_reorder(size_t sequences, int beams, const long long* 
         if (!states[i].data || states[i].stride < states[i].bytes) return FLSTM_E_INVALID;
         const size_t slabs = ceil_div(states[i].bytes, kThreads * 16);
         if (slabs > kMostBlocks || sequences > kMostBlocks / slabs) return FLSTM_E_TOO_LARGE;
-        a.states[a.count++] = State{static_cast<char*>(states[i].data), states[i].stride, states[i].bytes, unsigned(slabs), blocks};
         blocks += slabs * sequences;
+        if (blocks > kMostBlocks) return FLSTM_E_TOO_LARGE;
+        a.states[a.count++] = State{static_cast<char*>(states[i].data), states[i].stride, states[i].bytes, unsigned(slabs), unsigned(blocks - slabs * sequences)};
     }
-    if (blocks > kMostBlocks) return FLSTM_E_TOO_LARGE;
     if (blocks == 0) return 0;
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (beams <= 4) reorder_kernel<4><<<unsigned(blocks), kThreads, 0, s>>>(a);

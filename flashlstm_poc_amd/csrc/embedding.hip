@@ -352,10 +352,10 @@ template <class From, class To, int LANES, bool kNarrow, bool kPassing> __global
 
 // What each token's entries left in more than one group: the group that they begin in adds them up.
 template <class To, bool kNarrow> __global__ __launch_bounds__(kThreads) void join_kernel(Sums a, unsigned size) {
-    const size_t item = size_t(blockIdx.x) * kThreads + threadIdx.x;
-    unsigned group = unsigned(item / a.vectors);
+    const unsigned item = blockIdx.x * kThreads + threadIdx.x;
+    unsigned group = item / a.vectors;
     if (group + 1 >= a.groups) return;
-    const size_t c = column<kNarrow>(item - size_t(group) * a.vectors, a.width);
+    const size_t c = column<kNarrow>(item - group * a.vectors, a.width);
     const unsigned begin = group * size, last = begin + size - 1, token = a.keys[last];
     if (token >= a.vocabulary || a.keys[last + 1] != token || (begin > 0 && a.keys[begin - 1] == token)) return;
     const float* partial = a.partials + c;

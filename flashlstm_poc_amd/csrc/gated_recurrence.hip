@@ -593,9 +593,9 @@ __global__ __launch_bounds__(kThreads) void clear_kernel(u64* words, size_t coun
 }
 
 // One token of every sequence: vectors of eight channels.
-template <class T, bool kGate> __global__ __launch_bounds__(kThreads) void step_kernel(Recurrence a, unsigned vectors) {
-    const size_t item = size_t(blockIdx.x) * kThreads + threadIdx.x;
-    const size_t n = item / vectors, c = (item - n * vectors) * 8;
+template <class T, bool kGate> __global__ __launch_bounds__(kThreads) void step_kernel(Recurrence a, unsigned vectors, size_t first) {
+    const unsigned item = blockIdx.x * kThreads + threadIdx.x, in_launch = item / vectors;
+    const size_t n = first + in_launch, c = size_t(item - in_launch * vectors) * 8;
     if (n >= a.sequences) return;
     const int many = a.width - c < 8 ? int(a.width - c) : 8;
     const auto row = [&](const Rows& r) { return static_cast<T*>(r.data) + (long long)n * r.sequence + c; };
@@ -737,13 +737,18 @@ extern "C" int flstm_gated_recurrence_step(const flstm_recurrence* p, const flst
     a.sequences = p->sequences; a.width = unsigned(p->width); a.final = state;
     a.x = rows(x); a.forget = rows(forget); a.gate = rows(gate); a.y = rows(y);
     if (!a.x.data || !a.forget.data || !a.y.data || !state) return FLSTM_E_INVALID;
-    const size_t vectors = ceil_div(p->width, 8), grid = ceil_div(p->sequences * vectors, kThreads);
-    if (grid > kMostThreads / kThreads) return FLSTM_E_TOO_LARGE;
+    const size_t vectors = ceil_div(p->width, 8), most = (size_t(1) << 31) / vectors;   // sequences a launch
     return with_type(p->dtype, [&](auto zero) {
         typedef decltype(zero) T;
         hipStream_t s = static_cast<hipStream_t>(stream);
-        if (a.gate.data) step_kernel<T, true><<<unsigned(grid), kThreads, 0, s>>>(a, unsigned(vectors));
-        else step_kernel<T, false><<<unsigned(grid), kThreads, 0, s>>>(a, unsigned(vectors));
-        return launched();
+        for (size_t first = 0; first < p->sequences; first += most) {
+            const size_t some = p->sequences - first < most ? p->sequences - first : most;
+            a.sequences = first + some;
+            const unsigned grid = unsigned(ceil_div(some * vectors, kThreads));
+            if (a.gate.data) step_kernel<T, true><<<grid, kThreads, 0, s>>>(a, unsigned(vectors), first);
+            else step_kernel<T, false><<<grid, kThreads, 0, s>>>(a, unsigned(vectors), first);
+            if (const int rc = launched()) return rc;
+        }
+        return 0;
     });
 }
