@@ -35,7 +35,7 @@ struct Recurrence {
     const float *initial, *d_final;   // (sequences, width) or null
     float *final, *d_initial;
     float* saved;             // [batch slot][width]
-    unsigned* ticket;         // workgroups that have begun
+    unsigned* ticket;         // workgroups that have begun; behind it, whether one has waited in vain
     u64* made[3];             // [slot][width]: what segments, groups of kGroup segments and groups of these make of a state
 };
 
@@ -330,9 +330,10 @@ template <class T, int C, bool kGate, bool kPassing> __global__ __launch_bounds_
 // waits for have begun before it, and each publishes before it waits: every wait ends.  What a segment needs of those in front
 // of it is what the groups of groups, the groups in the last of these, and the segments in the last group make of a state; the last segment
 // of a group publishes the group's, as soon as it has its own group's.  A published pair is one word, which is its own flag: words are kNothing before.
+// (With cu_seqlens that do not ascend a group may have no last segment.  What is not there after a second reads as NaN, and nobody waits from then on.)
 
 constexpr u64 kNothing = ~u64(0);
-constexpr unsigned kMostPolls = 1u << 21;   // some seconds; what is not there then reads as NaN
+constexpr unsigned kMostPolls = 1u << 20;
 
 struct Made {
     float factor, sum;   // state -> factor * state + sum
@@ -350,7 +351,7 @@ __device__ __forceinline__ void publish(u64* row, unsigned at, Made m) {
 __device__ __forceinline__ u64 look(const u64* row, unsigned at) { return __hip_atomic_load(word_of(row, at), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
 // What the pairs of `count` rows from `row` on, `step` words apart, make of a state, one after the other.
-__device__ __forceinline__ Made read_made(const u64* row, ptrdiff_t step, long long count, unsigned at) {
+__device__ __forceinline__ Made read_made(const u64* row, ptrdiff_t step, long long count, unsigned at, unsigned* in_vain) {
     Made m{1.f, 0.f};
     constexpr int kAhead = 8;
     for (long long i = 0; i < count; i += kAhead, row += kAhead * step) {
@@ -361,9 +362,11 @@ __device__ __forceinline__ Made read_made(const u64* row, ptrdiff_t step, long l
 #pragma unroll
         for (int k = 0; k < kAhead; ++k)
             if (i + k < count) {
-                for (unsigned poll = 0; v[k] == kNothing && poll < kMostPolls; ++poll) {
+                for (unsigned poll = 1; v[k] == kNothing && poll <= kMostPolls; ++poll) {
                     __builtin_amdgcn_s_sleep(1);
                     v[k] = look(row + k * step, at);
+                    if (poll % 256 == 0 && __hip_atomic_load(in_vain, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) break;
+                    if (poll == kMostPolls) __hip_atomic_store(in_vain, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 }
                 m = then(m, __builtin_bit_cast(Made, v[k]));
             }
@@ -433,17 +436,17 @@ template <int C, int W, bool kBack> __device__ __forceinline__ void state_at(con
 #pragma unroll
         for (int w = 1; w < W; ++w) all = then(all, parts[w][ch]);
         publish(row_at(0, p.slot), word, all);
-        const Made front = read_made(row_at(0, kBack ? p.slot + few : p.slot - few), kBack ? -width : width, few, word);
+        const Made front = read_made(row_at(0, kBack ? p.slot + few : p.slot - few), kBack ? -width : width, few, word, a.ticket + 1);
         before[0][ch] = front;
         all = then(front, all);
         if (few == kGroup - 1) publish(row_at(1, first_slot(a, p.n, kSize * kGroup) + group), word, all);
     } else if (mine) {
-        if (role == 1) before[1][ch] = read_made(row_at(1, first_slot(a, p.n, kSize * kGroup) + group - few_groups), width, few_groups, word);
+        if (role == 1) before[1][ch] = read_made(row_at(1, first_slot(a, p.n, kSize * kGroup) + group - few_groups), width, few_groups, word, a.ticket + 1);
         if (role > 1 || kRoles == 2) {   // the groups of groups, in as many parts as there are roles for
             constexpr int kParts = kRoles == 2 ? 1 : kRoles - 2;
             const int part = kRoles == 2 ? 0 : role - 2;
             const long long some = (groups + kParts - 1) / kParts, begin = part * some, left = groups - begin < some ? groups - begin : some;
-            before[2 + part][ch] = read_made(row_at(2, first_slot(a, p.n, kSize * kGroup * kGroup) + begin), width, left, word);
+            before[2 + part][ch] = read_made(row_at(2, first_slot(a, p.n, kSize * kGroup * kGroup) + begin), width, left, word, a.ticket + 1);
         }
     }
     __syncthreads();
@@ -483,17 +486,24 @@ __global__ __launch_bounds__(W * kWave, C == 2 && sizeof(T) == 2 ? 6 : 3) void s
     };
     if (count == kBatch) load(std::true_type());
     else load(std::false_type());
+    // Of half of the tokens the factors stay in LDS, which is three workgroups' for that: two functions less a token (257 us instead of 277 for 131072 tokens
+    // of 1024 channels with a gate, bf16, where the vector units are the bound).
+    constexpr int kInLds = sizeof(T) == 2 ? kBatch / 2 : 0;
+    __shared__ Few<float, C> factors[kInLds ? kInLds : 1][kInLds ? W * kWave : 1];
     Made made[C];
 #pragma unroll
     for (int j = 0; j < C; ++j) made[j] = Made{1.f, 0.f};
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
         hold_factors<T, C>(u[i]);
+        float small[C];
 #pragma unroll
         for (int j = 0; j < C; ++j) {
             const Factor k = held_factor<T>(u[i][j]);
+            small[j] = __builtin_copysignf(k.small, k.keeps ? 1.f : -1.f);
             made[j] = Made{kept(k, made[j].factor), stepped(k, made[j].sum, x[i][j])};
         }
+        if (i < kInLds) __builtin_memcpy(&factors[i][threadIdx.x].word, small, sizeof(small));
     }
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
@@ -508,9 +518,12 @@ __global__ __launch_bounds__(W * kWave, C == 2 && sizeof(T) == 2 ? 6 : 3) void s
     for (int i = 0; i < kBatch; ++i) {
         if (i >= count) continue;
         float o[C];
+        Few<float, C> in_lds{};
+        if (i < kInLds) in_lds = factors[i][threadIdx.x];
 #pragma unroll
         for (int j = 0; j < C; ++j) {
-            s[j] = stepped(held_factor<T>(u[i][j]), s[j], x[i][j]);
+            const Factor k = i < kInLds ? held_factor<float>(in_lds[j]) : held_factor<T>(u[i][j]);
+            s[j] = stepped(k, s[j], x[i][j]);
             o[j] = s[j];
             if constexpr (kGate) o[j] *= sigmoid<T>(g[i][j]);
         }

@@ -49,7 +49,8 @@ def _check_backward(d_out, tokens, vocabulary, scale=1.0, dtype=torch.float32):
     held = (flat >= 0) & (flat < vocabulary)
     index = torch.where(held, flat, vocabulary).long()
     scale = float(torch.tensor(scale, dtype=torch.float32))
-    sums = lambda x: torch.zeros(vocabulary + 1, x.shape[1], device=x.device, dtype=torch.float64).index_add_(0, index, x)[:-1]
+    index = index.cpu()
+    sums = lambda x: torch.zeros(vocabulary + 1, x.shape[1], dtype=torch.float64).index_add_(0, index, x.cpu())[:-1].to(d.device)
     want, size, count = scale * sums(d), abs(scale) * sums(d.abs()), sums(torch.ones_like(d[:, :1]))
     assert_within(got, want, U32 * (count + 1) * size, f"{tuple(tokens.shape)} over {vocabulary} {d_out.dtype} to {dtype}")
     return got

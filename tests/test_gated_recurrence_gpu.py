@@ -27,7 +27,7 @@ def _problem(shape, dtype, states, gate=True, seed=0, keeps=3.0):
 
 
 def _one(x, u, g, state, dy, d_state):
-    """One sequence (tokens, width) token by token: every output with its bound."""
+    """Sequences of one length (tokens, .., width) token by token: every output with its bound."""
     x, u, dy = x.double(), u.double(), dy.double()
     f, z = torch.sigmoid(u), torch.sigmoid(-u)
     small, rel = torch.minimum(f, z), (u.abs() + 8) * U32
@@ -74,21 +74,24 @@ def _one(x, u, g, state, dy, d_state):
 
 
 def _definition(p, spans):
-    flat = {k: None if p[k] is None else p[k].reshape(-1, p[k].shape[-1]) for k in ("x", "forget", "gate", "dy")}
-    of_rows = {k: (torch.zeros_like(flat["x"], dtype=torch.float64), torch.zeros_like(flat["x"], dtype=torch.float64)) for k in
-               ("y", "dx", "dforget") + (("dgate",) if p["gate"] is not None else ())}
+    names = ("x", "forget", "gate", "dy")
+    rows = ("y", "dx", "dforget") + (("dgate",) if p["gate"] is not None else ())
+    zeros = torch.zeros(len(spans), p["x"].shape[-1], device="cuda")
+    state, d_state = (zeros if p[k] is None else p[k] for k in ("state", "d_state"))
+    if p["x"].dim() == 3:   # sequences of one length, all at once
+        part = {k: None if p[k] is None else p[k].transpose(0, 1) for k in names}
+        one = _one(part["x"], part["forget"], part["gate"], state, part["dy"], d_state)
+        return {k: tuple(t.transpose(0, 1) for t in v) if k in rows else v for k, v in one.items()}
+    out = {k: (torch.zeros_like(p["x"], dtype=torch.float64), torch.zeros_like(p["x"], dtype=torch.float64)) for k in rows}
     of_states = {"state": ([], []), "d_initial": ([], [])}
-    zeros = torch.zeros(p["x"].shape[-1], device="cuda")
     for n, (a, b) in enumerate(spans):
-        part = {k: None if v is None else v[a:b] for k, v in flat.items()}
-        one = _one(part["x"], part["forget"], part["gate"], zeros if p["state"] is None else p["state"][n], part["dy"],
-                   zeros if p["d_state"] is None else p["d_state"][n])
-        for k, pair in of_rows.items():
+        part = {k: None if p[k] is None else p[k][a:b] for k in names}
+        one = _one(part["x"], part["forget"], part["gate"], state[n], part["dy"], d_state[n])
+        for k, pair in out.items():
             pair[0][a:b], pair[1][a:b] = one[k]
         for k, pair in of_states.items():
             pair[0].append(one[k][0])
             pair[1].append(one[k][1])
-    out = {k: tuple(t.view(p["x"].shape) for t in pair) for k, pair in of_rows.items()}
     out.update({k: tuple(torch.stack(l) for l in pair) for k, pair in of_states.items() if pair[0]})
     return out
 
