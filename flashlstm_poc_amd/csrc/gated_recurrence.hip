@@ -208,8 +208,8 @@ template <int C> __device__ __forceinline__ unsigned first_channel(const Recurre
 struct Gradients {
     char *dx, *dforget, *dgate;   // rows, or null
 };
-template <class T, int C, bool kGate, bool kScalar, bool kPassing, class F>
-__device__ __forceinline__ void gradients(const Recurrence& a, const Gradients& to, int i, unsigned at, F&& factor, const Few<T, C>& u, const Few<T, C>& x, const Few<T, C>& d,
+template <class T, int C, bool kGate, bool kScalar, bool kPassing, class F, class U>
+__device__ __forceinline__ void gradients(const Recurrence& a, const Gradients& to, int i, unsigned at, F&& factor, const U& u, const Few<T, C>& x, const Few<T, C>& d,
                                           const Few<T, C>& g, const float (&before)[C], const float (&after)[C], float (&s)[C]) {
     float of_x[C], of_forget[C], of_gate[C];
 #pragma unroll
@@ -562,19 +562,24 @@ template <class T, int C, bool kGate, bool kPassing, int W> __global__ __launch_
     else load(std::false_type());
     Few<float, C> first{};
     if (count > 0) first = load_state<C>(a.saved, first_slot(a, p.n, kBatch) + t / kBatch, a, c);
+    constexpr int kInLds = sizeof(T) == 2 ? kBatch : 0;   // tokens whose factors stay in LDS
+    __shared__ Few<float, C> factors[kInLds ? kInLds : 1][kInLds ? W * kWave : 1];
     Made made[C];
 #pragma unroll
     for (int j = 0; j < C; ++j) made[j] = Made{1.f, 0.f};
 #pragma unroll
     for (int i = kBatch - 1; i >= 0; --i) {
         hold_factors<T, C>(u[i]);
+        float small[C];
 #pragma unroll
         for (int j = 0; j < C; ++j) {
             const Factor k = held_factor<T>(u[i][j]);
+            small[j] = __builtin_copysignf(k.small, k.keeps ? 1.f : -1.f);
             float dc = d[i][j];
             if constexpr (kGate) dc *= sigmoid<T>(g[i][j]);
             made[j] = Made{kept(k, made[j].factor), kept(k, made[j].sum + dc)};
         }
+        if (i < kInLds) __builtin_memcpy(&factors[i][threadIdx.x].word, small, sizeof(small));
     }
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
@@ -591,12 +596,15 @@ template <class T, int C, bool kGate, bool kPassing, int W> __global__ __launch_
     for (int i = 0; i < kBatch; ++i) {
         x[i].forget();   // (the states from here on)
 #pragma unroll
-        for (int j = 0; j < C; ++j) state[i + 1][j] = stepped(held_factor<T>(u[i][j]), state[i][j], x[i][j]);
+        for (int j = 0; j < C; ++j) state[i + 1][j] = stepped(i < kInLds ? held_factor<float>(factors[i][threadIdx.x][j]) : held_factor<T>(u[i][j]), state[i][j], x[i][j]);
     }
     const Gradients to = gradients_at<T>(a, p, t);
 #pragma unroll
     for (int i = kBatch - 1; i >= 0; --i)
-        if (i < count) gradients<T, C, kGate, true, kPassing>(a, to, i, at, held_factor<T>, u[i], x[i], d[i], g[i], state[i], state[i + 1], s);
+        if (i < count) {
+            if constexpr (kInLds > 0) gradients<T, C, kGate, true, kPassing>(a, to, i, at, held_factor<float>, factors[i][threadIdx.x], x[i], d[i], g[i], state[i], state[i + 1], s);
+            else gradients<T, C, kGate, true, kPassing>(a, to, i, at, held_factor<T>, u[i], x[i], d[i], g[i], state[i], state[i + 1], s);
+        }
     if (p.begin == 0 && wave == 0 && a.d_initial) store_state<C>(a.d_initial, p.n, a, c, s);
 }
 
