@@ -175,53 +175,84 @@ template <bool kPassing> __global__ __launch_bounds__(kSortThreads) void count_k
     for (unsigned b = threadIdx.x; b < bins; b += kSortThreads) a.counts[size_t(blockIdx.x) * bins + b] = counts[b];
 }
 
+// Adds the tiles' counts of every bin up: those in front of this workgroup's, and all.  A thread has P bins, kSortThreads apart, or where there are fewer bins
+// than threads some of the tiles.
+template <unsigned P> __device__ __forceinline__ void add_counts(const SortPass& a, unsigned* in_front, unsigned* in_all) {
+    constexpr unsigned kAhead = 16;   // tiles on their way together
+    const unsigned bins = 1u << a.bits, sharers = bins < kSortThreads ? kSortThreads / bins : 1, b = threadIdx.x % bins;
+    unsigned before[P], total[P];
+#pragma unroll
+    for (unsigned j = 0; j < P; ++j) before[j] = total[j] = 0;
+    for (unsigned first = threadIdx.x / bins; first < a.tiles; first += kAhead * sharers) {
+        unsigned n[P][kAhead];
+#pragma unroll
+        for (unsigned k = 0; k < kAhead; ++k)
+#pragma unroll
+            for (unsigned j = 0; j < P; ++j) {
+                const unsigned tile = first + k * sharers;
+                n[j][k] = a.counts[size_t(tile < a.tiles ? tile : first) * bins + b + j * kSortThreads];
+            }
+#pragma unroll
+        for (unsigned k = 0; k < kAhead; ++k)
+#pragma unroll
+            for (unsigned j = 0; j < P; ++j) {
+                const unsigned tile = first + k * sharers, v = tile < a.tiles ? n[j][k] : 0;
+                total[j] += v;
+                before[j] += tile < blockIdx.x ? v : 0;
+            }
+    }
+#pragma unroll
+    for (unsigned j = 0; j < P; ++j) {
+        if (total[j]) atomicAdd(&in_all[b + j * kSortThreads], total[j]);
+        if (before[j]) atomicAdd(&in_front[b + j * kSortThreads], before[j]);
+    }
+}
+
 template <bool kPassing> __global__ __launch_bounds__(kSortThreads) void scatter_kernel(SortPass a, Zeros zeros) {
     if (blockIdx.x >= zeros.first) return clear_share<kPassing>(zeros);
     __shared__ unsigned place[kSortWaves][1 << kMaxBits];   // counts of each wave's part, then where its next entry goes
-    __shared__ unsigned sums[kSortWaves];
+    __shared__ unsigned sums[(1 << kMaxBits) / kSortThreads][kSortWaves], in_front[1 << kMaxBits], in_all[1 << kMaxBits];
     const unsigned bins = 1u << a.bits, wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
     const unsigned begin = blockIdx.x * a.tile, end = a.count - begin < a.tile ? a.count : begin + a.tile;
     const unsigned part = a.tile / kSortWaves, from = begin + wave * part;
     const unsigned to = from >= end ? from : end - from < part ? end : from + part;
     for (unsigned b = lane; b < bins; b += kWave) place[wave][b] = 0;
     for (unsigned i = from + lane; i < to; i += kWave) atomicAdd(&place[wave][key_at(a, i) >> a.shift & (bins - 1)], 1u);
-    // entries of a bin in the tiles in front, and in all of them; a thread has `per` consecutive bins
-    const unsigned per = (bins + kSortThreads - 1) / kSortThreads;
-    unsigned before[(1 << kMaxBits) / kSortThreads], total[(1 << kMaxBits) / kSortThreads], all = 0;
-#pragma unroll
-    for (unsigned j = 0; j < (1 << kMaxBits) / kSortThreads; ++j) {
-        before[j] = total[j] = 0;
-        const unsigned b = threadIdx.x * per + j;
-        if (j < per && b < bins) {
-            constexpr unsigned kAhead = 16;   // on their way together
-            for (unsigned first = 0; first < a.tiles; first += kAhead) {
-                unsigned n[kAhead];
-#pragma unroll
-                for (unsigned k = 0; k < kAhead; ++k) n[k] = a.counts[size_t(first + k < a.tiles ? first + k : first) * bins + b];
-#pragma unroll
-                for (unsigned k = 0; k < kAhead; ++k) {
-                    const unsigned v = first + k < a.tiles ? n[k] : 0;
-                    total[j] += v;
-                    before[j] += first + k < blockIdx.x ? v : 0;
-                }
-            }
-        }
-        all += total[j];
-    }
-    unsigned at = all;   // the sum over the threads up to this one
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) {
-        const unsigned v = __shfl_up(at, d);
-        at += int(lane) >= d ? v : 0;
-    }
-    if (lane == kWave - 1) sums[wave] = at;
+    // entries of a bin in the tiles in front, and in all of them
+    constexpr unsigned kPer = (1 << kMaxBits) / kSortThreads;
+    for (unsigned b = threadIdx.x; b < bins; b += kSortThreads) in_front[b] = in_all[b] = 0;
     __syncthreads();
-    at -= all;
-    for (unsigned w = 0; w < wave; ++w) at += sums[w];
+    if (bins > kSortThreads) add_counts<kPer>(a, in_front, in_all);
+    else add_counts<1>(a, in_front, in_all);
+    __syncthreads();
+    unsigned before[kPer], total[kPer];
 #pragma unroll
-    for (unsigned j = 0; j < (1 << kMaxBits) / kSortThreads; ++j) {
-        const unsigned b = threadIdx.x * per + j;
-        if (j < per && b < bins) {
+    for (unsigned j = 0; j < kPer; ++j) {
+        const unsigned b = threadIdx.x + j * kSortThreads;
+        before[j] = b < bins ? in_front[b] : 0;
+        total[j] = b < bins ? in_all[b] : 0;
+    }
+    unsigned start = 0;   // of the thread's bins, the entries in all bins in front of the first
+#pragma unroll
+    for (unsigned j = 0; j < kPer; ++j) {
+        const unsigned b = threadIdx.x + j * kSortThreads;
+        unsigned at = total[j];   // the sum over the threads up to this one
+#pragma unroll
+        for (int d = 1; d < kWave; d *= 2) {
+            const unsigned v = __shfl_up(at, d);
+            at += int(lane) >= d ? v : 0;
+        }
+        if (lane == kWave - 1) sums[j][wave] = at;
+        __syncthreads();
+        at += start - total[j];
+        unsigned all = 0;
+#pragma unroll
+        for (unsigned w = 0; w < kSortWaves; ++w) {
+            at += w < wave ? sums[j][w] : 0;
+            all += sums[j][w];
+        }
+        start += all;
+        if (b < bins) {
             unsigned next = at + before[j];
 #pragma unroll
             for (int w = 0; w < kSortWaves; ++w) {
@@ -230,7 +261,6 @@ template <bool kPassing> __global__ __launch_bounds__(kSortThreads) void scatter
                 next += n;
             }
         }
-        at += total[j];
     }
     __syncthreads();
     // (the loop's count is the wave's own, so that all its lanes take part in the ballots)
@@ -284,8 +314,20 @@ template <class From, class To, int LANES, bool kNarrow, bool kPassing> __global
     const unsigned begin = group * size;
     const int here = a.count - begin < unsigned(size) ? int(a.count - begin) : size;
     constexpr unsigned kNone = ~0u;   // no token, and not the one behind the vocabulary
-    for (int i = tid; i < size + 2; i += kThreads) keys[i] = i <= here + 1 && (i > 0 || group > 0) && begin + i - 1 < a.count ? a.keys[begin + i - 1] : kNone;
-    for (int i = tid; i < size; i += kThreads) at[i] = a.at[i < here ? begin + i : begin];   // (any row, where there is none)
+#pragma unroll
+    for (int j = 0; j < kChunks * kMaxChunk / kThreads; ++j) {
+        const int i = tid + j * kThreads;
+        const unsigned from = i < here ? begin + i : begin;   // (any entry, where there is none)
+        const unsigned key = a.keys[from], place = a.at[from];
+        if (i < size) {
+            keys[i + 1] = i < here ? key : kNone;
+            at[i] = place;
+        }
+    }
+    if (tid < 2) {
+        const bool there = tid == 0 ? group > 0 : begin + size < a.count;
+        keys[tid == 0 ? 0 : size + 1] = there ? a.keys[tid == 0 ? begin - 1 : begin + size] : kNone;
+    }
     __syncthreads();
     if (slab * LANES + lane >= a.vectors) lane = a.vectors - 1 - slab * LANES;   // (a slab's last lanes do the last one's work again)
     const size_t c = column<kNarrow>(slab * LANES + lane, a.width);
@@ -367,7 +409,7 @@ template <class To, bool kNarrow> __global__ __launch_bounds__(kThreads) void jo
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             const unsigned g = group + 1 + j < a.groups ? group + 1 + j : a.groups - 1;
-            there[j] = group + 1 + j < a.groups && a.keys[g * size] == token;
+            there[j] = (group + 1 + j < a.groups) & (a.keys[g * size] == token);   // (no branch: all on their way together)
             v[j] = load_vector<kNarrow, false>(partial + size_t(g) * 2 * a.width, a.width);
         }
 #pragma unroll
