@@ -6,6 +6,7 @@
 // crosses a chunk's border is put together in LDS by the workgroup, whose chunks follow each other, and what crosses the workgroup's is left as partial
 // sums that a last kernel adds up in order.  No atomics on values: the result depends on tokens and sizes alone.
 // Few tokens are sorted by counting for each how many come in front of it, in one launch; many in stable passes over eight to ten bits.
+#include <algorithm>
 #include <type_traits>
 
 #include "lm_device.h"
@@ -27,26 +28,26 @@ __device__ __forceinline__ unsigned token_at(const Tokens& t, size_t i) {
     return v >= 0 && v < (long long)t.vocabulary ? unsigned(v) : t.vocabulary;
 }
 
-// Vector v of a row: eight columns from the returned one on, which the last two vectors of a width that is no multiple of eight have in part in
-// common; what is common is computed and written twice, alike.  So no lane has a branch of its own, behind which its loads would be waited for one
-// by one.  Rows of less than eight columns (kNarrow) are one vector.
-template <bool kNarrow> __device__ __forceinline__ size_t column(size_t v, size_t width) {
-    return kNarrow ? 0 : v * 8 + 8 <= width ? v * 8 : width - 8;
-}
-template <bool kNarrow, bool kPassing, class T> __device__ __forceinline__ float8 load_vector(const T* p, size_t width) {
-    typedef typename Vec8<T>::type __attribute__((aligned(sizeof(T)))) U;
-    if constexpr (kNarrow) return load8(p, int(width));
-    else if constexpr (kPassing) return __builtin_convertvector(__builtin_nontemporal_load(reinterpret_cast<const U*>(p)), float8);
-    else return load8(p);
-}
+// Rows are taken in vectors of N columns, sixteen bytes of what is read or written most, so that a wave's request is one piece; vector v is N columns from
+// the returned one on, which the last two of a width that is no multiple of N have in part in common: what is common is computed and written twice, alike.
+// So no lane has a branch of its own, behind which its loads would be waited for one by one.  Rows of less than a vector are taken column by column.
+template <class T> constexpr int kVector = 16 / int(sizeof(T));
+template <int N> using Floats = float __attribute__((ext_vector_type(N)));
+template <int N> __device__ __forceinline__ size_t column(size_t v, size_t width) { return v * N + N <= width ? v * N : width - N; }
 template <bool kPassing, class V, class T> __device__ __forceinline__ void store_any(T* p, V v) {
     typedef V __attribute__((aligned(sizeof(T)))) U;
     if constexpr (kPassing) __builtin_nontemporal_store(v, reinterpret_cast<U*>(p));
     else *reinterpret_cast<U*>(p) = v;
 }
-template <bool kNarrow, bool kPassing, class T> __device__ __forceinline__ void store_vector(T* p, float8 v, size_t width) {
-    if constexpr (kNarrow) store8(p, v, int(width));
-    else store_any<kPassing>(p, __builtin_convertvector(v, typename Vec8<T>::type));
+template <int N, bool kPassing, class T> __device__ __forceinline__ Floats<N> load_vector(const T* p) {
+    typedef T V __attribute__((ext_vector_type(N)));
+    typedef V __attribute__((aligned(sizeof(T)))) U;
+    if constexpr (kPassing) return __builtin_convertvector(__builtin_nontemporal_load(reinterpret_cast<const U*>(p)), Floats<N>);
+    else return __builtin_convertvector(*reinterpret_cast<const U*>(p), Floats<N>);
+}
+template <int N, bool kPassing, class T> __device__ __forceinline__ void store_vector(T* p, Floats<N> v) {
+    typedef T V __attribute__((ext_vector_type(N)));
+    store_any<kPassing>(p, __builtin_convertvector(v, V));
 }
 // Beyond what the L2s hold, looked-up rows and rows of zeros are written past them, and what the gradient sums is read past them (kPassing):
 // 65536 rows of 1024 fp16 are looked up in 39 us instead of 48, and their gradient's 50001 rows of 1024 fp32 take 65 instead of 80.
@@ -65,24 +66,25 @@ struct Lookup {
     float scale;
 };
 
-template <class From, class To, bool kNarrow, bool kPassing> __global__ __launch_bounds__(kThreads) void lookup_kernel(Lookup a) {
+// (fp32 results in vectors of eight, whose two stores each leave every other sixteen bytes, past the L2: 60000 rows of 500 in 44 us instead of 20.)
+template <class From, class To, int N, bool kPassing> __global__ __launch_bounds__(kThreads) void lookup_kernel(Lookup a) {
     unsigned token[kLookups];
     To* out[kLookups];
-    float8 v[kLookups];
+    Floats<N> v[kLookups];
     const unsigned item = blockIdx.x * (kThreads * kLookups) + threadIdx.x;
     const auto there = [&](int j) { return item + j * kThreads < a.items; };
 #pragma unroll
     for (int j = 0; j < kLookups; ++j) {
         const unsigned i = there(j) ? item + j * kThreads : 0, r = i / a.vectors;
-        const size_t row = a.first + r, c = column<kNarrow>(i - r * a.vectors, a.width);
+        const size_t row = a.first + r, c = column<N>(i - r * a.vectors, a.width);
         token[j] = token_at(a.t, row);
         out[j] = static_cast<To*>(a.out) + row * a.width + c;
-        v[j] = load_vector<kNarrow, false>(static_cast<const From*>(a.table) + (token[j] < a.t.vocabulary ? token[j] : 0) * a.ld + c, a.width);
+        v[j] = load_vector<N, false>(static_cast<const From*>(a.table) + (token[j] < a.t.vocabulary ? token[j] : 0) * a.ld + c);
     }
 #pragma unroll
     for (int j = 0; j < kLookups; ++j) {
-        const float8 zero = 0.f;
-        if (there(j)) store_vector<kNarrow, kPassing>(out[j], token[j] < a.t.vocabulary ? a.scale * v[j] : zero, a.width);
+        const Floats<N> zero = 0.f;
+        if (there(j)) store_vector<N, kPassing>(out[j], token[j] < a.t.vocabulary ? a.scale * v[j] : zero);
     }
 }
 
@@ -304,10 +306,10 @@ constexpr int kMaxChunk = 32;
 
 // A thread sums the entries of one chunk in one vector of columns; kThreads / LANES chunks behind one another and LANES vectors beside one
 // another are a workgroup's.
-template <class From, class To, int LANES, bool kNarrow, bool kPassing> __global__ __launch_bounds__(kThreads) void sum_kernel(Sums a) {
-    constexpr int kChunks = kThreads / LANES, kRows = sizeof(From) == 2 ? 8 : 4;   // rows on their way to a thread
+template <class From, class To, int N, int LANES, bool kPassing> __global__ __launch_bounds__(kThreads) void sum_kernel(Sums a) {
+    constexpr int kChunks = kThreads / LANES, kRows = 8;   // rows on their way to a thread
     __shared__ unsigned keys[kChunks * kMaxChunk + 2], at[kChunks * kMaxChunk];   // keys: with those in front of and behind the workgroup's
-    __shared__ float8 heads[kChunks][LANES], tails[kChunks][LANES];
+    __shared__ Floats<N> heads[kChunks][LANES], tails[kChunks][LANES];
     const unsigned group = blockIdx.x / a.slabs, slab = blockIdx.x - group * a.slabs;
     const int size = kChunks * a.chunk, tid = threadIdx.x, chunk = tid / LANES;
     int lane = tid % LANES;
@@ -330,22 +332,22 @@ template <class From, class To, int LANES, bool kNarrow, bool kPassing> __global
     }
     __syncthreads();
     if (slab * LANES + lane >= a.vectors) lane = a.vectors - 1 - slab * LANES;   // (a slab's last lanes do the last one's work again)
-    const size_t c = column<kNarrow>(slab * LANES + lane, a.width);
+    const size_t c = column<N>(slab * LANES + lane, a.width);
     const From* d = static_cast<const From*>(a.d_out) + c;
     To* out = static_cast<To*>(a.d_table) + c;
-    const auto put = [&](unsigned row, float8 v) { store_vector<kNarrow, false>(out + size_t(row) * a.width, a.scale * v, a.width); };
+    const auto put = [&](unsigned row, Floats<N> v) { store_vector<N, false>(out + size_t(row) * a.width, a.scale * v); };
     const unsigned* key = keys + 1;
     const int from = chunk * a.chunk, to = from + a.chunk;
     unsigned token = key[from];
-    float8 sum = 0.f;
+    Floats<N> sum = 0.f;
     bool began = key[from - 1] != token;   // the token's entries begin in this chunk
     for (int i = from; i < to; i += kRows) {
-        float8 row[kRows];
+        Floats<N> row[kRows];
         unsigned next[kRows];
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
             next[r] = key[i + r];
-            row[r] = load_vector<kNarrow, kPassing>(d + at[i + r] * a.ldd, a.width);
+            row[r] = load_vector<N, kPassing>(d + at[i + r] * a.ldd);
         }
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
@@ -376,12 +378,12 @@ template <class From, class To, int LANES, bool kNarrow, bool kPassing> __global
     for (int k = 0; k < kChunks; ++k) {
         const int first = k * a.chunk, last = first + a.chunk - 1;
         const unsigned front = key[first - 1], head = key[first], tail = key[last], behind = key[last + 1];
-        const float8 of_head = heads[k][lane], of_tail = tails[k][lane];
+        const Floats<N> of_head = heads[k][lane], of_tail = tails[k][lane];
         const bool enters = head < a.vocabulary && front == head, leaves = tail < a.vocabulary && behind == tail, whole = enters && head == tail;
         if (enters) sum += of_head;
         if (enters && !(whole && leaves)) {
             if (began) put(head, sum);
-            else store_vector<kNarrow, false>(partial, sum, a.width);
+            else store_vector<N, false>(partial, sum);
         }
         if (leaves && !whole) {
             sum = of_tail;
@@ -389,28 +391,28 @@ template <class From, class To, int LANES, bool kNarrow, bool kPassing> __global
         }
     }
     const unsigned tail = key[size - 1];
-    if (tail < a.vocabulary && key[size] == tail) store_vector<kNarrow, false>(partial + (began ? a.width : 0), sum, a.width);
+    if (tail < a.vocabulary && key[size] == tail) store_vector<N, false>(partial + (began ? a.width : 0), sum);
 }
 
 // What each token's entries left in more than one group: the group that they begin in adds them up.
-template <class To, bool kNarrow> __global__ __launch_bounds__(kThreads) void join_kernel(Sums a, unsigned size) {
+template <class To, int N> __global__ __launch_bounds__(kThreads) void join_kernel(Sums a, unsigned size) {
     const unsigned item = blockIdx.x * kThreads + threadIdx.x;
     unsigned group = item / a.vectors;
     if (group + 1 >= a.groups) return;
-    const size_t c = column<kNarrow>(item - group * a.vectors, a.width);
+    const size_t c = column<N>(item - group * a.vectors, a.width);
     const unsigned begin = group * size, last = begin + size - 1, token = a.keys[last];
     if (token >= a.vocabulary || a.keys[last + 1] != token || (begin > 0 && a.keys[begin - 1] == token)) return;
     const float* partial = a.partials + c;
-    float8 sum = load_vector<kNarrow, false>(partial + (size_t(group) * 2 + 1) * a.width, a.width);
+    Floats<N> sum = load_vector<N, false>(partial + (size_t(group) * 2 + 1) * a.width);
     constexpr int kAhead = 8;
     for (bool more = true; more;) {
-        float8 v[kAhead];
+        Floats<N> v[kAhead];
         bool there[kAhead];
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             const unsigned g = group + 1 + j < a.groups ? group + 1 + j : a.groups - 1;
             there[j] = (group + 1 + j < a.groups) & (a.keys[g * size] == token);   // (no branch: all on their way together)
-            v[j] = load_vector<kNarrow, false>(partial + size_t(g) * 2 * a.width, a.width);
+            v[j] = load_vector<N, false>(partial + size_t(g) * 2 * a.width);
         }
 #pragma unroll
         for (int j = 0; j < kAhead; ++j)
@@ -418,7 +420,7 @@ template <class To, bool kNarrow> __global__ __launch_bounds__(kThreads) void jo
         more = there[kAhead - 1];
         group += kAhead;
     }
-    store_vector<kNarrow, false>(static_cast<To*>(a.d_table) + size_t(token) * a.width + c, a.scale * sum, a.width);
+    store_vector<N, false>(static_cast<To*>(a.d_table) + size_t(token) * a.width + c, a.scale * sum);
 }
 
 // ---- host side
@@ -450,13 +452,14 @@ bool ranked(const flstm_embedding* p) { return p->tokens <= kMostRanked; }
 
 // Lanes beside one another for a row's vectors, and entries a thread sums: as many as leave enough workgroups.
 struct SumPlan {
-    int lanes, chunk;
+    int vector, lanes, chunk;   // columns; lanes; entries
     unsigned groups, slabs;
     size_t size() const { return size_t(kThreads / lanes) * chunk; }
 };
-SumPlan sum_plan(const flstm_embedding* p) {
-    const size_t vectors = ceil_div(p->width, 8);
+SumPlan sum_plan(const flstm_embedding* p, size_t element) {
     SumPlan s;
+    s.vector = p->width * element < 16 ? 1 : int(16 / element);
+    const size_t vectors = ceil_div(p->width, size_t(s.vector));
     s.lanes = vectors <= 4 ? 4 : vectors <= 8 ? 8 : 16;
     s.slabs = unsigned(ceil_div(vectors, s.lanes));
     for (s.chunk = kMaxChunk; s.chunk > 8 && ceil_div(p->tokens, s.size()) * s.slabs < 512;) s.chunk /= 2;
@@ -470,7 +473,7 @@ struct Room {   // of the workspace, in bytes
 Room room_of(const flstm_embedding* p) {
     const SortPlan s = sort_plan(p);
     return Room{round_up(p->tokens * 4, 16), size_t(ranked(p) ? 2 : 4), ranked(p) ? 0 : round_up((size_t(s.tiles) << s.bits) * 4, 16),
-                round_up(size_t(sum_plan(p).groups) * 2 * p->width * 4, 16)};
+                round_up(std::max(size_t(sum_plan(p, 2).groups), size_t(sum_plan(p, 4).groups)) * 2 * p->width * 4, 16)};   // (of any type)
 }
 
 }  // namespace
@@ -483,18 +486,21 @@ extern "C" int flstm_embedding_forward(const flstm_embedding* p, const void* tab
     if (!valid(p) || !valid_dtype(table_dtype) || !valid_dtype(dtype) || (ld < p->width && p->vocabulary > 1)) return FLSTM_E_INVALID;
     if (p->tokens == 0 || p->width == 0) return 0;
     if (!table || !out) return FLSTM_E_INVALID;
-    Lookup a{tokens_of(p), unsigned(ceil_div(p->width, 8)), 0, 0, p->width, ld, table, out, p->scale};
+    Lookup a{tokens_of(p), 0, 0, 0, p->width, ld, table, out, p->scale};
     return with_type(table_dtype, [&](auto from) {
         return with_type(dtype, [&](auto to) {
+            constexpr int N = kVector<decltype(to)>;
+            const size_t n = p->width < N ? 1 : N;
+            a.vectors = unsigned(ceil_div(p->width, n));
             const size_t most = (size_t(1) << 31) / a.vectors;   // rows a launch
             const bool passing = p->tokens * p->width * sizeof(to) > kMostKept;
             for (a.first = 0; a.first < p->tokens; a.first += most) {
                 a.items = unsigned((p->tokens - a.first < most ? p->tokens - a.first : most) * a.vectors);
                 const unsigned grid = unsigned(ceil_div(a.items, kThreads * kLookups));
                 hipStream_t s = static_cast<hipStream_t>(stream);
-                if (p->width < 8) lookup_kernel<decltype(from), decltype(to), true, false><<<grid, kThreads, 0, s>>>(a);
-                else if (passing) lookup_kernel<decltype(from), decltype(to), false, true><<<grid, kThreads, 0, s>>>(a);
-                else lookup_kernel<decltype(from), decltype(to), false, false><<<grid, kThreads, 0, s>>>(a);
+                if (n == 1) lookup_kernel<decltype(from), decltype(to), 1, false><<<grid, kThreads, 0, s>>>(a);
+                else if (passing) lookup_kernel<decltype(from), decltype(to), N, true><<<grid, kThreads, 0, s>>>(a);
+                else lookup_kernel<decltype(from), decltype(to), N, false><<<grid, kThreads, 0, s>>>(a);
                 if (const int rc = launched()) return rc;
             }
             return 0;
@@ -510,9 +516,9 @@ extern "C" int flstm_embedding_backward(const flstm_embedding* p, const void* d_
     if (p->width == 0) return 0;
     if (!d_table || (p->tokens > 0 && (!d_out || !workspace))) return FLSTM_E_INVALID;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const SumPlan plan = sum_plan(p);
+    const SumPlan plan = sum_plan(p, dtype == FLSTM_OP_F32 ? 4 : 2);
     Sums a{};
-    a.count = unsigned(p->tokens); a.vocabulary = unsigned(p->vocabulary); a.vectors = unsigned(ceil_div(p->width, 8));
+    a.count = unsigned(p->tokens); a.vocabulary = unsigned(p->vocabulary); a.vectors = unsigned(ceil_div(p->width, size_t(plan.vector)));
     a.groups = plan.groups; a.slabs = plan.slabs; a.chunk = plan.chunk;
     a.width = p->width; a.ldd = ldd; a.d_out = d_out; a.d_table = d_table; a.scale = p->scale;
     const size_t sums = size_t(a.groups) * a.slabs, joins = ceil_div(size_t(a.groups) * a.vectors, kThreads);
@@ -564,21 +570,21 @@ extern "C" int flstm_embedding_backward(const flstm_embedding* p, const void* d_
             typedef decltype(from) From;
             typedef decltype(to) To;
             const unsigned grid = unsigned(sums);
-            const auto sum = [&](auto lanes) {
-                constexpr int kLanes = decltype(lanes)::value;
-                if (p->tokens * p->width * sizeof(From) > kMostKept) sum_kernel<From, To, kLanes, false, true><<<grid, kThreads, 0, s>>>(a);
-                else sum_kernel<From, To, kLanes, false, false><<<grid, kThreads, 0, s>>>(a);
+            const bool passing = p->tokens * p->width * sizeof(From) > kMostKept;
+            const auto sum = [&](auto lanes, auto vector) {
+                constexpr int kLanes = decltype(lanes)::value, N = decltype(vector)::value;
+                if (N > 1 && passing) sum_kernel<From, To, N, kLanes, true><<<grid, kThreads, 0, s>>>(a);
+                else sum_kernel<From, To, N, kLanes, false><<<grid, kThreads, 0, s>>>(a);
+                if (const int rc = launched()) return rc;
+                if (a.groups > 1) join_kernel<To, N><<<unsigned(joins), kThreads, 0, s>>>(a, unsigned(plan.size()));
+                return launched();
             };
-            if (plan.lanes == 16) sum(std::integral_constant<int, 16>());
-            else if (plan.lanes == 8) sum(std::integral_constant<int, 8>());
-            else if (p->width >= 8) sum(std::integral_constant<int, 4>());
-            else sum_kernel<From, To, 4, true, false><<<grid, kThreads, 0, s>>>(a);
-            if (const int rc = launched()) return rc;
-            if (a.groups > 1) {
-                if (p->width >= 8) join_kernel<To, false><<<unsigned(joins), kThreads, 0, s>>>(a, unsigned(plan.size()));
-                else join_kernel<To, true><<<unsigned(joins), kThreads, 0, s>>>(a, unsigned(plan.size()));
-            }
-            return launched();
+            constexpr std::integral_constant<int, kVector<From>> whole;
+            constexpr std::integral_constant<int, 1> single;
+            if (plan.vector == 1) return plan.lanes == 4 ? sum(std::integral_constant<int, 4>(), single) : sum(std::integral_constant<int, 8>(), single);
+            if (plan.lanes == 16) return sum(std::integral_constant<int, 16>(), whole);
+            if (plan.lanes == 8) return sum(std::integral_constant<int, 8>(), whole);
+            return sum(std::integral_constant<int, 4>(), whole);
         });
     });
 }
