@@ -445,6 +445,22 @@ template <int B> __global__ __launch_bounds__(kThreads) void reorder_kernel(Reor
 
 // ---- host side
 
+// `count` rows of `bytes` at every `stride` from `at` on; whether two such have memory in common, where one launch would move it twice.  Rows of one
+// stride may lie between each other's (halves of a wider state); of unlike strides that is not looked into.
+struct Extent {
+    size_t at, stride, bytes, count;
+};
+bool meet(Extent x, Extent y) {
+    if (y.at < x.at) {
+        const Extent z = x;
+        x = y;
+        y = z;
+    }
+    const size_t apart = y.at - x.at;
+    if (apart / x.stride >= x.count || (apart / x.stride == x.count - 1 && apart % x.stride >= x.bytes)) return false;
+    return x.stride != y.stride || apart % x.stride < x.bytes || x.stride - apart % x.stride < y.bytes;
+}
+
 constexpr size_t kMostBlocks = 0xffffffffu / kThreads;
 
 bool valid(const flstm_beams* p) {
@@ -499,26 +515,37 @@ extern "C" int flstm_beam_select(const flstm_beams* p, float* scores, long long*
 }
 
 extern "C" int flstm_beam_reorder(size_t sequences, int beams, const long long* parents, const flstm_beam_state* states, int count, void* stream) {
-    if (beams < 1 || beams > kMaxBeams || count < 0 || count > kMaxStates || (count > 0 && !states)) return FLSTM_E_INVALID;
+    if (beams < 1 || beams > kMaxBeams || count < 0 || (count > 0 && !states)) return FLSTM_E_INVALID;
     if (sequences == 0 || count == 0 || beams == 1) return 0;
     if (!parents) return FLSTM_E_INVALID;
-    Reorder a{};
-    a.parents = parents; a.beams = beams;
-    size_t blocks = 0;
+    if (sequences > ~size_t(0) / kMaxBeams) return FLSTM_E_TOO_LARGE;
+    const Extent index{reinterpret_cast<size_t>(parents), sizeof(*parents), sizeof(*parents), sequences * beams};
+    const auto extent = [&](int i) { return Extent{reinterpret_cast<size_t>(states[i].data), states[i].stride, states[i].bytes, sequences * beams}; };
+    const auto slabs = [&](int i) { return ceil_div(states[i].bytes, kThreads * 16); };
     for (int i = 0; i < count; ++i) {
         if (states[i].bytes == 0) continue;
         if (!states[i].data || states[i].stride < states[i].bytes) return FLSTM_E_INVALID;
-        const size_t slabs = ceil_div(states[i].bytes, kThreads * 16);
-        if (slabs > kMostBlocks || sequences > kMostBlocks / slabs) return FLSTM_E_TOO_LARGE;
-        blocks += slabs * sequences;
-        if (blocks > kMostBlocks) return FLSTM_E_TOO_LARGE;
-        a.states[a.count++] = State{static_cast<char*>(states[i].data), states[i].stride, states[i].bytes, unsigned(slabs), unsigned(blocks - slabs * sequences)};
+        if (slabs(i) > kMostBlocks / sequences) return FLSTM_E_TOO_LARGE;
+        if (meet(index, extent(i))) return FLSTM_E_INVALID;
+        for (int j = 0; j < i; ++j)
+            if (states[j].bytes && meet(extent(j), extent(i))) return FLSTM_E_INVALID;
     }
-    if (blocks == 0) return 0;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (beams <= 4) reorder_kernel<4><<<unsigned(blocks), kThreads, 0, s>>>(a);
-    else if (beams <= 8) reorder_kernel<8><<<unsigned(blocks), kThreads, 0, s>>>(a);
-    else if (beams <= 16) reorder_kernel<16><<<unsigned(blocks), kThreads, 0, s>>>(a);
-    else reorder_kernel<32><<<unsigned(blocks), kThreads, 0, s>>>(a);
-    return launched();
+    for (int i = 0; i < count;) {
+        Reorder a{};
+        a.parents = parents; a.beams = beams;
+        size_t blocks = 0;
+        for (; i < count && a.count < kMaxStates && blocks + slabs(i) * sequences <= kMostBlocks; ++i) {
+            if (states[i].bytes == 0) continue;
+            a.states[a.count++] = State{static_cast<char*>(states[i].data), states[i].stride, states[i].bytes, unsigned(slabs(i)), unsigned(blocks)};
+            blocks += slabs(i) * sequences;
+        }
+        if (blocks == 0) break;
+        if (beams <= 4) reorder_kernel<4><<<unsigned(blocks), kThreads, 0, s>>>(a);
+        else if (beams <= 8) reorder_kernel<8><<<unsigned(blocks), kThreads, 0, s>>>(a);
+        else if (beams <= 16) reorder_kernel<16><<<unsigned(blocks), kThreads, 0, s>>>(a);
+        else reorder_kernel<32><<<unsigned(blocks), kThreads, 0, s>>>(a);
+        if (const int rc = launched()) return rc;
+    }
+    return 0;
 }

@@ -802,7 +802,7 @@ def gated_recurrence(x, forget, gate=None, *, state=None, cu_seqlens=None) -> Tu
 
 _BEAMS = struct.Struct("@NiiNPNiPPq")   # flstm_beams
 _BEAM_STATE = struct.Struct("@PNN")
-_MAX_BEAMS, _MAX_STATES = 32, 16
+_MAX_BEAMS = 32
 
 
 def beam_select(logits, scores, *, beams: Optional[int] = None, end: Optional[int] = None, finished=None) -> Tuple:
@@ -859,7 +859,7 @@ def beam_reorder(parents, *states) -> None:
     """Hypothesis b of sequence s becomes, in every one of `states`, what hypothesis parents[s, b] was, in place; rows that stay are not touched.
 
     parents (sequences, hypotheses) int64, as beam_select returns them; up to 32 hypotheses; one outside them leaves its row as it is.  states: tensors
-    of any type, (sequences * hypotheses, ..) or (sequences, hypotheses, ..), with contiguous rows.  No autograd."""
+    of any type, (sequences * hypotheses, ..) or (sequences, hypotheses, ..), with contiguous rows, that share no memory.  No autograd."""
     if not torch.is_tensor(parents) or not parents.is_cuda or parents.get_device() != torch._C._cuda_getDevice() or parents.dtype != torch.int64:
         raise ValueError("parents must be an int64 CUDA tensor on the current device")
     if parents.dim() != 2 or not 1 <= parents.shape[1] <= _MAX_BEAMS:
@@ -886,9 +886,10 @@ def beam_reorder(parents, *states) -> None:
             raise ValueError(f"state {i} needs a gradient: it would be changed in place")
         element = t.element_size()
         packed.append(_BEAM_STATE.pack(t.data_ptr(), max(stride, size) * element, size * element))
-    parents, lib = parents.contiguous(), _bind()
-    for at in range(0, len(packed), _MAX_STATES):
-        some = packed[at:at + _MAX_STATES]
-        _check(lib.flstm_beam_reorder(sequences, hypotheses, parents.data_ptr(), b"".join(some), len(some), _stream()), "flstm_beam_reorder")
+    parents = parents.contiguous()
+    rc = _bind().flstm_beam_reorder(sequences, hypotheses, parents.data_ptr(), b"".join(packed), len(packed), _stream())
+    if rc == 1:
+        raise ValueError("states must not share memory, with each other or with parents: it would be moved twice")
+    _check(rc, "flstm_beam_reorder")
     for t in states:
         _written(t)

@@ -225,8 +225,9 @@ size_t flstm_beam_select_workspace_bytes(const flstm_beams* problem);
 int flstm_beam_select(const flstm_beams* problem, float* scores, long long* parents, long long* tokens, unsigned char* finished,
                       void* workspace, void* stream);
 
-/* Row (s, b) of each of `count` (at most 16) tensors becomes what row (s, parents[s][b]) was, in place.  Rows of `bytes` bytes begin
- * (s * beams + b) * stride bytes behind data; 1 <= beams <= 32.  A parent outside 0 .. beams - 1 leaves its row as it is. */
+/* Row (s, b) of each of `count` tensors becomes what row (s, parents[s][b]) was, in place, sixteen tensors a launch.  Rows of `bytes` bytes begin
+ * (s * beams + b) * stride bytes behind data; 1 <= beams <= 32.  A parent outside 0 .. beams - 1 leaves its row as it is.  FLSTM_E_INVALID
+ * where tensors share memory with each other or with the parents; rows of one stride may lie between each other's. */
 typedef struct {
     void* data;
     size_t stride, bytes;

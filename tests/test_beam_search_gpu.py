@@ -256,6 +256,22 @@ def test_reorder_leaves_the_rest():
     assert torch.equal(lots, want)
 
 
+def test_reorder_of_shared_memory():
+    """What a call would move twice is refused before any of it moves; rows between each other's are each other's neighbours only."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    parents = torch.randint(0, 4, (6, 4), device="cuda", generator=g)
+    room = torch.randn(24, 100, device="cuda", generator=g)
+    before, others = room.clone(), [torch.randn(24, 3, device="cuda", generator=g) for _ in range(20)]
+    kept = [t.clone() for t in others]
+    for bad in ([room, room], [room[:, :50], room[:, 49:]], [others[0], *others], [room, room.flatten()[300:324]],
+                [room.view(48, 50)[:24], room.view(48, 50)[23:47]], [*others, parents]):
+        with pytest.raises(ValueError, match="share"):
+            fl.beam_reorder(parents, *bad)
+    assert torch.equal(room, before) and all(torch.equal(a, b) for a, b in zip(others, kept))
+    fl.beam_reorder(parents, room[:, :50], room[:, 50:99])
+    assert torch.equal(room[:, :99], _reordered(before, parents)[:, :99]) and torch.equal(room[:, 99], before[:, 99])
+
+
 def test_refusals():
     p = _problem(2, 3, 50)
     for bad, match in ((dict(logits=p["logits"].cpu()), "CUDA"), (dict(logits=p["logits"].double()), "dtype"), (dict(logits=p["logits"][0]), "logits"),

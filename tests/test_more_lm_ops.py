@@ -73,10 +73,16 @@ def test_beam_search_refuses_before_device_work():
     state = lambda data=4096, stride=16, size=16: lm_ops._BEAM_STATE.pack(data, stride, size)
     reorder = lambda n=2, beams=3, parents=SOME, states=state(), count=1: lib.flstm_beam_reorder(n, beams, parents, states, count, None)
     assert reorder(beams=0) == 1 and reorder(beams=33) == 1 and reorder(parents=None) == 1 and reorder(states=None) == 1
-    assert reorder(count=17) == 1 and reorder(count=-1) == 1 and reorder(states=state(0)) == 1 and reorder(states=state(stride=15)) == 1
+    assert reorder(count=-1) == 1 and reorder(states=state(0)) == 1 and reorder(states=state(stride=15)) == 1
     assert reorder(n=0, parents=None) == 0 and reorder(count=0, parents=None) == 0 and reorder(beams=1, parents=None) == 0
     assert reorder(states=state(0, 0, 0)) == 0
     assert reorder(n=1 << 20, states=state(stride=1 << 40, size=1 << 40)) == 2004
+    # six rows: the same ones twice, begun inside of one, at the last one's last byte, inside unlike strides; parents inside and at the end
+    two = lambda a, b, count=2: reorder(parents=1 << 30, states=a + b, count=count)
+    assert two(state(), state()) == 1 and two(state(), state(4096 + 33)) == 1 and two(state(), state(4096 - 95)) == 1 and two(state(), state(4096 + 95)) == 1
+    assert two(state(stride=32), state(4096 + 16, 48)) == 1 and two(state(stride=32), state(4096 + 15, 32)) == 1 and two(state(stride=32), state(4096 + 17, 32)) == 1
+    assert two(b"".join(state(4096 + i * 96) for i in range(20)), state(4096 + 96 + 95), 21) == 1
+    assert reorder(parents=4096 + 88) == 1 and reorder(parents=4096 - 40) == 1
 
 
 def test_host_tensors_are_refused():
