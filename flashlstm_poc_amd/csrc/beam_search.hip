@@ -17,6 +17,7 @@ constexpr int kMaxKeep = 32, kMaxBeams = 32;
 constexpr int kVectors = 4, kTile = kThreads * kVectors * 8;   // logits a workgroup holds at a time
 constexpr size_t kMaxParts = 64;   // one for each lane of a wave
 constexpr int kList = 1024;        // entries that are ordered at once
+static_assert(kTile <= kList * 8);
 constexpr float kLog2e = 1.4426950408889634f, kLowest = -3.4028234663852886e38f, kHighest = 3.4028234663852886e38f;
 
 struct Select {
@@ -108,9 +109,9 @@ template <class T> __device__ int fewer(const T* z, unsigned base, unsigned end,
 
 template <class T> __global__ __launch_bounds__(kThreads) void part_kernel(Select a) {
     __shared__ u64 list[kList + kMaxKeep], best[kMaxKeep], largest[kThreads / kWave];
-    __shared__ unsigned places[kList];
+    __shared__ unsigned places[kList];   // no fewer than a tile's vectors
     __shared__ float heads[kThreads / kWave][kMaxKeep], waves[kThreads / kWave];
-    __shared__ int count;
+    __shared__ int count, vectors;   // entries and vectors that reach the bound
     const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
     const unsigned in_launch = blockIdx.x / unsigned(a.parts), part = blockIdx.x - in_launch * unsigned(a.parts), begin = part * a.part;
     const size_t row = a.first + in_launch, block = row * unsigned(a.parts) + part;
@@ -154,7 +155,7 @@ template <class T> __global__ __launch_bounds__(kThreads) void part_kernel(Selec
         }
         m = groups_fold(fminf(m, kHighest), a.groups, [](float x, float y) { return fmaxf(x, y); });
         if (lane < a.groups) heads[wave][lane] = m;
-        if (tid == 0) count = 0;
+        if (tid == 0) count = vectors = 0;
         __syncthreads();
         m = heads[0][lane % a.groups];
 #pragma unroll
@@ -169,28 +170,23 @@ template <class T> __global__ __launch_bounds__(kThreads) void part_kernel(Selec
         const float shift = most * kLog2e;
         const float reached = __builtin_fmaf(bound, kLog2e, -shift);   // (rounding keeps the order)
         float more = 0.f;
-        unsigned reach = 0;   // a bit for each of this thread's entries: which reach the bound
+        unsigned reach = 0;   // a bit for each of this thread's vectors: whether an entry reaches the bound
 #pragma unroll
         for (int j = 0; j < kVectors; ++j) {
             asm volatile("" : "+v"(v[j]));
-            float d[8], largest_d = -__builtin_inff();
+            float largest_d = -__builtin_inff();
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                d[i] = __builtin_fmaf(float(v[j][i]), kLog2e, -shift);
-                more += __builtin_amdgcn_exp2f(d[i]);
-                largest_d = fmaxf(largest_d, d[i]);
+                const float d = __builtin_fmaf(float(v[j][i]), kLog2e, -shift);
+                more += __builtin_amdgcn_exp2f(d);
+                largest_d = fmaxf(largest_d, d);
             }
-            if (!(largest_d < reached)) {   // (a thread's eight hardly ever hold one that does, a wave's mostly)
-                unsigned bits = 0;
-#pragma unroll
-                for (int i = 7; i >= 0; --i) bits = bits + bits + unsigned(!(d[i] < reached));
-                reach |= bits << j * 8;
-            }
+            reach |= largest_d < reached ? 0u : 1u << j;
         }
         while (reach) {
-            const int e = __ffs(int(reach)) - 1, at = atomicAdd(&count, 1);
+            const int j = __ffs(int(reach)) - 1;
             reach &= reach - 1;
-            if (at < kList) places[at] = place_of(e / 8) + e % 8;
+            places[atomicAdd(&vectors, 1)] = base + (j * kThreads + tid) * 8;
         }
         if (more < __builtin_inff() && fabsf(shift) < __builtin_inff()) {
             more *= __builtin_amdgcn_exp2f(-__builtin_fmaf(most, kLog2e, -shift));
@@ -208,10 +204,23 @@ template <class T> __global__ __launch_bounds__(kThreads) void part_kernel(Selec
         }
         const u64 before = base > begin && tid < a.keep ? best[tid] : 0;   // of the tiles in front
         __syncthreads();
+        // which of the vectors' entries do: looked up again, a lane each, for fewer instructions than keeping account of all
+        for (int i = tid; i < vectors * 8; i += kThreads) {
+            const unsigned c = places[i / 8] + i % 8;
+            if (c >= end) continue;
+            const float x = number(float(z[c]));
+            if (!(x >= bound)) continue;
+            const int at = atomicAdd(&count, 1);
+            if (at < kList) list[at] = key_of(x, c);
+        }
+        __syncthreads();
         int some = count;
-        if (some > kList) some = fewer(z, base, end, bound, a.groups, places, heads, count);
+        if (some > kList) {
+            some = fewer(z, base, end, bound, a.groups, places, heads, count);
+            if (some <= kList)
+                for (int i = tid; i < some; i += kThreads) list[i] = key_of(number(float(z[places[i]])), places[i]);
+        }
         if (some <= kList) {
-            for (int i = tid; i < some; i += kThreads) list[i] = key_of(number(float(z[places[i]])), places[i]);
             if (base > begin) {
                 if (tid < a.keep) list[some + tid] = before;
                 some += a.keep;
