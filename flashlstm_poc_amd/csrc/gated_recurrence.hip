@@ -9,6 +9,8 @@
 // rounding of 1 - small would be the same at every token of a channel that mostly keeps its state, and add up over its memory.
 // The backward pass needs the states in front of all tokens.  They are walked again from the states that the forward pass leaves
 // every kBatch tokens, in 32 bits: y, rounded to 16 bits, would not give forget's gradient, which is a difference of states.
+// With a gate: 256 sequences of 1024 tokens and channels, fp16, walked whole, 420 us forward (5.3 TB/s) and 732 backward (5.2); one of 131072 tokens,
+// bf16, in segments, 237 forward (4.8 TB/s, where the vector units' five functions a token and channel are as much of a bound).
 #include <type_traits>
 
 #include "lm_device.h"
@@ -244,7 +246,8 @@ template <class T, int C> __device__ __forceinline__ void clear_rows(const Recur
 }
 
 // ---- whole sequences: a lane walks from the first token to the last.  A workgroup has neighbouring channels of one sequence, up to kWalkLanes lanes, so
-// that rows are read as wholes (64 lanes a workgroup: 487 us instead of 473; lanes of four channels, half as many waves: 513).
+// that rows are read as wholes.  (Measured with rows' addresses in scalar registers, forward: 473 us, workgroups of 64 lanes 487, lanes of four channels, half
+// as many waves, 513.)
 
 constexpr unsigned kWalkLanes = 256;
 
