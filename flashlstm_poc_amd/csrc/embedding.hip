@@ -6,8 +6,8 @@
 // crosses a chunk's border is put together in LDS by the workgroup, whose chunks follow each other, and what crosses the workgroup's is left as partial
 // sums that a last kernel adds up in order.  No atomics on values: the result depends on tokens and sizes alone.
 // Few tokens are sorted by counting for each how many come in front of it, in one launch; many in stable passes over eight to ten bits.
-// 65536 tokens of a text, 1024 fp16 channels, 50001 fp32 rows: lookup 39 us, 6.9 TB/s with what the caches hold of the table; sort 46, which writes
-// 205 MB of zeros meanwhile; sums 44, 4.6 TB/s; partial sums 5 to 8.
+// 65536 tokens of a text, 1024 fp16 channels, 50001 fp32 rows: lookup 38 us, 7.1 TB/s with what the caches hold of the table; sort 40, which writes
+// 205 MB of zeros meanwhile, 5.1 TB/s; sums 44, 4.6 TB/s; partial sums 5.
 #include <algorithm>
 #include <type_traits>
 
