@@ -6,7 +6,8 @@
 // makes of a state, a factor and a sum, is published, those in front of it are read, and the segment goes on from the state that they
 // give.  Every tensor is so read and written once, and the order of all sums depends on sizes alone.
 // Of f and 1 - f the smaller one is computed and the other's part left whole, c = x + f (c - x) or c = c + (1 - f)(x - c): a
-// rounding of 1 - small would be the same at every token of a channel that mostly keeps its state, and add up over its memory.
+// rounding of 1 - small would be the same at every token of a channel that mostly keeps its state, and add up over its memory.  Nor is it a product of factors
+// near one that segments publish, for the same reason, but what that lacks to one.
 // The backward pass needs the states in front of all tokens.  They are walked again from the states that the forward pass leaves
 // every kBatch tokens, in 32 bits: y, rounded to 16 bits, would not give forget's gradient, which is a difference of states.
 // With a gate: 256 sequences of 1024 tokens and channels, fp16, walked whole, 420 us forward (5.3 TB/s) and 732 backward (5.2); one of 131072 tokens,
@@ -98,10 +99,26 @@ struct Factor {
 template <class T> __device__ __forceinline__ Factor factor_of(float forget) { return Factor{small_sigmoid<T>(forget), forget > 0.f}; }
 __device__ __forceinline__ float keep(Factor f) { return f.keeps ? 1.f - f.small : f.small; }     // f
 __device__ __forceinline__ float kept(Factor f, float v) { return f.keeps ? __builtin_fmaf(-f.small, v, v) : f.small * v; }   // f v
+__device__ __forceinline__ float lost(Factor f, float v) { return f.keeps ? f.small * v : __builtin_fmaf(-f.small, v, v); }   // (1 - f) v
 __device__ __forceinline__ float stepped(Factor f, float c, float x) {
     const float base = f.keeps ? c : x, other = f.keeps ? x : c;
     return __builtin_fmaf(f.small, other - base, base);
 }
+__device__ __forceinline__ float small(Factor f) { return f.small; }
+// The same as one word, the smaller one as -f or 1 - f, and in an operation or two less, with the same results.  (Where a factor is computed again from its gate
+// the form above takes fewer registers: this one spills in the forward pass of 16-bit tensors.)
+struct Held {
+    float way;
+    __device__ __forceinline__ bool keeps() const { return __builtin_bit_cast(int, way) >= 0; }
+};
+__device__ __forceinline__ Factor factor(Factor f) { return f; }
+__device__ __forceinline__ Factor factor(Held f) { return Factor{fabsf(f.way), f.keeps()}; }
+__device__ __forceinline__ Held held(Held f) { return f; }
+__device__ __forceinline__ Held held(Factor f) { return Held{__builtin_copysignf(f.small, f.keeps ? 1.f : -1.f)}; }
+__device__ __forceinline__ float kept(Held f, float v) { return __builtin_fmaf(-f.way, v, f.keeps() ? v : 0.f); }
+__device__ __forceinline__ float lost(Held f, float v) { return __builtin_fmaf(f.way, v, f.keeps() ? 0.f : v); }
+__device__ __forceinline__ float stepped(Held f, float c, float x) { return __builtin_fmaf(f.way, x - c, f.keeps() ? c : x); }
+__device__ __forceinline__ float small(Held f) { return fabsf(f.way); }
 template <class T> __device__ __forceinline__ float sigmoid(float u) {
     if constexpr (sizeof(T) == 2) return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(u * -1.4426950408889634f));
     const float s = small_sigmoid<T>(u);
@@ -216,7 +233,7 @@ __device__ __forceinline__ void gradients(const Recurrence& a, const Gradients& 
     float of_x[C], of_forget[C], of_gate[C];
 #pragma unroll
     for (int j = 0; j < C; ++j) {
-        const Factor k = factor(u[j]);
+        const auto k = factor(u[j]);
         float dc = d[j];
         if constexpr (kGate) {
             const Factor o = factor_of<T>(g[j]);
@@ -224,8 +241,8 @@ __device__ __forceinline__ void gradients(const Recurrence& a, const Gradients& 
             dc *= keep(o);
         }
         const float total = dc + s[j];
-        of_x[j] = k.keeps ? k.small * total : __builtin_fmaf(-k.small, total, total);
-        of_forget[j] = total * (before[j] - x[j]) * (k.small * (1.f - k.small));
+        of_x[j] = lost(k, total);
+        of_forget[j] = total * (before[j] - x[j]) * (small(k) * (1.f - small(k)));
         s[j] = kept(k, total);
     }
     constexpr ptrdiff_t kSize = sizeof(T);
@@ -341,22 +358,43 @@ constexpr unsigned kMostPolls = 1u << 20;
 struct Made {
     float factor, sum;   // state -> factor * state + sum
 };
-__device__ __forceinline__ Made then(const Made& first, const Made& next) { return Made{next.factor * first.factor, __builtin_fmaf(next.factor, first.sum, next.sum)}; }
 __device__ __forceinline__ float of(const Made& m, float state) { return __builtin_fmaf(m.factor, state, m.sum); }
+// The same as it is handed on: 1 - factor, or of a factor up to 1/2 its negative.  A product of factors near one, each rounded to a multiple of 2^-24, is off by as
+// many of these as it has factors, all in one direction where the tokens' gates are alike; so what it lacks to one is added up beside it, from the tokens on.  (The
+// states of 41000 tokens of fp32 with forget gates of 8 to 12 are off by at most 12 times 2^-24; with products alone by 28 to 4600.)
+struct Packed {
+    float way, sum;
+};
+__device__ __forceinline__ Made unpacked(const Packed& p) { return Made{(Held{p.way}.keeps() ? 1.f : 0.f) - p.way, p.sum}; }
+// What tokens, or pieces of them, make of a state, one behind the other.
+struct Walk {
+    float factor = 1.f, sum = 0.f, less = 0.f;   // less: 1 - factor, as long as that is less than 1/2
+    template <class F> __device__ __forceinline__ void leaves(F f) {
+        less = __builtin_fmaf(small(f), factor, less);   // (where 1 - f is not the smaller one, factor is 1/2 at most from here on)
+        factor = kept(f, factor);
+    }
+    __device__ __forceinline__ void behind(const Packed& p) {
+        const Made next = unpacked(p);
+        less = __builtin_fmaf(fabsf(p.way), factor, less);
+        factor *= next.factor;
+        sum = of(next, sum);
+    }
+    __device__ __forceinline__ Packed packed() const { return Packed{factor > 0.5f ? less : -factor, sum}; }
+};
 // A row of published pairs: the same for all lanes, a lane's word `at` bytes behind it.
 __device__ __forceinline__ u64* word_of(const u64* row, unsigned at) {
     return reinterpret_cast<u64*>(const_cast<char*>(address<true>(reinterpret_cast<const char*>(row), at)));
 }
-__device__ __forceinline__ void publish(u64* row, unsigned at, Made m) {
-    if (m.factor != m.factor) m.factor = __builtin_nanf("");   // (not kNothing's)
-    __hip_atomic_store(word_of(row, at), __builtin_bit_cast(u64, m), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+__device__ __forceinline__ void publish(u64* row, unsigned at, Packed p) {
+    if (p.way != p.way) p.way = __builtin_nanf("");   // (not kNothing's)
+    __hip_atomic_store(word_of(row, at), __builtin_bit_cast(u64, p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 __device__ __forceinline__ u64 look(const u64* row, unsigned at) { return __hip_atomic_load(word_of(row, at), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
 // What the pairs of `count` rows from `row` on, `step` words apart, make of a state, one after the other.
-__device__ __forceinline__ Made read_made(const u64* row, ptrdiff_t step, long long count, unsigned at, unsigned* in_vain) {
-    Made m{1.f, 0.f};
-    constexpr int kAhead = 8;
+__device__ __forceinline__ Walk read_made(const u64* row, ptrdiff_t step, long long count, unsigned at, unsigned* in_vain) {
+    Walk m;
+    constexpr int kAhead = kGroup - 1;   // all there are of segments and groups (one more: registers that cost fp32 tensors with a gate a workgroup a CU, 6 % of the time)
     for (long long i = 0; i < count; i += kAhead, row += kAhead * step) {
         u64 v[kAhead];
 #pragma unroll
@@ -371,7 +409,7 @@ __device__ __forceinline__ Made read_made(const u64* row, ptrdiff_t step, long l
                     if (poll % 256 == 0 && __hip_atomic_load(in_vain, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) break;
                     if (poll == kMostPolls) __hip_atomic_store(in_vain, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 }
-                m = then(m, __builtin_bit_cast(Made, v[k]));
+                m.behind(__builtin_bit_cast(Packed, v[k]));
             }
     }
     return m;
@@ -383,15 +421,12 @@ template <class T, int C> __device__ __forceinline__ void hold_factors(Few<T, C>
     if constexpr (sizeof(T) == 4) {
         float s[C];
 #pragma unroll
-        for (int j = 0; j < C; ++j) {
-            const Factor f = factor_of<T>(u[j]);
-            s[j] = __builtin_copysignf(f.small, f.keeps ? 1.f : -1.f);
-        }
+        for (int j = 0; j < C; ++j) s[j] = held(factor_of<T>(u[j])).way;
         __builtin_memcpy(&u.word, s, sizeof(s));
     }
 }
-template <class T> __device__ __forceinline__ Factor held_factor(float u) {
-    if constexpr (sizeof(T) == 4) return Factor{fabsf(u), __builtin_bit_cast(int, u) >= 0};
+template <class T> __device__ __forceinline__ auto held_factor(float u) {
+    if constexpr (sizeof(T) == 4) return Held{u};
     else return factor_of<T>(u);
 }
 // A token that is none, which keeps the state.
@@ -416,14 +451,14 @@ template <bool kBack> __device__ __forceinline__ bool take_piece(const Recurrenc
 
 // The state in front of the wave's tokens (behind them, where kBack), from what its tokens make of one and all in front of them; `from` is the
 // sequence's first.  Publishes the segment's.  A wave and its neighbour see to half of the channels each, one a lane.
-template <int C, int W, bool kBack> __device__ __forceinline__ void state_at(const Recurrence& a, const Piece& p, unsigned c0, unsigned c, const Made (&own)[C],
+template <int C, int W, bool kBack> __device__ __forceinline__ void state_at(const Recurrence& a, const Piece& p, unsigned c0, unsigned c, const Walk (&own)[C],
                                                                              const float* from, float (&s)[C]) {
     constexpr int kChannels = kWave * C, kRoles = W / 2;
     constexpr long long kSize = W * kBatch;
-    __shared__ Made parts[W][kChannels], before[kRoles + 1][kChannels];
+    __shared__ Packed parts[W][kChannels], before[kRoles + 1][kChannels];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), order = kBack ? W - 1 - wave : wave;
 #pragma unroll
-    for (int j = 0; j < C; ++j) parts[order][c - c0 + j] = own[j];
+    for (int j = 0; j < C; ++j) parts[order][c - c0 + j] = own[j].packed();
     const long long place = p.begin / kSize;                                                 // in the sequence
     const long long at = kBack ? (span_of(a, p.n).length - 1) / kSize - place : place;       // as the walk goes
     const long long few = at % kGroup, group = at / kGroup, few_groups = group % kGroup, groups = group / kGroup;
@@ -433,35 +468,41 @@ template <int C, int W, bool kBack> __device__ __forceinline__ void state_at(con
     const ptrdiff_t width = a.width;
     const auto row_at = [&](int level, long long slot) { return a.made[level] + scalar(slot * width); };
     __syncthreads();
-    Made all{};
+    Packed all{};
     if (role == 0 && mine) {
-        all = parts[0][ch];
+        Walk here;
 #pragma unroll
-        for (int w = 1; w < W; ++w) all = then(all, parts[w][ch]);
+        for (int w = 0; w < W; ++w) here.behind(parts[w][ch]);
+        all = here.packed();
         publish(row_at(0, p.slot), word, all);
-        const Made front = read_made(row_at(0, kBack ? p.slot + few : p.slot - few), kBack ? -width : width, few, word, a.ticket + 1);
-        before[0][ch] = front;
-        all = then(front, all);
+        Walk walk = read_made(row_at(0, kBack ? p.slot + few : p.slot - few), kBack ? -width : width, few, word, a.ticket + 1);
+        before[0][ch] = walk.packed();
+        walk.behind(all);
+        all = walk.packed();
         if (few == kGroup - 1) publish(row_at(1, first_slot(a, p.n, kSize * kGroup) + group), word, all);
     } else if (mine) {
-        if (role == 1) before[1][ch] = read_made(row_at(1, first_slot(a, p.n, kSize * kGroup) + group - few_groups), width, few_groups, word, a.ticket + 1);
+        if (role == 1) before[1][ch] = read_made(row_at(1, first_slot(a, p.n, kSize * kGroup) + group - few_groups), width, few_groups, word, a.ticket + 1).packed();
         if (role > 1 || kRoles == 2) {   // the groups of groups, in as many parts as there are roles for
             constexpr int kParts = kRoles == 2 ? 1 : kRoles - 2;
             const int part = kRoles == 2 ? 0 : role - 2;
             const long long some = (groups + kParts - 1) / kParts, begin = part * some, left = groups - begin < some ? groups - begin : some;
-            before[2 + part][ch] = read_made(row_at(2, first_slot(a, p.n, kSize * kGroup * kGroup) + begin), width, left, word, a.ticket + 1);
+            before[2 + part][ch] = read_made(row_at(2, first_slot(a, p.n, kSize * kGroup * kGroup) + begin), width, left, word, a.ticket + 1).packed();
         }
     }
     __syncthreads();
-    if (role == 0 && mine && few == kGroup - 1 && few_groups == kGroup - 1)
-        publish(row_at(2, first_slot(a, p.n, kSize * kGroup * kGroup) + groups), word, then(before[1][ch], all));
+    if (role == 0 && mine && few == kGroup - 1 && few_groups == kGroup - 1) {
+        Walk walk;
+        walk.behind(before[1][ch]);
+        walk.behind(all);
+        publish(row_at(2, first_slot(a, p.n, kSize * kGroup * kGroup) + groups), word, walk.packed());
+    }
 #pragma unroll
     for (int j = 0; j < C; ++j) {
         s[j] = from ? from[p.n * a.width + c + j] : 0.f;
 #pragma unroll
-        for (int r = 2; r < (kRoles == 2 ? 3 : kRoles); ++r) s[j] = of(before[r][c - c0 + j], s[j]);
-        s[j] = of(before[0][c - c0 + j], of(before[1][c - c0 + j], s[j]));
-        for (int w = 0; w < order; ++w) s[j] = of(parts[w][c - c0 + j], s[j]);
+        for (int r = 2; r < (kRoles == 2 ? 3 : kRoles); ++r) s[j] = of(unpacked(before[r][c - c0 + j]), s[j]);
+        s[j] = of(unpacked(before[0][c - c0 + j]), of(unpacked(before[1][c - c0 + j]), s[j]));
+        for (int w = 0; w < order; ++w) s[j] = of(unpacked(parts[w][c - c0 + j]), s[j]);
     }
 }
 
@@ -493,20 +534,19 @@ __global__ __launch_bounds__(W * kWave, C == 2 && sizeof(T) == 2 ? 6 : 3) void s
     // of 1024 channels with a gate, bf16, where the vector units are the bound).
     constexpr int kInLds = sizeof(T) == 2 ? kBatch / 2 : 0;
     __shared__ Few<float, C> factors[kInLds ? kInLds : 1][kInLds ? W * kWave : 1];
-    Made made[C];
-#pragma unroll
-    for (int j = 0; j < C; ++j) made[j] = Made{1.f, 0.f};
+    Walk made[C];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
         hold_factors<T, C>(u[i]);
-        float small[C];
+        float way[C];
 #pragma unroll
         for (int j = 0; j < C; ++j) {
-            const Factor k = held_factor<T>(u[i][j]);
-            small[j] = __builtin_copysignf(k.small, k.keeps ? 1.f : -1.f);
-            made[j] = Made{kept(k, made[j].factor), stepped(k, made[j].sum, x[i][j])};
+            const Factor k = factor(held_factor<T>(u[i][j]));   // (as Held, 20 registers more of fp32 tensors without a gate, and 4 % of the time)
+            way[j] = held(k).way;
+            made[j].leaves(k);
+            made[j].sum = stepped(k, made[j].sum, x[i][j]);
         }
-        if (i < kInLds) __builtin_memcpy(&factors[i][threadIdx.x].word, small, sizeof(small));
+        if (i < kInLds) __builtin_memcpy(&factors[i][threadIdx.x].word, way, sizeof(way));
     }
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
@@ -525,8 +565,7 @@ __global__ __launch_bounds__(W * kWave, C == 2 && sizeof(T) == 2 ? 6 : 3) void s
         if (i < kInLds) in_lds = factors[i][threadIdx.x];
 #pragma unroll
         for (int j = 0; j < C; ++j) {
-            const Factor k = i < kInLds ? held_factor<float>(in_lds[j]) : held_factor<T>(u[i][j]);
-            s[j] = stepped(k, s[j], x[i][j]);
+            s[j] = i < kInLds ? stepped(Held{in_lds[j]}, s[j], x[i][j]) : stepped(held_factor<T>(u[i][j]), s[j], x[i][j]);
             o[j] = s[j];
             if constexpr (kGate) o[j] *= sigmoid<T>(g[i][j]);
         }
@@ -567,22 +606,21 @@ template <class T, int C, bool kGate, bool kPassing, int W> __global__ __launch_
     if (count > 0) first = load_state<C>(a.saved, first_slot(a, p.n, kBatch) + t / kBatch, a, c);
     constexpr int kInLds = sizeof(T) == 2 ? kBatch : 0;   // tokens whose factors stay in LDS
     __shared__ Few<float, C> factors[kInLds ? kInLds : 1][kInLds ? W * kWave : 1];
-    Made made[C];
-#pragma unroll
-    for (int j = 0; j < C; ++j) made[j] = Made{1.f, 0.f};
+    Walk made[C];
 #pragma unroll
     for (int i = kBatch - 1; i >= 0; --i) {
         hold_factors<T, C>(u[i]);
-        float small[C];
+        float way[C];
 #pragma unroll
         for (int j = 0; j < C; ++j) {
-            const Factor k = held_factor<T>(u[i][j]);
-            small[j] = __builtin_copysignf(k.small, k.keeps ? 1.f : -1.f);
+            const auto k = held_factor<T>(u[i][j]);
+            way[j] = held(k).way;
             float dc = d[i][j];
             if constexpr (kGate) dc *= sigmoid<T>(g[i][j]);
-            made[j] = Made{kept(k, made[j].factor), kept(k, made[j].sum + dc)};
+            made[j].leaves(k);
+            made[j].sum = kept(k, made[j].sum + dc);
         }
-        if (i < kInLds) __builtin_memcpy(&factors[i][threadIdx.x].word, small, sizeof(small));
+        if (i < kInLds) __builtin_memcpy(&factors[i][threadIdx.x].word, way, sizeof(way));
     }
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
@@ -599,7 +637,10 @@ template <class T, int C, bool kGate, bool kPassing, int W> __global__ __launch_
     for (int i = 0; i < kBatch; ++i) {
         x[i].forget();   // (the states from here on)
 #pragma unroll
-        for (int j = 0; j < C; ++j) state[i + 1][j] = stepped(i < kInLds ? held_factor<float>(factors[i][threadIdx.x][j]) : held_factor<T>(u[i][j]), state[i][j], x[i][j]);
+        for (int j = 0; j < C; ++j) {
+            if constexpr (kInLds > 0) state[i + 1][j] = stepped(Held{factors[i][threadIdx.x][j]}, state[i][j], x[i][j]);
+            else state[i + 1][j] = stepped(held_factor<T>(u[i][j]), state[i][j], x[i][j]);
+        }
     }
     const Gradients to = gradients_at<T>(a, p, t);
 #pragma unroll
