@@ -39,9 +39,9 @@ struct Select {
     size_t first;                   // the launch's first row, or sequence
 };
 
-// A logit as a whole number that orders alike; 0 for what is no candidate.
+// A logit as a whole number that orders alike, zeros of either sign the same; 0 for what is no candidate.
 __device__ __forceinline__ unsigned order_of(float z) {
-    const unsigned u = __builtin_bit_cast(unsigned, z);
+    const unsigned u = __builtin_bit_cast(unsigned, z + 0.f);   // (-0 + 0 is +0)
     return u ^ (unsigned(int(u) >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float logit_of(unsigned o) { return __builtin_bit_cast(float, o ^ (o >> 31 ? 0x80000000u : 0xffffffffu)); }
@@ -265,7 +265,7 @@ struct Candidate {
 };
 __device__ __forceinline__ bool ahead(const Candidate& x, const Candidate& y) { return x.order > y.order || (x.order == y.order && x.place < y.place); }
 __device__ __forceinline__ u64 order_of(double v) {
-    const u64 u = __builtin_bit_cast(u64, v);
+    const u64 u = __builtin_bit_cast(u64, v + 0.);
     return u ^ (u64(static_cast<long long>(u) >> 63) | u64(1) << 63);
 }
 __device__ __forceinline__ double value_of(u64 o) { return __builtin_bit_cast(double, o ^ (o >> 63 ? u64(1) << 63 : ~u64(0))); }
