@@ -168,8 +168,9 @@ template <class T> __global__ __launch_bounds__(kThreads) void part_kernel(Selec
         m = fmaxf(most, lanes_max<kWave>(m));
         sum *= __builtin_amdgcn_exp2f((most - m) * kLog2e);
         most = m;
-        // exponents as one operation each, z log2(e) - shift; what the rounding of shift is off by is put right behind the sum
-        const float shift = most * kLog2e;
+        // exponents as one operation each, z log2(e) - shift; what the rounding of shift is off by is put right behind the sum, as long as that leaves the sum's terms in
+        // range (most below 2^30, say: beyond it a step of shift can be a factor of 2^64 and more)
+        const float shift = most * kLog2e, off = __builtin_fmaf(most, kLog2e, -shift);
         const float reached = __builtin_fmaf(bound, kLog2e, -shift);   // (rounding keeps the order)
         float more = 0.f;
         unsigned reach = 0;   // a bit for each of this thread's vectors: whether an entry reaches the bound
@@ -190,8 +191,8 @@ template <class T> __global__ __launch_bounds__(kThreads) void part_kernel(Selec
             reach &= reach - 1;
             places[atomicAdd(&vectors, 1)] = base + (j * kThreads + tid) * 8;
         }
-        if (more < __builtin_inff() && fabsf(shift) < __builtin_inff()) {
-            more *= __builtin_amdgcn_exp2f(-__builtin_fmaf(most, kLog2e, -shift));
+        if (more < __builtin_inff() && fabsf(off) <= 64.f) {
+            more *= __builtin_amdgcn_exp2f(-off);
         } else {   // a NaN or an infinity among them, or exponents that are none: once more, number by number
             more = 0.f;
             for (int i = 0; i < kVectors * 8; ++i) {

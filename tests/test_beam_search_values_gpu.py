@@ -1,4 +1,5 @@
-"""Beam search's selection over values where numbers that are equal have more than one form.  Against the definition of test_beam_search_gpu.py, with its bounds."""
+"""Beam search's selection over values where numbers that are equal have more than one form, and where sums of exponentials leave the range of 32 bits
+on the way.  Against the definition of test_beam_search_gpu.py, with its bounds."""
 import pytest
 import torch
 
@@ -43,3 +44,20 @@ def test_scores_of_zero_of_either_sign_are_equal():
         assert parents.tolist() == [[0, 1]] and scores.tolist() == [[0, 0]] and tokens.tolist() == [[0, 0]]
         scores, parents, tokens, finished = fl.beam_select(torch.zeros(1, 2, 1, device="cuda"), torch.tensor([[0.0, -0.0]], device="cuda"), end=0, finished=flags)
         assert parents.tolist() == [[0, 1]] and scores.tolist() == [[0, 0]] and tokens.tolist() == [[0, 0]]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("size", [1e7, 1e9, 3e9, 1e10, 3e11, 1e12, 1e15, 3e18, 1e20, 1e25, 1e30, 1e38])
+def test_logits_of_any_size(size, dtype):
+    """Masks of a large negative value, over some or all of a row or over whole parts of it, and a row whose largest logit is as large."""
+    for vocabulary in (40, 9000, 50001):
+        p = _problem(5, 3, vocabulary, dtype, seed=17, finished=0)
+        z, half = p["logits"], vocabulary // 3
+        z[0, :, half:] = -size                          # the first tokens alone
+        z[1, :, :-2] = -size                            # the last ones alone
+        z[2, 1] = -size                                 # a row of nothing else
+        z[3] = -size * (1 + torch.rand(3, vocabulary, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))).to(dtype)
+        z[4, 1, half] = size
+        z[4, 2, ::2] = size
+        _check(p, f"{size} of {vocabulary} {dtype}")
+        _check(p, f"{size} of {vocabulary} {dtype}, its negative", logits=-z)
