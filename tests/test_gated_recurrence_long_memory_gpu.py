@@ -3,9 +3,9 @@ token adds up.
 
 Bounds, with u = 2^-24 and M the state (the gradient) with all its terms taken as magnitudes.  Cut into segments, a state is put together from what the
 16 tokens of a wave, the waves of a segment, 8 segments, 8 groups and all groups of groups in front make of one, and 16 tokens walked.
-* Every such step s -> F s + S rounds a difference S - (1 - F) s and a sum, of magnitudes below 2 M and M: 3 u M.  The steps inside of a piece do that to
-  the piece's own S, of which the pieces have M between them, and a piece keeps of an error no more than F <= 1.  At most 16 + 8 + 8 + 8 + 16 of
-  them and one for each of the groups of groups in front, G: 3 (56 + G) u M.
+* Every such step s -> F s + S rounds F, of a state of M at most, and the sum: 2 u M.  The steps inside of a piece do that to the piece's own S, of which
+  the pieces have M between them, and a piece keeps of an error no more than F <= 1.  At most 16 + 8 + 8 + 8 + 16 of them and one for each of the
+  groups of groups in front, G: 2 (56 + G) u M.
 * A token's smaller sigmoid is off by (|a| + 6) u of itself (see test_gated_recurrence_gpu.py), what its step rounds included (|a| + 8) u; and 1 - F by 2 u a
   step more, as its terms have one sign: 2 (16 + 8 + 8 + 8 + G).  A weight of x, s (1 - s)^n, changes by no more than (1 + s n / (1 - s)) of that, and the
   sum over n of s (1 - s)^n s n is below 1, where the values and the state that it starts from are of one size: 2 (|a| + 8) + 4 (40 + G) u M.
@@ -21,7 +21,7 @@ pytestmark = pytest.mark.gpu
 
 
 def _bound(gate, groups):
-    return (3 * (56 + groups) + 4 * (40 + groups) + 2 * (gate.abs() + 8)) * U32
+    return (2 * (56 + groups) + 4 * (40 + groups) + 2 * (gate.abs() + 8)) * U32
 
 
 def _walked(first, keep, take, x):
