@@ -5,7 +5,7 @@
 // another: chunks of the sorted list are summed in registers, in the order of the positions, and written once where a token's rows end.  What
 // crosses a chunk's border is put together in LDS by the workgroup, whose chunks follow each other, and what crosses the workgroup's is left as partial
 // sums that a last kernel adds up in order.  No atomics on values: the result depends on tokens and sizes alone.
-// Few tokens are sorted by counting for each how many come in front of it, in one launch; many in stable passes over eight to ten bits.
+// Few tokens are sorted by counting for each how many come in front of it, in one launch; many in stable passes over at most ten bits.
 // 65536 tokens of a text, 1024 fp16 channels, 50001 fp32 rows: lookup 38 us, 7.1 TB/s with what the caches hold of the table; sort 40, which writes
 // 205 MB of zeros meanwhile, 5.1 TB/s; sums 44, 4.6 TB/s; partial sums 5.
 #include <algorithm>
@@ -577,7 +577,8 @@ extern "C" int flstm_embedding_backward(const flstm_embedding* p, const void* d_
             const bool passing = p->tokens * p->width * sizeof(From) >= kMostRead && ldd * sizeof(From) % kLine == 0 && reinterpret_cast<uintptr_t>(d_out) % kLine == 0;
             const auto sum = [&](auto lanes, auto vector) {
                 constexpr int kLanes = decltype(lanes)::value, N = decltype(vector)::value;
-                if (N > 1 && passing) sum_kernel<From, To, N, kLanes, true><<<grid, kThreads, 0, s>>>(a);
+                constexpr bool kPassing = N > 1;   // (not for rows of less than a vector, column by column)
+                if (kPassing && passing) sum_kernel<From, To, N, kLanes, kPassing><<<grid, kThreads, 0, s>>>(a);
                 else sum_kernel<From, To, N, kLanes, false><<<grid, kThreads, 0, s>>>(a);
                 if (const int rc = launched()) return rc;
                 if (a.groups > 1) join_kernel<To, N><<<unsigned(joins), kThreads, 0, s>>>(a, unsigned(plan.size()));
