@@ -91,7 +91,8 @@ int flstm_decay_attention_backward(const flstm_decay_attention* shape, const fls
                                    const flstm_rows* v, const float* state_in, const float* d_state_out, const flstm_rows* dq,
                                    const flstm_rows* dk, const flstm_rows* dv, float* d_state_in, void* workspace, void* stream);
 size_t flstm_decay_attention_workspace_bytes(const flstm_decay_attention* shape, int backward);
-/* One token of every sequence (shape->tokens and cu_seqlens are not read), the state updated in place. */
+/* One token of every sequence, the state updated in place.  shape->tokens and cu_seqlens have to be what the forward pass takes (0 and null, say) and
+ * change nothing. */
 int flstm_decay_attention_step(const flstm_decay_attention* shape, const flstm_rows* q, const flstm_rows* k, const flstm_rows* v,
                                const flstm_rows* o, float* state, void* stream);
 
@@ -192,7 +193,8 @@ int flstm_gated_recurrence_backward(const flstm_recurrence* shape, const flstm_r
                                     const flstm_rows* dforget, const flstm_rows* dgate, float* d_state_in, void* workspace, void* stream);
 size_t flstm_gated_recurrence_workspace_bytes(const flstm_recurrence* shape, int backward);
 size_t flstm_gated_recurrence_saved_rows(const flstm_recurrence* shape);
-/* One token of every sequence (shape->tokens, cu_seqlens and .token are not read), the state updated in place. */
+/* One token of every sequence, the state updated in place.  shape->tokens and cu_seqlens have to be what the forward pass takes (0 and null, say) and
+ * change nothing; .token is not read. */
 int flstm_gated_recurrence_step(const flstm_recurrence* shape, const flstm_rows* x, const flstm_rows* forget, const flstm_rows* gate,
                                 const flstm_rows* y, float* state, void* stream);
 
