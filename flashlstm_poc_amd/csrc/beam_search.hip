@@ -457,8 +457,8 @@ template <int B> __global__ __launch_bounds__(kThreads) void reorder_kernel(Reor
 
 // ---- host side
 
-// `count` rows of `bytes` at every `stride` from `at` on; whether two such have memory in common, where one launch would move it twice.  Rows of one
-// stride may lie between each other's (halves of a wider state); of unlike strides that is not looked into.
+// `count` rows of `bytes` at every `stride` from `at` on; whether two such have memory in common, where one launch would move it twice.  Rows may lie between
+// each other's (halves of a wider state).
 struct Extent {
     size_t at, stride, bytes, count;
 };
@@ -470,7 +470,14 @@ bool meet(Extent x, Extent y) {
     }
     const size_t apart = y.at - x.at;
     if (apart / x.stride >= x.count || (apart / x.stride == x.count - 1 && apart % x.stride >= x.bytes)) return false;
-    return x.stride != y.stride || apart % x.stride < x.bytes || x.stride - apart % x.stride < y.bytes;
+    if (x.stride == y.stride) return apart % x.stride < x.bytes || x.stride - apart % x.stride < y.bytes;
+    for (size_t i = apart / x.stride, j = 0; i < x.count && j < y.count;) {   // a row each, of which the one in front does not reach the other
+        const size_t of_x = i * x.stride, of_y = apart + j * y.stride;
+        if (of_x <= of_y ? of_y - of_x < x.bytes : of_x - of_y < y.bytes) return true;
+        if (of_x <= of_y) i = of_y / x.stride > i ? of_y / x.stride : i + 1;
+        else j = (of_x - apart) / y.stride > j ? (of_x - apart) / y.stride : j + 1;
+    }
+    return false;
 }
 
 constexpr size_t kMostBlocks = 0xffffffffu / kThreads;

@@ -229,7 +229,7 @@ int flstm_beam_select(const flstm_beams* problem, float* scores, long long* pare
 
 /* Row (s, b) of each of `count` tensors becomes what row (s, parents[s][b]) was, in place, sixteen tensors a launch.  Rows of `bytes` bytes begin
  * (s * beams + b) * stride bytes behind data; 1 <= beams <= 32.  A parent outside 0 .. beams - 1 leaves its row as it is.  FLSTM_E_INVALID
- * where tensors share memory with each other or with the parents; rows of one stride may lie between each other's. */
+ * where tensors share memory with each other or with the parents; rows may lie between each other's. */
 typedef struct {
     void* data;
     size_t stride, bytes;
