@@ -116,26 +116,42 @@ def _ptr(t) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
-# An allocation without torch's dispatch of it, where torch has one: 0.8 us instead of 1.7, of calls that take 8.
+# An allocation without torch's dispatch of it, where torch has one of this signature: 0.8 us instead of 1.7, of calls that take 8.  Through torch where something
+# looks at what is dispatched (a mode that counts memory, say) or fills new memory (deterministic algorithms).
 _EMPTY_STRIDED = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
+_DISPATCH_MODES = getattr(torch._C, "_len_torch_dispatch_stack", None)
+_DETERMINISTIC = getattr(torch._C, "_get_deterministic_algorithms", torch.are_deterministic_algorithms_enabled)
 
 
-def _empty(shape, dtype):
-    """A contiguous tensor on the current device, of any content."""
-    if _EMPTY_STRIDED is None or 0 in shape:
-        return torch.empty(shape, device="cuda", dtype=dtype)
-    if len(shape) == 2:
-        return _EMPTY_STRIDED(tuple(shape), (shape[1], 1), dtype)
-    strides, stride = [], 1
-    for n in reversed(shape):
-        strides.append(stride)
-        stride *= n
-    return _EMPTY_STRIDED(tuple(shape), tuple(reversed(strides)), dtype)
+def _dispatched(shape, dtype):
+    return torch.empty(shape, device="cuda", dtype=dtype)
 
 
-def _scratch(size: int):
+def _direct(shape, dtype):
+    global _EMPTY_STRIDED
+    if 0 in shape:
+        return _dispatched(shape, dtype)
+    try:
+        if len(shape) == 2:
+            return _EMPTY_STRIDED(tuple(shape), (shape[1], 1), dtype)
+        strides, stride = [], 1
+        for n in reversed(shape):
+            strides.append(stride)
+            stride *= n
+        return _EMPTY_STRIDED(tuple(shape), tuple(reversed(strides)), dtype)
+    except TypeError:   # another signature, or none
+        _EMPTY_STRIDED = None
+        return _dispatched(shape, dtype)
+
+
+def _allocation():
+    """What allocates a call's tensors: (shape, dtype) -> a contiguous tensor on the current device, of any content."""
+    return _dispatched if _EMPTY_STRIDED is None or _DISPATCH_MODES is None or _DISPATCH_MODES() or _DETERMINISTIC() else _direct
+
+
+def _scratch(size: int, empty):
     """`size` bytes on the current device, None where there are to be none."""
-    return _empty((size,), torch.uint8) if size else None
+    return empty((size,), torch.uint8) if size else None
 
 
 # ---- layer norm
@@ -609,7 +625,7 @@ def embedding_forward(tokens, table, *, scale: float = 1.0, dtype=None):
     dtype = table.dtype if dtype is None else dtype
     out_code, scale = _op_dtype("dtype", dtype), _scale(scale)
     (vocabulary, width), tokens = table.shape, tokens.contiguous()
-    out = _empty((*tokens.shape, width), dtype)
+    out = _allocation()((*tokens.shape, width), dtype)
     if out.numel() == 0:
         return out
     rows, ld = table, width
@@ -633,14 +649,15 @@ def embedding_backward(d_out, tokens, vocabulary: int, *, scale: float = 1.0, dt
     if vocabulary < 1:
         raise ValueError("vocabulary must be >= 1")
     out_code, scale, width = _op_dtype("dtype", dtype), _scale(scale), d_out.shape[-1]
-    d_table = _empty((vocabulary, width), dtype)
+    empty = _allocation()
+    d_table = empty((vocabulary, width), dtype)
     if width == 0:
         return d_table
     tokens = tokens.contiguous()
     rows = _rows(d_out) if d_out.numel() else d_out.reshape(0, width)
     problem = _EMBEDDING.pack(tokens.numel(), vocabulary, width, tokens.data_ptr(), index_64, scale)
     lib = _bind()
-    workspace = _scratch(lib.flstm_embedding_workspace_bytes(problem))
+    workspace = _scratch(lib.flstm_embedding_workspace_bytes(problem), empty)
     _check(lib.flstm_embedding_backward(problem, rows.data_ptr(), rows.stride(0), code, d_table.data_ptr(), out_code, _ptr(workspace), _stream()),
            "flstm_embedding_backward")
     return d_table
@@ -723,15 +740,15 @@ def _channel_rows(t, packed: bool = False):
     return _ROWS.pack(t.data_ptr(), 0 if packed else s[0], s[-2] if packed or len(s) == 3 else 0, 0)
 
 
-def _like_channels(x):
+def _like_channels(x, empty):
     """An output in the memory order of x's rows."""
     if x.dim() == 3 and x.stride(0) < x.stride(1) and x.shape[0] > 1:
-        return _empty((x.shape[1], x.shape[0], x.shape[2]), x.dtype).transpose(0, 1)
-    return _empty(x.shape, x.dtype)
+        return empty((x.shape[1], x.shape[0], x.shape[2]), x.dtype).transpose(0, 1)
+    return empty(x.shape, x.dtype)
 
 
-def _recurrence_workspace(shape: bytes, backward: int):
-    return _scratch(_bind().flstm_gated_recurrence_workspace_bytes(shape, backward))
+def _recurrence_workspace(shape: bytes, backward: int, empty):
+    return _scratch(_bind().flstm_gated_recurrence_workspace_bytes(shape, backward), empty)
 
 
 def gated_recurrence_forward(x, forget, gate=None, *, state=None, cu_seqlens=None, want_state: bool = True, want_saved: bool = True) -> Tuple:
@@ -745,10 +762,11 @@ def gated_recurrence_forward(x, forget, gate=None, *, state=None, cu_seqlens=Non
     shape, states = _recurrence(x, forget, gate, state, cu_seqlens, 2 if packed else 3)
     x, forget = _last_axis_contiguous(x), _last_axis_contiguous(forget)
     gate = None if gate is None else _last_axis_contiguous(gate)
-    y, lib = _like_channels(x), _bind()
-    final = _empty(states, torch.float32) if want_state else None
-    saved = _empty((lib.flstm_gated_recurrence_saved_rows(shape), states[1]), torch.float32) if want_saved else None
-    workspace = _recurrence_workspace(shape, 0)
+    empty, lib = _allocation(), _bind()
+    y = _like_channels(x, empty)
+    final = empty(states, torch.float32) if want_state else None
+    saved = empty((lib.flstm_gated_recurrence_saved_rows(shape), states[1]), torch.float32) if want_saved else None
+    workspace = _recurrence_workspace(shape, 0, empty)
     _check(lib.flstm_gated_recurrence_forward(shape, _channel_rows(x, packed), _channel_rows(forget, packed), _channel_rows(gate, packed), _ptr(state),
                                               _channel_rows(y, packed), _ptr(final), _ptr(saved), _ptr(workspace), _stream()),
            "flstm_gated_recurrence_forward")
@@ -769,11 +787,12 @@ def gated_recurrence_backward(dy, x, forget, gate, saved, *, d_state=None, cu_se
         raise ValueError("saved must be what the forward pass returned")
     dy, x, forget = (_last_axis_contiguous(t) for t in (dy, x, forget))
     gate = None if gate is None else _last_axis_contiguous(gate)
-    dx = _like_channels(x) if want[0] else None
-    dforget = _like_channels(x) if want[1] else None
-    dgate = _like_channels(x) if want[2] and gate is not None else None
-    d_initial = _empty(states, torch.float32) if want[3] else None
-    workspace = _recurrence_workspace(shape, 1)
+    empty = _allocation()
+    dx = _like_channels(x, empty) if want[0] else None
+    dforget = _like_channels(x, empty) if want[1] else None
+    dgate = _like_channels(x, empty) if want[2] and gate is not None else None
+    d_initial = empty(states, torch.float32) if want[3] else None
+    workspace = _recurrence_workspace(shape, 1, empty)
     _check(lib.flstm_gated_recurrence_backward(
         shape, _channel_rows(dy, packed), _channel_rows(x, packed), _channel_rows(forget, packed), _channel_rows(gate, packed), saved.data_ptr(),
         _ptr(d_state), _channel_rows(dx, packed), _channel_rows(dforget, packed), _channel_rows(dgate, packed), _ptr(d_initial), _ptr(workspace),
@@ -789,7 +808,7 @@ def gated_recurrence_step(x, forget, state, gate=None):
     shape, states = _recurrence(x, forget, gate, state, None, 2)
     x, forget = _last_axis_contiguous(x), _last_axis_contiguous(forget)
     gate = None if gate is None else _last_axis_contiguous(gate)
-    y = _empty(states, x.dtype)
+    y = _allocation()(states, x.dtype)
     _check(_bind().flstm_gated_recurrence_step(shape, _channel_rows(x), _channel_rows(forget), _channel_rows(gate), _channel_rows(y), state.data_ptr(),
                                                _stream()), "flstm_gated_recurrence_step")
     _written(state)
@@ -868,12 +887,13 @@ def beam_select(logits, scores, *, beams: Optional[int] = None, end: Optional[in
         if ld < vocabulary:   # (rows that share memory)
             rows, ld = rows.contiguous(), vocabulary
     shape = (sequences, keep)
-    out_scores, parents, tokens = _empty(shape, torch.float32), _empty(shape, torch.int64), _empty(shape, torch.int64)
-    out_finished = None if end is None else _empty(shape, torch.bool)
+    empty = _allocation()
+    out_scores, parents, tokens = empty(shape, torch.float32), empty(shape, torch.int64), empty(shape, torch.int64)
+    out_finished = None if end is None else empty(shape, torch.bool)
     problem = _BEAMS.pack(sequences, hypotheses, keep, vocabulary, rows.data_ptr(), ld, code, scores.data_ptr(), _ptr(finished) or 0,
                           -1 if end is None else end)
     lib = _bind()
-    workspace = _scratch(lib.flstm_beam_select_workspace_bytes(problem))
+    workspace = _scratch(lib.flstm_beam_select_workspace_bytes(problem), empty)
     _check(lib.flstm_beam_select(problem, out_scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(), _ptr(out_finished), _ptr(workspace),
                                  _stream()), "flstm_beam_select")
     return out_scores, parents, tokens, out_finished
