@@ -685,7 +685,10 @@ def embedding(tokens, table, *, scale: float = 1.0, dtype=None):
 
 
 class Embedding(torch.nn.Module):
-    """Rows of a table of fp32 parameters, named and initialised as torch.nn.Embedding's, scaled, as activations of type `dtype`."""
+    """Rows of a table of fp32 parameters, named and initialised as torch.nn.Embedding's, scaled, as activations of type `dtype`; zeros for tokens outside
+    the vocabulary, which are what pads (none of those inside does)."""
+
+    padding_idx = None
 
     def __init__(self, vocabulary: int, width: int, *, scale: float = 1.0, dtype=torch.float32, device="cuda"):
         super().__init__()
@@ -695,6 +698,14 @@ class Embedding(torch.nn.Module):
         self.vocabulary, self.width, self.scale, self.dtype = int(vocabulary), int(width), _scale(scale), dtype
         self.weight = torch.nn.Parameter(torch.empty((self.vocabulary, self.width), device=device, dtype=torch.float32))
         torch.nn.init.normal_(self.weight)
+
+    @property
+    def num_embeddings(self) -> int:
+        return self.vocabulary
+
+    @property
+    def embedding_dim(self) -> int:
+        return self.width
 
     def forward(self, tokens):
         return embedding(tokens, self.weight, scale=self.scale, dtype=self.dtype)

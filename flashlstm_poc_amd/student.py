@@ -92,7 +92,8 @@ class RecurrentLayer(torch.nn.Module):
 
 
 class RecurrentStudent(torch.nn.Module):
-    """Tokens (T, B) -> logits (T, B, vocabulary) fp16; parameters fp32, activations fp16."""
+    """Tokens (T, B) -> logits (T, B, vocabulary) fp16; parameters fp32, activations fp16.  Tokens outside the vocabulary (-1, say) are padding: their
+    embeddings are zeros, and nothing is learnt from them."""
 
     def __init__(self, vocabulary: int, width: int, heads: int, layers: int = 1, device="cuda", recurrence: str = "lstm"):
         super().__init__()
@@ -173,6 +174,8 @@ def train(student: RecurrentStudent, teacher, steps: int, *, length: int = 64, b
     loss_scale: on the mean, so that fp16 gradients of a logit (about 1 / (rows * vocabulary)) lie in that type's range; taken out
     of the parameters' gradients."""
     logits, index = teacher
+    if logits.shape[0] > student.embedding.vocabulary:   # (of which the student would take the last tokens for padding)
+        raise ValueError(f"the teacher has {logits.shape[0]} tokens, the student {student.embedding.vocabulary}")
     device = logits.device
     g = torch.Generator(device=device).manual_seed(seed)
     optimizer = torch.optim.Adam(student.parameters(), lr=rate)
