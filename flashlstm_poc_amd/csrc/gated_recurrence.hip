@@ -691,7 +691,9 @@ bool valid_shape(const flstm_recurrence* p) {
 // a gate, 1024 channels): one sequence of 64 tokens 18 / 15 and 25 / 25, of 128 18 / 22 and 24 / 44, of 512 19 / 75 and 25 / 158; 64 of 128 27 / 25 and 43 /
 // 48, of 2048 237 / 417 and 427 / 724; 128 of 128 43 / 32 and 63 / 56, of 1024 233 / 234 and 416 / 402; 256 of 512 224 / 214 and 400 / 380.
 // Of packed sequences the longest decides how long the whole walk takes, and is not known: 200 of up to 2000 tokens 387 / 543 and 688 / 934, 400 of up
-// to 1000 429 / 474 and 758 / 823, but 200 of up to 100 51 / 34 and 67 / 55.
+// to 1000 429 / 474 and 758 / 823, but 200 of up to 100 51 / 34 and 67 / 55.  All of these are of lengths spread evenly up to the longest: the rule knows the mean alone,
+// and one long sequence among many short ones is walked whole however long it is (199 of 50 tokens and one of 10000: 1511 and 3103 us; 511 of 10 and one of
+// 60000: 10720 and 19393).
 bool split(const flstm_recurrence* p) {
     const size_t lanes = round_up(ceil_div(p->width, 2), kWave);
     if (p->tokens <= 64) return false;

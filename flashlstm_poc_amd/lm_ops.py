@@ -862,7 +862,8 @@ _MAX_BEAMS = 32
 
 def beam_select(logits, scores, *, beams: Optional[int] = None, end: Optional[int] = None, finished=None) -> Tuple:
     """The best continuations of every sequence's hypotheses by one token, by scores + log_softmax(logits), the best first and of equal ones
-    that of the lower hypothesis and token.
+    that of the lower hypothesis and token.  (The sum in log_softmax is held in 32 bits: continuations of different hypotheses that are nearer than 48 * 2^-24
+    may come in either order, unless logits and scores are equal.)
 
     logits (sequences, hypotheses, vocabulary) float32 / float16 / bfloat16, scores (sequences, hypotheses) float32 (minus infinity: no
     hypothesis).  beams: how many are kept, as many as there are where None; up to 32 of both.  end: the token that ends a hypothesis;

@@ -207,7 +207,8 @@ int flstm_gated_recurrence_step(const flstm_recurrence* shape, const flstm_rows*
  * logits are not read.  Logits of minus infinity and NaN are no continuations; plus infinity counts as the largest number of fp32.  Where
  * there are fewer than `keep`, the places behind them get the score minus infinity, the token -1 and the place itself as parent (0 from
  * `beams` on).  A returned hypothesis is finished if its token is `end` or -1.
- * Scores are compared in 64 bits and returned in 32.  Row (s, b) of the logits begins (s * beams + b) * ld elements behind the first.
+ * Scores are compared in 64 bits and returned in 32.  The sum of exponentials is held in 32 bits, its logarithm off by up to 48 * 2^-24: continuations of
+ * different hypotheses whose scores are nearer than that may come in either order, unless rows and scores are equal.  Row (s, b) of the logits begins (s * beams + b) * ld elements behind the first.
  * 1 <= beams, keep <= 32, vocabulary below 2^31 - 65536.  Results must not lie in the inputs.
  * `workspace`: flstm_beam_select_workspace_bytes() bytes, 16-byte aligned. */
 typedef struct {
