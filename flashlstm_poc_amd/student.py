@@ -174,8 +174,8 @@ def train(student: RecurrentStudent, teacher, steps: int, *, length: int = 64, b
     loss_scale: on the mean, so that fp16 gradients of a logit (about 1 / (rows * vocabulary)) lie in that type's range; taken out
     of the parameters' gradients."""
     logits, index = teacher
-    if logits.shape[0] > student.embedding.vocabulary:   # (of which the student would take the last tokens for padding)
-        raise ValueError(f"the teacher has {logits.shape[0]} tokens, the student {student.embedding.vocabulary}")
+    if logits.shape[0] > student.embedding.num_embeddings:   # (of which the student would take the last tokens for padding)
+        raise ValueError(f"the teacher has {logits.shape[0]} tokens, the student {student.embedding.num_embeddings}")
     device = logits.device
     g = torch.Generator(device=device).manual_seed(seed)
     optimizer = torch.optim.Adam(student.parameters(), lr=rate)
