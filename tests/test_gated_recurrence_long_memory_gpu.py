@@ -16,6 +16,7 @@ import torch
 
 import flashlstm_poc_amd as fl
 from lm_helpers import DTYPES, U32, assert_within
+from test_gated_recurrence_gpu import _check, _problem
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +64,16 @@ def test_gates_that_stay_the_same(dtype, sign):
             ("dx", dx[0], z * total, z * (of_total + (rel + 2 * U32) * size)),
             ("dforget", dforget[0], total * way * f * z, f * z * (of_total * way.abs() + size * of_way + (2 * rel + 4 * U32) * size * (of_c[:-1] + x.double().abs())))):
         assert_within(got.cpu(), want, bound, f"{dtype} {name}")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_gates_of_all_sizes(dtype):
+    """Factors of pieces from nothing to one, in every order, over states of all sizes; bounds of test_gated_recurrence_gpu.py."""
+    p = _problem((2, 20000, 12), dtype, 2, True, seed=22)
+    g = torch.Generator(device="cuda").manual_seed(23)
+    sizes = torch.tensor([-60.0, -7.0, -1.0, 0.0, 0.5, 3.0, 9.0, 14.0, 40.0], device="cuda")
+    drawn = sizes[torch.randint(0, 9, (2, 20000, 12), device="cuda", generator=g)].to(dtype)
+    keeps = torch.rand(2, 20000, 12, device="cuda", generator=g) < torch.tensor([0.0, 0.5, 0.99, 0.999, 0.9999, 1.0], device="cuda").repeat(2)
+    p["forget"] = torch.where(keeps, drawn.abs() + 6, drawn)
+    p["state"], p["d_state"] = p["state"] * 10.0 ** torch.arange(-6, 6, device="cuda"), p["d_state"] * 10.0 ** torch.arange(5, -7, -1, device="cuda")
+    _check(p, f"{dtype}")
